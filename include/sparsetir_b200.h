@@ -43,7 +43,7 @@ extern "C" {
 #ifndef DLPACK_DLPACK_H_
 typedef enum { kDLCPU = 1, kDLCUDA = 2, kDLCUDAHost = 3 } SpDLDeviceType;
 typedef struct { int32_t device_type; int32_t device_id; } DLDevice;
-typedef enum { kDLInt = 0U, kDLUInt = 1U, kDLFloat = 2U } SpDLDataTypeCode;
+typedef enum { kDLInt = 0U, kDLUInt = 1U, kDLFloat = 2U, kDLBfloat = 4U } SpDLDataTypeCode;
 typedef struct { uint8_t code; uint8_t bits; uint16_t lanes; } DLDataType;
 typedef struct {
   void* data;
@@ -317,6 +317,78 @@ SPARSETIR_API int sparsetir_rgms_ell3d_f16(SPARSETIR_PACKED_ARGS);
  * (examples/rgms/sparse_conv/sparse_conv.py:93-125), which takes every other shape. */
 SPARSETIR_API int sparsetir_sparse_conv_f16(SPARSETIR_PACKED_ARGS);
 
+/* ---- mixture of experts: RGMS whose structure is made on the GPU in every call ------------------
+ * (no counterpart in the reference.)  Tokens t = 0 .. T-1 choose top_k of num_experts experts each; pair
+ * p = t*top_k + j is the j-th choice of token t.  Expert order puts the pairs side by side by expert, those of
+ * one expert in the order of the tokens: indptr i32[num_experts+1] bounds the experts' rows like the row pointers
+ * of a CSR matrix, slots i32[T*top_k] is the row of every pair, or -1 for a pair without an expert.
+ * Element types: f32, f16, bf16 (DLPack code kDLBfloat); sums are formed in f32 whatever the type.  top_k <= 32,
+ * num_experts <= 1024.  Results do not depend on the order in which blocks run. */
+#define SPARSETIR_MOE_RENORMALIZE 1 /* gates of a token are divided by their sum */
+#define SPARSETIR_MOE_MAX_TOP_K 32
+#define SPARSETIR_MOE_MAX_EXPERTS 1024
+
+/* Router: for every token the top_k experts with the largest logits, largest first, of equal ones the lower
+ * index; gates = softmax over all logits of the token (with RENORMALIZE over the chosen ones), and the pairs'
+ * places in expert order.  A logit that is -inf or NaN masks its expert: never chosen, no part of the sum.  A token
+ * with fewer than top_k experts left has -1 for the missing ones in experts and slots, and gate 0.
+ * args: (logits f32|f16|bf16 [T*num_experts], gates f32[T*top_k], experts i32[T*top_k], slots i32[T*top_k],
+ *        indptr i32[num_experts+1], num_experts, top_k [, flags]). */
+SPARSETIR_API int sparsetir_moe_route(SPARSETIR_PACKED_ARGS);
+
+/* Gradient of the gates with respect to the logits; the probabilities are formed again from the logits.
+ *   d_logits[i] = [i chosen as j] d_gates[j] gates[j] - p[i] sum_j d_gates[j] gates[j]
+ * with RENORMALIZE  gates[j] (d_gates[j] - sum d_gates gates) at the chosen experts and 0 elsewhere.
+ * args: (logits [T*num_experts], gates f32[T*top_k], experts i32[T*top_k], d_gates f32[T*top_k],
+ *        d_logits (type of logits) [T*num_experts], num_experts, top_k [, flags]); gates and experts as
+ * sparsetir_moe_route wrote them. */
+SPARSETIR_API int sparsetir_moe_route_grad(SPARSETIR_PACKED_ARGS);
+
+/* Rows of the tokens to expert order: z[slots[t*top_k+j], :] = x[t, :].  Rows of z that no pair names are not
+ * written.  Its gradient is sparsetir_moe_combine without gates.
+ * args: (x [T*feat], slots i32[T*top_k], z (type of x) [S*feat], feat, top_k). */
+SPARSETIR_API int sparsetir_moe_dispatch(SPARSETIR_PACKED_ARGS);
+
+/* The same, quantised to 8 bits with a scale for each row:
+ *   a = max |x[t,:]|,  scale = a / 127,  q = round(x * (127 / a)), ties to even.
+ * A row whose a is below 2^-119 becomes zeros with scale 0; one that holds an infinity or a NaN zeros with
+ * that as its scale.  slots may be null with top_k 1: row t goes to row t.
+ * args: (x [T*feat], slots i32[T*top_k] or null, q i8[S*feat], scale f32[S], feat, top_k). */
+SPARSETIR_API int sparsetir_moe_dispatch_i8(SPARSETIR_PACKED_ARGS);
+
+/* Rows in expert order back to the tokens: y[t, :] = sum_j gates[t*top_k+j] * z[slots[t*top_k+j], :], the sum in
+ * ascending j; gates null: all 1.  Pairs without a slot add nothing.
+ * args: (z [S*feat], slots i32[T*top_k], gates f32[T*top_k] or null, y (type of z, or f32) [T*feat], feat, top_k). */
+SPARSETIR_API int sparsetir_moe_combine(SPARSETIR_PACKED_ARGS);
+
+/* Gradient of sparsetir_moe_combine: dz[slots[p], :] = gates[p] * dy[t, :] and d_gates[p] = <dy[t, :], z[slots[p], :]>,
+ * 0 for a pair without a slot.  Rows of dz that no pair names are not written.
+ * args: (dy [T*feat], z [S*feat], slots i32[T*top_k], gates f32[T*top_k], dz (type of z) [S*feat],
+ *        d_gates f32[T*top_k], feat, top_k); dy and z of one type. */
+SPARSETIR_API int sparsetir_moe_combine_grad(SPARSETIR_PACKED_ARGS);
+
+/* Products grouped by expert, ragged sizes: y[s, :] = x[s, :] * W[g] for the rows s in [indptr[g], indptr[g+1]).
+ * W is [num_groups, feat_in, feat_out], or with SPARSETIR_GROUPED_W_OUT_IN [num_groups, feat_out, feat_in]; the
+ * gradient with respect to x is the same call on dy with the flag the other way round and the sizes exchanged.
+ * Rows of no group are not written.  indptr may be null with num_groups 1: all rows.
+ * args: (x f16|bf16 [S*feat_in], w (type of x), y (type of x, or f32) [S*feat_out], indptr i32[num_groups+1] or null,
+ *        num_groups, feat_in, feat_out [, flags]). */
+#define SPARSETIR_GROUPED_W_OUT_IN 1
+SPARSETIR_API int sparsetir_grouped_mm(SPARSETIR_PACKED_ARGS);
+
+/* Gradient of sparsetir_grouped_mm with respect to W, in W's layout:
+ *   dw[g, fi, fo] = sum over the rows s of group g of x[s, fi] * dy[s, fo];  zeros for a group without rows.
+ * args: (x f16|bf16 [S*feat_in], dy (type of x) [S*feat_out], dw (type of x, or f32) [num_groups*feat_in*feat_out],
+ *        indptr i32[num_groups+1] or null, num_groups, feat_in, feat_out [, flags]). */
+SPARSETIR_API int sparsetir_grouped_mm_grad_w(SPARSETIR_PACKED_ARGS);
+
+/* The product in 8-bit integers with a scale for each row of x and each output feature of each group, sums exact in
+ * 32-bit integers:  y[s, fo] = x_scale[s] * w_scale[g, fo] * sum_fi x[s, fi] * w[g, fo, fi].
+ * args: (x i8[S*feat_in], x_scale f32[S], w i8[num_groups*feat_out*feat_in], w_scale f32[num_groups*feat_out],
+ *        y f16|bf16|f32 [S*feat_out], indptr i32[num_groups+1] or null, num_groups, feat_in, feat_out);
+ * feat_in < 131072. */
+SPARSETIR_API int sparsetir_grouped_mm_i8(SPARSETIR_PACKED_ARGS);
+
 /* ---- operators, plain-pointer form (device pointers; stream is a cudaStream_t) -------- */
 SPARSETIR_API int sparsetir_csrmm_raw(const float* a, const float* b, float* c,
                                       const int32_t* indptr, const int32_t* indices, int m, int n,
@@ -450,6 +522,41 @@ SPARSETIR_API int sparsetir_rgms_noalloc(const float* a, const float* w, const f
                                          const int32_t* indptr_j, const int32_t* indices_j, int m,
                                          int n, int num_rels, int feat, int nnz_i, int nnz_j,
                                          int device_id, void* stream);
+
+/* Mixture of experts (see above).  Element types of the operands: */
+#define SPARSETIR_F32 0
+#define SPARSETIR_F16 1
+#define SPARSETIR_BF16 2
+SPARSETIR_API int sparsetir_moe_route_raw(const void* logits, int logits_type, float* gates, int32_t* experts,
+                                          int32_t* slots, int32_t* indptr, int tokens, int num_experts, int top_k,
+                                          int flags, int device_id, void* stream);
+SPARSETIR_API int sparsetir_moe_route_grad_raw(const void* logits, int logits_type, const float* gates,
+                                               const int32_t* experts, const float* d_gates, void* d_logits,
+                                               int tokens, int num_experts, int top_k, int flags, int device_id,
+                                               void* stream);
+/* rows: how many z, q, dz have; a slot outside of [0, rows) is taken as -1 */
+SPARSETIR_API int sparsetir_moe_dispatch_raw(const void* x, const int32_t* slots, void* z, int type, int tokens,
+                                             int rows, int feat, int top_k, int device_id, void* stream);
+SPARSETIR_API int sparsetir_moe_dispatch_i8_raw(const void* x, int type, const int32_t* slots, int8_t* q, float* scale,
+                                                int tokens, int rows, int feat, int top_k, int device_id,
+                                                void* stream);
+SPARSETIR_API int sparsetir_moe_combine_raw(const void* z, int z_type, const int32_t* slots, const float* gates,
+                                            void* y, int y_type, int tokens, int rows, int feat, int top_k,
+                                            int device_id, void* stream);
+SPARSETIR_API int sparsetir_moe_combine_grad_raw(const void* dy, const void* z, int type, const int32_t* slots,
+                                                 const float* gates, void* dz, float* d_gates, int tokens, int rows,
+                                                 int feat, int top_k, int device_id, void* stream);
+/* rows: how many x and y have; row pointers outside of [0, rows] are taken as the nearer bound */
+SPARSETIR_API int sparsetir_grouped_mm_raw(const void* x, const void* w, int type, void* y, int y_type,
+                                           const int32_t* indptr, int rows, int num_groups, int feat_in, int feat_out,
+                                           int flags, int device_id, void* stream);
+SPARSETIR_API int sparsetir_grouped_mm_grad_w_raw(const void* x, const void* dy, int type, void* dw, int dw_type,
+                                                  const int32_t* indptr, int rows, int num_groups, int feat_in,
+                                                  int feat_out, int flags, int device_id, void* stream);
+SPARSETIR_API int sparsetir_grouped_mm_i8_raw(const int8_t* x, const float* x_scale, const int8_t* w,
+                                              const float* w_scale, void* y, int y_type, const int32_t* indptr,
+                                              int rows, int num_groups, int feat_in, int feat_out, int device_id,
+                                              void* stream);
 
 /* ---- host-side format conversion (CPU int32 arrays) ----------------------------------- */
 

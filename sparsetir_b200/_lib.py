@@ -57,12 +57,15 @@ class EllBucket(ctypes.Structure):
 
 
 kDLCPU, kDLCUDA, kDLCUDAHost = 1, 2, 3
-kDLInt, kDLUInt, kDLFloat = 0, 1, 2
+kDLInt, kDLUInt, kDLFloat, kDLBfloat = 0, 1, 2, 4
 kTVMArgInt, kTVMArgFloat, kTVMOpaqueHandle, kTVMNullptr = 0, 2, 3, 4
 kTVMDLTensorHandle, kTVMNDArrayHandle = 7, 13
 
 HYB_ZERO_C, HYB_REARM, HYB_ALL_ATOMIC = 1, 2, 4
 HYB_MAX_BUCKETS = 64
+MOE_RENORMALIZE = 1
+MOE_MAX_TOP_K, MOE_MAX_EXPERTS = 32, 1024
+GROUPED_W_OUT_IN = 1
 
 PACKED_SYMBOLS = (
     "sparsetir_csrmm",
@@ -82,6 +85,15 @@ PACKED_SYMBOLS = (
     "sparsetir_csr2bsr",
     "sparsetir_ellmm",
     "sparsetir_fusedmm",
+    "sparsetir_moe_route",
+    "sparsetir_moe_route_grad",
+    "sparsetir_moe_dispatch",
+    "sparsetir_moe_dispatch_i8",
+    "sparsetir_moe_combine",
+    "sparsetir_moe_combine_grad",
+    "sparsetir_grouped_mm",
+    "sparsetir_grouped_mm_grad_w",
+    "sparsetir_grouped_mm_i8",
 )
 
 # every other exported symbol: name -> (restype, argtypes)
@@ -127,6 +139,15 @@ PLAIN_SYMBOLS = {
     "sparsetir_rgms_ell3d_f16_raw": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "sparsetir_sparse_conv_f16_raw": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "sparsetir_rgms_noalloc": (_i, [_vp] * 8 + [_i] * 7 + [_vp]),
+    "sparsetir_moe_route_raw": (_i, [_vp, _i] + [_vp] * 4 + [_i] * 5 + [_vp]),
+    "sparsetir_moe_route_grad_raw": (_i, [_vp, _i] + [_vp] * 4 + [_i] * 5 + [_vp]),
+    "sparsetir_moe_dispatch_raw": (_i, [_vp] * 3 + [_i] * 6 + [_vp]),
+    "sparsetir_moe_dispatch_i8_raw": (_i, [_vp, _i] + [_vp] * 3 + [_i] * 5 + [_vp]),
+    "sparsetir_moe_combine_raw": (_i, [_vp, _i, _vp, _vp, _vp] + [_i] * 6 + [_vp]),
+    "sparsetir_moe_combine_grad_raw": (_i, [_vp, _vp, _i] + [_vp] * 4 + [_i] * 5 + [_vp]),
+    "sparsetir_grouped_mm_raw": (_i, [_vp, _vp, _i, _vp, _i, _vp] + [_i] * 6 + [_vp]),
+    "sparsetir_grouped_mm_grad_w_raw": (_i, [_vp, _vp, _i, _vp, _i, _vp] + [_i] * 6 + [_vp]),
+    "sparsetir_grouped_mm_i8_raw": (_i, [_vp] * 5 + [_i, _vp] + [_i] * 5 + [_vp]),
     "sparsetir_column_part_hyb": (_vp, [_i, _i, _i32p, _i32p, _i, _i32p, _i, _i]),
     "sparsetir_hyb_num_rows": (_i64, [_vp, _i, _i]),
     "sparsetir_hyb_copy_bucket": (_i, [_vp, _i, _i, _i32p, _i32p, _i32p, _i32p, _f32p, _f32p]),

@@ -57,6 +57,27 @@ struct Packed {
     return 0;
   }
 
+  // The same for operators that take several element types: SPARSETIR_F32 / F16 / BF16 of argument i, which is
+  // to be one of the types in `allowed` (a bit mask).
+  int floating(int i, const char* name, unsigned allowed, int* type, void** data, int64_t* len) {
+    *type = SPARSETIR_F32;
+    if (is_tensor(i) && v[i].v_handle != nullptr) {
+      const DLDataType dt = static_cast<const DLTensor*>(v[i].v_handle)->dtype;
+      const int found = dt.lanes != 1 ? -1 : dt.code == kDLFloat && dt.bits == 32 ? SPARSETIR_F32
+                        : dt.code == kDLFloat && dt.bits == 16 ? SPARSETIR_F16
+                        : dt.code == kDLBfloat && dt.bits == 16 ? SPARSETIR_BF16 : -1;
+      if (found < 0 || (allowed & (1u << found)) == 0)
+        return fail("%s: %s.dtype is expected to be%s%s%s, got code=%d bits=%d lanes=%d", fn, name,
+                    allowed & (1u << SPARSETIR_F32) ? " float32" : "", allowed & (1u << SPARSETIR_F16) ? " float16" : "",
+                    allowed & (1u << SPARSETIR_BF16) ? " bfloat16" : "", dt.code, dt.bits, dt.lanes);
+      *type = found;
+    }
+    return tensor(i, name, *type == SPARSETIR_BF16 ? kDLBfloat : kDLFloat, *type == SPARSETIR_F32 ? 32 : 16, data, len);
+  }
+
+  // A tensor, or a null handle where the operator can do without: *data stays null.
+  bool absent(int i) const { return i < n && tc[i] == kTVMNullptr; }
+
   int integer(int i, const char* name, int64_t* out) {
     if (i >= n) return fail("%s: missing argument %d (%s)", fn, i, name);
     if (tc[i] != kTVMArgInt)
@@ -743,6 +764,290 @@ int sparsetir_fusedmm(SPARSETIR_PACKED_ARGS) {
                                static_cast<const int32_t*>(indptr), static_cast<const int32_t*>(indices),
                                (int)m, (int)n, (int)nnz, (int)feat, p.device_id,
                                sptir::stream_for(p.device_id));
+}
+
+
+// ---- mixture of experts
+static constexpr unsigned kAnyFloat = 1u << SPARSETIR_F32 | 1u << SPARSETIR_F16 | 1u << SPARSETIR_BF16;
+static constexpr unsigned kHalves = 1u << SPARSETIR_F16 | 1u << SPARSETIR_BF16;
+
+// Rows of a buffer of `len` elements, `feat` to a row.
+static int whole_rows(const char* fn, const char* name, int64_t len, int64_t feat, int64_t* rows) {
+  if (feat <= 0) return fail("%s: the number of features must be positive", fn);
+  if (len % feat != 0)
+    return fail("%s: len(%s) = %lld is not a multiple of %lld features", fn, name, (long long)len, (long long)feat);
+  *rows = len / feat;
+  return fits_i32(fn, "the number of rows", *rows);
+}
+
+static int check_top_k(const char* fn, int64_t top_k) {
+  if (top_k < 1 || top_k > SPARSETIR_MOE_MAX_TOP_K)
+    return fail("%s: top_k = %lld is not in [1, %d]", fn, (long long)top_k, SPARSETIR_MOE_MAX_TOP_K);
+  return 0;
+}
+
+// num_experts, top_k and flags behind the tensors of the router and its gradient
+static int route_scalars(Packed& p, int at, int64_t len, int64_t* tokens, int64_t* experts, int64_t* top_k, int64_t* flags) {
+  TRY(p.integer(at, "num_experts", experts));
+  TRY(p.integer(at + 1, "top_k", top_k));
+  if (p.n == at + 3) TRY(p.integer(at + 2, "flags", flags));
+  if (*experts < 1 || *experts > SPARSETIR_MOE_MAX_EXPERTS)
+    return fail("%s: num_experts = %lld is not in [1, %d]", p.fn, (long long)*experts, SPARSETIR_MOE_MAX_EXPERTS);
+  TRY(check_top_k(p.fn, *top_k));
+  if (*top_k > *experts)
+    return fail("%s: top_k = %lld exceeds num_experts = %lld", p.fn, (long long)*top_k, (long long)*experts);
+  if (*flags & ~int64_t{SPARSETIR_MOE_RENORMALIZE}) return fail("%s: unknown flags %lld", p.fn, (long long)*flags);
+  TRY(whole_rows(p.fn, "logits", len, *experts, tokens));
+  return fits_i32(p.fn, "the number of pairs", *tokens * *top_k);
+}
+
+int sparsetir_moe_route(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_moe_route", args, type_codes, num_args};
+  if (num_args != 7 && num_args != 8) return fail("sparsetir_moe_route: num_args should be 7 or 8, got %d", num_args);
+  void *logits = nullptr, *gates = nullptr, *experts = nullptr, *slots = nullptr, *indptr = nullptr;
+  int64_t ll = 0, lg = 0, le = 0, ls = 0, lp = 0, tokens = 0, num = 0, k = 0, flags = 0;
+  int type = 0;
+  TRY(p.floating(0, "logits", kAnyFloat, &type, &logits, &ll));
+  TRY(p.tensor(1, "gates", kDLFloat, 32, &gates, &lg));
+  TRY(p.tensor(2, "experts", kDLInt, 32, &experts, &le));
+  TRY(p.tensor(3, "slots", kDLInt, 32, &slots, &ls));
+  TRY(p.tensor(4, "indptr", kDLInt, 32, &indptr, &lp));
+  TRY(route_scalars(p, 5, ll, &tokens, &num, &k, &flags));
+  TRY(check_len(p.fn, "gates", lg, tokens * k));
+  TRY(check_len(p.fn, "experts", le, tokens * k));
+  TRY(check_len(p.fn, "slots", ls, tokens * k));
+  TRY(check_len(p.fn, "indptr", lp, num + 1));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_moe_route_raw(logits, type, static_cast<float*>(gates), static_cast<int32_t*>(experts),
+                                 static_cast<int32_t*>(slots), static_cast<int32_t*>(indptr), (int)tokens, (int)num, (int)k,
+                                 (int)flags, p.device_id, sptir::stream_for(p.device_id));
+}
+
+int sparsetir_moe_route_grad(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_moe_route_grad", args, type_codes, num_args};
+  if (num_args != 7 && num_args != 8)
+    return fail("sparsetir_moe_route_grad: num_args should be 7 or 8, got %d", num_args);
+  void *logits = nullptr, *gates = nullptr, *experts = nullptr, *dg = nullptr, *dl = nullptr;
+  int64_t ll = 0, lg = 0, le = 0, ldg = 0, ldl = 0, tokens = 0, num = 0, k = 0, flags = 0;
+  int type = 0, dtype = 0;
+  TRY(p.floating(0, "logits", kAnyFloat, &type, &logits, &ll));
+  TRY(p.tensor(1, "gates", kDLFloat, 32, &gates, &lg));
+  TRY(p.tensor(2, "experts", kDLInt, 32, &experts, &le));
+  TRY(p.tensor(3, "d_gates", kDLFloat, 32, &dg, &ldg));
+  TRY(p.floating(4, "d_logits", 1u << type, &dtype, &dl, &ldl));
+  TRY(route_scalars(p, 5, ll, &tokens, &num, &k, &flags));
+  TRY(check_len(p.fn, "gates", lg, tokens * k));
+  TRY(check_len(p.fn, "experts", le, tokens * k));
+  TRY(check_len(p.fn, "d_gates", ldg, tokens * k));
+  TRY(check_len(p.fn, "d_logits", ldl, tokens * num));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_moe_route_grad_raw(logits, type, static_cast<const float*>(gates), static_cast<const int32_t*>(experts),
+                                      static_cast<const float*>(dg), dl, (int)tokens, (int)num, (int)k, (int)flags,
+                                      p.device_id, sptir::stream_for(p.device_id));
+}
+
+int sparsetir_moe_dispatch(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_moe_dispatch", args, type_codes, num_args};
+  if (num_args != 5) return fail("sparsetir_moe_dispatch: num_args should be 5, got %d", num_args);
+  void *x = nullptr, *slots = nullptr, *z = nullptr;
+  int64_t lx = 0, ls = 0, lz = 0, feat = 0, k = 0, tokens = 0, rows = 0;
+  int type = 0, ztype = 0;
+  TRY(p.floating(0, "x", kAnyFloat, &type, &x, &lx));
+  TRY(p.tensor(1, "slots", kDLInt, 32, &slots, &ls));
+  TRY(p.floating(2, "z", 1u << type, &ztype, &z, &lz));
+  TRY(p.integer(3, "feat_size", &feat));
+  TRY(p.integer(4, "top_k", &k));
+  TRY(check_top_k(p.fn, k));
+  TRY(whole_rows(p.fn, "x", lx, feat, &tokens));
+  TRY(whole_rows(p.fn, "z", lz, feat, &rows));
+  TRY(fits_i32(p.fn, "feat_size", feat)); TRY(fits_i32(p.fn, "the number of pairs", tokens * k));
+  TRY(check_len(p.fn, "slots", ls, tokens * k));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_moe_dispatch_raw(x, static_cast<const int32_t*>(slots), z, type, (int)tokens, (int)rows, (int)feat, (int)k,
+                                    p.device_id, sptir::stream_for(p.device_id));
+}
+
+int sparsetir_moe_dispatch_i8(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_moe_dispatch_i8", args, type_codes, num_args};
+  if (num_args != 6) return fail("sparsetir_moe_dispatch_i8: num_args should be 6, got %d", num_args);
+  void *x = nullptr, *slots = nullptr, *q = nullptr, *scale = nullptr;
+  int64_t lx = 0, ls = 0, lq = 0, lc = 0, feat = 0, k = 0, tokens = 0, rows = 0;
+  int type = 0;
+  TRY(p.floating(0, "x", kAnyFloat, &type, &x, &lx));
+  if (!p.absent(1)) TRY(p.tensor(1, "slots", kDLInt, 32, &slots, &ls));
+  TRY(p.tensor(2, "q", kDLInt, 8, &q, &lq));
+  TRY(p.tensor(3, "scale", kDLFloat, 32, &scale, &lc));
+  TRY(p.integer(4, "feat_size", &feat));
+  TRY(p.integer(5, "top_k", &k));
+  TRY(check_top_k(p.fn, k));
+  TRY(whole_rows(p.fn, "x", lx, feat, &tokens));
+  TRY(whole_rows(p.fn, "q", lq, feat, &rows));
+  TRY(fits_i32(p.fn, "feat_size", feat)); TRY(fits_i32(p.fn, "the number of pairs", tokens * k));
+  TRY(check_len(p.fn, "scale", lc, rows));
+  if (p.absent(1)) {
+    if (k != 1) return fail("sparsetir_moe_dispatch_i8: slots may be null with top_k 1 only, got %lld", (long long)k);
+    TRY(check_len(p.fn, "q", lq, lx));
+  } else {
+    TRY(check_len(p.fn, "slots", ls, tokens * k));
+  }
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_moe_dispatch_i8_raw(x, type, static_cast<const int32_t*>(slots), static_cast<int8_t*>(q),
+                                       static_cast<float*>(scale), (int)tokens, (int)rows, (int)feat, (int)k, p.device_id,
+                                       sptir::stream_for(p.device_id));
+}
+
+int sparsetir_moe_combine(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_moe_combine", args, type_codes, num_args};
+  if (num_args != 6) return fail("sparsetir_moe_combine: num_args should be 6, got %d", num_args);
+  void *z = nullptr, *slots = nullptr, *gates = nullptr, *y = nullptr;
+  int64_t lz = 0, ls = 0, lg = 0, ly = 0, feat = 0, k = 0, tokens = 0, rows = 0;
+  int type = 0, ytype = 0;
+  TRY(p.floating(0, "z", kAnyFloat, &type, &z, &lz));
+  TRY(p.tensor(1, "slots", kDLInt, 32, &slots, &ls));
+  if (!p.absent(2)) TRY(p.tensor(2, "gates", kDLFloat, 32, &gates, &lg));
+  TRY(p.floating(3, "y", 1u << type | 1u << SPARSETIR_F32, &ytype, &y, &ly));
+  TRY(p.integer(4, "feat_size", &feat));
+  TRY(p.integer(5, "top_k", &k));
+  TRY(check_top_k(p.fn, k));
+  TRY(whole_rows(p.fn, "y", ly, feat, &tokens));
+  TRY(whole_rows(p.fn, "z", lz, feat, &rows));
+  TRY(fits_i32(p.fn, "feat_size", feat)); TRY(fits_i32(p.fn, "the number of pairs", tokens * k));
+  TRY(check_len(p.fn, "slots", ls, tokens * k));
+  if (!p.absent(2)) TRY(check_len(p.fn, "gates", lg, tokens * k));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_moe_combine_raw(z, type, static_cast<const int32_t*>(slots), static_cast<const float*>(gates), y, ytype,
+                                   (int)tokens, (int)rows, (int)feat, (int)k, p.device_id, sptir::stream_for(p.device_id));
+}
+
+int sparsetir_moe_combine_grad(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_moe_combine_grad", args, type_codes, num_args};
+  if (num_args != 8) return fail("sparsetir_moe_combine_grad: num_args should be 8, got %d", num_args);
+  void *dy = nullptr, *z = nullptr, *slots = nullptr, *gates = nullptr, *dz = nullptr, *dg = nullptr;
+  int64_t ldy = 0, lz = 0, ls = 0, lg = 0, ldz = 0, ldg = 0, feat = 0, k = 0, tokens = 0, rows = 0;
+  int type = 0, same = 0;
+  TRY(p.floating(0, "dy", kAnyFloat, &type, &dy, &ldy));
+  TRY(p.floating(1, "z", 1u << type, &same, &z, &lz));
+  TRY(p.tensor(2, "slots", kDLInt, 32, &slots, &ls));
+  TRY(p.tensor(3, "gates", kDLFloat, 32, &gates, &lg));
+  TRY(p.floating(4, "dz", 1u << type, &same, &dz, &ldz));
+  TRY(p.tensor(5, "d_gates", kDLFloat, 32, &dg, &ldg));
+  TRY(p.integer(6, "feat_size", &feat));
+  TRY(p.integer(7, "top_k", &k));
+  TRY(check_top_k(p.fn, k));
+  TRY(whole_rows(p.fn, "dy", ldy, feat, &tokens));
+  TRY(whole_rows(p.fn, "z", lz, feat, &rows));
+  TRY(fits_i32(p.fn, "feat_size", feat)); TRY(fits_i32(p.fn, "the number of pairs", tokens * k));
+  TRY(check_len(p.fn, "slots", ls, tokens * k));
+  TRY(check_len(p.fn, "gates", lg, tokens * k));
+  TRY(check_len(p.fn, "dz", ldz, lz));
+  TRY(check_len(p.fn, "d_gates", ldg, tokens * k));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_moe_combine_grad_raw(dy, z, type, static_cast<const int32_t*>(slots), static_cast<const float*>(gates), dz,
+                                        static_cast<float*>(dg), (int)tokens, (int)rows, (int)feat, (int)k, p.device_id,
+                                        sptir::stream_for(p.device_id));
+}
+
+// indptr, num_groups, feat_in, feat_out and flags of the grouped products, from argument `at` on
+struct Groups {
+  void* indptr = nullptr;
+  int64_t num = 0, feat_in = 0, feat_out = 0, flags = 0;
+};
+static int groups(Packed& p, int at, bool with_flags, Groups* g) {
+  int64_t lp = 0;
+  if (!p.absent(at)) TRY(p.tensor(at, "indptr", kDLInt, 32, &g->indptr, &lp));
+  TRY(p.integer(at + 1, "num_groups", &g->num));
+  TRY(p.integer(at + 2, "feat_in", &g->feat_in));
+  TRY(p.integer(at + 3, "feat_out", &g->feat_out));
+  if (with_flags && p.n == at + 5) TRY(p.integer(at + 4, "flags", &g->flags));
+  TRY(fits_i32(p.fn, "num_groups", g->num));
+  if (g->feat_in < 1 || g->feat_out < 1) return fail("%s: feat_in and feat_out must be positive", p.fn);
+  TRY(fits_i32(p.fn, "feat_in", g->feat_in)); TRY(fits_i32(p.fn, "feat_out", g->feat_out));
+  if (g->flags & ~int64_t{SPARSETIR_GROUPED_W_OUT_IN}) return fail("%s: unknown flags %lld", p.fn, (long long)g->flags);
+  if (p.absent(at)) {
+    if (g->num != 1) return fail("%s: indptr may be null with num_groups 1 only, got %lld", p.fn, (long long)g->num);
+    return 0;
+  }
+  return check_len(p.fn, "indptr", lp, g->num + 1);
+}
+
+// num_groups matrices of feat_in x feat_out
+static int check_weights(const char* fn, const char* name, int64_t len, const Groups& g) {
+  const int64_t each = g.feat_in * g.feat_out;  // both below 2^31
+  if (g.num > 0 && each > INT64_MAX / g.num) return fail("%s: %s is too large", fn, name);
+  return check_len(fn, name, len, g.num * each);
+}
+
+int sparsetir_grouped_mm(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_grouped_mm", args, type_codes, num_args};
+  if (num_args != 7 && num_args != 8) return fail("sparsetir_grouped_mm: num_args should be 7 or 8, got %d", num_args);
+  void *x = nullptr, *w = nullptr, *y = nullptr;
+  int64_t lx = 0, lw = 0, ly = 0, rows = 0;
+  int type = 0, same = 0, ytype = 0;
+  Groups g;
+  TRY(p.floating(0, "x", kHalves, &type, &x, &lx));
+  TRY(p.floating(1, "w", 1u << type, &same, &w, &lw));
+  TRY(p.floating(2, "y", 1u << type | 1u << SPARSETIR_F32, &ytype, &y, &ly));
+  TRY(groups(p, 3, true, &g));
+  TRY(whole_rows(p.fn, "x", lx, g.feat_in, &rows));
+  TRY(check_weights(p.fn, "w", lw, g));
+  TRY(check_len(p.fn, "y", ly, rows * g.feat_out));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_grouped_mm_raw(x, w, type, y, ytype, static_cast<const int32_t*>(g.indptr), (int)rows, (int)g.num,
+                                  (int)g.feat_in, (int)g.feat_out, (int)g.flags, p.device_id, sptir::stream_for(p.device_id));
+}
+
+int sparsetir_grouped_mm_grad_w(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_grouped_mm_grad_w", args, type_codes, num_args};
+  if (num_args != 7 && num_args != 8)
+    return fail("sparsetir_grouped_mm_grad_w: num_args should be 7 or 8, got %d", num_args);
+  void *x = nullptr, *dy = nullptr, *dw = nullptr;
+  int64_t lx = 0, ldy = 0, lw = 0, rows = 0;
+  int type = 0, same = 0, wtype = 0;
+  Groups g;
+  TRY(p.floating(0, "x", kHalves, &type, &x, &lx));
+  TRY(p.floating(1, "dy", 1u << type, &same, &dy, &ldy));
+  TRY(p.floating(2, "dw", 1u << type | 1u << SPARSETIR_F32, &wtype, &dw, &lw));
+  TRY(groups(p, 3, true, &g));
+  TRY(whole_rows(p.fn, "x", lx, g.feat_in, &rows));
+  TRY(check_weights(p.fn, "dw", lw, g));
+  TRY(check_len(p.fn, "dy", ldy, rows * g.feat_out));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_grouped_mm_grad_w_raw(x, dy, type, dw, wtype, static_cast<const int32_t*>(g.indptr), (int)rows, (int)g.num,
+                                         (int)g.feat_in, (int)g.feat_out, (int)g.flags, p.device_id,
+                                         sptir::stream_for(p.device_id));
+}
+
+int sparsetir_grouped_mm_i8(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_grouped_mm_i8", args, type_codes, num_args};
+  if (num_args != 9) return fail("sparsetir_grouped_mm_i8: num_args should be 9, got %d", num_args);
+  void *x = nullptr, *xs = nullptr, *w = nullptr, *ws = nullptr, *y = nullptr;
+  int64_t lx = 0, lxs = 0, lw = 0, lws = 0, ly = 0, rows = 0;
+  int ytype = 0;
+  Groups g;
+  TRY(p.tensor(0, "x", kDLInt, 8, &x, &lx));
+  TRY(p.tensor(1, "x_scale", kDLFloat, 32, &xs, &lxs));
+  TRY(p.tensor(2, "w", kDLInt, 8, &w, &lw));
+  TRY(p.tensor(3, "w_scale", kDLFloat, 32, &ws, &lws));
+  TRY(p.floating(4, "y", kAnyFloat, &ytype, &y, &ly));
+  TRY(groups(p, 5, false, &g));
+  TRY(whole_rows(p.fn, "x", lx, g.feat_in, &rows));
+  TRY(check_len(p.fn, "x_scale", lxs, rows));
+  TRY(check_weights(p.fn, "w", lw, g));
+  TRY(check_len(p.fn, "w_scale", lws, g.num * g.feat_out));
+  TRY(check_len(p.fn, "y", ly, rows * g.feat_out));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_grouped_mm_i8_raw(static_cast<const int8_t*>(x), static_cast<const float*>(xs), static_cast<const int8_t*>(w),
+                                     static_cast<const float*>(ws), y, ytype, static_cast<const int32_t*>(g.indptr), (int)rows,
+                                     (int)g.num, (int)g.feat_in, (int)g.feat_out, p.device_id, sptir::stream_for(p.device_id));
 }
 
 }  // extern "C"

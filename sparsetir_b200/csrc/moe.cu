@@ -1,0 +1,618 @@
+// Router of a mixture of experts, and the exchange of rows between the order of the tokens and that of the experts.
+// The products between the two are in grouped.cu.
+#include <algorithm>
+#include <cmath>
+
+#include "common.h"
+#include "launch.cuh"
+#include "lowp.cuh"
+
+namespace sptir {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr unsigned kFull = 0xffffffffu;
+
+// ---- router ---------------------------------------------------------------------------------------------------------
+
+// Floats in an order of unsigned integers: larger float, larger key.  0 for what masks an expert (-inf, NaN); both
+// zeros have one key, so that the lower index wins between them as between other equal logits.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (!(v > -INFINITY)) return 0u;
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b ^ ((b >> 31) != 0u ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k ^ ((k >> 31) != 0u ? 0x80000000u : 0xffffffffu));
+}
+// exp(v - top) for the logits of a token; those of the largest are 1 even if it is +inf
+__device__ __forceinline__ float over_top(uint32_t key, uint32_t top) {
+  if (key == 0u) return 0.f;
+  return key == top ? 1.f : expf(key_value(key) - key_value(top));
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+
+// A token's logits, R to a lane: lane l has those of the experts l, l + 32, ...
+template <class T, int R>
+__device__ __forceinline__ void load_keys(const T* row, int num_experts, int lane, uint32_t (&key)[R]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = lane + 32 * r;
+    key[r] = 0u;
+    if (i < num_experts) key[r] = order_key(to_float(ld_global(row + i)));
+  }
+}
+
+// One warp per token.  p[i] = exp(z[i] - max z) / sum; the top_k largest are found one after the other, each by a
+// maximum over the keys of the warp and the lowest index that has it.
+template <class T, int R>
+__global__ void __launch_bounds__(kWarps * 32)
+choose_kernel(const T* logits, float* gates, int32_t* experts, int tokens, int num_experts, int top_k, int renormalize) {
+  chain_wait();
+  const int lane = threadIdx.x & 31;
+  const int t = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  uint32_t key[R];
+  load_keys<T, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, lane, key);
+  uint32_t most = 0u;
+#pragma unroll
+  for (int r = 0; r < R; ++r) most = max(most, key[r]);
+  const uint32_t top = __reduce_max_sync(kFull, most);
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) sum += over_top(key[r], top);
+  sum = warp_sum(sum);
+  int expert = -1;     // of choice `lane`
+  float value = 0.f;   // exp(z - top) of it
+  for (int j = 0; j < top_k; ++j) {
+    uint32_t best = 0u;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (key[r] > best) { best = key[r]; at = lane + 32 * r; }
+    const uint32_t found = __reduce_max_sync(kFull, best);
+    if (found == 0u) break;
+    const int who = __reduce_min_sync(kFull, best == found ? at : 0x7fffffff);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (lane + 32 * r == who) key[r] = 0u;
+    if (lane == j) {
+      expert = who;
+      value = over_top(found, top);
+    }
+  }
+  if (renormalize) sum = warp_sum(value);
+  if (lane < top_k) {
+    const size_t p = static_cast<size_t>(t) * top_k + lane;
+    experts[p] = expert;
+    gates[p] = expert < 0 ? 0.f : value / sum;
+  }
+}
+
+// Stable counting sort of the pairs by expert, in one block.
+__global__ void __launch_bounds__(1024)
+place_kernel(const int32_t* experts, int32_t* slots, int32_t* indptr, int pairs, int num_experts) {
+  __shared__ int next[SPARSETIR_MOE_MAX_EXPERTS];
+  chain_wait();
+  const int tid = threadIdx.x, lane = tid & 31;
+  next[tid] = 0;
+  __syncthreads();
+  for (int p = tid; p < pairs; p += 1024) {
+    const int e = ld_global(experts + p);
+    if (e >= 0) atomicAdd(&next[e], 1);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int sum = 0;
+    for (int e = 0; e < num_experts; ++e) {
+      indptr[e] = sum;
+      const int n = next[e];
+      next[e] = sum;
+      sum += n;
+    }
+    indptr[num_experts] = sum;
+  }
+  __syncthreads();
+  if (tid >= 32) return;
+  for (int p0 = 0; p0 < pairs; p0 += 32) {
+    const int p = p0 + lane;
+    const int e = p < pairs ? ld_global(experts + p) : -1;
+    const unsigned same = __match_any_sync(kFull, e);
+    const int before = __popc(same & ((1u << lane) - 1u));
+    int slot = -1;
+    if (e >= 0) slot = next[e] + before;
+    __syncwarp();
+    if (e >= 0 && before == 0) next[e] += __popc(same);
+    __syncwarp();
+    if (p < pairs) slots[p] = slot;
+  }
+}
+
+template <class T, int R>
+__global__ void __launch_bounds__(kWarps * 32)
+route_grad_kernel(const T* logits, const float* gates, const int32_t* experts, const float* d_gates, T* d_logits, int tokens,
+                  int num_experts, int top_k, int renormalize) {
+  chain_wait();
+  const int lane = threadIdx.x & 31;
+  const int t = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  uint32_t key[R];
+  load_keys<T, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, lane, key);
+  int expert = -1;
+  float gate = 0.f, dg = 0.f;
+  if (lane < top_k) {
+    const size_t p = static_cast<size_t>(t) * top_k + lane;
+    expert = ld_global(experts + p);
+    if (expert >= 0) {
+      gate = ld_global(gates + p);
+      dg = ld_global(d_gates + p);
+    }
+  }
+  const float mean = warp_sum(gate * dg);
+  float grad[R];
+  if (renormalize) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) grad[r] = 0.f;
+    dg -= mean;
+  } else {
+    uint32_t most = 0u;
+#pragma unroll
+    for (int r = 0; r < R; ++r) most = max(most, key[r]);
+    const uint32_t top = __reduce_max_sync(kFull, most);
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      grad[r] = over_top(key[r], top);
+      sum += grad[r];
+    }
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int r = 0; r < R; ++r) grad[r] = key[r] != 0u ? -mean * (grad[r] / sum) : 0.f;
+  }
+  for (int j = 0; j < top_k; ++j) {
+    const int e = __shfl_sync(kFull, expert, j);
+    const float add = __shfl_sync(kFull, gate * dg, j);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (lane + 32 * r == e) grad[r] += add;
+  }
+  T* out = d_logits + static_cast<size_t>(t) * num_experts;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (lane + 32 * r < num_experts) out[lane + 32 * r] = from_float<T>(grad[r]);
+}
+
+// f(integral constant R) with R * 32 >= num_experts
+template <class F>
+int with_lane_share(int num_experts, F&& f) {
+  if (num_experts <= 32) return f(std::integral_constant<int, 1>{});
+  if (num_experts <= 64) return f(std::integral_constant<int, 2>{});
+  if (num_experts <= 128) return f(std::integral_constant<int, 4>{});
+  if (num_experts <= 256) return f(std::integral_constant<int, 8>{});
+  if (num_experts <= 512) return f(std::integral_constant<int, 16>{});
+  return f(std::integral_constant<int, 32>{});
+}
+
+// ---- rows -----------------------------------------------------------------------------------------------------------
+
+constexpr int kHold = 4;  // pieces of a row that a lane has in flight
+
+// Slot of pair t * top_k + lane, -1 where there is none
+__device__ __forceinline__ int pair_slot(const int32_t* slots, int t, int top_k, int rows, int lane) {
+  int s = -1;
+  if (lane < top_k) s = ld_global(slots + static_cast<size_t>(t) * top_k + lane);
+  return static_cast<unsigned>(s) < static_cast<unsigned>(rows) ? s : -1;
+}
+
+// A warp copies up to kHold * 32 pieces of a token's row to its slots: the row is read once.
+template <int B>
+__global__ void __launch_bounds__(kWarps * 32)
+dispatch_kernel(const Piece<B>* x, const int32_t* slots, Piece<B>* z, int tokens, int rows, int pieces, int chunks, int top_k) {
+  chain_wait();
+  const int lane = threadIdx.x & 31;
+  const long long item = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int t = static_cast<int>(item / chunks), c = static_cast<int>(item - static_cast<long long>(t) * chunks);
+  if (t >= tokens) return;
+  const int slot = pair_slot(slots, t, top_k, rows, lane);
+  const int first = c * (kHold * 32) + lane;
+  Piece<B> v[kHold];
+#pragma unroll
+  for (int i = 0; i < kHold; ++i)
+    if (first + 32 * i < pieces) v[i] = ld_global(x + static_cast<size_t>(t) * pieces + first + 32 * i);
+  for (int j = 0; j < top_k; ++j) {
+    const int s = __shfl_sync(kFull, slot, j);
+    if (s < 0) continue;
+    Piece<B>* to = z + static_cast<size_t>(s) * pieces + first;
+#pragma unroll
+    for (int i = 0; i < kHold; ++i)
+      if (first + 32 * i < pieces) to[32 * i] = v[i];
+  }
+}
+
+// A warp sums up to 64 pieces of a token's rows, four rows requested together.
+template <class T, class OutT, int B>
+__global__ void __launch_bounds__(kWarps * 32)
+combine_kernel(const Piece<B>* z, const int32_t* slots, const float* gates, OutT* y, int tokens, int rows, int pieces,
+               int chunks, int top_k) {
+  constexpr int N = B / sizeof(T), U = 2, J = 4;
+  chain_wait();
+  const int lane = threadIdx.x & 31;
+  const long long item = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int t = static_cast<int>(item / chunks), c = static_cast<int>(item - static_cast<long long>(t) * chunks);
+  if (t >= tokens) return;
+  const int slot = pair_slot(slots, t, top_k, rows, lane);
+  float gate = 1.f;
+  if (gates != nullptr && lane < top_k) gate = ld_global(gates + static_cast<size_t>(t) * top_k + lane);
+  const int first = c * (U * 32) + lane;
+  float acc[U][N];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[u][n] = 0.f;
+  for (int j0 = 0; j0 < top_k; j0 += J) {
+    Piece<B> v[J][U];
+    int s[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      s[j] = j0 + j < top_k ? __shfl_sync(kFull, slot, (j0 + j) & 31) : -1;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (s[j] >= 0 && first + 32 * u < pieces) v[j][u] = ld_global(z + static_cast<size_t>(s[j]) * pieces + first + 32 * u);
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const float w = __shfl_sync(kFull, gate, (j0 + j) & 31);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (s[j] >= 0 && first + 32 * u < pieces) {
+          float f[N];
+          unpack<T, B>(v[j][u], f);
+#pragma unroll
+          for (int n = 0; n < N; ++n) acc[u][n] = fmaf(w, f[n], acc[u][n]);
+        }
+      }
+    }
+  }
+  constexpr int OB = N * static_cast<int>(sizeof(OutT)) > 16 ? 16 : N * static_cast<int>(sizeof(OutT));
+  constexpr int ON = OB / sizeof(OutT);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (first + 32 * u >= pieces) continue;
+    OutT* to = y + (static_cast<size_t>(t) * pieces + first + 32 * u) * N;
+#pragma unroll
+    for (int q = 0; q < N / ON; ++q) {
+      float part[ON];
+#pragma unroll
+      for (int n = 0; n < ON; ++n) part[n] = acc[u][q * ON + n];
+      *reinterpret_cast<Piece<OB>*>(to + q * ON) = pack<OutT, OB>(part);
+    }
+  }
+}
+
+constexpr int kRowThreads = 128;  // a block per token
+constexpr int kRowWarps = kRowThreads / 32;
+
+// Block per token: dy in registers, kHold pieces to a thread at a time, the rows of z one after the other.
+template <class T, int B>
+__global__ void __launch_bounds__(kRowThreads)
+combine_grad_kernel(const Piece<B>* dy, const Piece<B>* z, const int32_t* slots, const float* gates, Piece<B>* dz, float* d_gates,
+                    int rows, int pieces, int top_k) {
+  constexpr int N = B / sizeof(T);
+  __shared__ float part[SPARSETIR_MOE_MAX_TOP_K][kRowWarps];
+  chain_wait();
+  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int slot = pair_slot(slots, t, top_k, rows, lane);
+  float gate = 0.f;
+  if (lane < top_k) {
+    gate = ld_global(gates + static_cast<size_t>(t) * top_k + lane);
+    part[lane][warp] = 0.f;
+  }
+  __syncwarp();
+  for (int base = 0; base < pieces; base += kHold * kRowThreads) {
+    const int first = base + tid;
+    Piece<B> d[kHold];
+#pragma unroll
+    for (int i = 0; i < kHold; ++i)
+      if (first + i * kRowThreads < pieces) d[i] = ld_global(dy + static_cast<size_t>(t) * pieces + first + i * kRowThreads);
+    for (int j = 0; j < top_k; ++j) {
+      const int s = __shfl_sync(kFull, slot, j);
+      const float w = __shfl_sync(kFull, gate, j);
+      if (s < 0) continue;
+      const size_t row = static_cast<size_t>(s) * pieces + first;
+      Piece<B> v[kHold];
+#pragma unroll
+      for (int i = 0; i < kHold; ++i)
+        if (first + i * kRowThreads < pieces) v[i] = ld_global(z + row + i * kRowThreads);
+      float dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < kHold; ++i) {
+        if (first + i * kRowThreads < pieces) {
+          float a[N], b[N], o[N];
+          unpack<T, B>(d[i], a);
+          unpack<T, B>(v[i], b);
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            dot = fmaf(a[n], b[n], dot);
+            o[n] = w * a[n];
+          }
+          dz[row + i * kRowThreads] = pack<T, B>(o);
+        }
+      }
+      dot = warp_sum(dot);
+      if (lane == 0) part[j][warp] += dot;
+    }
+  }
+  __syncthreads();
+  if (tid < top_k) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) sum += part[tid][w];
+    d_gates[static_cast<size_t>(t) * top_k + tid] = slot >= 0 ? sum : 0.f;
+  }
+}
+
+// Block per token: the largest magnitude, as the bits of a float without its sign (so that an infinity or a NaN is
+// larger than all numbers and stays), then the quotients.  Rows of up to kHold pieces to a thread are read once.
+template <class T, int B>
+__global__ void __launch_bounds__(kRowThreads)
+dispatch_i8_kernel(const Piece<B>* x, const int32_t* slots, Piece<B / sizeof(T)>* q, float* scale, int rows, int pieces,
+                   int top_k) {
+  constexpr int N = B / sizeof(T);
+  __shared__ uint32_t most[kRowWarps];
+  chain_wait();
+  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int slot = slots != nullptr ? pair_slot(slots, t, top_k, rows, lane) : (lane == 0 ? t : -1);
+  const Piece<B>* xr = x + static_cast<size_t>(t) * pieces;
+  Piece<B> v[kHold];
+  uint32_t bits = 0u;
+  for (int base = 0; base < pieces; base += kHold * kRowThreads) {
+#pragma unroll
+    for (int i = 0; i < kHold; ++i)
+      if (base + tid + i * kRowThreads < pieces) v[i] = ld_global(xr + base + tid + i * kRowThreads);
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {
+      if (base + tid + i * kRowThreads < pieces) {
+        float f[N];
+        unpack<T, B>(v[i], f);
+#pragma unroll
+        for (int n = 0; n < N; ++n) bits = max(bits, __float_as_uint(f[n]) & 0x7fffffffu);
+      }
+    }
+  }
+  bits = __reduce_max_sync(kFull, bits);
+  if (lane == 0) most[warp] = bits;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kRowWarps; ++w) bits = max(bits, most[w]);
+  const float a = __uint_as_float(bits);
+  const bool zeros = !(a >= 0x1p-119f && a < INFINITY);
+  const float inv = zeros ? 0.f : 127.f / a;
+  if (tid < top_k && slot >= 0) scale[slot] = a < 0x1p-119f ? 0.f : a / 127.f;
+  for (int base = 0; base < pieces; base += kHold * kRowThreads) {
+    if (pieces > kHold * kRowThreads) {  // otherwise they are here still
+#pragma unroll
+      for (int i = 0; i < kHold; ++i)
+        if (base + tid + i * kRowThreads < pieces) v[i] = ld_global(xr + base + tid + i * kRowThreads);
+    }
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {
+      const int at = base + tid + i * kRowThreads;
+      Piece<N> o;
+      if (at < pieces) {
+        float f[N];
+        unpack<T, B>(v[i], f);
+        int8_t* b = reinterpret_cast<int8_t*>(&o);
+#pragma unroll
+        for (int n = 0; n < N; ++n) b[n] = zeros ? 0 : static_cast<int8_t>(__float2int_rn(f[n] * inv));
+      }
+      for (int j = 0; j < top_k; ++j) {
+        const int s = __shfl_sync(kFull, slot, j);
+        if (s >= 0 && at < pieces) q[static_cast<size_t>(s) * pieces + at] = o;
+      }
+    }
+  }
+}
+
+// Widest piece, in bytes, that divides rows of `row_bytes` and fits the pointers.
+int piece_bytes(size_t row_bytes, uintptr_t pointers) {
+  for (int b : {16, 8, 4})
+    if (row_bytes % b == 0 && pointers % b == 0) return b;
+  return 2;
+}
+uintptr_t bits_of(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// f(integral constant B) for pieces of b bytes of elements of `size` bytes
+template <int SIZE, class F>
+int with_piece(int b, F&& f) {
+  if (b == 16) return f(std::integral_constant<int, 16>{});
+  if (b == 8) return f(std::integral_constant<int, 8>{});
+  if (b == 4) return f(std::integral_constant<int, 4>{});
+  if constexpr (SIZE == 2) return f(std::integral_constant<int, 2>{});
+  return fail("misaligned f32 operand");
+}
+
+int check_rows(const char* fn, int type, int tokens, int rows, int feat, int top_k) {
+  if (type < SPARSETIR_F32 || type > SPARSETIR_BF16) return fail("%s: unknown element type %d", fn, type);
+  if (tokens < 0 || rows < 0 || feat < 0) return fail("%s: negative size", fn);
+  if (top_k < 1 || top_k > SPARSETIR_MOE_MAX_TOP_K)
+    return fail("%s: top_k = %d is not in [1, %d]", fn, top_k, SPARSETIR_MOE_MAX_TOP_K);
+  return 0;
+}
+int check_slots(const char* fn, const int32_t* slots, int tokens, int rows, int top_k, cudaStream_t st) {
+  if (!validate_enabled()) return 0;
+  return validate_range(fn, "slots", slots, static_cast<long long>(tokens) * top_k, rows, st, /*lowest=*/-1);
+}
+size_t element(int type) { return type == SPARSETIR_F32 ? 4 : 2; }
+
+int check_route(const char* fn, int type, int tokens, int num_experts, int top_k, int flags) {
+  if (check_rows(fn, type, tokens, 0, 0, top_k) != 0) return -1;
+  if (num_experts < top_k || num_experts > SPARSETIR_MOE_MAX_EXPERTS)
+    return fail("%s: num_experts = %d is not in [top_k, %d]", fn, num_experts, SPARSETIR_MOE_MAX_EXPERTS);
+  if ((flags & ~SPARSETIR_MOE_RENORMALIZE) != 0) return fail("%s: unknown flags %d", fn, flags);
+  if (static_cast<long long>(tokens) * top_k > INT32_MAX) return fail("%s: too many pairs for 32-bit indices", fn);
+  return 0;
+}
+
+}  // namespace
+}  // namespace sptir
+
+using namespace sptir;
+
+extern "C" int sparsetir_moe_route_raw(const void* logits, int logits_type, float* gates, int32_t* experts, int32_t* slots,
+                                       int32_t* indptr, int tokens, int num_experts, int top_k, int flags, int device_id,
+                                       void* stream) {
+  const char* fn = "sparsetir_moe_route";
+  if (check_route(fn, logits_type, tokens, num_experts, top_k, flags) != 0) return -1;
+  if (!indptr || (tokens > 0 && (!logits || !gates || !experts || !slots))) return fail("%s: null pointer argument", fn);
+  if (use_device(device_id) != 0) return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (tokens > 0) {
+    const int rc = with_type(logits_type, [&](auto t) {
+      using T = decltype(t);
+      return with_lane_share(num_experts, [&](auto r) {
+        launch_chained(choose_kernel<T, r.value>, ceil_div(tokens, kWarps), kWarps * 32, 0, st, static_cast<const T*>(logits),
+                       gates, experts, tokens, num_experts, top_k, flags & SPARSETIR_MOE_RENORMALIZE);
+        SPTIR_LAUNCH_OK("choose_kernel");
+        return 0;
+      });
+    });
+    if (rc != 0) return rc;
+  }
+  launch_chained(place_kernel, 1, 1024, 0, st, experts, slots, indptr, tokens * top_k, num_experts);
+  SPTIR_LAUNCH_OK("place_kernel");
+  return 0;
+}
+
+extern "C" int sparsetir_moe_route_grad_raw(const void* logits, int logits_type, const float* gates, const int32_t* experts,
+                                            const float* d_gates, void* d_logits, int tokens, int num_experts, int top_k,
+                                            int flags, int device_id, void* stream) {
+  const char* fn = "sparsetir_moe_route_grad";
+  if (check_route(fn, logits_type, tokens, num_experts, top_k, flags) != 0) return -1;
+  if (tokens == 0) return 0;
+  if (!logits || !gates || !experts || !d_gates || !d_logits) return fail("%s: null pointer argument", fn);
+  if (use_device(device_id) != 0) return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (validate_enabled() && validate_range(fn, "experts", experts, static_cast<long long>(tokens) * top_k, num_experts, st,
+                                           /*lowest=*/-1) != 0)
+    return -1;
+  return with_type(logits_type, [&](auto t) {
+    using T = decltype(t);
+    return with_lane_share(num_experts, [&](auto r) {
+      launch_chained(route_grad_kernel<T, r.value>, ceil_div(tokens, kWarps), kWarps * 32, 0, st, static_cast<const T*>(logits),
+                     gates, experts, d_gates, static_cast<T*>(d_logits), tokens, num_experts, top_k,
+                     flags & SPARSETIR_MOE_RENORMALIZE);
+      SPTIR_LAUNCH_OK("route_grad_kernel");
+      return 0;
+    });
+  });
+}
+
+extern "C" int sparsetir_moe_dispatch_raw(const void* x, const int32_t* slots, void* z, int type, int tokens, int rows, int feat,
+                                          int top_k, int device_id, void* stream) {
+  const char* fn = "sparsetir_moe_dispatch";
+  if (check_rows(fn, type, tokens, rows, feat, top_k) != 0) return -1;
+  if (tokens == 0 || rows == 0 || feat == 0) return 0;
+  if (!x || !slots || !z) return fail("%s: null pointer argument", fn);
+  if (use_device(device_id) != 0) return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (check_slots(fn, slots, tokens, rows, top_k, st) != 0) return -1;
+  const size_t row_bytes = element(type) * feat;
+  const int b = piece_bytes(row_bytes, bits_of(x) | bits_of(z));
+  return with_piece<2>(b, [&](auto bytes) {
+    using P = Piece<bytes.value>;
+    const int pieces = static_cast<int>(row_bytes / bytes.value), chunks = ceil_div(pieces, kHold * 32);
+    const long long blocks = (static_cast<long long>(tokens) * chunks + kWarps - 1) / kWarps;
+    if (blocks > INT32_MAX) return fail("%s: too large for one launch", fn);
+    launch_chained(dispatch_kernel<bytes.value>, static_cast<unsigned>(blocks), kWarps * 32, 0, st, static_cast<const P*>(x), slots,
+                   static_cast<P*>(z), tokens, rows, pieces, chunks, top_k);
+    SPTIR_LAUNCH_OK("dispatch_kernel");
+    return 0;
+  });
+}
+
+extern "C" int sparsetir_moe_dispatch_i8_raw(const void* x, int type, const int32_t* slots, int8_t* q, float* scale, int tokens,
+                                             int rows, int feat, int top_k, int device_id, void* stream) {
+  const char* fn = "sparsetir_moe_dispatch_i8";
+  if (check_rows(fn, type, tokens, rows, feat, top_k) != 0) return -1;
+  if (!slots && (top_k != 1 || rows != tokens)) return fail("%s: slots may be null with top_k 1 and a row per token only", fn);
+  if (tokens == 0 || rows == 0 || feat == 0) return 0;
+  if (!x || !q || !scale) return fail("%s: null pointer argument", fn);
+  if (use_device(device_id) != 0) return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (slots && check_slots(fn, slots, tokens, rows, top_k, st) != 0) return -1;
+  return with_type(type, [&](auto t) {
+    using T = decltype(t);
+    // a piece of N elements leaves as N bytes
+    int b = piece_bytes(sizeof(T) * feat, bits_of(x));
+    while (b > static_cast<int>(sizeof(T)) && bits_of(q) % (b / sizeof(T)) != 0) b /= 2;
+    return with_piece<sizeof(T)>(b, [&](auto bytes) {
+      constexpr int B = bytes.value;
+      using Q = Piece<B / sizeof(T)>;
+      launch_chained(dispatch_i8_kernel<T, B>, tokens, kRowThreads, 0, st, static_cast<const Piece<B>*>(x), slots,
+                     reinterpret_cast<Q*>(q), scale, rows, static_cast<int>(sizeof(T) * feat / B), top_k);
+      SPTIR_LAUNCH_OK("dispatch_i8_kernel");
+      return 0;
+    });
+  });
+}
+
+extern "C" int sparsetir_moe_combine_raw(const void* z, int z_type, const int32_t* slots, const float* gates, void* y, int y_type,
+                                         int tokens, int rows, int feat, int top_k, int device_id, void* stream) {
+  const char* fn = "sparsetir_moe_combine";
+  if (check_rows(fn, z_type, tokens, rows, feat, top_k) != 0) return -1;
+  if (y_type != z_type && y_type != SPARSETIR_F32) return fail("%s: y has the type of z, or f32", fn);
+  if (tokens == 0 || feat == 0) return 0;
+  if ((!z && rows > 0) || !slots || !y) return fail("%s: null pointer argument", fn);
+  if (use_device(device_id) != 0) return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (check_slots(fn, slots, tokens, rows, top_k, st) != 0) return -1;
+  return with_type(z_type, [&](auto t) {
+    using T = decltype(t);
+    // a piece of N elements leaves in stores of up to 16 bytes
+    int b = piece_bytes(sizeof(T) * feat, bits_of(z));
+    while (b > static_cast<int>(sizeof(T)) && bits_of(y) % std::min<size_t>(16, b / sizeof(T) * element(y_type)) != 0) b /= 2;
+    return with_piece<sizeof(T)>(b, [&](auto bytes) {
+      constexpr int B = bytes.value;
+      const int pieces = static_cast<int>(sizeof(T) * feat / B), chunks = ceil_div(pieces, 64);
+      const long long blocks = (static_cast<long long>(tokens) * chunks + kWarps - 1) / kWarps;
+      if (blocks > INT32_MAX) return fail("%s: too large for one launch", fn);
+      const dim3 grid(static_cast<unsigned>(blocks));
+      if (y_type == z_type)
+        launch_chained(combine_kernel<T, T, B>, grid, kWarps * 32, 0, st, static_cast<const Piece<B>*>(z), slots, gates,
+                       static_cast<T*>(y), tokens, rows, pieces, chunks, top_k);
+      else
+        launch_chained(combine_kernel<T, float, B>, grid, kWarps * 32, 0, st, static_cast<const Piece<B>*>(z), slots, gates,
+                       static_cast<float*>(y), tokens, rows, pieces, chunks, top_k);
+      SPTIR_LAUNCH_OK("combine_kernel");
+      return 0;
+    });
+  });
+}
+
+extern "C" int sparsetir_moe_combine_grad_raw(const void* dy, const void* z, int type, const int32_t* slots, const float* gates,
+                                              void* dz, float* d_gates, int tokens, int rows, int feat, int top_k, int device_id,
+                                              void* stream) {
+  const char* fn = "sparsetir_moe_combine_grad";
+  if (check_rows(fn, type, tokens, rows, feat, top_k) != 0) return -1;
+  if (tokens == 0) return 0;
+  if (!slots || !gates || !d_gates || (feat > 0 && (!dy || (rows > 0 && (!z || !dz))))) return fail("%s: null pointer argument", fn);
+  if (use_device(device_id) != 0) return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (check_slots(fn, slots, tokens, rows, top_k, st) != 0) return -1;
+  return with_type(type, [&](auto t) {
+    using T = decltype(t);
+    const int b = piece_bytes(sizeof(T) * feat, bits_of(dy) | bits_of(z) | bits_of(dz));
+    return with_piece<sizeof(T)>(b, [&](auto bytes) {
+      constexpr int B = bytes.value;
+      launch_chained(combine_grad_kernel<T, B>, tokens, kRowThreads, 0, st, static_cast<const Piece<B>*>(dy),
+                     static_cast<const Piece<B>*>(z), slots, gates, static_cast<Piece<B>*>(dz), d_gates, rows,
+                     static_cast<int>(sizeof(T) * feat / B), top_k);
+      SPTIR_LAUNCH_OK("combine_grad_kernel");
+      return 0;
+    });
+  });
+}

@@ -25,9 +25,12 @@ namespace {
 using PackedFn = int (*)(TVMValue*, int*, int, TVMValue*, int*, void*);
 using SetStreamFn = int (*)(int, void*);
 
-bool dl_type(at::ScalarType t, DLDataType* out) {
+// The types of the reference's operators; with `more`, also those that the mixture-of-experts operators take.
+bool dl_type(at::ScalarType t, bool more, DLDataType* out) {
   out->lanes = 1;
   switch (t) {
+    case at::kBFloat16: out->code = kDLBfloat; out->bits = 16; return more;
+    case at::kChar: out->code = kDLInt; out->bits = 8; return more;
     case at::kFloat: out->code = kDLFloat; out->bits = 32; return true;
     case at::kHalf: out->code = kDLFloat; out->bits = 16; return true;
     case at::kDouble: out->code = kDLFloat; out->bits = 64; return true;
@@ -67,7 +70,8 @@ int run(PackedFn fn, SetStreamFn set_stream, TVMValue* values, int* codes, int n
 // end the process.
 
 // invoke(fn, set_stream, args) -> return code, or None when an argument is of a kind that only the
-// general packing on the Python side takes (or refuses with its message).
+// general packing on the Python side takes (or refuses with its message).  invoke_more takes bfloat16 and int8 too.
+template <bool MORE>
 PyObject* invoke(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   HANDLE_TH_ERRORS
   if (argc != 3 || !PyTuple_Check(argv[2])) {
@@ -105,7 +109,7 @@ PyObject* invoke(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     if (THPVariable_Check(o)) {
       const at::Tensor& t = THPVariable_Unpack(o);
       DLTensor& d = dl[i];
-      if (t.layout() != c10::kStrided || !(t.is_cuda() || t.is_cpu()) || !dl_type(t.scalar_type(), &d.dtype))
+      if (t.layout() != c10::kStrided || !(t.is_cuda() || t.is_cpu()) || !dl_type(t.scalar_type(), MORE, &d.dtype))
         Py_RETURN_NONE;
       d.data = t.numel() > 0 ? t.data_ptr() : nullptr;
       d.ndim = static_cast<int32_t>(t.dim());
@@ -183,7 +187,8 @@ PyObject* flatten(PyObject*, PyObject* list) {
 }
 
 PyMethodDef methods[] = {
-    {"invoke", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(invoke)), METH_FASTCALL, nullptr},
+    {"invoke", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(invoke<false>)), METH_FASTCALL, nullptr},
+    {"invoke_more", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(invoke<true>)), METH_FASTCALL, nullptr},
     {"invoke_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(invoke_packed)), METH_FASTCALL, nullptr},
     {"flatten", flatten, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},

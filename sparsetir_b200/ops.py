@@ -8,7 +8,8 @@ stream, a raised error when the callee returns -1.  Tensors are ``torch.Tensor``
 CUDA device; torch is used only for device memory and streams.
 
 The module-level callables ``csrmm``, ``hyb_spmm``, ``sddmm``, ``sddmm_edge_to_row``, ``bsrmm``
-and ``rgms`` are the packed entry points of ``include/sparsetir_b200.h``.
+and ``rgms`` are the packed entry points of ``include/sparsetir_b200.h``; so are ``moe_*`` and ``grouped_mm*``, the
+operators of a mixture-of-experts layer (``sparsetir_b200.moe`` runs them together).
 """
 from __future__ import annotations
 
@@ -34,13 +35,16 @@ _DTYPES = {
     torch.int64: (L.kDLInt, 64),
     torch.uint8: (L.kDLUInt, 8),
 }
+# what the mixture-of-experts operators take besides
+_MORE_DTYPES = {**_DTYPES, torch.bfloat16: (L.kDLBfloat, 16), torch.int8: (L.kDLInt, 8)}
 
 
-def to_dltensor(t: torch.Tensor, keepalive: List) -> L.DLTensor:
-    """Borrowed DLTensor view of a torch tensor (no copy)."""
-    if t.dtype not in _DTYPES:
+def to_dltensor(t: torch.Tensor, keepalive: List, more: bool = False) -> L.DLTensor:
+    """Borrowed DLTensor view of a torch tensor (no copy); with ``more``, of bfloat16 and int8 too."""
+    dtypes = _MORE_DTYPES if more else _DTYPES
+    if t.dtype not in dtypes:
         raise TypeError(f"unsupported dtype {t.dtype}")
-    code, bits = _DTYPES[t.dtype]
+    code, bits = dtypes[t.dtype]
     shape = (ctypes.c_int64 * max(1, t.dim()))(*t.shape)
     strides = None
     if not t.is_contiguous():
@@ -87,10 +91,12 @@ class PreparedCall:
 
 
 class PackedFunc:
-    """A TVMBackendPackedCFunc symbol of the library, callable like the reference's functions."""
+    """A TVMBackendPackedCFunc symbol of the library, callable like the reference's functions.  ``more``: it takes
+    bfloat16 and int8 tensors besides the types of the reference's operators."""
 
-    def __init__(self, symbol: str):
+    def __init__(self, symbol: str, more: bool = False):
         self.symbol = symbol
+        self._more = more
         self._fn = None
         self._entry = None
 
@@ -101,7 +107,8 @@ class PackedFunc:
     def _resolve(self):
         if self._fn is None:
             self._fn = getattr(L.load(), self.symbol)
-            self._entry = (L.pycall().invoke, _addr(self._fn), _addr(L.load().sparsetir_set_stream))
+            invoke = L.pycall().invoke_more if self._more else L.pycall().invoke
+            self._entry = (invoke, _addr(self._fn), _addr(L.load().sparsetir_set_stream))
         return self._fn
 
     def __call__(self, *args) -> None:
@@ -125,7 +132,7 @@ class PackedFunc:
         device = None
         for i, a in enumerate(args):
             if isinstance(a, torch.Tensor):
-                dl = to_dltensor(a, keep)
+                dl = to_dltensor(a, keep, self._more)
                 keep.append(dl)
                 values[i].v_handle = ctypes.cast(ctypes.pointer(dl), ctypes.c_void_p)
                 codes[i] = L.kTVMDLTensorHandle
@@ -187,6 +194,17 @@ sparse_softmax = PackedFunc("sparsetir_sparse_softmax")
 csr2bsr = PackedFunc("sparsetir_csr2bsr")
 ellmm = PackedFunc("sparsetir_ellmm")
 fusedmm = PackedFunc("sparsetir_fusedmm")
+moe_route = PackedFunc("sparsetir_moe_route", more=True)
+moe_route_grad = PackedFunc("sparsetir_moe_route_grad", more=True)
+moe_dispatch = PackedFunc("sparsetir_moe_dispatch", more=True)
+moe_dispatch_i8 = PackedFunc("sparsetir_moe_dispatch_i8", more=True)
+moe_combine = PackedFunc("sparsetir_moe_combine", more=True)
+moe_combine_grad = PackedFunc("sparsetir_moe_combine_grad", more=True)
+grouped_mm = PackedFunc("sparsetir_grouped_mm", more=True)
+grouped_mm_grad_w = PackedFunc("sparsetir_grouped_mm_grad_w", more=True)
+grouped_mm_i8 = PackedFunc("sparsetir_grouped_mm_i8", more=True)
+
+MOE_RENORMALIZE, GROUPED_W_OUT_IN = L.MOE_RENORMALIZE, L.GROUPED_W_OUT_IN
 
 
 def hyb_args(x: torch.Tensor, y: torch.Tensor, buckets: Sequence[Sequence[torch.Tensor]],
