@@ -41,6 +41,7 @@ int rgms_tc_timeouts(unsigned int* count);  // the same counter of rgms_tc.cu
 int rgms_f16_timeouts(unsigned int* count);  // ... and of rgms_f16.cu
 int rgms_fused_timeouts(unsigned int* count);  // ... and of rgms_fused.cu
 int conv_timeouts(unsigned int* count);        // ... and of sparse_conv.cu
+int grouped_timeouts(unsigned int* count);     // ... and of grouped.cu
 
 namespace {
 
@@ -603,6 +604,8 @@ extern "C" int sparsetir_tc_timeouts(int device_id, unsigned int* count) {
   if (rgms_fused_timeouts(&rf) != 0) return -1;
   unsigned int cv = 0;
   if (conv_timeouts(&cv) != 0) return -1;
-  *count = bsr + rgms + rh + rf + cv;
+  unsigned int gr = 0;
+  if (grouped_timeouts(&gr) != 0) return -1;
+  *count = bsr + rgms + rh + rf + cv + gr;
   return 0;
 }

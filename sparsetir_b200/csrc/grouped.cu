@@ -1,112 +1,450 @@
-// Products grouped by expert, ragged sizes: the simplest form that is right for every size, on CUDA cores.
+// Products grouped by expert, ragged sizes, on the tensor cores:
+//   grouped_mm         y[s, :] = x[s, :] * W[g]                       s in [indptr[g], indptr[g + 1])
+//   grouped_mm_i8      the same in 8-bit integers, scaled per row and per output feature
+//   grouped_mm_grad_w  dW[g, a, b] = sum over the rows s of group g of pa[s, a] * pb[s, b]
+//
+// All three are one kernel.  A pair of blocks (cta_group::2) holds 256 of what is contiguous in the result (output
+// features; b) as the rows of the tensor core's left operand, and up to 256 of what is not (rows of the group; a) as the columns:
+// the result comes out of TMEM with neighbouring lanes at neighbouring addresses, and a ragged group costs its rows rounded
+// up to 32, whatever the group's neighbours are.  How many rows a group has is read from indptr on the device, by every
+// role of the block for itself.
 #include <algorithm>
 
 #include "common.h"
 #include "launch.cuh"
 #include "lowp.cuh"
+#include "tc05.cuh"
+#include "tmap.h"
+#include "vec.cuh"
 
 namespace sptir {
 namespace {
 
-constexpr int kTile = 64, kStep = 16;
+constexpr int kM = 128;               // features per block
+constexpr int kN = 256;               // columns per pair
+constexpr int kHalfBytes = 16 * 1024; // one operand of a stage: 128 rows of 128 bytes
+constexpr int kStageBytes = 2 * kHalfBytes;
+constexpr int kStages = 6;
+constexpr int kAtom = 8 * 1024;       // 64 rows of 128 bytes
+constexpr int kThreads = 256;         // warp 0 loads, 1 issues, 2-3 clear the tails of groups (grad_w), 4-7 epilogue
+constexpr int kSmem = kStages * kStageBytes + 1024;
+constexpr int kTmemCols = 2 * kN;
+constexpr int kBand = 8;              // column tiles of a group that are walked side by side
+
+__device__ unsigned int g_grouped_timeouts = 0;
+
+struct Args {
+  void* out;
+  const int32_t* indptr;
+  const float* x_scale;
+  const float* w_scale;
+  int rows, groups;
+  int k;          // depth of the product; grad_w: unused
+  int features;   // contiguous in the result
+  int columns;    // grad_w: rows of each dW
+  int mt, nt;     // tiles of 256 features; grad_w: of 256 columns
+  int max_tiles;  // no valid indptr has more
+  uint32_t idesc; // without N
+  int a_mn;       // the left operand is contiguous along the features
+};
 
 // First and past the last row of group g, inside the array whatever the pointers say.
-__device__ __forceinline__ void group_rows(const int32_t* indptr, int g, int rows, int* first, int* last) {
-  if (indptr == nullptr) { *first = 0; *last = rows; return; }
-  *first = min(max(ld_global(indptr + g), 0), rows);
-  *last = max(min(ld_global(indptr + g + 1), rows), *first);
+__device__ __forceinline__ void group_rows(const Args& p, int g, int* first, int* last) {
+  if (p.indptr == nullptr) { *first = 0; *last = p.rows; return; }
+  *first = min(max(ld_global(p.indptr + g), 0), p.rows);
+  *last = max(min(ld_global(p.indptr + g + 1), p.rows), *first);
 }
 
-__device__ __forceinline__ float number(float v) { return v; }
-__device__ __forceinline__ float number(__half v) { return __half2float(v); }
-__device__ __forceinline__ float number(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ int number(int8_t v) { return v; }
-
-template <class T> struct SumOf { using type = float; };
-template <> struct SumOf<int8_t> { using type = int; };
-
-// c[64 x 64] += a[64 x 16] * b[16 x 64] out of shared memory, 4 x 4 results to a thread
-template <class S>
-__device__ __forceinline__ void multiply(S (&c)[4][4], const S (&a)[kStep][kTile + 1], const S (&b)[kStep][kTile + 1]) {
-  const int r = threadIdx.x / 16, q = threadIdx.x % 16;
-#pragma unroll
-  for (int k = 0; k < kStep; ++k)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) c[i][j] += a[k][r + 16 * i] * b[k][q + 16 * j];
+// A group of m rows in equal tiles of a multiple of 32 up to 256.
+__device__ __forceinline__ void split(int m, int* size, int* count) {
+  const int n = (m + kN - 1) / kN;
+  *size = n == 0 ? kN : ((m + n - 1) / n + 31) & ~31;
+  *count = (m + *size - 1) / *size;
 }
 
-// Block = 64 features of 64 rows of one group; blockIdx.y counts the row tiles of all groups.
-template <class T, class OutT>
-__global__ void __launch_bounds__(256)
-grouped_kernel(const T* x, const T* w, OutT* y, const float* x_scale, const float* w_scale, const int32_t* indptr, int rows,
-               int groups, int fi, int fo, int out_in) {
-  using S = typename SumOf<T>::type;
-  __shared__ S a[kStep][kTile + 1], b[kStep][kTile + 1];
-  chain_wait();
-  int tile = blockIdx.y, g = 0, first = 0, last = 0;
-  for (; g < groups; ++g) {
-    group_rows(indptr, g, rows, &first, &last);
-    const int n = (last - first + kTile - 1) / kTile;
-    if (tile < n) break;
-    tile -= n;
-  }
-  if (g == groups) return;
-  first += tile * kTile;
-  const int f0 = blockIdx.x * kTile;
-  S c[4][4] = {};
-  const T* wg = w + static_cast<size_t>(g) * fi * fo;
-  for (int k0 = 0; k0 < fi; k0 += kStep) {
-    for (int e = threadIdx.x; e < kStep * kTile; e += 256) {
-      const int k = e % kStep, i = e / kStep;
-      a[k][i] = 0;
-      if (first + i < last && k0 + k < fi) a[k][i] = number(x[static_cast<size_t>(first + i) * fi + k0 + k]);
-      b[k][i] = 0;
-      if (f0 + i < fo && k0 + k < fi)
-        b[k][i] = number(out_in ? wg[static_cast<size_t>(f0 + i) * fi + k0 + k] : wg[static_cast<size_t>(k0 + k) * fo + f0 + i]);
-    }
-    __syncthreads();
-    multiply(c, a, b);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int r = first + threadIdx.x / 16 + 16 * i, f = f0 + threadIdx.x % 16 + 16 * j;
-      if (r >= last || f >= fo) continue;
-      float v = static_cast<float>(c[i][j]);
-      if (x_scale != nullptr) v *= x_scale[r] * w_scale[static_cast<size_t>(g) * fo + f];
-      y[static_cast<size_t>(r) * fo + f] = from_float<OutT>(v);
-    }
-}
+struct Tile {
+  int group, feat0;
+  int col0, n, n_mma;   // columns: first, how many there are, rounded up to 32
+  int row0, depth;      // grad_w: rows of the group
+};
 
-// Block = 64 x 64 of one group's dw: the sum over the group's rows of a[s, i] * b[s, j]
-template <class T, class OutT>
-__global__ void __launch_bounds__(256)
-grouped_grad_kernel(const T* pa, const T* pb, OutT* dw, const int32_t* indptr, int rows, int fa, int fb) {
-  __shared__ float a[kStep][kTile + 1], b[kStep][kTile + 1];
-  chain_wait();
-  const int g = blockIdx.z, i0 = blockIdx.y * kTile, j0 = blockIdx.x * kTile;
+// The tiles of one pair: t, t + pairs, ...  All lanes of a warp call next() together; lane l holds the prefix of tile counts
+// of group base + l.  Sums stop at 2^30: wild pointers give tiles inside the arrays, and no more than max_tiles of them.
+template <bool GRAD>
+struct Walker {
+  const Args& p;
+  int t, step, base = -32;
+  unsigned before = 0, upto = 0;  // tiles ahead of the group of lane 0, and up to the group of this lane
+  unsigned all = 0;               // up to the last of the 32
   int first = 0, last = 0;
-  group_rows(indptr, g, rows, &first, &last);
-  float c[4][4] = {};
-  for (int s0 = first; s0 < last; s0 += kStep) {
-    for (int e = threadIdx.x; e < kStep * kTile; e += 256) {
-      const int i = e % kTile, k = e / kTile;
-      a[k][i] = 0.f;
-      b[k][i] = 0.f;
-      if (s0 + k < last && i0 + i < fa) a[k][i] = number(pa[static_cast<size_t>(s0 + k) * fa + i0 + i]);
-      if (s0 + k < last && j0 + i < fb) b[k][i] = number(pb[static_cast<size_t>(s0 + k) * fb + j0 + i]);
+  __device__ __forceinline__ Walker(const Args& a, int pair, int pairs) : p(a), t(pair), step(pairs) {}
+  __device__ __forceinline__ bool next(Tile* out) {
+    if (t >= p.max_tiles) return false;
+    if constexpr (GRAD) {
+      const int per = p.mt * p.nt, g = t / per, r = t - g * per;
+      int f, l;
+      group_rows(p, g, &f, &l);
+      place(r, p.nt, out);
+      out->group = g;
+      out->col0 *= kN;
+      out->n = min(kN, p.columns - out->col0);
+      out->row0 = f;
+      out->depth = l - f;
+    } else {
+      const int lane = threadIdx.x & 31;
+      while (static_cast<unsigned>(t) >= all) {
+        base += 32;
+        if (base >= p.groups) return false;
+        before = all;
+        unsigned mine = 0;
+        first = last = 0;
+        if (base + lane < p.groups) {
+          group_rows(p, base + lane, &first, &last);
+          int size, count;
+          split(last - first, &size, &count);
+          mine = static_cast<unsigned>(min(static_cast<long long>(count) * p.mt, 1ll << 30));
+        }
+        upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned up = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto = min(upto + up, 1u << 30);
+        }
+        upto = min(upto + before, 1u << 30);
+        all = __shfl_sync(0xffffffffu, upto, 31);
+      }
+      const int src = __ffs(__ballot_sync(0xffffffffu, upto > static_cast<unsigned>(t))) - 1;
+      const unsigned prev = __shfl_sync(0xffffffffu, upto, max(src - 1, 0));
+      const int f = __shfl_sync(0xffffffffu, first, src), l = __shfl_sync(0xffffffffu, last, src);
+      int size, count;
+      split(l - f, &size, &count);
+      place(t - static_cast<int>(src == 0 ? before : prev), count, out);
+      out->group = base + src;
+      out->col0 = f + out->col0 * size;
+      out->n = min(size, l - out->col0);
+      out->row0 = 0;
+      out->depth = p.k;
     }
-    __syncthreads();
-    multiply(c, a, b);
-    __syncthreads();
+    out->n_mma = (out->n + 31) & ~31;
+    t += step;
+    return true;
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int r = i0 + threadIdx.x / 16 + 16 * i, f = j0 + threadIdx.x % 16 + 16 * j;
-      if (r < fa && f < fb) dw[(static_cast<size_t>(g) * fa + r) * fb + f] = from_float<OutT>(c[i][j]);
+  // Tile r of a group with `cols` column tiles: bands of kBand column tiles, in a band one column tile after the other.
+  // col0 is left in tiles.
+  __device__ __forceinline__ void place(int r, int cols, Tile* out) const {
+    const int band = r / (kBand * p.mt), in = r - band * (kBand * p.mt);
+    const int width = min(kBand, cols - band * kBand);
+    const int f = in / width;
+    out->feat0 = f * (2 * kM);
+    out->col0 = band * kBand + in - f * width;
+  }
+};
+
+template <bool I8, bool GRAD, class OutT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b64,
+               const __grid_constant__ CUtensorMap tm_b16, const __grid_constant__ Args p) {
+  constexpr int kDepth = I8 ? 128 : 64;  // of K per stage
+  constexpr int kInstr = I8 ? 32 : 16;   // of K per instruction
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t bar_full[kStages];   // rank 0: both blocks' operands are there
+  __shared__ __align__(8) uint64_t bar_empty[kStages];  // the tensor core has read the stage
+  __shared__ __align__(8) uint64_t bar_tail[kStages];   // the last rows of a group are there, to be cleared past its end
+  __shared__ __align__(8) uint64_t bar_acc_full[2];
+  __shared__ __align__(8) uint64_t bar_acc_empty[2];    // rank 0: both blocks have taken the result
+  __shared__ __align__(8) uint64_t bar_drain;
+  __shared__ uint32_t s_tmem;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = tc05::pair::rank();
+  const uint32_t base = (tc05::smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int s = 0; s < kStages; ++s) {
+        tc05::mbar_init(&bar_full[s], 2);
+        tc05::mbar_init(&bar_empty[s], 1);
+        tc05::mbar_init(&bar_tail[s], 1);
+      }
+      for (int b = 0; b < 2; ++b) {
+        tc05::mbar_init(&bar_acc_full[b], 1);
+        tc05::mbar_init(&bar_acc_empty[b], 8);
+      }
+      tc05::mbar_init(&bar_drain, 1);
+      tc05::fence_mbar_init();
+      tc05::prefetch_tensormap(&tm_a);
+      tc05::prefetch_tensormap(&tm_b64);
     }
+    __syncwarp();
+    tc05::pair::tmem_alloc(&s_tmem, kTmemCols);
+  }
+  chain_wait();
+  tc05::fence_before_sync();
+  __syncthreads();
+  tc05::pair::sync();  // the other block's barriers are there
+  chain_trigger();
+  tc05::fence_after_sync();
+  const uint32_t tmem = s_tmem;
+  bool ok = true;
+  int armed = 0;
+
+  // Stage and phase of the ring move by whole tiles in all lanes of a role's warp; its elected thread walks them step by step.
+  int stage = 0;
+  uint32_t phase = 0;
+  auto advance = [&](int steps) {
+    const int q = stage + steps;
+    phase ^= static_cast<uint32_t>(q / kStages) & 1u;
+    stage = q % kStages;
+  };
+  Walker<GRAD> walk(p, pair, pairs);
+  Tile tile;
+
+  if (warp == 0) {
+    // ---- loads.  Each block fetches its 128 features and its half of the columns, and tells rank 0's barrier.
+    while (ok && walk.next(&tile)) {
+      const int half = tile.n_mma / 2, units = half / 16;
+      const int feat = tile.feat0 + static_cast<int>(rank) * kM, col = tile.col0 + static_cast<int>(rank) * half;
+      const int steps = (tile.depth + kDepth - 1) / kDepth;
+      if (tc05::elect_one()) {
+        const uint32_t bytes = kHalfBytes + (GRAD ? (half > 64 ? 2 : 1) * kAtom : units * 2048);
+        int s = stage;
+        uint32_t ph = phase;
+        for (int k = 0; k < steps; ++k) {
+          if (!tc05::mbar_wait(&bar_empty[s], ph ^ 1u)) { ok = false; break; }
+          const uint32_t st = base + s * kStageBytes;
+          uint32_t bar;
+          if (GRAD && k == steps - 1 && tile.depth % kDepth != 0) {
+            bar = tc05::smem_u32(&bar_tail[s]);
+            tc05::mbar_arrive_expect_tx(&bar_tail[s], bytes);
+          } else {
+            bar = tc05::pair::at_first(&bar_full[s]);
+            tc05::pair::arrive_expect_tx(bar, bytes);
+          }
+          if constexpr (GRAD) {
+            const int row = tile.row0 + k * kDepth;
+            tc05::pair::tma_load_2d(st, &tm_a, feat, row, bar);
+            tc05::pair::tma_load_2d(st + kAtom, &tm_a, feat + 64, row, bar);
+            tc05::pair::tma_load_2d(st + kHalfBytes, &tm_b64, col, row, bar);
+            if (half > 64) tc05::pair::tma_load_2d(st + kHalfBytes + kAtom, &tm_b64, col + 64, row, bar);
+          } else {
+            if (p.a_mn) {
+              tc05::pair::tma_load_3d(st, &tm_a, feat, k * kDepth, tile.group, bar);
+              tc05::pair::tma_load_3d(st + kAtom, &tm_a, feat + 64, k * kDepth, tile.group, bar);
+            } else {
+              tc05::pair::tma_load_3d(st, &tm_a, k * kDepth, feat, tile.group, bar);
+            }
+            int u = 0;
+            for (; u + 4 <= units; u += 4) tc05::pair::tma_load_2d(st + kHalfBytes + u * 2048, &tm_b64, k * kDepth, col + u * 16, bar);
+            for (; u < units; ++u) tc05::pair::tma_load_2d(st + kHalfBytes + u * 2048, &tm_b16, k * kDepth, col + u * 16, bar);
+          }
+          ++armed;
+          if (++s == kStages) { s = 0; ph ^= 1u; }
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      advance(steps);
+    }
+  } else if (warp == 1) {
+    // ---- MMAs of both blocks, from rank 0: M = 256 features, N = the tile's columns
+    int acc = 0;
+    const bool a_mn = GRAD || p.a_mn != 0;
+    const uint32_t a_step = a_mn ? 2048u : 32u, b_step = GRAD ? 2048u : 32u;
+    const uint64_t da0 = tc05::smem_desc_swizzled(base, a_mn ? kAtom : 0, 1024, tc05::kSwizzle128B);
+    const uint64_t db0 = tc05::smem_desc_swizzled(base + kHalfBytes, GRAD ? kAtom : 0, 1024, tc05::kSwizzle128B);
+    while (rank == 0 && ok && walk.next(&tile)) {
+      const int steps = (tile.depth + kDepth - 1) / kDepth;
+      if (steps == 0) continue;
+      if (tc05::elect_one()) {
+        const int buf = acc & 1;
+        const uint32_t idesc = p.idesc | static_cast<uint32_t>(tile.n_mma >> 3) << 17;
+        const uint32_t d = tmem + buf * kN;
+        int s = stage;
+        uint32_t ph = phase;
+        ok = tc05::pair::mbar_wait(&bar_acc_empty[buf], ((acc >> 1) & 1) ^ 1);
+        tc05::fence_after_sync();
+        for (int k = 0; k < steps && ok; ++k) {
+          if (!tc05::pair::mbar_wait(&bar_full[s], ph)) { ok = false; break; }
+          tc05::fence_after_sync();
+          const uint64_t da = tc05::desc_advance(da0, s * kStageBytes), db = tc05::desc_advance(db0, s * kStageBytes);
+          const int left = tile.depth - k * kDepth;
+#pragma unroll
+          for (int i = 0; i < kDepth / kInstr; ++i)
+            if (i * kInstr < left)
+              tc05::pair::mma<I8>(d, tc05::desc_advance(da, i * a_step), tc05::desc_advance(db, i * b_step), idesc,
+                                  (k > 0 || i > 0) ? 1u : 0u);
+          tc05::pair::mma_commit(&bar_empty[s]);
+          if (++s == kStages) { s = 0; ph ^= 1u; }
+        }
+        tc05::pair::mma_commit(&bar_acc_full[buf]);
+        if (!ok) {  // gave up: what has been issued is over before the block's memory is released
+          tc05::pair::mma_commit(&bar_drain);
+          tc05::mbar_wait(&bar_drain, 0);
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      ++acc;
+      advance(steps);
+    }
+  } else if (GRAD && warp == 2) {
+    // ---- The last step of a group holds rows of its neighbours: zeros in their place, in both operands (0 times what is
+    // not a number would not be zero), up to where the instructions read.
+    uint32_t tail_phase = 0;
+    while (ok && walk.next(&tile)) {
+      const int steps = (tile.depth + kDepth - 1) / kDepth, rem = tile.depth % kDepth;
+      if (rem != 0) {
+        const int s = (stage + steps - 1) % kStages;
+        ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_tail[s], (tail_phase >> s) & 1u));
+        tail_phase ^= 1u << s;
+        const int clear = (((rem + kInstr - 1) / kInstr) * kInstr - rem) * 8;  // pieces of 16 bytes in each of the four atoms
+        unsigned char* at = smem_raw + (base - tc05::smem_u32(smem_raw)) + s * kStageBytes + rem * 128;
+        for (int i = lane; i < 4 * clear; i += 32) {
+          const int atom = i / clear;
+          *reinterpret_cast<uint4*>(at + atom * kAtom + (i - atom * clear) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        tc05::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) tc05::pair::arrive(tc05::pair::at_first(&bar_full[s]));
+      }
+      advance(steps);
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue: lane = feature, columns 32 at a time
+    int acc = 0;
+    OutT* const out = static_cast<OutT*>(p.out);
+    while (ok && walk.next(&tile)) {
+      const int feat = tile.feat0 + static_cast<int>(rank) * kM + (warp & 3) * 32 + lane;
+      const bool live = feat < p.features;
+      size_t row = static_cast<size_t>(tile.col0);
+      if constexpr (GRAD) row += static_cast<size_t>(tile.group) * p.columns;
+      OutT* to = out + row * p.features + feat;
+      if (GRAD && tile.depth == 0) {
+        for (int c = 0; c < tile.n; ++c)
+          if (live) to[static_cast<size_t>(c) * p.features] = from_float<OutT>(0.f);
+        continue;
+      }
+      float ws = 0.f;
+      if constexpr (I8) {
+        if (live) ws = ld_global(p.w_scale + static_cast<size_t>(tile.group) * p.features + feat);
+      }
+      const int buf = acc & 1;
+      ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_acc_full[buf], (acc >> 1) & 1));
+      if (!ok) break;
+      tc05::fence_after_sync();
+      const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + buf * kN;
+      for (int c0 = 0; c0 < tile.n; c0 += 32) {
+        float xs = 0.f;
+        if constexpr (I8) {
+          if (c0 + lane < tile.n) xs = ld_global(p.x_scale + tile.col0 + c0 + lane);
+        }
+        uint32_t r[32];
+        tc05::tmem_ld32(taddr + c0, r);
+        if (c0 + 32 >= tile.n) {  // the result is in registers: the accumulator may be written again
+          tc05::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc05::pair::arrive(tc05::pair::at_first(&bar_acc_empty[buf]));
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          float v;
+          if constexpr (I8)
+            v = static_cast<float>(static_cast<int>(r[c])) * (__shfl_sync(0xffffffffu, xs, c) * ws);
+          else
+            v = __uint_as_float(r[c]);
+          if (live && c0 + c < tile.n) to[static_cast<size_t>(c0 + c) * p.features] = from_float<OutT>(v);
+        }
+      }
+      ++acc;
+    }
+  }
+
+  const bool all_ok = !__syncthreads_or(!ok);
+  if (!all_ok) {
+    if (tid == 0) atomicAdd(&g_grouped_timeouts, 1u);
+    // gave up: the loads that have been issued land (bounded) before the blocks' memory is released
+    if (rank == 0)
+      for (int it = max(0, armed - kStages); it < armed; ++it) tc05::mbar_wait(&bar_full[it % kStages], (it / kStages) & 1);
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  }
+  __syncwarp();
+  tc05::fence_before_sync();
+  tc05::pair::sync();
+  if (warp == 0) tc05::pair::tmem_dealloc(tmem, kTmemCols);
+}
+
+// ---- rows at aligned addresses: TMA wants pitches that are multiples of 16 bytes
+
+template <class E>  // an element of 1 or 2 bytes
+__global__ void __launch_bounds__(256) pad_rows_kernel(const E* src, uint4* dst, long long rows, int cols, int pieces) {
+  constexpr int N = 16 / sizeof(E);
+  chain_wait();
+  const long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const long long row = at / pieces;
+  const int c0 = static_cast<int>(at - row * pieces) * N;
+  if (row >= rows) return;
+  const E* from = src + row * cols + c0;
+  Piece<16> v = make_uint4(0u, 0u, 0u, 0u);
+  E* e = reinterpret_cast<E*>(&v);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (c0 + i < cols) e[i] = from[i];
+  dst[at] = v;
+}
+
+// A row-major operand of elements of `size` bytes as TMA can read it: where it is, or a padded copy.
+struct Operand {
+  const void* data;
+  long long rows;
+  int cols, size;
+  size_t pitch = 0;  // bytes of a row
+  bool fits() const { return aligned16(data) && static_cast<size_t>(cols) * size % 16 == 0; }
+  size_t padded() const { return (static_cast<size_t>(cols) * size + 15) / 16 * 16; }
+  size_t copy_bytes() const { return fits() ? 0 : (padded() * rows + 255) / 256 * 256; }
+};
+int place_operand(Operand* o, char** scratch, cudaStream_t st) {
+  o->pitch = o->padded();
+  if (o->fits() || o->rows == 0) return 0;
+  const int pieces = static_cast<int>(o->pitch / 16);
+  const long long blocks = (o->rows * pieces + 255) / 256;
+  if (blocks > INT32_MAX) return fail("operand too large to be copied to aligned rows");
+  uint4* to = reinterpret_cast<uint4*>(*scratch);
+  if (o->size == 2)
+    launch_chained(pad_rows_kernel<uint16_t>, static_cast<unsigned>(blocks), 256, 0, st, static_cast<const uint16_t*>(o->data), to,
+                   o->rows, o->cols, pieces);
+  else
+    launch_chained(pad_rows_kernel<uint8_t>, static_cast<unsigned>(blocks), 256, 0, st, static_cast<const uint8_t*>(o->data), to,
+                   o->rows, o->cols, pieces);
+  SPTIR_LAUNCH_OK("pad_rows_kernel");
+  *scratch += o->copy_bytes();
+  o->data = to;
+  return 0;
+}
+
+template <bool I8, bool GRAD, class OutT>
+int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap& tm_b16, const Args& p, cudaStream_t st) {
+  static thread_local int configured_device = -1, pairs = 0;
+  int dev = 0;
+  SPTIR_CUDA_OK(cudaGetDevice(&dev));
+  if (configured_device != dev) {
+    SPTIR_CUDA_OK(cudaFuncSetAttribute(grouped_kernel<I8, GRAD, OutT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    // as many pairs as can run at a time: each walks its share of the tiles
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = kNumSMs;
+    cfg.blockDim = kThreads;
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    SPTIR_CUDA_OK(cudaOccupancyMaxActiveClusters(&pairs, grouped_kernel<I8, GRAD, OutT>, &cfg));
+    if (pairs < 1) return fail("no pair of blocks fits this device");
+    pairs = std::min(pairs, kNumSMs / 2);
+    configured_device = dev;
+  }
+  launch_chained(grouped_kernel<I8, GRAD, OutT>, 2 * std::min(pairs, p.max_tiles), kThreads, kSmem, st, tm_a, tm_b64, tm_b16, p);
+  SPTIR_LAUNCH_OK("grouped_kernel");
+  return 0;
 }
 
 int check_groups(const char* fn, const int32_t* indptr, int rows, int groups, int fi, int fo, int flags) {
@@ -121,17 +459,66 @@ int check_pointers(const char* fn, const int32_t* indptr, int rows, int groups, 
   if (validate_indptr(fn, "indptr", indptr, groups, -1, st) != 0) return -1;
   return validate_range(fn, "indptr", indptr, groups + 1ll, rows + 1ll, st);
 }
-
-template <class T, class OutT>
-int run(const T* x, const T* w, OutT* y, const float* xs, const float* ws, const int32_t* indptr, int rows, int groups, int fi,
-        int fo, int out_in, cudaStream_t st) {
-  const dim3 grid(ceil_div(fo, kTile), ceil_div(rows, kTile) + groups);
-  launch_chained(grouped_kernel<T, OutT>, grid, 256, 0, st, x, w, y, xs, ws, indptr, rows, groups, fi, fo, out_in);
-  SPTIR_LAUNCH_OK("grouped_kernel");
+int set_tiles(const char* fn, Args* p, long long column_tiles) {
+  p->mt = ceil_div(p->features, 2 * kM);
+  if (column_tiles > (1 << 30) / p->mt) return fail("%s: too many tiles for 32-bit indices", fn);
+  p->max_tiles = static_cast<int>(column_tiles * p->mt);
   return 0;
 }
 
+CUtensorMapDataType map_type(int type) {
+  return type == SPARSETIR_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+         : type == SPARSETIR_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+}
+uint32_t map_format(int type) { return type == SPARSETIR_F16 ? tc05::kFmtF16 : tc05::kFmtBF16; }
+
+// y = x * W: `type` of the elements of x and W, -1 for 8-bit integers
+int product(const char* fn, const void* x, const void* w, int type, void* y, int y_type, const float* xs, const float* ws,
+            const int32_t* indptr, int rows, int groups, int fi, int fo, bool out_in, int device_id, cudaStream_t st) {
+  const bool i8 = type < 0;
+  const int size = i8 ? 1 : 2, depth = 128 / size;
+  Args p{};
+  p.out = y;
+  p.indptr = indptr;
+  p.x_scale = xs;
+  p.w_scale = ws;
+  p.rows = rows;
+  p.groups = groups;
+  p.k = fi;
+  p.features = fo;
+  p.a_mn = out_in ? 0 : 1;
+  p.idesc = i8 ? tc05::instr_desc_i8(2 * kM, 0) : tc05::instr_desc(map_format(type), 2 * kM, 0, p.a_mn, 0);
+  if (set_tiles(fn, &p, rows / kN + static_cast<long long>(std::min(groups, rows))) != 0) return -1;
+  Operand ox{x, rows, fi, size}, ow{w, static_cast<long long>(groups) * (out_in ? fo : fi), out_in ? fi : fo, size};
+  const size_t copies = ox.copy_bytes() + ow.copy_bytes();
+  CallScratch cs;
+  if (copies > 0 && take_scratch(device_id, st, copies, 0, &cs) != 0) return -1;
+  char* scratch = cs.scratch;
+  if (place_operand(&ox, &scratch, st) != 0 || place_operand(&ow, &scratch, st) != 0) return -1;
+  CUtensorMap tm_w, tm_x64, tm_x16;
+  const cuuint64_t each = out_in ? fo : fi;  // rows of one W
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(ow.cols), each, static_cast<cuuint64_t>(groups)};
+  const cuuint64_t strides[2] = {ow.pitch, ow.pitch * each};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(out_in ? depth : 64), static_cast<cuuint32_t>(out_in ? kM : depth), 1};
+  const CUtensorMapDataType dt = map_type(type);
+  if (make_tmap(&tm_w, dt, ow.data, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
+      make_tmap_2d(&tm_x64, dt, ox.data, fi, rows, ox.pitch, depth, 64, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
+      make_tmap_2d(&tm_x16, dt, ox.data, fi, rows, ox.pitch, depth, 16, CU_TENSOR_MAP_SWIZZLE_128B) != 0)
+    return -1;
+  const int rc = with_type(y_type, [&](auto o) {
+    using O = decltype(o);
+    return i8 ? launch<true, false, O>(tm_w, tm_x64, tm_x16, p, st) : launch<false, false, O>(tm_w, tm_x64, tm_x16, p, st);
+  });
+  return rc != 0 ? rc : return_scratch(cs, st);
+}
+
 }  // namespace
+
+int grouped_timeouts(unsigned int* count) {
+  SPTIR_CUDA_OK(cudaMemcpyFromSymbol(count, g_grouped_timeouts, sizeof(unsigned int)));
+  return 0;
+}
+
 }  // namespace sptir
 
 using namespace sptir;
@@ -148,41 +535,8 @@ extern "C" int sparsetir_grouped_mm_raw(const void* x, const void* w, int type, 
   if (use_device(device_id) != 0) return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (check_pointers(fn, indptr, rows, num_groups, st) != 0) return -1;
-  return with_type(type, [&](auto t) {
-    using T = decltype(t);
-    return with_type(y_type, [&](auto o) {
-      using O = decltype(o);
-      return run(static_cast<const T*>(x), static_cast<const T*>(w), static_cast<O*>(y), nullptr, nullptr, indptr, rows, num_groups,
-                 feat_in, feat_out, flags & SPARSETIR_GROUPED_W_OUT_IN, st);
-    });
-  });
-}
-
-extern "C" int sparsetir_grouped_mm_grad_w_raw(const void* x, const void* dy, int type, void* dw, int dw_type,
-                                               const int32_t* indptr, int rows, int num_groups, int feat_in, int feat_out,
-                                               int flags, int device_id, void* stream) {
-  const char* fn = "sparsetir_grouped_mm_grad_w";
-  if (check_groups(fn, indptr, rows, num_groups, feat_in, feat_out, flags) != 0) return -1;
-  if (type != SPARSETIR_F16 && type != SPARSETIR_BF16) return fail("%s: x and dy are f16 or bf16", fn);
-  if (dw_type != type && dw_type != SPARSETIR_F32) return fail("%s: dw has the type of x, or f32", fn);
-  if (num_groups == 0) return 0;
-  if (!dw || (rows > 0 && (!x || !dy))) return fail("%s: null pointer argument", fn);
-  if (use_device(device_id) != 0) return -1;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (check_pointers(fn, indptr, rows, num_groups, st) != 0) return -1;
-  const bool out_in = (flags & SPARSETIR_GROUPED_W_OUT_IN) != 0;
-  const int fa = out_in ? feat_out : feat_in, fb = out_in ? feat_in : feat_out;
-  return with_type(type, [&](auto t) {
-    using T = decltype(t);
-    return with_type(dw_type, [&](auto o) {
-      using O = decltype(o);
-      const dim3 grid(ceil_div(fb, kTile), ceil_div(fa, kTile), num_groups);
-      launch_chained(grouped_grad_kernel<T, O>, grid, 256, 0, st, static_cast<const T*>(out_in ? dy : x),
-                     static_cast<const T*>(out_in ? x : dy), static_cast<O*>(dw), indptr, rows, fa, fb);
-      SPTIR_LAUNCH_OK("grouped_grad_kernel");
-      return 0;
-    });
-  });
+  return product(fn, x, w, type, y, y_type, nullptr, nullptr, indptr, rows, num_groups, feat_in, feat_out,
+                 (flags & SPARSETIR_GROUPED_W_OUT_IN) != 0, device_id, st);
 }
 
 extern "C" int sparsetir_grouped_mm_i8_raw(const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale, void* y,
@@ -197,8 +551,49 @@ extern "C" int sparsetir_grouped_mm_i8_raw(const int8_t* x, const float* x_scale
   if (use_device(device_id) != 0) return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (check_pointers(fn, indptr, rows, num_groups, st) != 0) return -1;
-  return with_type(y_type, [&](auto o) {
-    using O = decltype(o);
-    return run(x, w, static_cast<O*>(y), x_scale, w_scale, indptr, rows, num_groups, feat_in, feat_out, 1, st);
-  });
+  return product(fn, x, w, /*type=*/-1, y, y_type, x_scale, w_scale, indptr, rows, num_groups, feat_in, feat_out, /*out_in=*/true,
+                 device_id, st);
+}
+
+extern "C" int sparsetir_grouped_mm_grad_w_raw(const void* x, const void* dy, int type, void* dw, int dw_type,
+                                               const int32_t* indptr, int rows, int num_groups, int feat_in, int feat_out,
+                                               int flags, int device_id, void* stream) {
+  const char* fn = "sparsetir_grouped_mm_grad_w";
+  if (check_groups(fn, indptr, rows, num_groups, feat_in, feat_out, flags) != 0) return -1;
+  if (type != SPARSETIR_F16 && type != SPARSETIR_BF16) return fail("%s: x and dy are f16 or bf16", fn);
+  if (dw_type != type && dw_type != SPARSETIR_F32) return fail("%s: dw has the type of x, or f32", fn);
+  if (num_groups == 0) return 0;
+  if (!dw || (rows > 0 && (!x || !dy))) return fail("%s: null pointer argument", fn);
+  if (use_device(device_id) != 0) return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {
+    const size_t bytes = static_cast<size_t>(num_groups) * feat_in * feat_out * (dw_type == SPARSETIR_F32 ? 4 : 2);
+    SPTIR_CUDA_OK(cudaMemsetAsync(dw, 0, bytes, st));
+    return 0;
+  }
+  if (check_pointers(fn, indptr, rows, num_groups, st) != 0) return -1;
+  const bool out_in = (flags & SPARSETIR_GROUPED_W_OUT_IN) != 0;
+  Args p{};
+  p.out = dw;
+  p.indptr = indptr;
+  p.rows = rows;
+  p.groups = num_groups;
+  p.features = out_in ? feat_in : feat_out;
+  p.columns = out_in ? feat_out : feat_in;
+  p.nt = ceil_div(p.columns, kN);
+  p.idesc = tc05::instr_desc(map_format(type), 2 * kM, 0, 1, 1);
+  if (set_tiles(fn, &p, static_cast<long long>(num_groups) * p.nt) != 0) return -1;
+  Operand oa{out_in ? x : dy, rows, p.features, 2}, ob{out_in ? dy : x, rows, p.columns, 2};
+  const size_t copies = oa.copy_bytes() + ob.copy_bytes();
+  CallScratch cs;
+  if (copies > 0 && take_scratch(device_id, st, copies, 0, &cs) != 0) return -1;
+  char* scratch = cs.scratch;
+  if (place_operand(&oa, &scratch, st) != 0 || place_operand(&ob, &scratch, st) != 0) return -1;
+  CUtensorMap tm_a, tm_b;
+  const CUtensorMapDataType dt = map_type(type);
+  if (make_tmap_2d(&tm_a, dt, oa.data, oa.cols, rows, oa.pitch, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
+      make_tmap_2d(&tm_b, dt, ob.data, ob.cols, rows, ob.pitch, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) != 0)
+    return -1;
+  const int rc = with_type(dw_type, [&](auto o) { return launch<false, true, decltype(o)>(tm_a, tm_b, tm_b, p, st); });
+  return rc != 0 ? rc : return_scratch(cs, st);
 }
