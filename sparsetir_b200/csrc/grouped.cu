@@ -27,7 +27,8 @@ constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kStages = 6;
 constexpr int kAtom = 8 * 1024;       // 64 rows of 128 bytes
 constexpr int kThreads = 256;         // warp 0 loads, 1 issues, 2-3 clear the tails of groups (grad_w), 4-7 epilogue
-constexpr int kSmem = kStages * kStageBytes + 1024;
+constexpr int kStagedBytes = 32 * 64;  // 32 columns of 32 features on their way out, per epilogue warp
+constexpr int kSmem = kStages * kStageBytes + 4 * kStagedBytes + 1024;
 constexpr int kTmemCols = 2 * kN;
 constexpr int kBand = 8;              // column tiles of a group that are walked side by side
 
@@ -46,6 +47,7 @@ struct Args {
   int max_tiles;  // no valid indptr has more
   uint32_t idesc; // without N
   int a_mn;       // the left operand is contiguous along the features
+  int wide;       // rows of the result start at 16-byte addresses
 };
 
 // First and past the last row of group g, inside the array whatever the pointers say.
@@ -140,6 +142,107 @@ struct Walker {
   }
 };
 
+__device__ __forceinline__ float sum_of(uint32_t bits, bool i8) {
+  return i8 ? static_cast<float>(static_cast<int>(bits)) : __uint_as_float(bits);
+}
+template <class OutT> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return reinterpret_cast<const uint32_t&>(v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return reinterpret_cast<const uint32_t&>(v);
+}
+
+// n columns of 32 features from TMEM to rows of the result, 16-bit elements at 16-byte addresses.  The fragments of 8
+// columns and 32 features are transposed on their way to shared memory (rows of 32 features, pieces of 16 bytes exchanged
+// so that neither side collides) and leave as 16 bytes to a lane.  With a 2-byte store per lane and column the epilogue took
+// longer than the products of 2048-deep tiles: 576 us where this takes REPLACE (65,536 rows, 2048 -> 2048).
+template <bool I8, class OutT, class Take>
+__device__ __forceinline__ void store_halves(OutT* to, int pitch, int feats, int n, uint32_t taddr, unsigned char* staged,
+                                             const float* xs, const float* ws, int lane, Take&& take) {
+  float scale[4] = {};  // of features lane / 4 + 8 q
+  if constexpr (I8) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (lane / 4 + 8 * q < feats) scale[q] = ld_global(ws + lane / 4 + 8 * q);
+  }
+  const uint32_t put = tc05::smem_u32(staged);
+  const int get_row = lane >> 2, get_piece = lane & 3;
+  const unsigned char* get = staged + get_row * 64 + ((get_piece ^ ((get_row >> 1) & 3)) << 4);  // rows 8 apart alike
+  OutT* out = to + static_cast<size_t>(get_row) * pitch + get_piece * 8;
+  const bool live = get_piece * 8 < feats;
+  for (int c0 = 0; c0 < n; c0 += 32) {
+    uint32_t a[16], b[16];
+    tc05::tmem_ld16x32(taddr + c0, a);
+    tc05::tmem_ld16x32(taddr + (16u << 16) + c0, b);
+    float x[8];
+    if constexpr (I8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = c0 + 8 * (i >> 1) + 2 * (lane & 3) + (i & 1);
+        x[i] = c < n ? ld_global(xs + c) : 0.f;
+      }
+    }
+    tc05::tmem_ld_wait();
+    take(c0);
+    __syncwarp();  // the reads of the last 32 columns are over
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // columns 8 i .. 8 i + 7
+      uint32_t v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t* f = q < 2 ? a : b;
+        float lo = sum_of(f[4 * i + 2 * (q & 1)], I8), hi = sum_of(f[4 * i + 2 * (q & 1) + 1], I8);
+        if constexpr (I8) {
+          lo *= x[2 * i] * scale[q];
+          hi *= x[2 * i + 1] * scale[q];
+        }
+        v[q] = pack2<OutT>(lo, hi);
+      }
+      const int r = 8 * i + (lane & 7), q = lane >> 3;  // row and piece that this lane addresses
+      asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(put + r * 64 + ((q ^ ((r >> 1) & 3)) << 4)),
+                   "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                   : "memory");
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(get + 8 * i * 64);
+      if (live && c0 + 8 * i + get_row < n) *reinterpret_cast<uint4*>(out + static_cast<size_t>(c0 + 8 * i) * pitch) = v;
+    }
+  }
+}
+
+// The same for 32-bit elements and for rows at any address: lane = feature, a store per column.
+template <bool I8, class OutT, class Take>
+__device__ __forceinline__ void store_lanes(OutT* to, int pitch, int feats, int n, uint32_t taddr, const float* xs, const float* ws,
+                                            int lane, Take&& take) {
+  const bool live = lane < feats;
+  float scale = 0.f;
+  if constexpr (I8) {
+    if (live) scale = ld_global(ws + lane);
+  }
+  OutT* out = to + lane;
+  for (int c0 = 0; c0 < n; c0 += 32) {
+    float x = 0.f;
+    if constexpr (I8) {
+      if (c0 + lane < n) x = ld_global(xs + c0 + lane);
+    }
+    uint32_t r[32];
+    tc05::tmem_ld32(taddr + c0, r);
+    take(c0);
+#pragma unroll
+    for (int c = 0; c < 32; ++c) {
+      float v = sum_of(r[c], I8);
+      if constexpr (I8) v *= __shfl_sync(0xffffffffu, x, c) * scale;
+      if (live && c0 + c < n) *out = from_float<OutT>(v);
+      out += pitch;
+    }
+  }
+}
+
 template <bool I8, bool GRAD, class OutT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b64,
@@ -218,7 +321,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             tc05::mbar_arrive_expect_tx(&bar_tail[s], bytes);
           } else {
             bar = tc05::pair::at_first(&bar_full[s]);
-            tc05::pair::arrive_expect_tx(bar, bytes);
+            if (rank == 0) {  // for both blocks: an arrival from the other one at every step took 1 us each
+              tc05::mbar_arrive_expect_tx(&bar_full[s], 2 * bytes);
+              tc05::mbar_arrive(&bar_full[s]);
+            }
           }
           if constexpr (GRAD) {
             const int row = tile.row0 + k * kDepth;
@@ -263,7 +369,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         ok = tc05::pair::mbar_wait(&bar_acc_empty[buf], ((acc >> 1) & 1) ^ 1);
         tc05::fence_after_sync();
         for (int k = 0; k < steps && ok; ++k) {
-          if (!tc05::pair::mbar_wait(&bar_full[s], ph)) { ok = false; break; }
+          const bool cleared = GRAD && k == steps - 1 && tile.depth % kDepth != 0;  // by threads of both blocks
+          if (!(cleared ? tc05::pair::mbar_wait(&bar_full[s], ph) : tc05::mbar_wait(&bar_full[s], ph))) { ok = false; break; }
           tc05::fence_after_sync();
           const uint64_t da = tc05::desc_advance(da0, s * kStageBytes), db = tc05::desc_advance(db0, s * kStageBytes);
           const int left = tile.depth - k * kDepth;
@@ -308,51 +415,42 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       advance(steps);
     }
   } else if (warp >= 4) {
-    // ---- epilogue: lane = feature, columns 32 at a time
+    // ---- epilogue: a warp takes 32 features, columns 32 at a time
     int acc = 0;
-    OutT* const out = static_cast<OutT*>(p.out);
+    unsigned char* const staged = smem_raw + (base - tc05::smem_u32(smem_raw)) + kStages * kStageBytes + (warp & 3) * kStagedBytes;
     while (ok && walk.next(&tile)) {
-      const int feat = tile.feat0 + static_cast<int>(rank) * kM + (warp & 3) * 32 + lane;
-      const bool live = feat < p.features;
+      const int feat0 = tile.feat0 + static_cast<int>(rank) * kM + (warp & 3) * 32;
       size_t row = static_cast<size_t>(tile.col0);
       if constexpr (GRAD) row += static_cast<size_t>(tile.group) * p.columns;
-      OutT* to = out + row * p.features + feat;
+      OutT* const to = static_cast<OutT*>(p.out) + row * p.features + feat0;  // column 0, feature 0 of the warp's
+      const int feats = p.features - feat0;  // live ones of the warp's, may be <= 0 or > 32
       if (GRAD && tile.depth == 0) {
-        for (int c = 0; c < tile.n; ++c)
-          if (live) to[static_cast<size_t>(c) * p.features] = from_float<OutT>(0.f);
+        if (lane < feats)
+          for (int c = 0; c < tile.n; ++c) to[static_cast<size_t>(c) * p.features + lane] = from_float<OutT>(0.f);
         continue;
-      }
-      float ws = 0.f;
-      if constexpr (I8) {
-        if (live) ws = ld_global(p.w_scale + static_cast<size_t>(tile.group) * p.features + feat);
       }
       const int buf = acc & 1;
       ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_acc_full[buf], (acc >> 1) & 1));
       if (!ok) break;
       tc05::fence_after_sync();
       const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + buf * kN;
-      for (int c0 = 0; c0 < tile.n; c0 += 32) {
-        float xs = 0.f;
-        if constexpr (I8) {
-          if (c0 + lane < tile.n) xs = ld_global(p.x_scale + tile.col0 + c0 + lane);
-        }
-        uint32_t r[32];
-        tc05::tmem_ld32(taddr + c0, r);
-        if (c0 + 32 >= tile.n) {  // the result is in registers: the accumulator may be written again
-          tc05::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) tc05::pair::arrive(tc05::pair::at_first(&bar_acc_empty[buf]));
-        }
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          float v;
-          if constexpr (I8)
-            v = static_cast<float>(static_cast<int>(r[c])) * (__shfl_sync(0xffffffffu, xs, c) * ws);
-          else
-            v = __uint_as_float(r[c]);
-          if (live && c0 + c < tile.n) to[static_cast<size_t>(c0 + c) * p.features] = from_float<OutT>(v);
+      const uint32_t taken = tc05::pair::at_first(&bar_acc_empty[buf]);
+      auto take = [&](int c0) {  // the last columns are in registers: the accumulator may be written again
+        if (c0 + 32 < tile.n) return;
+        tc05::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc05::pair::arrive(taken);
+      };
+      const float* const xs = I8 ? p.x_scale + tile.col0 : nullptr;
+      const float* const ws = I8 ? p.w_scale + static_cast<size_t>(tile.group) * p.features + feat0 : nullptr;
+      bool done = false;
+      if constexpr (sizeof(OutT) == 2) {
+        if (p.wide) {
+          store_halves<I8>(to, p.features, feats, tile.n, taddr, staged, xs, ws, lane, take);
+          done = true;
         }
       }
+      if (!done) store_lanes<I8>(to, p.features, feats, tile.n, taddr, xs, ws, lane, take);
       ++acc;
     }
   }
@@ -472,6 +570,10 @@ CUtensorMapDataType map_type(int type) {
 }
 uint32_t map_format(int type) { return type == SPARSETIR_F16 ? tc05::kFmtF16 : tc05::kFmtBF16; }
 
+bool wide_rows(const void* out, int type, int features) {
+  return type != SPARSETIR_F32 && aligned16(out) && features % 8 == 0;
+}
+
 // y = x * W: `type` of the elements of x and W, -1 for 8-bit integers
 int product(const char* fn, const void* x, const void* w, int type, void* y, int y_type, const float* xs, const float* ws,
             const int32_t* indptr, int rows, int groups, int fi, int fo, bool out_in, int device_id, cudaStream_t st) {
@@ -487,6 +589,7 @@ int product(const char* fn, const void* x, const void* w, int type, void* y, int
   p.k = fi;
   p.features = fo;
   p.a_mn = out_in ? 0 : 1;
+  p.wide = wide_rows(y, y_type, fo);
   p.idesc = i8 ? tc05::instr_desc_i8(2 * kM, 0) : tc05::instr_desc(map_format(type), 2 * kM, 0, p.a_mn, 0);
   if (set_tiles(fn, &p, rows / kN + static_cast<long long>(std::min(groups, rows))) != 0) return -1;
   Operand ox{x, rows, fi, size}, ow{w, static_cast<long long>(groups) * (out_in ? fo : fi), out_in ? fi : fo, size};
@@ -581,6 +684,7 @@ extern "C" int sparsetir_grouped_mm_grad_w_raw(const void* x, const void* dy, in
   p.features = out_in ? feat_in : feat_out;
   p.columns = out_in ? feat_out : feat_in;
   p.nt = ceil_div(p.columns, kN);
+  p.wide = wide_rows(dw, dw_type, p.features);
   p.idesc = tc05::instr_desc(map_format(type), 2 * kM, 0, 1, 1);
   if (set_tiles(fn, &p, static_cast<long long>(num_groups) * p.nt) != 0) return -1;
   Operand oa{out_in ? x : dy, rows, p.features, 2}, ob{out_in ? dy : x, rows, p.columns, 2};
