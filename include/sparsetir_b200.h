@@ -534,6 +534,8 @@ SPARSETIR_API int sparsetir_moe_route_grad_raw(const void* logits, int logits_ty
                                                const int32_t* experts, const float* d_gates, void* d_logits,
                                                int tokens, int num_experts, int top_k, int flags, int device_id,
                                                void* stream);
+/* Scratch bytes of sparsetir_moe_route: the experts' counts in the shares of a large batch. */
+SPARSETIR_API int sparsetir_moe_route_workspace(int tokens, int num_experts, size_t* scratch_bytes);
 /* rows: how many z, q, dz have; a slot outside of [0, rows) is taken as -1 */
 SPARSETIR_API int sparsetir_moe_dispatch_raw(const void* x, const int32_t* slots, void* z, int type, int tokens,
                                              int rows, int feat, int top_k, int device_id, void* stream);
@@ -546,6 +548,10 @@ SPARSETIR_API int sparsetir_moe_combine_raw(const void* z, int z_type, const int
 SPARSETIR_API int sparsetir_moe_combine_grad_raw(const void* dy, const void* z, int type, const int32_t* slots,
                                                  const float* gates, void* dz, float* d_gates, int tokens, int rows,
                                                  int feat, int top_k, int device_id, void* stream);
+/* Scratch bytes of the grouped products at most: copies of operands of element_bytes (1 or 2) whose rows do not start at
+ * 16-byte addresses.  Operands at aligned addresses with rows of a multiple of 16 bytes need none. */
+SPARSETIR_API int sparsetir_grouped_mm_workspace(int rows, int num_groups, int feat_in, int feat_out, int element_bytes,
+                                                 int flags, size_t* scratch_bytes);
 /* rows: how many x and y have; row pointers outside of [0, rows] are taken as the nearer bound */
 SPARSETIR_API int sparsetir_grouped_mm_raw(const void* x, const void* w, int type, void* y, int y_type,
                                            const int32_t* indptr, int rows, int num_groups, int feat_in, int feat_out,

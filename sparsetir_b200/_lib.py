@@ -139,6 +139,8 @@ PLAIN_SYMBOLS = {
     "sparsetir_rgms_ell3d_f16_raw": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "sparsetir_sparse_conv_f16_raw": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "sparsetir_rgms_noalloc": (_i, [_vp] * 8 + [_i] * 7 + [_vp]),
+    "sparsetir_moe_route_workspace": (_i, [_i, _i, ctypes.POINTER(ctypes.c_size_t)]),
+    "sparsetir_grouped_mm_workspace": (_i, [_i] * 6 + [ctypes.POINTER(ctypes.c_size_t)]),
     "sparsetir_moe_route_raw": (_i, [_vp, _i] + [_vp] * 4 + [_i] * 5 + [_vp]),
     "sparsetir_moe_route_grad_raw": (_i, [_vp, _i] + [_vp] * 4 + [_i] * 5 + [_vp]),
     "sparsetir_moe_dispatch_raw": (_i, [_vp] * 3 + [_i] * 6 + [_vp]),

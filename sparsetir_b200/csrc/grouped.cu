@@ -57,13 +57,6 @@ __device__ __forceinline__ void group_rows(const Args& p, int g, int* first, int
   *last = max(min(ld_global(p.indptr + g + 1), p.rows), *first);
 }
 
-// A group of m rows in equal tiles of a multiple of 32 up to 256.
-__device__ __forceinline__ void split(int m, int* size, int* count) {
-  const int n = (m + kN - 1) / kN;
-  *size = n == 0 ? kN : ((m + n - 1) / n + 31) & ~31;
-  *count = (m + *size - 1) / *size;
-}
-
 struct Tile {
   int group, feat0;
   int col0, n, n_mma;   // columns: first, how many there are, rounded up to 32
@@ -102,9 +95,7 @@ struct Walker {
         first = last = 0;
         if (base + lane < p.groups) {
           group_rows(p, base + lane, &first, &last);
-          int size, count;
-          split(last - first, &size, &count);
-          mine = static_cast<unsigned>(min(static_cast<long long>(count) * p.mt, 1ll << 30));
+          mine = static_cast<unsigned>(min(static_cast<long long>((last - first + kN - 1) / kN) * p.mt, 1ll << 30));
         }
         upto = mine;
 #pragma unroll
@@ -118,12 +109,10 @@ struct Walker {
       const int src = __ffs(__ballot_sync(0xffffffffu, upto > static_cast<unsigned>(t))) - 1;
       const unsigned prev = __shfl_sync(0xffffffffu, upto, max(src - 1, 0));
       const int f = __shfl_sync(0xffffffffu, first, src), l = __shfl_sync(0xffffffffu, last, src);
-      int size, count;
-      split(l - f, &size, &count);
-      place(t - static_cast<int>(src == 0 ? before : prev), count, out);
+      place(t - static_cast<int>(src == 0 ? before : prev), (l - f + kN - 1) / kN, out);
       out->group = base + src;
-      out->col0 = f + out->col0 * size;
-      out->n = min(size, l - out->col0);
+      out->col0 = f + out->col0 * kN;
+      out->n = min(kN, l - out->col0);
       out->row0 = 0;
       out->depth = p.k;
     }
@@ -700,4 +689,16 @@ extern "C" int sparsetir_grouped_mm_grad_w_raw(const void* x, const void* dy, in
     return -1;
   const int rc = with_type(dw_type, [&](auto o) { return launch<false, true, decltype(o)>(tm_a, tm_b, tm_b, p, st); });
   return rc != 0 ? rc : return_scratch(cs, st);
+}
+
+extern "C" int sparsetir_grouped_mm_workspace(int rows, int num_groups, int feat_in, int feat_out, int element_bytes, int flags,
+                                              size_t* scratch_bytes) {
+  const char* fn = "sparsetir_grouped_mm_workspace";
+  if (check_groups(fn, nullptr, rows, std::min(num_groups, 1), feat_in, feat_out, flags) != 0) return -1;
+  if ((element_bytes != 1 && element_bytes != 2) || !scratch_bytes) return fail("%s: bad argument", fn);
+  auto copy = [&](long long n, int cols) -> size_t { return (Operand{nullptr, n, cols, element_bytes}.padded() * n + 255) / 256 * 256; };
+  const bool out_in = (flags & SPARSETIR_GROUPED_W_OUT_IN) != 0;
+  const size_t w = copy(static_cast<long long>(num_groups) * (out_in ? feat_out : feat_in), out_in ? feat_in : feat_out);
+  *scratch_bytes = copy(rows, feat_in) + std::max(w, copy(rows, feat_out));
+  return 0;
 }

@@ -47,89 +47,166 @@ __device__ __forceinline__ void load_keys(const T* row, int num_experts, int lan
   }
 }
 
-// One warp per token.  p[i] = exp(z[i] - max z) / sum; the top_k largest are found one after the other, each by a
-// maximum over the keys of the warp and the lowest index that has it.
-template <class T, int R>
-__global__ void __launch_bounds__(kWarps * 32)
-choose_kernel(const T* logits, float* gates, int32_t* experts, int tokens, int num_experts, int top_k, int renormalize) {
-  chain_wait();
-  const int lane = threadIdx.x & 31;
-  const int t = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (t >= tokens) return;
-  uint32_t key[R];
-  load_keys<T, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, lane, key);
-  uint32_t most = 0u;
+// The router is two launches, or one where a single block has all tokens.  Each block of the first chooses for its share of
+// the tokens, a warp per token, and counts the pairs of every expert; each block of the second sums the counts of all
+// shares (they are few: 148 at most) and places its share's pairs.  Nothing depends on the order in which blocks run.
+constexpr int kRouteThreads = 1024, kRouteWarps = kRouteThreads / 32;
+constexpr int kRouteTokens = 128;  // of a share, more where there would be over 148 of them
+
+struct PlaceShared {
+  int next[SPARSETIR_MOE_MAX_EXPERTS];  // where the share's next pair of every expert goes
+  unsigned char count[kRouteWarps][SPARSETIR_MOE_MAX_EXPERTS];
+  int sums[kRouteWarps];
+};
+
+// next[e] += the sum of total[0 .. e-1], one expert to a thread; the sum of all is returned.
+__device__ __forceinline__ int add_bases(PlaceShared& s, int total) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int upto = total;
 #pragma unroll
-  for (int r = 0; r < R; ++r) most = max(most, key[r]);
-  const uint32_t top = __reduce_max_sync(kFull, most);
-  float sum = 0.f;
-#pragma unroll
-  for (int r = 0; r < R; ++r) sum += over_top(key[r], top);
-  sum = warp_sum(sum);
-  int expert = -1;     // of choice `lane`
-  float value = 0.f;   // exp(z - top) of it
-  for (int j = 0; j < top_k; ++j) {
-    uint32_t best = 0u;
-    int at = 0x7fffffff;
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (key[r] > best) { best = key[r]; at = lane + 32 * r; }
-    const uint32_t found = __reduce_max_sync(kFull, best);
-    if (found == 0u) break;
-    const int who = __reduce_min_sync(kFull, best == found ? at : 0x7fffffff);
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (lane + 32 * r == who) key[r] = 0u;
-    if (lane == j) {
-      expert = who;
-      value = over_top(found, top);
-    }
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(kFull, upto, o);
+    if (lane >= o) upto += up;
   }
-  if (renormalize) sum = warp_sum(value);
-  if (lane < top_k) {
-    const size_t p = static_cast<size_t>(t) * top_k + lane;
-    experts[p] = expert;
-    gates[p] = expert < 0 ? 0.f : value / sum;
+  if (lane == 31) s.sums[warp] = upto;
+  __syncthreads();
+  int before = 0, all = s.sums[lane];
+  for (int w = 0; w < warp; ++w) before += s.sums[w];
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) all += __shfl_xor_sync(kFull, all, o);
+  s.next[tid] += before + upto - total;
+  return all;
+}
+
+// Pairs [first, last) in order: the place of each is next of its expert plus the pairs of that expert ahead of it, in its
+// warp by a match, in the warps ahead by their counts.
+__device__ __forceinline__ void place_pairs(PlaceShared& s, const int32_t* experts, int32_t* slots, int first, int last,
+                                            int num_experts) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int p0 = first; p0 < last; p0 += kRouteThreads) {
+    const int p = p0 + tid;
+    const int e = p < last ? ld_global(experts + p) : -1;
+    for (int i = lane; i * 4 < num_experts; i += 32) reinterpret_cast<uint32_t*>(s.count[warp])[i] = 0u;
+    __syncwarp();
+    const unsigned same = __match_any_sync(kFull, e);
+    const int ahead = __popc(same & ((1u << lane) - 1u));
+    if (e >= 0 && ahead == 0) s.count[warp][e] = static_cast<unsigned char>(__popc(same));
+    __syncthreads();
+    if (p < last) {
+      int slot = -1;
+      if (e >= 0) {
+        slot = s.next[e] + ahead;
+        for (int w = 0; w < warp; ++w) slot += s.count[w][e];
+      }
+      slots[p] = slot;
+    }
+    __syncthreads();
+    if (p0 + kRouteThreads < last && tid < num_experts) {
+      int sum = 0;
+      for (int w = 0; w < kRouteWarps; ++w) sum += s.count[w][tid];
+      s.next[tid] += sum;
+    }
+    __syncthreads();
   }
 }
 
-// Stable counting sort of the pairs by expert, in one block.
-__global__ void __launch_bounds__(1024)
-place_kernel(const int32_t* experts, int32_t* slots, int32_t* indptr, int pairs, int num_experts) {
-  __shared__ int next[SPARSETIR_MOE_MAX_EXPERTS];
+// p[i] = exp(z[i] - max z) / sum; the top_k largest are found one after the other, each by a maximum over the keys of the
+// warp and the lowest index that has it.
+template <class T, int R>
+__global__ void __launch_bounds__(kRouteThreads)
+choose_kernel(const T* logits, float* gates, int32_t* experts, int32_t* slots, int32_t* indptr, int32_t* counts, int tokens,
+              int share, int num_experts, int top_k, int renormalize) {
+  __shared__ PlaceShared s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  s.next[tid] = 0;
   chain_wait();
-  const int tid = threadIdx.x, lane = tid & 31;
-  next[tid] = 0;
   __syncthreads();
-  for (int p = tid; p < pairs; p += 1024) {
-    const int e = ld_global(experts + p);
-    if (e >= 0) atomicAdd(&next[e], 1);
-  }
-  __syncthreads();
-  if (tid == 0) {
-    int sum = 0;
-    for (int e = 0; e < num_experts; ++e) {
-      indptr[e] = sum;
-      const int n = next[e];
-      next[e] = sum;
-      sum += n;
+  const int t0 = blockIdx.x * share, t1 = t0 + min(share, tokens - t0);
+  for (int t = t0 + warp; t < t1; t += kRouteWarps) {
+    uint32_t key[R];
+    load_keys<T, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, lane, key);
+    uint32_t most = 0u;
+#pragma unroll
+    for (int r = 0; r < R; ++r) most = max(most, key[r]);
+    const uint32_t top = __reduce_max_sync(kFull, most);
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) sum += over_top(key[r], top);
+    sum = warp_sum(sum);
+    int expert = -1;     // of choice `lane`
+    float value = 0.f;   // exp(z - top) of it
+    for (int j = 0; j < top_k; ++j) {
+      uint32_t best = 0u;
+      int at = 0x7fffffff;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (key[r] > best) { best = key[r]; at = lane + 32 * r; }
+      const uint32_t found = __reduce_max_sync(kFull, best);
+      if (found == 0u) break;
+      const int who = __reduce_min_sync(kFull, best == found ? at : 0x7fffffff);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (lane + 32 * r == who) key[r] = 0u;
+      if (lane == j) {
+        expert = who;
+        value = over_top(found, top);
+      }
     }
-    indptr[num_experts] = sum;
+    if (renormalize) sum = warp_sum(value);
+    if (lane < top_k) {
+      const size_t p = static_cast<size_t>(t) * top_k + lane;
+      experts[p] = expert;
+      gates[p] = expert < 0 ? 0.f : value / sum;
+      if (expert >= 0) atomicAdd(&s.next[expert], 1);
+    }
   }
   __syncthreads();
-  if (tid >= 32) return;
-  for (int p0 = 0; p0 < pairs; p0 += 32) {
-    const int p = p0 + lane;
-    const int e = p < pairs ? ld_global(experts + p) : -1;
-    const unsigned same = __match_any_sync(kFull, e);
-    const int before = __popc(same & ((1u << lane) - 1u));
-    int slot = -1;
-    if (e >= 0) slot = next[e] + before;
-    __syncwarp();
-    if (e >= 0 && before == 0) next[e] += __popc(same);
-    __syncwarp();
-    if (p < pairs) slots[p] = slot;
+  const int mine = s.next[tid];
+  if (counts != nullptr) {
+    if (tid < num_experts) counts[static_cast<size_t>(blockIdx.x) * num_experts + tid] = mine;
+    return;
   }
+  s.next[tid] = 0;
+  const int all = add_bases(s, mine);
+  __syncthreads();
+  if (tid < num_experts) indptr[tid] = s.next[tid];
+  if (tid == 0) indptr[num_experts] = all;
+  place_pairs(s, experts, slots, 0, tokens * top_k, num_experts);
+}
+
+__global__ void __launch_bounds__(kRouteThreads)
+place_kernel(const int32_t* experts, int32_t* slots, int32_t* indptr, const int32_t* counts, int tokens, int share, int num_experts,
+             int top_k) {
+  __shared__ PlaceShared s;
+  __shared__ int total[SPARSETIR_MOE_MAX_EXPERTS];
+  const int tid = threadIdx.x;
+  s.next[tid] = 0;
+  total[tid] = 0;
+  chain_wait();
+  __syncthreads();
+  // of every expert: the pairs of the shares ahead, and of all; several threads share an expert's column of counts
+  const int shares = gridDim.x, block = blockIdx.x;
+  const int rows = kRouteThreads / num_experts, row = tid / num_experts, e = tid - row * num_experts;
+  if (row < rows) {
+    int before = 0, all = 0;
+#pragma unroll 8
+    for (int b = row; b < shares; b += rows) {
+      const int c = ld_global(counts + static_cast<size_t>(b) * num_experts + e);
+      all += c;
+      before += b < block ? c : 0;
+    }
+    atomicAdd(&s.next[e], before);
+    atomicAdd(&total[e], all);
+  }
+  __syncthreads();
+  const int all = add_bases(s, total[tid]);
+  __syncthreads();
+  if (block == 0) {
+    if (tid < num_experts) indptr[tid] = s.next[tid];
+    if (tid == 0) indptr[num_experts] = all;
+  }
+  const int t0 = block * share, t1 = t0 + min(share, tokens - t0);
+  place_pairs(s, experts, slots, t0 * top_k, t1 * top_k, num_experts);
 }
 
 template <class T, int R>
@@ -453,9 +530,12 @@ int check_route(const char* fn, int type, int tokens, int num_experts, int top_k
   if (num_experts < top_k || num_experts > SPARSETIR_MOE_MAX_EXPERTS)
     return fail("%s: num_experts = %d is not in [top_k, %d]", fn, num_experts, SPARSETIR_MOE_MAX_EXPERTS);
   if ((flags & ~SPARSETIR_MOE_RENORMALIZE) != 0) return fail("%s: unknown flags %d", fn, flags);
-  if (static_cast<long long>(tokens) * top_k > INT32_MAX) return fail("%s: too many pairs for 32-bit indices", fn);
+  if (static_cast<long long>(tokens) * top_k > INT32_MAX - 2 * kRouteThreads) return fail("%s: too many pairs for 32-bit indices", fn);
   return 0;
 }
+
+int route_share(int tokens) { return std::max(kRouteTokens, ceil_div(tokens, kNumSMs)); }
+size_t route_counts(int shares, int num_experts) { return static_cast<size_t>(shares) * num_experts * sizeof(int32_t); }
 
 }  // namespace
 }  // namespace sptir
@@ -470,20 +550,30 @@ extern "C" int sparsetir_moe_route_raw(const void* logits, int logits_type, floa
   if (!indptr || (tokens > 0 && (!logits || !gates || !experts || !slots))) return fail("%s: null pointer argument", fn);
   if (use_device(device_id) != 0) return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (tokens > 0) {
-    const int rc = with_type(logits_type, [&](auto t) {
-      using T = decltype(t);
-      return with_lane_share(num_experts, [&](auto r) {
-        launch_chained(choose_kernel<T, r.value>, ceil_div(tokens, kWarps), kWarps * 32, 0, st, static_cast<const T*>(logits),
-                       gates, experts, tokens, num_experts, top_k, flags & SPARSETIR_MOE_RENORMALIZE);
-        SPTIR_LAUNCH_OK("choose_kernel");
-        return 0;
-      });
+  const int share = route_share(tokens), shares = std::max(1, ceil_div(tokens, share));
+  CallScratch cs;
+  if (shares > 1 && take_scratch(device_id, st, route_counts(shares, num_experts), 0, &cs) != 0) return -1;
+  int32_t* counts = reinterpret_cast<int32_t*>(cs.scratch);
+  const int rc = with_type(logits_type, [&](auto t) {
+    using T = decltype(t);
+    return with_lane_share(num_experts, [&](auto r) {
+      launch_chained(choose_kernel<T, r.value>, shares, kRouteThreads, 0, st, static_cast<const T*>(logits), gates, experts, slots,
+                     indptr, counts, tokens, share, num_experts, top_k, flags & SPARSETIR_MOE_RENORMALIZE);
+      SPTIR_LAUNCH_OK("choose_kernel");
+      return 0;
     });
-    if (rc != 0) return rc;
-  }
-  launch_chained(place_kernel, 1, 1024, 0, st, experts, slots, indptr, tokens * top_k, num_experts);
+  });
+  if (rc != 0 || shares == 1) return rc;
+  launch_chained(place_kernel, shares, kRouteThreads, 0, st, experts, slots, indptr, counts, tokens, share, num_experts, top_k);
   SPTIR_LAUNCH_OK("place_kernel");
+  return return_scratch(cs, st);
+}
+
+extern "C" int sparsetir_moe_route_workspace(int tokens, int num_experts, size_t* scratch_bytes) {
+  if (tokens < 0 || num_experts < 1 || num_experts > SPARSETIR_MOE_MAX_EXPERTS || !scratch_bytes)
+    return fail("sparsetir_moe_route_workspace: bad argument");
+  const int shares = ceil_div(tokens, route_share(tokens));
+  *scratch_bytes = shares > 1 ? route_counts(shares, num_experts) : 0;
   return 0;
 }
 

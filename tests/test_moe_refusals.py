@@ -138,3 +138,23 @@ def test_plain_pointer_forms():
     raw("a row per token", "sparsetir_moe_dispatch_i8_raw", None, 1, None, None, None, 4, 5, 8, 1, 0, None)
     raw("num_experts = 3", "sparsetir_moe_route_raw", None, 0, None, None, None, None, 4, 3, 4, 0, 0, None)
     assert lib.sparsetir_grouped_mm_raw(None, None, 1, None, 1, None, 0, 1, 8, 8, 0, 0, None) == 0  # no rows: nothing to do
+
+
+def test_scratch_queries():
+    import ctypes
+
+    out = ctypes.c_size_t(99)
+
+    def ask(name, *sizes):
+        assert getattr(L.load(), name)(*sizes, ctypes.byref(out)) == 0, L.last_error()
+        return out.value
+
+    assert ask("sparsetir_moe_route_workspace", 0, 8) == ask("sparsetir_moe_route_workspace", 128, 1024) == 0
+    assert ask("sparsetir_moe_route_workspace", 129, 8) == 2 * 8 * 4
+    assert ask("sparsetir_moe_route_workspace", 2 ** 31 - 1, 1024) <= 148 * 1024 * 4
+    # copies at rows of a multiple of 16 bytes
+    assert ask("sparsetir_grouped_mm_workspace", 100, 4, 9, 16, 2, 1) == 100 * 32 + 128 + max(4 * 16 * 32, 100 * 32 + 128)
+    assert ask("sparsetir_grouped_mm_workspace", 0, 4, 17, 16, 1, 0) == 4 * 17 * 16 + 192
+    for name, sizes in (("sparsetir_moe_route_workspace", (-1, 8)), ("sparsetir_moe_route_workspace", (4, 0)),
+                        ("sparsetir_grouped_mm_workspace", (4, 4, 0, 8, 2, 0)), ("sparsetir_grouped_mm_workspace", (4, 4, 8, 8, 3, 0))):
+        assert getattr(L.load(), name)(*sizes, ctypes.byref(out)) == -1
