@@ -21,16 +21,20 @@ namespace sptir {
 namespace {
 
 constexpr int kM = 128;               // features per block
-constexpr int kN = 256;               // columns per pair
-constexpr int kHalfBytes = 16 * 1024; // one operand of a stage: 128 rows of 128 bytes
-constexpr int kStageBytes = 2 * kHalfBytes;
-constexpr int kStages = 6;
+constexpr int kABytes = 16 * 1024;    // left operand of a stage: 128 rows of 128 bytes
 constexpr int kAtom = 8 * 1024;       // 64 rows of 128 bytes
 constexpr int kThreads = 256;         // warp 0 loads, 1 issues, 2-3 clear the tails of groups (grad_w), 4-7 epilogue
-constexpr int kStagedBytes = 32 * 64;  // 32 columns of 32 features on their way out, per epilogue warp
-constexpr int kSmem = kStages * kStageBytes + 4 * kStagedBytes + 1024;
-constexpr int kTmemCols = 2 * kN;
+constexpr int kStagedBytes = 32 * 64; // 32 columns of 32 features on their way out, per epilogue warp
 constexpr int kBand = 8;              // column tiles of a group that are walked side by side
+
+// Columns of a tile, and what follows from them.
+template <int N> struct Shape {
+  static constexpr int kBytes = kABytes + N / 2 * 128;  // of a stage
+  static constexpr int kStages = N == 256 ? 6 : 4;
+  static constexpr int kBlocks = N == 256 ? 1 : 2;      // per SM
+  static constexpr int kTmemCols = 2 * N;               // two accumulators
+  static constexpr int kSmem = kStages * kBytes + 4 * kStagedBytes + 1024;
+};
 
 __device__ unsigned int g_grouped_timeouts = 0;
 
@@ -43,8 +47,11 @@ struct Args {
   int k;          // depth of the product; grad_w: unused
   int features;   // contiguous in the result
   int columns;    // grad_w: rows of each dW
-  int mt, nt;     // tiles of 256 features; grad_w: of 256 columns
-  int max_tiles;  // no valid indptr has more
+  int mt, nt;     // tiles of 256 features; grad_w: column tiles
+  int max_tiles;  // no valid indptr has more; times splits
+  int splits;     // units that share the depth of a tile, each with sums of its own in `parts`
+  void* parts;    // [splits][rows of the result][features], 32 bits each
+  long long part; // elements of one split's
   uint32_t idesc; // without N
   int a_mn;       // the left operand is contiguous along the features
   int wide;       // rows of the result start at 16-byte addresses
@@ -59,22 +66,25 @@ __device__ __forceinline__ void group_rows(const Args& p, int g, int* first, int
 
 struct Tile {
   int group, feat0;
-  int col0, n, n_mma;   // columns: first, how many there are, rounded up to 32
-  int row0, depth;      // grad_w: rows of the group
+  int col0, n, n_mma;      // columns: first, how many there are, rounded up to 32
+  int row0, depth;         // depth: of K; grad_w: the rows of the group, from row0 on
+  int split, step0, steps; // the unit's share of the depth
 };
 
-// The tiles of one pair: t, t + pairs, ...  All lanes of a warp call next() together; lane l holds the prefix of tile counts
+// The units of one pair: `pair`, pair + pairs, ...  All lanes of a warp call next() together; lane l holds the prefix of tile counts
 // of group base + l.  Sums stop at 2^30: wild pointers give tiles inside the arrays, and no more than max_tiles of them.
-template <bool GRAD>
+template <bool GRAD, int kN, int kDepth>
 struct Walker {
   const Args& p;
-  int t, step, base = -32;
+  int unit, step, base = -32;
   unsigned before = 0, upto = 0;  // tiles ahead of the group of lane 0, and up to the group of this lane
   unsigned all = 0;               // up to the last of the 32
   int first = 0, last = 0;
-  __device__ __forceinline__ Walker(const Args& a, int pair, int pairs) : p(a), t(pair), step(pairs) {}
+  __device__ __forceinline__ Walker(const Args& a, int pair, int pairs) : p(a), unit(pair), step(pairs) {}
   __device__ __forceinline__ bool next(Tile* out) {
-    if (t >= p.max_tiles) return false;
+    if (unit >= p.max_tiles) return false;
+    const int t = unit / p.splits;
+    out->split = unit - t * p.splits;
     if constexpr (GRAD) {
       const int per = p.mt * p.nt, g = t / per, r = t - g * per;
       int f, l;
@@ -117,7 +127,10 @@ struct Walker {
       out->depth = p.k;
     }
     out->n_mma = (out->n + 31) & ~31;
-    t += step;
+    const int steps = (out->depth + kDepth - 1) / kDepth, share = (steps + p.splits - 1) / p.splits;
+    out->step0 = min(out->split * share, steps);
+    out->steps = min(share, steps - out->step0);
+    unit += step;
     return true;
   }
   // Tile r of a group with `cols` column tiles: bands of kBand column tiles, in a band one column tile after the other.
@@ -232,12 +245,13 @@ __device__ __forceinline__ void store_lanes(OutT* to, int pitch, int feats, int 
   }
 }
 
-template <bool I8, bool GRAD, class OutT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+template <bool I8, bool GRAD, class OutT, int kN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Shape<kN>::kBlocks)
 grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b64,
                const __grid_constant__ CUtensorMap tm_b16, const __grid_constant__ Args p) {
   constexpr int kDepth = I8 ? 128 : 64;  // of K per stage
   constexpr int kInstr = I8 ? 32 : 16;   // of K per instruction
+  constexpr int kStages = Shape<kN>::kStages, kStageBytes = Shape<kN>::kBytes, kTmemCols = Shape<kN>::kTmemCols;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kStages];   // rank 0: both blocks' operands are there
   __shared__ __align__(8) uint64_t bar_empty[kStages];  // the tensor core has read the stage
@@ -288,7 +302,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     phase ^= static_cast<uint32_t>(q / kStages) & 1u;
     stage = q % kStages;
   };
-  Walker<GRAD> walk(p, pair, pairs);
+  Walker<GRAD, kN, kDepth> walk(p, pair, pairs);
   Tile tile;
 
   if (warp == 0) {
@@ -296,16 +310,15 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     while (ok && walk.next(&tile)) {
       const int half = tile.n_mma / 2, units = half / 16;
       const int feat = tile.feat0 + static_cast<int>(rank) * kM, col = tile.col0 + static_cast<int>(rank) * half;
-      const int steps = (tile.depth + kDepth - 1) / kDepth;
       if (tc05::elect_one()) {
-        const uint32_t bytes = kHalfBytes + (GRAD ? (half > 64 ? 2 : 1) * kAtom : units * 2048);
+        const uint32_t bytes = kABytes + (GRAD ? (half > 64 ? 2 : 1) * kAtom : units * 2048);
         int s = stage;
         uint32_t ph = phase;
-        for (int k = 0; k < steps; ++k) {
+        for (int k = tile.step0; k < tile.step0 + tile.steps; ++k) {
           if (!tc05::mbar_wait(&bar_empty[s], ph ^ 1u)) { ok = false; break; }
           const uint32_t st = base + s * kStageBytes;
           uint32_t bar;
-          if (GRAD && k == steps - 1 && tile.depth % kDepth != 0) {
+          if (GRAD && (k + 1) * kDepth > tile.depth) {
             bar = tc05::smem_u32(&bar_tail[s]);
             tc05::mbar_arrive_expect_tx(&bar_tail[s], bytes);
           } else {
@@ -319,8 +332,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             const int row = tile.row0 + k * kDepth;
             tc05::pair::tma_load_2d(st, &tm_a, feat, row, bar);
             tc05::pair::tma_load_2d(st + kAtom, &tm_a, feat + 64, row, bar);
-            tc05::pair::tma_load_2d(st + kHalfBytes, &tm_b64, col, row, bar);
-            if (half > 64) tc05::pair::tma_load_2d(st + kHalfBytes + kAtom, &tm_b64, col + 64, row, bar);
+            tc05::pair::tma_load_2d(st + kABytes, &tm_b64, col, row, bar);
+            if (half > 64) tc05::pair::tma_load_2d(st + kABytes + kAtom, &tm_b64, col + 64, row, bar);
           } else {
             if (p.a_mn) {
               tc05::pair::tma_load_3d(st, &tm_a, feat, k * kDepth, tile.group, bar);
@@ -329,15 +342,15 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
               tc05::pair::tma_load_3d(st, &tm_a, k * kDepth, feat, tile.group, bar);
             }
             int u = 0;
-            for (; u + 4 <= units; u += 4) tc05::pair::tma_load_2d(st + kHalfBytes + u * 2048, &tm_b64, k * kDepth, col + u * 16, bar);
-            for (; u < units; ++u) tc05::pair::tma_load_2d(st + kHalfBytes + u * 2048, &tm_b16, k * kDepth, col + u * 16, bar);
+            for (; u + 4 <= units; u += 4) tc05::pair::tma_load_2d(st + kABytes + u * 2048, &tm_b64, k * kDepth, col + u * 16, bar);
+            for (; u < units; ++u) tc05::pair::tma_load_2d(st + kABytes + u * 2048, &tm_b16, k * kDepth, col + u * 16, bar);
           }
           ++armed;
           if (++s == kStages) { s = 0; ph ^= 1u; }
         }
       }
       ok = __all_sync(0xffffffffu, ok);
-      advance(steps);
+      advance(tile.steps);
     }
   } else if (warp == 1) {
     // ---- MMAs of both blocks, from rank 0: M = 256 features, N = the tile's columns
@@ -345,10 +358,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     const bool a_mn = GRAD || p.a_mn != 0;
     const uint32_t a_step = a_mn ? 2048u : 32u, b_step = GRAD ? 2048u : 32u;
     const uint64_t da0 = tc05::smem_desc_swizzled(base, a_mn ? kAtom : 0, 1024, tc05::kSwizzle128B);
-    const uint64_t db0 = tc05::smem_desc_swizzled(base + kHalfBytes, GRAD ? kAtom : 0, 1024, tc05::kSwizzle128B);
+    const uint64_t db0 = tc05::smem_desc_swizzled(base + kABytes, GRAD ? kAtom : 0, 1024, tc05::kSwizzle128B);
     while (rank == 0 && ok && walk.next(&tile)) {
-      const int steps = (tile.depth + kDepth - 1) / kDepth;
-      if (steps == 0) continue;
+      if (tile.steps == 0) continue;
       if (tc05::elect_one()) {
         const int buf = acc & 1;
         const uint32_t idesc = p.idesc | static_cast<uint32_t>(tile.n_mma >> 3) << 17;
@@ -357,8 +369,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         uint32_t ph = phase;
         ok = tc05::pair::mbar_wait(&bar_acc_empty[buf], ((acc >> 1) & 1) ^ 1);
         tc05::fence_after_sync();
-        for (int k = 0; k < steps && ok; ++k) {
-          const bool cleared = GRAD && k == steps - 1 && tile.depth % kDepth != 0;  // by threads of both blocks
+        for (int k = tile.step0; k < tile.step0 + tile.steps && ok; ++k) {
+          const bool cleared = GRAD && (k + 1) * kDepth > tile.depth;  // by threads of both blocks
           if (!(cleared ? tc05::pair::mbar_wait(&bar_full[s], ph) : tc05::mbar_wait(&bar_full[s], ph))) { ok = false; break; }
           tc05::fence_after_sync();
           const uint64_t da = tc05::desc_advance(da0, s * kStageBytes), db = tc05::desc_advance(db0, s * kStageBytes);
@@ -367,7 +379,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
           for (int i = 0; i < kDepth / kInstr; ++i)
             if (i * kInstr < left)
               tc05::pair::mma<I8>(d, tc05::desc_advance(da, i * a_step), tc05::desc_advance(db, i * b_step), idesc,
-                                  (k > 0 || i > 0) ? 1u : 0u);
+                                  (k > tile.step0 || i > 0) ? 1u : 0u);
           tc05::pair::mma_commit(&bar_empty[s]);
           if (++s == kStages) { s = 0; ph ^= 1u; }
         }
@@ -379,21 +391,21 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       }
       ok = __all_sync(0xffffffffu, ok);
       ++acc;
-      advance(steps);
+      advance(tile.steps);
     }
   } else if (GRAD && warp == 2) {
     // ---- The last step of a group holds rows of its neighbours: zeros in their place, in both operands (0 times what is
     // not a number would not be zero), up to where the instructions read.
     uint32_t tail_phase = 0;
     while (ok && walk.next(&tile)) {
-      const int steps = (tile.depth + kDepth - 1) / kDepth, rem = tile.depth % kDepth;
-      if (rem != 0) {
-        const int s = (stage + steps - 1) % kStages;
+      const int rem = tile.depth % kDepth;
+      if (rem != 0 && tile.steps > 0 && (tile.step0 + tile.steps) * kDepth > tile.depth) {
+        const int s = (stage + tile.steps - 1) % kStages;
         ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_tail[s], (tail_phase >> s) & 1u));
         tail_phase ^= 1u << s;
-        const int clear = (((rem + kInstr - 1) / kInstr) * kInstr - rem) * 8;  // pieces of 16 bytes in each of the four atoms
+        const int clear = (((rem + kInstr - 1) / kInstr) * kInstr - rem) * 8;  // pieces of 16 bytes in each atom
         unsigned char* at = smem_raw + (base - tc05::smem_u32(smem_raw)) + s * kStageBytes + rem * 128;
-        for (int i = lane; i < 4 * clear; i += 32) {
+        for (int i = lane; i < kStageBytes / kAtom * clear; i += 32) {
           const int atom = i / clear;
           *reinterpret_cast<uint4*>(at + atom * kAtom + (i - atom * clear) * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
@@ -401,7 +413,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         __syncwarp();
         if (lane == 0) tc05::pair::arrive(tc05::pair::at_first(&bar_full[s]));
       }
-      advance(steps);
+      advance(tile.steps);
     }
   } else if (warp >= 4) {
     // ---- epilogue: a warp takes 32 features, columns 32 at a time
@@ -411,11 +423,18 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       const int feat0 = tile.feat0 + static_cast<int>(rank) * kM + (warp & 3) * 32;
       size_t row = static_cast<size_t>(tile.col0);
       if constexpr (GRAD) row += static_cast<size_t>(tile.group) * p.columns;
-      OutT* const to = static_cast<OutT*>(p.out) + row * p.features + feat0;  // column 0, feature 0 of the warp's
+      const size_t at = row * p.features + feat0;  // column 0, feature 0 of the warp's
+      OutT* const to = static_cast<OutT*>(p.out) + at;
+      uint32_t* const part = p.splits > 1 ? static_cast<uint32_t*>(p.parts) + tile.split * p.part + at : nullptr;
       const int feats = p.features - feat0;  // live ones of the warp's, may be <= 0 or > 32
-      if (GRAD && tile.depth == 0) {
+      if (tile.steps == 0) {  // a group without rows, or nothing of the depth left for this unit
         if (lane < feats)
-          for (int c = 0; c < tile.n; ++c) to[static_cast<size_t>(c) * p.features + lane] = from_float<OutT>(0.f);
+          for (int c = 0; c < tile.n; ++c) {
+            if (part != nullptr)
+              part[static_cast<size_t>(c) * p.features + lane] = 0u;
+            else
+              to[static_cast<size_t>(c) * p.features + lane] = from_float<OutT>(0.f);
+          }
         continue;
       }
       const int buf = acc & 1;
@@ -433,8 +452,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       const float* const xs = I8 ? p.x_scale + tile.col0 : nullptr;
       const float* const ws = I8 ? p.w_scale + static_cast<size_t>(tile.group) * p.features + feat0 : nullptr;
       bool done = false;
+      if (part != nullptr) {
+        store_lanes<false>(reinterpret_cast<float*>(part), p.features, feats, tile.n, taddr, xs, ws, lane, take);
+        done = true;
+      }
       if constexpr (sizeof(OutT) == 2) {
-        if (p.wide) {
+        if (!done && p.wide) {
           store_halves<I8>(to, p.features, feats, tile.n, taddr, staged, xs, ws, lane, take);
           done = true;
         }
@@ -456,6 +479,50 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
   tc05::fence_before_sync();
   tc05::pair::sync();
   if (warp == 0) tc05::pair::tmem_dealloc(tmem, kTmemCols);
+}
+
+// ---- the sums of the units that share a tile, added in their order: thread = an element of the result
+template <bool I8, bool GRAD, class OutT>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args p) {
+  chain_wait();
+  const int lane = threadIdx.x & 31;
+  const long long row = blockIdx.y + static_cast<long long>(blockIdx.z) * gridDim.y;
+  const int feat = blockIdx.x * 256 + threadIdx.x;
+  int group = 0;
+  if constexpr (!GRAD) {  // rows of no group are not written; 8-bit integers: the group's scales
+    if (row >= p.rows) return;
+    if (p.indptr != nullptr) {
+      if (row < ld_global(p.indptr) || row >= ld_global(p.indptr + p.groups)) return;
+      if constexpr (I8) {  // the last group that starts at or before the row: 32 pointers at a time
+        int lo = 0, n = p.groups;
+        while (n > 1) {
+          const int step = (n + 31) / 32;
+          const bool in = lane * step < n && ld_global(p.indptr + lo + min(lane * step, n - 1)) <= row;
+          const int last = 31 - __clz(__ballot_sync(0xffffffffu, in) | 1u);
+          lo += last * step;
+          n = min(step, n - last * step);
+        }
+        group = lo;
+      }
+    }
+  } else if (row >= static_cast<long long>(p.groups) * p.columns) {
+    return;
+  }
+  if (feat >= p.features) return;
+  const size_t at = static_cast<size_t>(row) * p.features + feat;
+  const uint32_t* from = static_cast<const uint32_t*>(p.parts) + at;
+  float v;
+  if constexpr (I8) {
+    int sum = 0;
+#pragma unroll 8
+    for (int s = 0; s < p.splits; ++s) sum += static_cast<int>(ld_global(from + s * p.part));
+    v = static_cast<float>(sum) * (ld_global(p.x_scale + row) * ld_global(p.w_scale + static_cast<size_t>(group) * p.features + feat));
+  } else {
+    v = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < p.splits; ++s) v += __uint_as_float(ld_global(from + s * p.part));
+  }
+  static_cast<OutT*>(p.out)[at] = from_float<OutT>(v);
 }
 
 // ---- rows at aligned addresses: TMA wants pitches that are multiples of 16 bytes
@@ -506,32 +573,55 @@ int place_operand(Operand* o, char** scratch, cudaStream_t st) {
   return 0;
 }
 
-template <bool I8, bool GRAD, class OutT>
+template <bool I8, bool GRAD, class OutT, int N>
 int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap& tm_b16, const Args& p, cudaStream_t st) {
   static thread_local int configured_device = -1, pairs = 0;
+  constexpr int smem = Shape<N>::kSmem;
   int dev = 0;
   SPTIR_CUDA_OK(cudaGetDevice(&dev));
   if (configured_device != dev) {
-    SPTIR_CUDA_OK(cudaFuncSetAttribute(grouped_kernel<I8, GRAD, OutT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    SPTIR_CUDA_OK(cudaFuncSetAttribute(grouped_kernel<I8, GRAD, OutT, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    SPTIR_CUDA_OK(cudaFuncSetAttribute(grouped_kernel<I8, GRAD, OutT, N>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                       cudaSharedmemCarveoutMaxShared));
     // as many pairs as can run at a time: each walks its share of the tiles
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = 2;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = kNumSMs;
+    cfg.gridDim = 2 * kNumSMs;
     cfg.blockDim = kThreads;
-    cfg.dynamicSmemBytes = kSmem;
+    cfg.dynamicSmemBytes = smem;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    SPTIR_CUDA_OK(cudaOccupancyMaxActiveClusters(&pairs, grouped_kernel<I8, GRAD, OutT>, &cfg));
+    SPTIR_CUDA_OK(cudaOccupancyMaxActiveClusters(&pairs, grouped_kernel<I8, GRAD, OutT, N>, &cfg));
     if (pairs < 1) return fail("no pair of blocks fits this device");
-    pairs = std::min(pairs, kNumSMs / 2);
+    // the query counts one pair to two SMs; two run there
+    pairs *= Shape<N>::kBlocks;
     configured_device = dev;
   }
-  launch_chained(grouped_kernel<I8, GRAD, OutT>, 2 * std::min(pairs, p.max_tiles), kThreads, kSmem, st, tm_a, tm_b64, tm_b16, p);
+  launch_chained(grouped_kernel<I8, GRAD, OutT, N>, 2 * std::min(pairs, p.max_tiles), kThreads, smem, st, tm_a, tm_b64, tm_b16, p);
   SPTIR_LAUNCH_OK("grouped_kernel");
+  if (p.splits > 1) {
+    const long long rows = p.part / p.features;
+    const unsigned y = static_cast<unsigned>(std::min<long long>(rows, 32768));
+    const dim3 grid(ceil_div(p.features, 256), y, ceil_div(rows, y));
+    launch_chained(join_kernel<I8, GRAD, OutT>, grid, 256, 0, st, p);
+    SPTIR_LAUNCH_OK("join_kernel");
+  }
   return 0;
+}
+
+// The kernel for results of `type`, with tiles of `columns` columns.
+template <bool I8, bool GRAD>
+int launch_type(int columns, int type, const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap& tm_b16, const Args& p,
+                cudaStream_t st) {
+  return with_type(type, [&](auto o) {
+    using O = decltype(o);
+    if constexpr (!GRAD)
+      if (columns == 128) return launch<I8, false, O, 128>(tm_a, tm_b64, tm_b16, p, st);
+    return launch<I8, GRAD, O, 256>(tm_a, tm_b64, tm_b16, p, st);
+  });
 }
 
 int check_groups(const char* fn, const int32_t* indptr, int rows, int groups, int fi, int fo, int flags) {
@@ -546,12 +636,23 @@ int check_pointers(const char* fn, const int32_t* indptr, int rows, int groups, 
   if (validate_indptr(fn, "indptr", indptr, groups, -1, st) != 0) return -1;
   return validate_range(fn, "indptr", indptr, groups + 1ll, rows + 1ll, st);
 }
-int set_tiles(const char* fn, Args* p, long long column_tiles) {
+// Sets the tiles of p, and how many units share the depth of a tile, from what the host knows: `bound(n)` column tiles of n
+// at most, about `some(n)` of them, `depth` steps each, and `rows` rows of the result.  Returns the columns of a tile, or -1.
+template <class Bound, class Some>
+int set_tiles(const char* fn, Args* p, bool few_columns, Bound&& bound, Some&& some, int depth, long long rows) {
   p->mt = ceil_div(p->features, 2 * kM);
-  if (column_tiles > (1 << 30) / p->mt) return fail("%s: too many tiles for 32-bit indices", fn);
-  p->max_tiles = static_cast<int>(column_tiles * p->mt);
-  return 0;
+  const long long tiles = some(256) * p->mt;
+  const int columns = few_columns && tiles > kNumSMs / 2 ? 128 : 256;
+  p->splits = 1;
+  if (columns == 256)
+    p->splits = static_cast<int>(std::max<long long>(1, std::min<long long>(kNumSMs / 2 / std::max<long long>(tiles, 1), depth / 4)));
+  const long long units = bound(columns) * p->mt;
+  if (units > (1 << 30) / p->splits) return fail("%s: too many tiles for 32-bit indices", fn);
+  p->max_tiles = static_cast<int>(units) * p->splits;
+  p->part = rows * p->features;
+  return columns;
 }
+size_t part_bytes(const Args& p) { return p.splits > 1 ? p.part * p.splits * sizeof(float) : 0; }
 
 CUtensorMapDataType map_type(int type) {
   return type == SPARSETIR_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
@@ -580,13 +681,17 @@ int product(const char* fn, const void* x, const void* w, int type, void* y, int
   p.a_mn = out_in ? 0 : 1;
   p.wide = wide_rows(y, y_type, fo);
   p.idesc = i8 ? tc05::instr_desc_i8(2 * kM, 0) : tc05::instr_desc(map_format(type), 2 * kM, 0, p.a_mn, 0);
-  if (set_tiles(fn, &p, rows / kN + static_cast<long long>(std::min(groups, rows))) != 0) return -1;
+  const long long used = std::min(groups, rows);
+  const int columns = set_tiles(fn, &p, rows <= 128 * used, [&](int n) { return rows / n + used; },
+                                [&](int n) { return used * ((rows + used * n - 1) / (used * n)); }, ceil_div(fi, depth), rows);
+  if (columns < 0) return -1;
   Operand ox{x, rows, fi, size}, ow{w, static_cast<long long>(groups) * (out_in ? fo : fi), out_in ? fi : fo, size};
-  const size_t copies = ox.copy_bytes() + ow.copy_bytes();
+  const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + part_bytes(p);
   CallScratch cs;
-  if (copies > 0 && take_scratch(device_id, st, copies, 0, &cs) != 0) return -1;
+  if (bytes > 0 && take_scratch(device_id, st, bytes, 0, &cs) != 0) return -1;
   char* scratch = cs.scratch;
   if (place_operand(&ox, &scratch, st) != 0 || place_operand(&ow, &scratch, st) != 0) return -1;
+  p.parts = scratch;
   CUtensorMap tm_w, tm_x64, tm_x16;
   const cuuint64_t each = out_in ? fo : fi;  // rows of one W
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(ow.cols), each, static_cast<cuuint64_t>(groups)};
@@ -597,10 +702,8 @@ int product(const char* fn, const void* x, const void* w, int type, void* y, int
       make_tmap_2d(&tm_x64, dt, ox.data, fi, rows, ox.pitch, depth, 64, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
       make_tmap_2d(&tm_x16, dt, ox.data, fi, rows, ox.pitch, depth, 16, CU_TENSOR_MAP_SWIZZLE_128B) != 0)
     return -1;
-  const int rc = with_type(y_type, [&](auto o) {
-    using O = decltype(o);
-    return i8 ? launch<true, false, O>(tm_w, tm_x64, tm_x16, p, st) : launch<false, false, O>(tm_w, tm_x64, tm_x16, p, st);
-  });
+  const int rc = i8 ? launch_type<true, false>(columns, y_type, tm_w, tm_x64, tm_x16, p, st)
+                    : launch_type<false, false>(columns, y_type, tm_w, tm_x64, tm_x16, p, st);
   return rc != 0 ? rc : return_scratch(cs, st);
 }
 
@@ -672,22 +775,25 @@ extern "C" int sparsetir_grouped_mm_grad_w_raw(const void* x, const void* dy, in
   p.groups = num_groups;
   p.features = out_in ? feat_in : feat_out;
   p.columns = out_in ? feat_out : feat_in;
-  p.nt = ceil_div(p.columns, kN);
   p.wide = wide_rows(dw, dw_type, p.features);
   p.idesc = tc05::instr_desc(map_format(type), 2 * kM, 0, 1, 1);
-  if (set_tiles(fn, &p, static_cast<long long>(num_groups) * p.nt) != 0) return -1;
+  auto tiles = [&](int n) { return static_cast<long long>(num_groups) * ceil_div(p.columns, n); };
+  const int columns = set_tiles(fn, &p, false, tiles, tiles, ceil_div(ceil_div(rows, num_groups), 64), static_cast<long long>(num_groups) * p.columns);
+  if (columns < 0) return -1;
+  p.nt = ceil_div(p.columns, columns);
   Operand oa{out_in ? x : dy, rows, p.features, 2}, ob{out_in ? dy : x, rows, p.columns, 2};
-  const size_t copies = oa.copy_bytes() + ob.copy_bytes();
+  const size_t bytes = oa.copy_bytes() + ob.copy_bytes() + part_bytes(p);
   CallScratch cs;
-  if (copies > 0 && take_scratch(device_id, st, copies, 0, &cs) != 0) return -1;
+  if (bytes > 0 && take_scratch(device_id, st, bytes, 0, &cs) != 0) return -1;
   char* scratch = cs.scratch;
   if (place_operand(&oa, &scratch, st) != 0 || place_operand(&ob, &scratch, st) != 0) return -1;
+  p.parts = scratch;
   CUtensorMap tm_a, tm_b;
   const CUtensorMapDataType dt = map_type(type);
   if (make_tmap_2d(&tm_a, dt, oa.data, oa.cols, rows, oa.pitch, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
       make_tmap_2d(&tm_b, dt, ob.data, ob.cols, rows, ob.pitch, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) != 0)
     return -1;
-  const int rc = with_type(dw_type, [&](auto o) { return launch<false, true, decltype(o)>(tm_a, tm_b, tm_b, p, st); });
+  const int rc = launch_type<false, true>(columns, dw_type, tm_a, tm_b, tm_b, p, st);
   return rc != 0 ? rc : return_scratch(cs, st);
 }
 
