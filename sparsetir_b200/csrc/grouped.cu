@@ -23,7 +23,7 @@ namespace {
 constexpr int kM = 128;               // features per block
 constexpr int kABytes = 16 * 1024;    // left operand of a stage: 128 rows of 128 bytes
 constexpr int kAtom = 8 * 1024;       // 64 rows of 128 bytes
-constexpr int kThreads = 256;         // warp 0 loads, 1 issues, 2-3 clear the tails of groups (grad_w), 4-7 epilogue
+constexpr int kFirstEpilogue = 4;     // warp 0 loads, 1 issues, 2 clears the tails of groups (grad_w), from 4 on the epilogue
 constexpr int kStagedBytes = 32 * 64; // 32 columns of 32 features on their way out, per epilogue warp
 constexpr int kBand = 8;              // column tiles of a group that are walked side by side
 
@@ -33,10 +33,27 @@ template <int N> struct Shape {
   static constexpr int kStages = N == 256 ? 6 : 4;
   static constexpr int kBlocks = N == 256 ? 1 : 2;      // per SM
   static constexpr int kTmemCols = 2 * N;               // two accumulators
-  static constexpr int kSmem = kStages * kBytes + 4 * kStagedBytes + 1024;
+  static constexpr int kEpilogue = N == 256 ? 8 : 4;    // warps
+  static constexpr int kThreads = (kFirstEpilogue + kEpilogue) * 32;
+  static constexpr int kSmem = kStages * kBytes + kEpilogue * kStagedBytes + 1024;
 };
 
 __device__ unsigned int g_grouped_timeouts = 0;
+
+// Quotients by numbers that the host knows, of dividends below 2^31: a product and a shift (a division is tens of
+// instructions, and every role makes several per tile).
+struct Divisor {
+  uint32_t by = 1, mul = 1u << 31;
+  int shift = 31;
+  Divisor() = default;
+  explicit Divisor(uint32_t d) : by(d), shift(31) {
+    while ((1ull << (shift - 31)) < d) ++shift;
+    mul = static_cast<uint32_t>(((1ull << shift) + d - 1) / d);
+  }
+  __device__ __forceinline__ int quotient(int n) const {
+    return static_cast<int>((static_cast<unsigned long long>(static_cast<uint32_t>(n)) * mul) >> shift);
+  }
+};
 
 struct Args {
   void* out;
@@ -48,6 +65,7 @@ struct Args {
   int features;   // contiguous in the result
   int columns;    // grad_w: rows of each dW
   int mt, nt;     // tiles of 256 features; grad_w: column tiles
+  Divisor per_split, per_group, per_band;  // splits; grad_w: mt * nt; kBand * mt
   int max_tiles;  // no valid indptr has more; times splits
   int splits;     // units that share the depth of a tile, each with sums of its own in `parts`
   void* parts;    // [splits][rows of the result][features], 32 bits each
@@ -80,15 +98,26 @@ struct Walker {
   unsigned before = 0, upto = 0;  // tiles ahead of the group of lane 0, and up to the group of this lane
   unsigned all = 0;               // up to the last of the 32
   int first = 0, last = 0;
-  __device__ __forceinline__ Walker(const Args& a, int pair, int pairs) : p(a), unit(pair), step(pairs) {}
+  __device__ __forceinline__ Walker(const Args& a, int pair, int pairs) : p(a), unit(pair), step(pairs) {
+    if constexpr (GRAD) ask(pair);
+  }
+  // grad_w: the row pointers of a unit's group are asked for one unit ahead
+  __device__ __forceinline__ void ask(int u) {
+    first = 0;
+    last = p.rows;
+    if (p.indptr == nullptr || u >= p.max_tiles) return;
+    const int g = p.per_group.quotient(p.per_split.quotient(u));
+    first = ld_global(p.indptr + g);
+    last = ld_global(p.indptr + g + 1);
+  }
   __device__ __forceinline__ bool next(Tile* out) {
     if (unit >= p.max_tiles) return false;
-    const int t = unit / p.splits;
+    const int t = p.per_split.quotient(unit);
     out->split = unit - t * p.splits;
     if constexpr (GRAD) {
-      const int per = p.mt * p.nt, g = t / per, r = t - g * per;
-      int f, l;
-      group_rows(p, g, &f, &l);
+      const int g = p.per_group.quotient(t), r = t - g * static_cast<int>(p.per_group.by);
+      const int f = min(max(first, 0), p.rows), l = max(min(last, p.rows), f);
+      ask(unit + step);
       place(r, p.nt, out);
       out->group = g;
       out->col0 *= kN;
@@ -127,7 +156,7 @@ struct Walker {
       out->depth = p.k;
     }
     out->n_mma = (out->n + 31) & ~31;
-    const int steps = (out->depth + kDepth - 1) / kDepth, share = (steps + p.splits - 1) / p.splits;
+    const int steps = (out->depth + kDepth - 1) / kDepth, share = p.per_split.quotient(steps + p.splits - 1);
     out->step0 = min(out->split * share, steps);
     out->steps = min(share, steps - out->step0);
     unit += step;
@@ -136,9 +165,14 @@ struct Walker {
   // Tile r of a group with `cols` column tiles: bands of kBand column tiles, in a band one column tile after the other.
   // col0 is left in tiles.
   __device__ __forceinline__ void place(int r, int cols, Tile* out) const {
-    const int band = r / (kBand * p.mt), in = r - band * (kBand * p.mt);
+    // ceil(2^32 / width): exact for quotients of less than 2^29
+    constexpr uint32_t kInverse[kBand + 1] = {0u, 0u, 0x80000000u, 0x55555556u, 0x40000000u, 0x33333334u, 0x2aaaaaabu, 0x24924925u, 0x20000000u};
+    const int band = p.per_band.quotient(r), in = r - band * static_cast<int>(p.per_band.by);
     const int width = min(kBand, cols - band * kBand);
-    const int f = in / width;
+    uint32_t inverse = 0u;
+#pragma unroll
+    for (int w = 2; w <= kBand; ++w) inverse = width == w ? kInverse[w] : inverse;
+    const int f = width == 1 ? in : static_cast<int>(__umulhi(static_cast<uint32_t>(in), inverse));
     out->feat0 = f * (2 * kM);
     out->col0 = band * kBand + in - f * width;
   }
@@ -157,12 +191,12 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
   return reinterpret_cast<const uint32_t&>(v);
 }
 
-// n columns of 32 features from TMEM to rows of the result, 16-bit elements at 16-byte addresses.  The fragments of 8
+// Columns first .. n - 1, 32 of every STEP, of 32 features from TMEM to rows of the result, 16-bit elements at 16-byte addresses.  The fragments of 8
 // columns and 32 features are transposed on their way to shared memory (rows of 32 features, pieces of 16 bytes exchanged
 // so that neither side collides) and leave as 16 bytes to a lane.  With a 2-byte store per lane and column the epilogue took
 // longer than the products of 2048-deep tiles: 576 us where this takes REPLACE (65,536 rows, 2048 -> 2048).
-template <bool I8, class OutT, class Take>
-__device__ __forceinline__ void store_halves(OutT* to, int pitch, int feats, int n, uint32_t taddr, unsigned char* staged,
+template <bool I8, int STEP, class OutT, class Take>
+__device__ __forceinline__ void store_halves(OutT* to, int pitch, int feats, int first, int n, uint32_t taddr, unsigned char* staged,
                                              const float* xs, const float* ws, int lane, Take&& take) {
   float scale[4] = {};  // of features lane / 4 + 8 q
   if constexpr (I8) {
@@ -175,7 +209,7 @@ __device__ __forceinline__ void store_halves(OutT* to, int pitch, int feats, int
   const unsigned char* get = staged + get_row * 64 + ((get_piece ^ ((get_row >> 1) & 3)) << 4);  // rows 8 apart alike
   OutT* out = to + static_cast<size_t>(get_row) * pitch + get_piece * 8;
   const bool live = get_piece * 8 < feats;
-  for (int c0 = 0; c0 < n; c0 += 32) {
+  for (int c0 = first; c0 < n; c0 += STEP) {
     uint32_t a[16], b[16];
     tc05::tmem_ld16x32(taddr + c0, a);
     tc05::tmem_ld16x32(taddr + (16u << 16) + c0, b);
@@ -218,16 +252,16 @@ __device__ __forceinline__ void store_halves(OutT* to, int pitch, int feats, int
 }
 
 // The same for 32-bit elements and for rows at any address: lane = feature, a store per column.
-template <bool I8, class OutT, class Take>
-__device__ __forceinline__ void store_lanes(OutT* to, int pitch, int feats, int n, uint32_t taddr, const float* xs, const float* ws,
+template <bool I8, int STEP, class OutT, class Take>
+__device__ __forceinline__ void store_lanes(OutT* to, int pitch, int feats, int first, int n, uint32_t taddr, const float* xs, const float* ws,
                                             int lane, Take&& take) {
   const bool live = lane < feats;
   float scale = 0.f;
   if constexpr (I8) {
     if (live) scale = ld_global(ws + lane);
   }
-  OutT* out = to + lane;
-  for (int c0 = 0; c0 < n; c0 += 32) {
+  for (int c0 = first; c0 < n; c0 += STEP) {
+    OutT* out = to + static_cast<size_t>(c0) * pitch + lane;
     float x = 0.f;
     if constexpr (I8) {
       if (c0 + lane < n) x = ld_global(xs + c0 + lane);
@@ -246,12 +280,13 @@ __device__ __forceinline__ void store_lanes(OutT* to, int pitch, int feats, int 
 }
 
 template <bool I8, bool GRAD, class OutT, int kN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Shape<kN>::kBlocks)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kN>::kThreads, Shape<kN>::kBlocks)
 grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b64,
                const __grid_constant__ CUtensorMap tm_b16, const __grid_constant__ Args p) {
   constexpr int kDepth = I8 ? 128 : 64;  // of K per stage
   constexpr int kInstr = I8 ? 32 : 16;   // of K per instruction
   constexpr int kStages = Shape<kN>::kStages, kStageBytes = Shape<kN>::kBytes, kTmemCols = Shape<kN>::kTmemCols;
+  constexpr int kEpilogue = Shape<kN>::kEpilogue;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kStages];   // rank 0: both blocks' operands are there
   __shared__ __align__(8) uint64_t bar_empty[kStages];  // the tensor core has read the stage
@@ -274,7 +309,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       }
       for (int b = 0; b < 2; ++b) {
         tc05::mbar_init(&bar_acc_full[b], 1);
-        tc05::mbar_init(&bar_acc_empty[b], 8);
+        tc05::mbar_init(&bar_acc_empty[b], 2 * kEpilogue);
       }
       tc05::mbar_init(&bar_drain, 1);
       tc05::fence_mbar_init();
@@ -415,10 +450,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       }
       advance(tile.steps);
     }
-  } else if (warp >= 4) {
-    // ---- epilogue: a warp takes 32 features, columns 32 at a time
+  } else if (warp >= kFirstEpilogue) {
+    // ---- epilogue: a warp takes the 32 features of its lanes of TMEM, columns 32 at a time; two warps share them
     int acc = 0;
-    unsigned char* const staged = smem_raw + (base - tc05::smem_u32(smem_raw)) + kStages * kStageBytes + (warp & 3) * kStagedBytes;
+    const int mine = (warp - kFirstEpilogue) / 4 * 32;  // first columns of the warp
+    constexpr int kStep = kEpilogue / 4 * 32;
+    unsigned char* const staged = smem_raw + (base - tc05::smem_u32(smem_raw)) + kStages * kStageBytes + (warp - kFirstEpilogue) * kStagedBytes;
     while (ok && walk.next(&tile)) {
       const int feat0 = tile.feat0 + static_cast<int>(rank) * kM + (warp & 3) * 32;
       size_t row = static_cast<size_t>(tile.col0);
@@ -429,7 +466,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       const int feats = p.features - feat0;  // live ones of the warp's, may be <= 0 or > 32
       if (tile.steps == 0) {  // a group without rows, or nothing of the depth left for this unit
         if (lane < feats)
-          for (int c = 0; c < tile.n; ++c) {
+          for (int c = mine / 32; c < tile.n; c += kEpilogue / 4) {
             if (part != nullptr)
               part[static_cast<size_t>(c) * p.features + lane] = 0u;
             else
@@ -443,26 +480,27 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       tc05::fence_after_sync();
       const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + buf * kN;
       const uint32_t taken = tc05::pair::at_first(&bar_acc_empty[buf]);
-      auto take = [&](int c0) {  // the last columns are in registers: the accumulator may be written again
-        if (c0 + 32 < tile.n) return;
+      auto take = [&](int c0) {  // the warp's last columns are in registers: the accumulator may be written again
+        if (c0 + kStep < tile.n) return;
         tc05::fence_before_sync();
         __syncwarp();
         if (lane == 0) tc05::pair::arrive(taken);
       };
+      if (mine >= tile.n) take(tile.n);
       const float* const xs = I8 ? p.x_scale + tile.col0 : nullptr;
       const float* const ws = I8 ? p.w_scale + static_cast<size_t>(tile.group) * p.features + feat0 : nullptr;
       bool done = false;
       if (part != nullptr) {
-        store_lanes<false>(reinterpret_cast<float*>(part), p.features, feats, tile.n, taddr, xs, ws, lane, take);
+        store_lanes<false, kStep>(reinterpret_cast<float*>(part), p.features, feats, mine, tile.n, taddr, xs, ws, lane, take);
         done = true;
       }
       if constexpr (sizeof(OutT) == 2) {
         if (!done && p.wide) {
-          store_halves<I8>(to, p.features, feats, tile.n, taddr, staged, xs, ws, lane, take);
+          store_halves<I8, kStep>(to, p.features, feats, mine, tile.n, taddr, staged, xs, ws, lane, take);
           done = true;
         }
       }
-      if (!done) store_lanes<I8>(to, p.features, feats, tile.n, taddr, xs, ws, lane, take);
+      if (!done) store_lanes<I8, kStep>(to, p.features, feats, mine, tile.n, taddr, xs, ws, lane, take);
       ++acc;
     }
   }
@@ -590,7 +628,7 @@ int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = 2 * kNumSMs;
-    cfg.blockDim = kThreads;
+    cfg.blockDim = Shape<N>::kThreads;
     cfg.dynamicSmemBytes = smem;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
@@ -600,7 +638,7 @@ int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap
     pairs *= Shape<N>::kBlocks;
     configured_device = dev;
   }
-  launch_chained(grouped_kernel<I8, GRAD, OutT, N>, 2 * std::min(pairs, p.max_tiles), kThreads, smem, st, tm_a, tm_b64, tm_b16, p);
+  launch_chained(grouped_kernel<I8, GRAD, OutT, N>, 2 * std::min(pairs, p.max_tiles), Shape<N>::kThreads, smem, st, tm_a, tm_b64, tm_b16, p);
   SPTIR_LAUNCH_OK("grouped_kernel");
   if (p.splits > 1) {
     const long long rows = p.part / p.features;
@@ -649,6 +687,8 @@ int set_tiles(const char* fn, Args* p, bool few_columns, Bound&& bound, Some&& s
   const long long units = bound(columns) * p->mt;
   if (units > (1 << 30) / p->splits) return fail("%s: too many tiles for 32-bit indices", fn);
   p->max_tiles = static_cast<int>(units) * p->splits;
+  p->per_split = Divisor(p->splits);
+  p->per_band = Divisor(kBand * p->mt);
   p->part = rows * p->features;
   return columns;
 }
@@ -781,6 +821,7 @@ extern "C" int sparsetir_grouped_mm_grad_w_raw(const void* x, const void* dy, in
   const int columns = set_tiles(fn, &p, false, tiles, tiles, ceil_div(ceil_div(rows, num_groups), 64), static_cast<long long>(num_groups) * p.columns);
   if (columns < 0) return -1;
   p.nt = ceil_div(p.columns, columns);
+  p.per_group = Divisor(p.mt * p.nt);
   Operand oa{out_in ? x : dy, rows, p.features, 2}, ob{out_in ? dy : x, rows, p.columns, 2};
   const size_t bytes = oa.copy_bytes() + ob.copy_bytes() + part_bytes(p);
   CallScratch cs;
