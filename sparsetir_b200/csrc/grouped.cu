@@ -23,8 +23,9 @@ namespace {
 constexpr int kM = 128;               // features per block
 constexpr int kABytes = 16 * 1024;    // left operand of a stage: 128 rows of 128 bytes
 constexpr int kAtom = 8 * 1024;       // 64 rows of 128 bytes
-constexpr int kFirstEpilogue = 4;     // warp 0 loads, 1 issues, 2 clears the tails of groups (grad_w), from 4 on the epilogue
+constexpr int kFirstEpilogue = 4;     // warp 0 loads, 1 issues, 2 clears the tails of groups (grad_w), 3 hands out tiles, from 4 on the epilogue
 constexpr int kStagedBytes = 32 * 64; // 32 columns of 32 features on their way out, per epilogue warp
+constexpr int kTiles = 4;             // entries of the ring of tiles
 constexpr int kBand = 8;              // column tiles of a group that are walked side by side
 
 // Columns of a tile, and what follows from them.
@@ -67,6 +68,7 @@ struct Args {
   int mt, nt;     // tiles of 256 features; grad_w: column tiles
   Divisor per_split, per_group, per_band;  // splits; grad_w: mt * nt; kBand * mt
   int max_tiles;  // no valid indptr has more; times splits
+  int deal;       // more of them than pairs of blocks run at a time
   int splits;     // units that share the depth of a tile, each with sums of its own in `parts`
   void* parts;    // [splits][rows of the result][features], 32 bits each
   long long part; // elements of one split's
@@ -89,35 +91,23 @@ struct Tile {
   int split, step0, steps; // the unit's share of the depth
 };
 
-// The units of one pair: `pair`, pair + pairs, ...  All lanes of a warp call next() together; lane l holds the prefix of tile counts
-// of group base + l.  Sums stop at 2^30: wild pointers give tiles inside the arrays, and no more than max_tiles of them.
+// The tile of a unit.  All lanes of a warp call at() together; lane l holds the prefix of tile counts of group base + l.
+// Sums stop at 2^30: wild pointers give tiles inside the arrays, and no more than max_tiles of them.
 template <bool GRAD, int kN, int kDepth>
 struct Walker {
   const Args& p;
-  int unit, step, base = -32;
+  int base = -32;
   unsigned before = 0, upto = 0;  // tiles ahead of the group of lane 0, and up to the group of this lane
   unsigned all = 0;               // up to the last of the 32
   int first = 0, last = 0;
-  __device__ __forceinline__ Walker(const Args& a, int pair, int pairs) : p(a), unit(pair), step(pairs) {
-    if constexpr (GRAD) ask(pair);
-  }
-  // grad_w: the row pointers of a unit's group are asked for one unit ahead
-  __device__ __forceinline__ void ask(int u) {
-    first = 0;
-    last = p.rows;
-    if (p.indptr == nullptr || u >= p.max_tiles) return;
-    const int g = p.per_group.quotient(p.per_split.quotient(u));
-    first = ld_global(p.indptr + g);
-    last = ld_global(p.indptr + g + 1);
-  }
-  __device__ __forceinline__ bool next(Tile* out) {
-    if (unit >= p.max_tiles) return false;
+  __device__ __forceinline__ explicit Walker(const Args& a) : p(a) {}
+  __device__ __forceinline__ bool at(int unit, Tile* out) {
     const int t = p.per_split.quotient(unit);
     out->split = unit - t * p.splits;
     if constexpr (GRAD) {
       const int g = p.per_group.quotient(t), r = t - g * static_cast<int>(p.per_group.by);
-      const int f = min(max(first, 0), p.rows), l = max(min(last, p.rows), f);
-      ask(unit + step);
+      int f, l;
+      group_rows(p, g, &f, &l);
       place(r, p.nt, out);
       out->group = g;
       out->col0 *= kN;
@@ -126,6 +116,10 @@ struct Walker {
       out->depth = l - f;
     } else {
       const int lane = threadIdx.x & 31;
+      if (static_cast<unsigned>(t) < before) {
+        base = -32;
+        before = all = 0;
+      }
       while (static_cast<unsigned>(t) >= all) {
         base += 32;
         if (base >= p.groups) return false;
@@ -159,7 +153,6 @@ struct Walker {
     const int steps = (out->depth + kDepth - 1) / kDepth, share = p.per_split.quotient(steps + p.splits - 1);
     out->step0 = min(out->split * share, steps);
     out->steps = min(share, steps - out->step0);
-    unit += step;
     return true;
   }
   // Tile r of a group with `cols` column tiles: bands of kBand column tiles, in a band one column tile after the other.
@@ -294,11 +287,16 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
   __shared__ __align__(8) uint64_t bar_acc_full[2];
   __shared__ __align__(8) uint64_t bar_acc_empty[2];    // rank 0: both blocks have taken the result
   __shared__ __align__(8) uint64_t bar_drain;
+  __shared__ __align__(8) uint64_t bar_tile_full[kTiles];
+  __shared__ __align__(8) uint64_t bar_tile_empty[kTiles];  // rank 0: the roles of both blocks have read the entry
+  __shared__ __align__(8) uint64_t bar_answer;
+  __shared__ __align__(16) int4 s_tiles[kTiles][2];
+  __shared__ __align__(16) int4 s_answer;
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = tc05::pair::rank();
   const uint32_t base = (tc05::smem_u32(smem_raw) + 1023u) & ~1023u;
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int pair = blockIdx.x >> 1;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -312,6 +310,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         tc05::mbar_init(&bar_acc_empty[b], 2 * kEpilogue);
       }
       tc05::mbar_init(&bar_drain, 1);
+      for (int b = 0; b < kTiles; ++b) {
+        tc05::mbar_init(&bar_tile_full[b], 1);
+        tc05::mbar_init(&bar_tile_empty[b], 3 + 2 * kEpilogue + (GRAD ? 2 : 0));
+      }
+      tc05::mbar_init(&bar_answer, 1);
       tc05::fence_mbar_init();
       tc05::prefetch_tensormap(&tm_a);
       tc05::prefetch_tensormap(&tm_b64);
@@ -337,12 +340,30 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     phase ^= static_cast<uint32_t>(q / kStages) & 1u;
     stage = q % kStages;
   };
-  Walker<GRAD, kN, kDepth> walk(p, pair, pairs);
+  Walker<GRAD, kN, kDepth> walk(p);
   Tile tile;
+  // A role's next tile: the pair's own, then those that warp 3 of rank 0 hands to both blocks.
+  int turn = -1;
+  auto next = [&]() {
+    if (turn < 0) {
+      turn = 0;
+      return walk.at(pair, &tile);
+    }
+    if (p.deal == 0) return false;
+    const int s = turn % kTiles;
+    ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_tile_full[s], (turn / kTiles) & 1));
+    if (!ok) return false;
+    const int4 a = s_tiles[s][0], b = s_tiles[s][1];
+    __syncwarp();
+    if (lane == 0) tc05::pair::arrive_relaxed(tc05::pair::at_first(&bar_tile_empty[s]));
+    ++turn;
+    tile = Tile{a.x, a.y, a.z, a.w & 0xffff, ((a.w & 0xffff) + 31) & ~31, b.x, b.y, a.w >> 16, b.z, b.w};
+    return tile.steps >= 0;
+  };
 
   if (warp == 0) {
     // ---- loads.  Each block fetches its 128 features and its half of the columns, and tells rank 0's barrier.
-    while (ok && walk.next(&tile)) {
+    while (ok && next()) {
       const int half = tile.n_mma / 2, units = half / 16;
       const int feat = tile.feat0 + static_cast<int>(rank) * kM, col = tile.col0 + static_cast<int>(rank) * half;
       if (tc05::elect_one()) {
@@ -394,7 +415,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     const uint32_t a_step = a_mn ? 2048u : 32u, b_step = GRAD ? 2048u : 32u;
     const uint64_t da0 = tc05::smem_desc_swizzled(base, a_mn ? kAtom : 0, 1024, tc05::kSwizzle128B);
     const uint64_t db0 = tc05::smem_desc_swizzled(base + kABytes, GRAD ? kAtom : 0, 1024, tc05::kSwizzle128B);
-    while (rank == 0 && ok && walk.next(&tile)) {
+    while (rank == 0 && ok && next()) {
       if (tile.steps == 0) continue;
       if (tc05::elect_one()) {
         const int buf = acc & 1;
@@ -432,7 +453,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     // ---- The last step of a group holds rows of its neighbours: zeros in their place, in both operands (0 times what is
     // not a number would not be zero), up to where the instructions read.
     uint32_t tail_phase = 0;
-    while (ok && walk.next(&tile)) {
+    while (ok && next()) {
       const int rem = tile.depth % kDepth;
       if (rem != 0 && tile.steps > 0 && (tile.step0 + tile.steps) * kDepth > tile.depth) {
         const int s = (stage + tile.steps - 1) % kStages;
@@ -450,13 +471,44 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       }
       advance(tile.steps);
     }
+  } else if (warp == 3) {
+    // ---- tiles.  The launch has a pair of blocks for every unit, and those that are not running yet are waited for by nobody:
+    // a pair that is takes the next one's work until there is none.  (Units dealt out beforehand: REPLACE.)
+    int at = 0;
+    bool more = rank == 0 && p.deal != 0 && walk.at(pair, &tile);  // there are readers
+    while (rank == 0 && p.deal != 0) {
+      if (lane == 0) {
+        tc05::mbar_arrive_expect_tx(&bar_answer, 16);
+        tc05::pair::try_cancel(&s_answer, &bar_answer);
+      }
+      ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_answer, at & 1));
+      ++at;
+      int block = 0;
+      const bool one = ok && tc05::pair::cancelled(&s_answer, &block);
+      tc05::fence_async_smem();  // the answer has been read before it is written again
+      __syncwarp();
+      if (more) {
+        if (!one || !walk.at(block >> 1, &tile)) tile.steps = -1;  // the readers' last entry
+        more = tile.steps >= 0;
+        const int n = turn < 0 ? 0 : turn, s = n % kTiles;
+        turn = n + 1;
+        ok = ok && __all_sync(0xffffffffu, tc05::mbar_wait(&bar_tile_empty[s], ((n / kTiles) & 1) ^ 1));
+        if (ok && lane < 2) {  // to the block of rank `lane`
+          const uint32_t to = tc05::pair::at_rank(&s_tiles[s][0], lane), bar = tc05::pair::at_rank(&bar_tile_full[s], lane);
+          tc05::pair::arrive_expect_tx(bar, 32);
+          tc05::pair::store_async(to, make_int4(tile.group, tile.feat0, tile.col0, tile.n | tile.split << 16), bar);
+          tc05::pair::store_async(to + 16, make_int4(tile.row0, tile.depth, tile.step0, tile.steps), bar);
+        }
+      }
+      if (!one || !ok) break;
+    }
   } else if (warp >= kFirstEpilogue) {
     // ---- epilogue: a warp takes the 32 features of its lanes of TMEM, columns 32 at a time; two warps share them
     int acc = 0;
     const int mine = (warp - kFirstEpilogue) / 4 * 32;  // first columns of the warp
     constexpr int kStep = kEpilogue / 4 * 32;
     unsigned char* const staged = smem_raw + (base - tc05::smem_u32(smem_raw)) + kStages * kStageBytes + (warp - kFirstEpilogue) * kStagedBytes;
-    while (ok && walk.next(&tile)) {
+    while (ok && next()) {
       const int feat0 = tile.feat0 + static_cast<int>(rank) * kM + (warp & 3) * 32;
       size_t row = static_cast<size_t>(tile.col0);
       if constexpr (GRAD) row += static_cast<size_t>(tile.group) * p.columns;
@@ -613,7 +665,7 @@ int place_operand(Operand* o, char** scratch, cudaStream_t st) {
 
 template <bool I8, bool GRAD, class OutT, int N>
 int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap& tm_b16, const Args& p, cudaStream_t st) {
-  static thread_local int configured_device = -1, pairs = 0;
+  static thread_local int configured_device = -1;
   constexpr int smem = Shape<N>::kSmem;
   int dev = 0;
   SPTIR_CUDA_OK(cudaGetDevice(&dev));
@@ -621,24 +673,9 @@ int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap
     SPTIR_CUDA_OK(cudaFuncSetAttribute(grouped_kernel<I8, GRAD, OutT, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     SPTIR_CUDA_OK(cudaFuncSetAttribute(grouped_kernel<I8, GRAD, OutT, N>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                        cudaSharedmemCarveoutMaxShared));
-    // as many pairs as can run at a time: each walks its share of the tiles
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = 2 * kNumSMs;
-    cfg.blockDim = Shape<N>::kThreads;
-    cfg.dynamicSmemBytes = smem;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    SPTIR_CUDA_OK(cudaOccupancyMaxActiveClusters(&pairs, grouped_kernel<I8, GRAD, OutT, N>, &cfg));
-    if (pairs < 1) return fail("no pair of blocks fits this device");
-    // the query counts one pair to two SMs; two run there
-    pairs *= Shape<N>::kBlocks;
     configured_device = dev;
   }
-  launch_chained(grouped_kernel<I8, GRAD, OutT, N>, 2 * std::min(pairs, p.max_tiles), Shape<N>::kThreads, smem, st, tm_a, tm_b64, tm_b16, p);
+  launch_chained(grouped_kernel<I8, GRAD, OutT, N>, 2 * p.max_tiles, Shape<N>::kThreads, smem, st, tm_a, tm_b64, tm_b16, p);
   SPTIR_LAUNCH_OK("grouped_kernel");
   if (p.splits > 1) {
     const long long rows = p.part / p.features;
@@ -685,8 +722,9 @@ int set_tiles(const char* fn, Args* p, bool few_columns, Bound&& bound, Some&& s
   if (columns == 256)
     p->splits = static_cast<int>(std::max<long long>(1, std::min<long long>(kNumSMs / 2 / std::max<long long>(tiles, 1), depth / 4)));
   const long long units = bound(columns) * p->mt;
-  if (units > (1 << 30) / p->splits) return fail("%s: too many tiles for 32-bit indices", fn);
+  if (units > (1 << 29) / p->splits) return fail("%s: too many tiles for 32-bit indices", fn);
   p->max_tiles = static_cast<int>(units) * p->splits;
+  p->deal = p->max_tiles > kNumSMs / 2 * (columns == 128 ? Shape<128>::kBlocks : Shape<256>::kBlocks);
   p->per_split = Divisor(p->splits);
   p->per_band = Divisor(kBand * p->mt);
   p->part = rows * p->features;

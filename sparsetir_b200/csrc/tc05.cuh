@@ -268,14 +268,51 @@ __device__ __forceinline__ uint32_t rank() {
 __device__ __forceinline__ void sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Address of rank 0's copy of a shared-memory object
-__device__ __forceinline__ uint32_t at_first(const void* p) {
+// Address of a rank's copy of a shared-memory object
+__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
   uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
+__device__ __forceinline__ uint32_t at_first(const void* p) { return at_rank(p, 0); }
 __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The same where nothing that this thread has done is to be seen behind it.
+__device__ __forceinline__ void arrive_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// 16 bytes to shared memory of a block of the cluster; they count at its barrier when they are there.
+__device__ __forceinline__ void store_async(uint32_t to, int4 v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(v.x),
+               "r"(v.y), "r"(v.z), "r"(v.w), "r"(bar)
+               : "memory");
+}
+// Takes over the work of a cluster of this launch that has not been started: 16 bytes for cancelled() at `answer`, which
+// count at `bar`.  Not to be asked again once there was none.
+__device__ __forceinline__ void try_cancel(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// Whether there was one; *block is the x index of its first block.
+__device__ __forceinline__ bool cancelled(const void* answer, int* block) {
+  uint32_t yes, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, r;\n\t}"
+      : "=r"(yes), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  *block = static_cast<int>(x);
+  return yes != 0;
 }
 // mbar_wait for a barrier at which threads of the other block arrive
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
