@@ -355,7 +355,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     if (!ok) return false;
     const int4 a = s_tiles[s][0], b = s_tiles[s][1];
     __syncwarp();
-    if (lane == 0) tc05::pair::arrive_relaxed(tc05::pair::at_first(&bar_tile_empty[s]));
+    if (lane == 0) tc05::pair::arrive_here(tc05::pair::at_first(&bar_tile_empty[s]));
     ++turn;
     tile = Tile{a.x, a.y, a.z, a.w & 0xffff, ((a.w & 0xffff) + 31) & ~31, b.x, b.y, a.w >> 16, b.z, b.w};
     return tile.steps >= 0;
@@ -536,7 +536,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         if (c0 + kStep < tile.n) return;
         tc05::fence_before_sync();
         __syncwarp();
-        if (lane == 0) tc05::pair::arrive(taken);
+        if (lane == 0) tc05::pair::arrive_here(taken);
       };
       if (mine >= tile.n) take(tile.n);
       const float* const xs = I8 ? p.x_scale + tile.col0 : nullptr;

@@ -278,9 +278,10 @@ __device__ __forceinline__ uint32_t at_first(const void* p) { return at_rank(p, 
 __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// The same where nothing that this thread has done is to be seen behind it.
-__device__ __forceinline__ void arrive_relaxed(uint32_t bar) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// The same where what this thread has written need not be seen behind it: the form above waits until all of its stores
+// have arrived, those to global memory among them.
+__device__ __forceinline__ void arrive_here(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void arrive_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
