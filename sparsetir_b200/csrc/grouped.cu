@@ -11,6 +11,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "grouped.h"
 #include "launch.cuh"
 #include "lowp.cuh"
 #include "tc05.cuh"
@@ -202,10 +203,11 @@ __device__ __forceinline__ void store_halves(OutT* to, int pitch, int feats, int
   const unsigned char* get = staged + get_row * 64 + ((get_piece ^ ((get_row >> 1) & 3)) << 4);  // rows 8 apart alike
   OutT* out = to + static_cast<size_t>(get_row) * pitch + get_piece * 8;
   const bool live = get_piece * 8 < feats;
+  if (first >= n) return;
+  uint32_t a[16], b[16];
+  tc05::tmem_ld16x32(taddr + first, a);
+  tc05::tmem_ld16x32(taddr + (16u << 16) + first, b);
   for (int c0 = first; c0 < n; c0 += STEP) {
-    uint32_t a[16], b[16];
-    tc05::tmem_ld16x32(taddr + c0, a);
-    tc05::tmem_ld16x32(taddr + (16u << 16) + c0, b);
     float x[8];
     if constexpr (I8) {
 #pragma unroll
@@ -234,6 +236,10 @@ __device__ __forceinline__ void store_halves(OutT* to, int pitch, int feats, int
       asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(put + r * 64 + ((q ^ ((r >> 1) & 3)) << 4)),
                    "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                    : "memory");
+    }
+    if (c0 + STEP < n) {  // the next columns while these leave
+      tc05::tmem_ld16x32(taddr + c0 + STEP, a);
+      tc05::tmem_ld16x32(taddr + (16u << 16) + c0 + STEP, b);
     }
     __syncwarp();
 #pragma unroll
@@ -355,7 +361,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     if (!ok) return false;
     const int4 a = s_tiles[s][0], b = s_tiles[s][1];
     __syncwarp();
-    if (lane == 0) tc05::pair::arrive_here(tc05::pair::at_first(&bar_tile_empty[s]));
+    if (lane == 0) tc05::pair::arrive(tc05::pair::at_first(&bar_tile_empty[s]));
     ++turn;
     tile = Tile{a.x, a.y, a.z, a.w & 0xffff, ((a.w & 0xffff) + 31) & ~31, b.x, b.y, a.w >> 16, b.z, b.w};
     return tile.steps >= 0;
@@ -536,7 +542,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         if (c0 + kStep < tile.n) return;
         tc05::fence_before_sync();
         __syncwarp();
-        if (lane == 0) tc05::pair::arrive_here(taken);
+        if (lane == 0) tc05::pair::arrive(taken);
       };
       if (mine >= tile.n) take(tile.n);
       const float* const xs = I8 ? p.x_scale + tile.col0 : nullptr;
@@ -719,8 +725,10 @@ int set_tiles(const char* fn, Args* p, bool few_columns, Bound&& bound, Some&& s
   const long long tiles = some(256) * p->mt;
   const int columns = few_columns && tiles > kNumSMs / 2 ? 128 : 256;
   p->splits = 1;
-  if (columns == 256)
-    p->splits = static_cast<int>(std::max<long long>(1, std::min<long long>(kNumSMs / 2 / std::max<long long>(tiles, 1), depth / 4)));
+  if (columns == 256) {
+    const int most = static_cast<int>(std::min<long long>(kNumSMs / 2 / std::max<long long>(tiles, 1), depth / 4));
+    if (most > 1 && depth - depth / most >= 12) p->splits = most;
+  }
   const long long units = bound(columns) * p->mt;
   if (units > (1 << 29) / p->splits) return fail("%s: too many tiles for 32-bit indices", fn);
   p->max_tiles = static_cast<int>(units) * p->splits;
@@ -740,6 +748,18 @@ uint32_t map_format(int type) { return type == SPARSETIR_F16 ? tc05::kFmtF16 : t
 
 bool wide_rows(const void* out, int type, int features) {
   return type != SPARSETIR_F32 && aligned16(out) && features % 8 == 0;
+}
+
+// Whether the kernel for groups of a few rows takes a product, from what the host knows (us, that kernel / this one, 16-bit elements
+// unless said otherwise; rows, groups, features): W contiguous along the depth 2, 1, 4096 -> 4096 7.9 / 13.4; 16, 1, 4096 -> 4096
+// 9.0 / 14.0; 16, 8, 1024 -> 1024 3.8 / 8.8; 64, 8, 2048 -> 2048 15.5 / 15.8; 8-bit integers 1, 1, 4096 -> 8192 8.2 / 14; but 128, 8, 2048 -> 2048 20 / 16 and
+// 500, 64, 2048 -> 2048 114 / 90, which have tiles enough; along the features 16, 8, 512 -> 512 3.9 / 6.5, but 16, 8, 2048 ->
+// 2048 17.7 / 14.4.  The bound on the rows is for batches that meet in one group, which it walks 16 rows at a time.
+bool few_rows_pay(int rows, int groups, int fi, int fo, bool along_k) {
+  const long long used = std::min(groups, rows);
+  const long long tiles = used * ceil_div(fo, 2 * kM);
+  if (rows > 256 || rows > (tiles < kNumSMs / 4 ? 16 : 8) * used || groups > 65535) return false;
+  return along_k ? tiles <= 256 : used * fi <= (8 << 20) / fo;
 }
 
 // y = x * W: `type` of the elements of x and W, -1 for 8-bit integers
@@ -770,6 +790,11 @@ int product(const char* fn, const void* x, const void* w, int type, void* y, int
   char* scratch = cs.scratch;
   if (place_operand(&ox, &scratch, st) != 0 || place_operand(&ow, &scratch, st) != 0) return -1;
   p.parts = scratch;
+  if (few_rows_pay(rows, groups, fi, fo, out_in)) {
+    FewArgs f{ox.data, ow.data, y, xs, ws, indptr, ox.pitch, ow.pitch, rows, groups, fi, fo, fi * size, 0, 0, 0};
+    const int done = few_rows(f, type, y_type, out_in, st);
+    return done != 0 ? done : return_scratch(cs, st);
+  }
   CUtensorMap tm_w, tm_x64, tm_x16;
   const cuuint64_t each = out_in ? fo : fi;  // rows of one W
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(ow.cols), each, static_cast<cuuint64_t>(groups)};

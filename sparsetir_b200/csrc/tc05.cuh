@@ -275,12 +275,9 @@ __device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
   return a;
 }
 __device__ __forceinline__ uint32_t at_first(const void* p) { return at_rank(p, 0); }
+// An arrival at a barrier of either block.  (With release.cluster it waits until all stores of this thread have arrived, those
+// to global memory among them.)
 __device__ __forceinline__ void arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// The same where what this thread has written need not be seen behind it: the form above waits until all of its stores
-// have arrived, those to global memory among them.
-__device__ __forceinline__ void arrive_here(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void arrive_expect_tx(uint32_t bar, uint32_t bytes) {
