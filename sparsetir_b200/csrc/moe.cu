@@ -39,11 +39,15 @@ __device__ __forceinline__ float warp_sum(float v) {
 // A token's logits, R to a lane: lane l has those of the experts l, l + 32, ...
 template <class T, int R>
 __device__ __forceinline__ void load_keys(const T* row, int num_experts, int lane, uint32_t (&key)[R]) {
+  constexpr int G = R < 8 ? R : 8;  // in flight
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = lane + 32 * r;
-    key[r] = 0u;
-    if (i < num_experts) key[r] = order_key(to_float(ld_global(row + i)));
+  for (int r0 = 0; r0 < R; r0 += G) {
+    T v[G];
+#pragma unroll
+    for (int r = 0; r < G; ++r)
+      if (lane + 32 * (r0 + r) < num_experts) v[r] = ld_global(row + lane + 32 * (r0 + r));
+#pragma unroll
+    for (int r = 0; r < G; ++r) key[r0 + r] = lane + 32 * (r0 + r) < num_experts ? order_key(to_float(v[r])) : 0u;
   }
 }
 
@@ -51,11 +55,12 @@ __device__ __forceinline__ void load_keys(const T* row, int num_experts, int lan
 // the tokens, a warp per token, and counts the pairs of every expert; each block of the second sums the counts of all
 // shares (they are few: 148 at most) and places its share's pairs.  Nothing depends on the order in which blocks run.
 constexpr int kRouteThreads = 1024, kRouteWarps = kRouteThreads / 32;
-constexpr int kRouteTokens = 128;  // of a share, more where there would be over 148 of them
+constexpr int kRouteAlone = 128;   // tokens that a single block takes
+constexpr int kRouteTokens = 32;   // of a share at least; more where there would be over 148 shares
 
 struct PlaceShared {
   int next[SPARSETIR_MOE_MAX_EXPERTS];  // where the share's next pair of every expert goes
-  unsigned char count[kRouteWarps][SPARSETIR_MOE_MAX_EXPERTS];
+  uint4 count[SPARSETIR_MOE_MAX_EXPERTS][kRouteWarps / 16];  // a byte for every warp
   int sums[kRouteWarps];
 };
 
@@ -70,12 +75,22 @@ __device__ __forceinline__ int add_bases(PlaceShared& s, int total) {
   }
   if (lane == 31) s.sums[warp] = upto;
   __syncthreads();
-  int before = 0, all = s.sums[lane];
-  for (int w = 0; w < warp; ++w) before += s.sums[w];
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) all += __shfl_xor_sync(kFull, all, o);
+  const int sum = s.sums[lane];
+  const int before = __reduce_add_sync(kFull, lane < warp ? sum : 0);
   s.next[tid] += before + upto - total;
-  return all;
+  return __reduce_add_sync(kFull, sum);
+}
+// Sum of the first n bytes of 32
+__device__ __forceinline__ int sum_bytes(const uint4 (&c)[kRouteWarps / 16], int n) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(c);
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < kRouteWarps / 4; ++i) {
+    const int left = min(max(n - 4 * i, 0), 4);
+    const uint32_t ones = left == 4 ? 0x01010101u : 0x01010101u & ((1u << (8 * left)) - 1u);
+    sum = __dp4a(w[i], ones, static_cast<uint32_t>(sum));
+  }
+  return sum;
 }
 
 // Pairs [first, last) in order: the place of each is next of its expert plus the pairs of that expert ahead of it, in its
@@ -86,27 +101,18 @@ __device__ __forceinline__ void place_pairs(PlaceShared& s, const int32_t* exper
   for (int p0 = first; p0 < last; p0 += kRouteThreads) {
     const int p = p0 + tid;
     const int e = p < last ? ld_global(experts + p) : -1;
-    for (int i = lane; i * 4 < num_experts; i += 32) reinterpret_cast<uint32_t*>(s.count[warp])[i] = 0u;
-    __syncwarp();
+    if (tid < num_experts) s.count[tid][0] = s.count[tid][1] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
     const unsigned same = __match_any_sync(kFull, e);
     const int ahead = __popc(same & ((1u << lane) - 1u));
-    if (e >= 0 && ahead == 0) s.count[warp][e] = static_cast<unsigned char>(__popc(same));
+    if (e >= 0 && ahead == 0) reinterpret_cast<unsigned char*>(s.count[e])[warp] = static_cast<unsigned char>(__popc(same));
     __syncthreads();
-    if (p < last) {
-      int slot = -1;
-      if (e >= 0) {
-        slot = s.next[e] + ahead;
-        for (int w = 0; w < warp; ++w) slot += s.count[w][e];
-      }
-      slots[p] = slot;
+    if (p < last) slots[p] = e >= 0 ? s.next[e] + ahead + sum_bytes(s.count[e], warp) : -1;
+    __syncthreads();
+    if (p0 + kRouteThreads < last) {
+      if (tid < num_experts) s.next[tid] += sum_bytes(s.count[tid], kRouteWarps);
+      __syncthreads();
     }
-    __syncthreads();
-    if (p0 + kRouteThreads < last && tid < num_experts) {
-      int sum = 0;
-      for (int w = 0; w < kRouteWarps; ++w) sum += s.count[w][tid];
-      s.next[tid] += sum;
-    }
-    __syncthreads();
   }
 }
 
@@ -134,24 +140,36 @@ choose_kernel(const T* logits, float* gates, int32_t* experts, int32_t* slots, i
     for (int r = 0; r < R; ++r) sum += over_top(key[r], top);
     sum = warp_sum(sum);
     int expert = -1;     // of choice `lane`
-    float value = 0.f;   // exp(z - top) of it
-    for (int j = 0; j < top_k; ++j) {
-      uint32_t best = 0u;
-      int at = 0x7fffffff;
+    uint32_t chosen = 0u;
+    uint32_t best = 0u;  // the lane's largest that is left, and its first place
+    int at = 0;
+    auto look = [&]() {
+      best = 0u;
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (key[r] > best) { best = key[r]; at = lane + 32 * r; }
+        if (key[r] > best) { best = key[r]; at = r; }
+    };
+    look();
+    for (int j = 0; j < top_k; ++j) {
       const uint32_t found = __reduce_max_sync(kFull, best);
       if (found == 0u) break;
-      const int who = __reduce_min_sync(kFull, best == found ? at : 0x7fffffff);
+      const unsigned have = __ballot_sync(kFull, best == found);
+      // several lanes: the lowest expert, whose row of 32 comes first, and then its lane
+      int src = __ffs(have) - 1;
+      if ((have & (have - 1u)) != 0u) src = __reduce_min_sync(kFull, best == found ? at * 32 + lane : 0x7fffffff) & 31;
+      const int who = __shfl_sync(kFull, at, src) * 32 + src;
+      if (lane == src) {
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (lane + 32 * r == who) key[r] = 0u;
+        for (int r = 0; r < R; ++r)
+          if (r == at) key[r] = 0u;
+        look();
+      }
       if (lane == j) {
         expert = who;
-        value = over_top(found, top);
+        chosen = found;
       }
     }
+    const float value = over_top(chosen, top);
     if (renormalize) sum = warp_sum(value);
     if (lane < top_k) {
       const size_t p = static_cast<size_t>(t) * top_k + lane;
@@ -217,18 +235,17 @@ route_grad_kernel(const T* logits, const float* gates, const int32_t* experts, c
   const int lane = threadIdx.x & 31;
   const int t = blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (t >= tokens) return;
-  uint32_t key[R];
-  load_keys<T, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, lane, key);
   int expert = -1;
   float gate = 0.f, dg = 0.f;
   if (lane < top_k) {
     const size_t p = static_cast<size_t>(t) * top_k + lane;
     expert = ld_global(experts + p);
-    if (expert >= 0) {
-      gate = ld_global(gates + p);
-      dg = ld_global(d_gates + p);
-    }
+    gate = ld_global(gates + p);
+    dg = ld_global(d_gates + p);
   }
+  uint32_t key[R];
+  load_keys<T, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, lane, key);
+  if (expert < 0) gate = dg = 0.f;
   const float mean = warp_sum(gate * dg);
   float grad[R];
   if (renormalize) {
@@ -395,15 +412,19 @@ combine_grad_kernel(const Piece<B>* dy, const Piece<B>* z, const int32_t* slots,
 #pragma unroll
     for (int i = 0; i < kHold; ++i)
       if (first + i * kRowThreads < pieces) d[i] = ld_global(dy + static_cast<size_t>(t) * pieces + first + i * kRowThreads);
-    for (int j = 0; j < top_k; ++j) {
-      const int s = __shfl_sync(kFull, slot, j);
-      const float w = __shfl_sync(kFull, gate, j);
-      if (s < 0) continue;
-      const size_t row = static_cast<size_t>(s) * pieces + first;
-      Piece<B> v[kHold];
+    // the pieces of the next row are asked for before this one's are used
+    auto ask = [&](int j, Piece<B> (&v)[kHold]) {
+      const int s = j < top_k ? __shfl_sync(kFull, slot, j) : -1;
+      if (s < 0) return s;
 #pragma unroll
       for (int i = 0; i < kHold; ++i)
-        if (first + i * kRowThreads < pieces) v[i] = ld_global(z + row + i * kRowThreads);
+        if (first + i * kRowThreads < pieces) v[i] = ld_global(z + static_cast<size_t>(s) * pieces + first + i * kRowThreads);
+      return s;
+    };
+    auto use = [&](int j, int s, const Piece<B> (&v)[kHold]) {
+      if (s < 0) return;
+      const float w = __shfl_sync(kFull, gate, j);
+      Piece<B>* to = dz + static_cast<size_t>(s) * pieces + first;
       float dot = 0.f;
 #pragma unroll
       for (int i = 0; i < kHold; ++i) {
@@ -416,11 +437,19 @@ combine_grad_kernel(const Piece<B>* dy, const Piece<B>* z, const int32_t* slots,
             dot = fmaf(a[n], b[n], dot);
             o[n] = w * a[n];
           }
-          dz[row + i * kRowThreads] = pack<T, B>(o);
+          to[i * kRowThreads] = pack<T, B>(o);
         }
       }
       dot = warp_sum(dot);
       if (lane == 0) part[j][warp] += dot;
+    };
+    Piece<B> u[kHold], v[kHold];
+    int su = ask(0, u);
+    for (int j = 0; j < top_k; j += 2) {
+      const int sv = ask(j + 1, v);
+      use(j, su, u);
+      su = ask(j + 2, u);
+      if (j + 1 < top_k) use(j + 1, sv, v);
     }
   }
   __syncthreads();
@@ -534,7 +563,7 @@ int check_route(const char* fn, int type, int tokens, int num_experts, int top_k
   return 0;
 }
 
-int route_share(int tokens) { return std::max(kRouteTokens, ceil_div(tokens, kNumSMs)); }
+int route_share(int tokens) { return tokens <= kRouteAlone ? kRouteAlone : std::max(kRouteTokens, ceil_div(tokens, kNumSMs)); }
 size_t route_counts(int shares, int num_experts) { return static_cast<size_t>(shares) * num_experts * sizeof(int32_t); }
 
 }  // namespace
