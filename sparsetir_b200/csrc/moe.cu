@@ -55,7 +55,7 @@ __device__ __forceinline__ void load_keys(const T* row, int num_experts, int lan
 // the tokens, a warp per token, and counts the pairs of every expert; each block of the second sums the counts of all
 // shares (they are few: 148 at most) and places its share's pairs.  Nothing depends on the order in which blocks run.
 constexpr int kRouteThreads = 1024, kRouteWarps = kRouteThreads / 32;
-constexpr int kRouteAlone = 128;   // tokens that a single block takes
+constexpr int kRouteAlone = 32;   // tokens that a single block takes
 constexpr int kRouteTokens = 32;   // of a share at least; more where there would be over 148 shares
 
 struct PlaceShared {
@@ -141,33 +141,26 @@ choose_kernel(const T* logits, float* gates, int32_t* experts, int32_t* slots, i
     sum = warp_sum(sum);
     int expert = -1;     // of choice `lane`
     uint32_t chosen = 0u;
-    uint32_t best = 0u;  // the lane's largest that is left, and its first place
-    int at = 0;
-    auto look = [&]() {
-      best = 0u;
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (key[r] > best) { best = key[r]; at = r; }
-    };
-    look();
     for (int j = 0; j < top_k; ++j) {
+      uint32_t best = 0u;  // the lane's largest that is left, and its first place
+      int at = 0;
+#pragma unroll
+      for (int r = R - 1; r >= 0; --r) {
+        at = key[r] >= best ? r : at;
+        best = max(best, key[r]);
+      }
       const uint32_t found = __reduce_max_sync(kFull, best);
       if (found == 0u) break;
       const unsigned have = __ballot_sync(kFull, best == found);
       // several lanes: the lowest expert, whose row of 32 comes first, and then its lane
       int src = __ffs(have) - 1;
       if ((have & (have - 1u)) != 0u) src = __reduce_min_sync(kFull, best == found ? at * 32 + lane : 0x7fffffff) & 31;
-      const int who = __shfl_sync(kFull, at, src) * 32 + src;
-      if (lane == src) {
+      const int row = __shfl_sync(kFull, at, src);
+      const int gone = lane == src ? row : -1;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (r == at) key[r] = 0u;
-        look();
-      }
-      if (lane == j) {
-        expert = who;
-        chosen = found;
-      }
+      for (int r = 0; r < R; ++r) key[r] = gone == r ? 0u : key[r];
+      expert = lane == j ? row * 32 + src : expert;
+      chosen = lane == j ? found : chosen;
     }
     const float value = over_top(chosen, top);
     if (renormalize) sum = warp_sum(value);
@@ -208,7 +201,8 @@ place_kernel(const int32_t* experts, int32_t* slots, int32_t* indptr, const int3
   if (row < rows) {
     int before = 0, all = 0;
 #pragma unroll 8
-    for (int b = row; b < shares; b += rows) {
+    for (int i = row; i < shares; i += rows) {
+      const int b = i + block < shares ? i + block : i + block - shares;  // no two blocks at the same place at a time
       const int c = ld_global(counts + static_cast<size_t>(b) * num_experts + e);
       all += c;
       before += b < block ? c : 0;
@@ -389,8 +383,9 @@ combine_kernel(const Piece<B>* z, const int32_t* slots, const float* gates, OutT
 
 constexpr int kRowThreads = 128;  // a block per token
 constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kRowHold = 2;       // pieces of a row that a thread of it has in flight
 
-// Block per token: dy in registers, kHold pieces to a thread at a time, the rows of z one after the other.
+// Block per token: dy in registers, kRowHold pieces to a thread at a time, the rows of z one after the other.
 template <class T, int B>
 __global__ void __launch_bounds__(kRowThreads)
 combine_grad_kernel(const Piece<B>* dy, const Piece<B>* z, const int32_t* slots, const float* gates, Piece<B>* dz, float* d_gates,
@@ -406,28 +401,28 @@ combine_grad_kernel(const Piece<B>* dy, const Piece<B>* z, const int32_t* slots,
     part[lane][warp] = 0.f;
   }
   __syncwarp();
-  for (int base = 0; base < pieces; base += kHold * kRowThreads) {
+  for (int base = 0; base < pieces; base += kRowHold * kRowThreads) {
     const int first = base + tid;
-    Piece<B> d[kHold];
+    Piece<B> d[kRowHold];
 #pragma unroll
-    for (int i = 0; i < kHold; ++i)
+    for (int i = 0; i < kRowHold; ++i)
       if (first + i * kRowThreads < pieces) d[i] = ld_global(dy + static_cast<size_t>(t) * pieces + first + i * kRowThreads);
     // the pieces of the next row are asked for before this one's are used
-    auto ask = [&](int j, Piece<B> (&v)[kHold]) {
+    auto ask = [&](int j, Piece<B> (&v)[kRowHold]) {
       const int s = j < top_k ? __shfl_sync(kFull, slot, j) : -1;
       if (s < 0) return s;
 #pragma unroll
-      for (int i = 0; i < kHold; ++i)
+      for (int i = 0; i < kRowHold; ++i)
         if (first + i * kRowThreads < pieces) v[i] = ld_global(z + static_cast<size_t>(s) * pieces + first + i * kRowThreads);
       return s;
     };
-    auto use = [&](int j, int s, const Piece<B> (&v)[kHold]) {
+    auto use = [&](int j, int s, const Piece<B> (&v)[kRowHold]) {
       if (s < 0) return;
       const float w = __shfl_sync(kFull, gate, j);
       Piece<B>* to = dz + static_cast<size_t>(s) * pieces + first;
       float dot = 0.f;
 #pragma unroll
-      for (int i = 0; i < kHold; ++i) {
+      for (int i = 0; i < kRowHold; ++i) {
         if (first + i * kRowThreads < pieces) {
           float a[N], b[N], o[N];
           unpack<T, B>(d[i], a);
@@ -443,7 +438,7 @@ combine_grad_kernel(const Piece<B>* dy, const Piece<B>* z, const int32_t* slots,
       dot = warp_sum(dot);
       if (lane == 0) part[j][warp] += dot;
     };
-    Piece<B> u[kHold], v[kHold];
+    Piece<B> u[kRowHold], v[kRowHold];
     int su = ask(0, u);
     for (int j = 0; j < top_k; j += 2) {
       const int sv = ask(j + 1, v);
@@ -462,7 +457,7 @@ combine_grad_kernel(const Piece<B>* dy, const Piece<B>* z, const int32_t* slots,
 }
 
 // Block per token: the largest magnitude, as the bits of a float without its sign (so that an infinity or a NaN is
-// larger than all numbers and stays), then the quotients.  Rows of up to kHold pieces to a thread are read once.
+// larger than all numbers and stays), then the quotients.  Rows of up to kRowHold pieces to a thread are read once.
 template <class T, int B>
 __global__ void __launch_bounds__(kRowThreads)
 dispatch_i8_kernel(const Piece<B>* x, const int32_t* slots, Piece<B / sizeof(T)>* q, float* scale, int rows, int pieces,
@@ -473,14 +468,14 @@ dispatch_i8_kernel(const Piece<B>* x, const int32_t* slots, Piece<B / sizeof(T)>
   const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slot = slots != nullptr ? pair_slot(slots, t, top_k, rows, lane) : (lane == 0 ? t : -1);
   const Piece<B>* xr = x + static_cast<size_t>(t) * pieces;
-  Piece<B> v[kHold];
+  Piece<B> v[kRowHold];
   uint32_t bits = 0u;
-  for (int base = 0; base < pieces; base += kHold * kRowThreads) {
+  for (int base = 0; base < pieces; base += kRowHold * kRowThreads) {
 #pragma unroll
-    for (int i = 0; i < kHold; ++i)
+    for (int i = 0; i < kRowHold; ++i)
       if (base + tid + i * kRowThreads < pieces) v[i] = ld_global(xr + base + tid + i * kRowThreads);
 #pragma unroll
-    for (int i = 0; i < kHold; ++i) {
+    for (int i = 0; i < kRowHold; ++i) {
       if (base + tid + i * kRowThreads < pieces) {
         float f[N];
         unpack<T, B>(v[i], f);
@@ -498,14 +493,14 @@ dispatch_i8_kernel(const Piece<B>* x, const int32_t* slots, Piece<B / sizeof(T)>
   const bool zeros = !(a >= 0x1p-119f && a < INFINITY);
   const float inv = zeros ? 0.f : 127.f / a;
   if (tid < top_k && slot >= 0) scale[slot] = a < 0x1p-119f ? 0.f : a / 127.f;
-  for (int base = 0; base < pieces; base += kHold * kRowThreads) {
-    if (pieces > kHold * kRowThreads) {  // otherwise they are here still
+  for (int base = 0; base < pieces; base += kRowHold * kRowThreads) {
+    if (pieces > kRowHold * kRowThreads) {  // otherwise they are here still
 #pragma unroll
-      for (int i = 0; i < kHold; ++i)
+      for (int i = 0; i < kRowHold; ++i)
         if (base + tid + i * kRowThreads < pieces) v[i] = ld_global(xr + base + tid + i * kRowThreads);
     }
 #pragma unroll
-    for (int i = 0; i < kHold; ++i) {
+    for (int i = 0; i < kRowHold; ++i) {
       const int at = base + tid + i * kRowThreads;
       Piece<N> o;
       if (at < pieces) {
