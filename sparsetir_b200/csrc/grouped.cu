@@ -250,7 +250,24 @@ __device__ __forceinline__ void store_halves(OutT* to, int pitch, int feats, int
   }
 }
 
-// The same for 32-bit elements and for rows at any address: lane = feature, a store per column.
+// Zeros to the same places.
+template <int STEP, class OutT>
+__device__ __forceinline__ void store_zeros(OutT* to, int pitch, int feats, int first, int n, bool wide, int lane) {
+  for (int c0 = first; c0 < n; c0 += STEP) {
+    if (sizeof(OutT) == 2 && wide) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + 8 * i + (lane >> 2), f = (lane & 3) * 8;
+        if (c < n && f < feats) *reinterpret_cast<uint4*>(to + static_cast<size_t>(c) * pitch + f) = make_uint4(0u, 0u, 0u, 0u);
+      }
+    } else if (lane < feats) {
+#pragma unroll 8
+      for (int c = c0; c < min(c0 + 32, n); ++c) to[static_cast<size_t>(c) * pitch + lane] = OutT{};
+    }
+  }
+}
+
+// The same as store_halves for 32-bit elements and for rows at any address: lane = feature, a store per column.
 template <bool I8, int STEP, class OutT, class Take>
 __device__ __forceinline__ void store_lanes(OutT* to, int pitch, int feats, int first, int n, uint32_t taddr, const float* xs, const float* ws,
                                             int lane, Take&& take) {
@@ -523,13 +540,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       uint32_t* const part = p.splits > 1 ? static_cast<uint32_t*>(p.parts) + tile.split * p.part + at : nullptr;
       const int feats = p.features - feat0;  // live ones of the warp's, may be <= 0 or > 32
       if (tile.steps == 0) {  // a group without rows, or nothing of the depth left for this unit
-        if (lane < feats)
-          for (int c = mine / 32; c < tile.n; c += kEpilogue / 4) {
-            if (part != nullptr)
-              part[static_cast<size_t>(c) * p.features + lane] = 0u;
-            else
-              to[static_cast<size_t>(c) * p.features + lane] = from_float<OutT>(0.f);
-          }
+        if (part != nullptr) {
+          store_zeros<kStep>(part, p.features, feats, mine, tile.n, false, lane);
+        } else {
+          store_zeros<kStep>(to, p.features, feats, mine, tile.n, p.wide != 0, lane);
+        }
         continue;
       }
       const int buf = acc & 1;

@@ -414,6 +414,20 @@ def test_grouped_large(cuda_device, sizes, fi, fo, out_in):
     check_grouped(sizes, fi, fo, torch.bfloat16, out_in, torch.bfloat16, cuda_device)
 
 
+@pytest.mark.parametrize("sizes,fi,fo", [([100], 4096, 520), ([33, 0, 50, 41], 2056, 200), ([300], 8200, 72)])
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.float16, torch.float16), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("out_in", [False, True])
+def test_grouped_depth_shared_by_several_units(cuda_device, sizes, fi, fo, dtype, out_dtype, out_in):
+    check_grouped(sizes, fi, fo, dtype, out_in, out_dtype, cuda_device, tail=9)
+
+
+@pytest.mark.parametrize("sizes,fi,fo", [([3], 4096, 2000), ([5, 0, 16, 17, 1, 0, 33], 1024, 520), ([1] * 70, 136, 40), ([9], 200, 9)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("out_in", [False, True])
+def test_grouped_few_rows(cuda_device, sizes, fi, fo, dtype, out_in):
+    check_grouped(sizes, fi, fo, dtype, out_in, dtype, cuda_device, tail=3)
+
+
 def test_grouped_values_stay_in_their_rows_and_groups(cuda_device):
     sizes, fi, fo = [40, 0, 25, 130], 96, 136
     g = gen(3, cuda_device)
@@ -458,6 +472,17 @@ def test_grouped_with_wild_pointers_stays_inside(cuda_device, bad):
     assert (dw[:1000] == 9).all() and (dw[-1000:] == 9).all()
 
 
+@pytest.mark.parametrize("fi,rows", [(2048, 30), (64, 3000), (4096, 900)])
+def test_grouped_with_wild_pointers_in_every_kernel(cuda_device, fi, rows):
+    fo = 264
+    x, w = torch.ones(rows * fi, device=cuda_device).half(), torch.ones(3 * fi * fo, device=cuda_device).half()
+    for bad in ([0, rows, 5, rows + 9], [-3, rows // 2, 2 ** 31 - 1, 0], [rows, 7, -2 ** 31, rows]):
+        guard = torch.full((1000 + rows * fo + 1000,), 9.0, device=cuda_device)
+        ptr = torch.tensor(bad, device=cuda_device).int()
+        ops.grouped_mm(x, w, guard[1000:1000 + rows * fo], ptr, 3, fi, fo)
+        assert (guard[:1000] == 9).all() and (guard[-1000:] == 9).all()
+
+
 def check_grad_w(sizes, fi, fo, dtype, out_in, out_dtype, device, shift=0, tail=0):
     g = gen(fi * 5 + fo, device)
     n, rows = len(sizes), sum(sizes)
@@ -499,6 +524,18 @@ def test_grad_w_operands_at_odd_addresses(cuda_device, shift, fi, fo):
 @pytest.mark.parametrize("sizes,fi,fo", [([2000, 100, 1700], 1024, 1000), ([700] * 8, 512, 768), ([5000], 264, 520)])
 def test_grad_w_large(cuda_device, sizes, fi, fo):
     check_grad_w(sizes, fi, fo, torch.bfloat16, False, torch.bfloat16, cuda_device)
+
+
+@pytest.mark.parametrize("sizes,fi,fo", [([3000, 0, 130, 2870], 72, 136), ([6001], 40, 8), ([0, 0, 5000], 264, 24)])
+@pytest.mark.parametrize("out_dtype", [torch.float16, torch.float32])
+def test_grad_w_depth_shared_by_several_units(cuda_device, sizes, fi, fo, out_dtype):
+    check_grad_w(sizes, fi, fo, torch.float16, False, out_dtype, cuda_device, tail=70)
+
+
+@pytest.mark.parametrize("out_in", [False, True])
+@pytest.mark.parametrize("fo", [200, 203])
+def test_grad_w_of_groups_without_rows(cuda_device, out_in, fo):
+    check_grad_w([0] * 20 + [3] + [0] * 20, 264, fo, torch.bfloat16, out_in, torch.bfloat16, cuda_device)
 
 
 def test_grad_w_rows_of_other_groups_do_not_matter(cuda_device):
@@ -578,6 +615,11 @@ def test_i8_features(cuda_device, fi, fo, out_dtype):
 @pytest.mark.parametrize("fi,fo", [(64, 72), (63, 40)])
 def test_i8_operands_at_odd_addresses(cuda_device, shift, fi, fo):
     check_i8([30, 100], fi, fo, torch.float32, cuda_device, shift=shift)
+
+
+@pytest.mark.parametrize("sizes,fi,fo", [([100], 8200, 520), ([33, 0, 50, 41] * 10, 4112, 72), ([3], 4096, 2000), ([5, 0, 16, 17, 1, 0, 33], 1040, 520)])
+def test_i8_depth_shared(cuda_device, sizes, fi, fo):
+    check_i8(sizes, fi, fo, torch.float32, cuda_device, tail=9)
 
 
 def test_i8_extremes_and_one_dense_product(cuda_device):
