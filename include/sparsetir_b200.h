@@ -548,8 +548,8 @@ SPARSETIR_API int sparsetir_moe_combine_raw(const void* z, int z_type, const int
 SPARSETIR_API int sparsetir_moe_combine_grad_raw(const void* dy, const void* z, int type, const int32_t* slots,
                                                  const float* gates, void* dz, float* d_gates, int tokens, int rows,
                                                  int feat, int top_k, int device_id, void* stream);
-/* Scratch bytes of the grouped products at most: copies of operands of element_bytes (1 or 2) whose rows do not start at
- * 16-byte addresses.  Operands at aligned addresses with rows of a multiple of 16 bytes need none. */
+/* Scratch bytes at most of sparsetir_grouped_mm and its gradient (element_bytes 2) or of sparsetir_grouped_mm_i8 (1): copies of
+ * operands whose rows do not start at 16-byte addresses, and sums of thread blocks that share a tile (20 MB at most). */
 SPARSETIR_API int sparsetir_grouped_mm_workspace(int rows, int num_groups, int feat_in, int feat_out, int element_bytes,
                                                  int flags, size_t* scratch_bytes);
 /* rows: how many x and y have; row pointers outside of [0, rows] are taken as the nearer bound */

@@ -6,8 +6,19 @@
 // All three are one kernel.  A pair of blocks (cta_group::2) holds 256 of what is contiguous in the result (output
 // features; b) as the rows of the tensor core's left operand, and up to 256 of what is not (rows of the group; a) as the columns:
 // the result comes out of TMEM with neighbouring lanes at neighbouring addresses, and a ragged group costs its rows rounded
-// up to 32, whatever the group's neighbours are.  How many rows a group has is read from indptr on the device, by every
-// role of the block for itself.
+// up to 32, whatever the group's neighbours are.  Rows of the neighbours that a load brings along become columns that nobody
+// stores; in the gradient, where rows are the depth, they are cleared in shared memory.  How many rows a group has is read from
+// indptr on the device.
+//
+// A ring of six stages of 32 KB is fed by TMA, MMAs of 256 x 256 x 16 (x 32) go to one of two accumulators while eight warps
+// take the other one out; tiles that are not running yet are taken over by pairs that are done (cluster launch control).
+// With all operands in L2 a step of K (64 deep, 512 clocks of the tensor core) takes 0.28 us of loads, 117 GB/s into each SM:
+// loads and MMAs are even, and beyond about 1.2 PFLOP/s the power limit lowers the clock.  65,536 rows in 64 ragged groups, 2048 ->
+// 2048, bf16: 0.45-0.51 ms, 1.08-1.2 PFLOP/s, by the clock (8192^3 in one group: 0.71-0.83 ms; torch.matmul 0.75).  The
+// gradient of 64 weights of 2048 x 1024 over 32,768 rows, 8 steps to a tile, 0.13-0.17 ms: its 470 MB alone are 72 us.
+// Tried and taken back: equal column tiles instead of 256 and a remainder (more, smaller loads: 54 -> 45 us on 6,001 rows); a
+// prefetch of the next tiles' operands to L2 (44 -> 60); the whole tiles of all groups first (no change); one arrival
+// of the loading thread at the other block's barrier per step (935 us where now 500).
 #include <algorithm>
 
 #include "common.h"
@@ -29,7 +40,9 @@ constexpr int kStagedBytes = 32 * 64; // 32 columns of 32 features on their way 
 constexpr int kTiles = 4;             // entries of the ring of tiles
 constexpr int kBand = 8;              // column tiles of a group that are walked side by side
 
-// Columns of a tile, and what follows from them.
+// Columns of a tile, and what follows from them.  128 leave room for two pairs of blocks on two SMs: for many groups of few rows,
+// where the loads of one pair hide the other's beginning and end (us, 256 / 128 columns: 64 groups of 16 rows, 512 -> 512
+// 13.6 / 7.6; 500 rows in 64 groups, 2048 -> 2048 91.4 / 90.3; 8 groups of 500 rows 39 / 41).
 template <int N> struct Shape {
   static constexpr int kBytes = kABytes + N / 2 * 128;  // of a stage
   static constexpr int kStages = N == 256 ? 6 : 4;
@@ -185,10 +198,10 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
   return reinterpret_cast<const uint32_t&>(v);
 }
 
-// Columns first .. n - 1, 32 of every STEP, of 32 features from TMEM to rows of the result, 16-bit elements at 16-byte addresses.  The fragments of 8
-// columns and 32 features are transposed on their way to shared memory (rows of 32 features, pieces of 16 bytes exchanged
-// so that neither side collides) and leave as 16 bytes to a lane.  With a 2-byte store per lane and column the epilogue took
-// longer than the products of 2048-deep tiles: 576 us where this takes REPLACE (65,536 rows, 2048 -> 2048).
+// Columns first .. n - 1, 32 of every STEP, of 32 features from TMEM to rows of the result, 16-bit elements at 16-byte
+// addresses.  The fragments of 8 columns and 32 features are transposed on their way to shared memory (rows of 32 features,
+// pieces of 16 bytes exchanged so that neither side collides) and leave as 16 bytes to a lane.  With a 2-byte store per lane and column the epilogue took
+// longer than the products of shallow tiles (us, then / with this: gradient of 64 weights of 2048 x 1024 287 / 175).
 template <bool I8, int STEP, class OutT, class Take>
 __device__ __forceinline__ void store_halves(OutT* to, int pitch, int feats, int first, int n, uint32_t taddr, unsigned char* staged,
                                              const float* xs, const float* ws, int lane, Take&& take) {
@@ -495,8 +508,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       advance(tile.steps);
     }
   } else if (warp == 3) {
-    // ---- tiles.  The launch has a pair of blocks for every unit, and those that are not running yet are waited for by nobody:
-    // a pair that is takes the next one's work until there is none.  (Units dealt out beforehand: REPLACE.)
+    // ---- tiles.  The launch has a pair of blocks for every unit; a pair that runs takes over the work of one that does not yet,
+    // until there is none.  (us, units dealt out beforehand / this: 65,536 rows in 64 groups, 512 -> 2048 170 / 148; 16,000
+    // rows, 1024 -> 1024 61 / 57.)
     int at = 0;
     bool more = rank == 0 && p.deal != 0 && walk.at(pair, &tile);  // there are readers
     while (rank == 0 && p.deal != 0) {
@@ -734,6 +748,9 @@ int check_pointers(const char* fn, const int32_t* indptr, int rows, int groups, 
 }
 // Sets the tiles of p, and how many units share the depth of a tile, from what the host knows: `bound(n)` column tiles of n
 // at most, about `some(n)` of them, `depth` steps each, and `rows` rows of the result.  Returns the columns of a tile, or -1.
+// Units share a depth where the tiles are half as many as the pairs or fewer, into parts of four steps at least, and where that
+// spares the twelve steps that the second launch costs (us, one unit / several: 100 rows, 4096 -> 4096 23 / 14; gradient of one
+// 504 x 1000 weight over 60,000 rows 263 / 67; 300 rows, 4096 -> 4096, two units, 23 / 24).
 template <class Bound, class Some>
 int set_tiles(const char* fn, Args* p, bool few_columns, Bound&& bound, Some&& some, int depth, long long rows) {
   p->mt = ceil_div(p->features, 2 * kM);
@@ -751,6 +768,22 @@ int set_tiles(const char* fn, Args* p, bool few_columns, Bound&& bound, Some&& s
   p->per_split = Divisor(p->splits);
   p->per_band = Divisor(kBand * p->mt);
   p->part = rows * p->features;
+  return columns;
+}
+// For rows, groups, k and features of p, steps of `depth` of K.
+int plan_product(const char* fn, Args* p, int depth) {
+  const long long rows = p->rows, used = std::min(p->groups, p->rows);
+  return set_tiles(fn, p, rows <= 128 * used, [&](int n) { return rows / n + used; },
+                   [&](int n) { return used * ((rows + used * n - 1) / (used * n)); }, ceil_div(p->k, depth), rows);
+}
+// For rows, groups, features and columns of p.
+int plan_grad(const char* fn, Args* p) {
+  auto tiles = [&](int n) { return static_cast<long long>(p->groups) * ceil_div(p->columns, n); };
+  const int columns = set_tiles(fn, p, false, tiles, tiles, ceil_div(ceil_div(p->rows, p->groups), 64),
+                                static_cast<long long>(p->groups) * p->columns);
+  if (columns < 0) return -1;
+  p->nt = ceil_div(p->columns, columns);
+  p->per_group = Divisor(p->mt * p->nt);
   return columns;
 }
 size_t part_bytes(const Args& p) { return p.splits > 1 ? p.part * p.splits * sizeof(float) : 0; }
@@ -794,9 +827,7 @@ int product(const char* fn, const void* x, const void* w, int type, void* y, int
   p.a_mn = out_in ? 0 : 1;
   p.wide = wide_rows(y, y_type, fo);
   p.idesc = i8 ? tc05::instr_desc_i8(2 * kM, 0) : tc05::instr_desc(map_format(type), 2 * kM, 0, p.a_mn, 0);
-  const long long used = std::min(groups, rows);
-  const int columns = set_tiles(fn, &p, rows <= 128 * used, [&](int n) { return rows / n + used; },
-                                [&](int n) { return used * ((rows + used * n - 1) / (used * n)); }, ceil_div(fi, depth), rows);
+  const int columns = plan_product(fn, &p, depth);
   if (columns < 0) return -1;
   Operand ox{x, rows, fi, size}, ow{w, static_cast<long long>(groups) * (out_in ? fo : fi), out_in ? fi : fo, size};
   const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + part_bytes(p);
@@ -895,11 +926,8 @@ extern "C" int sparsetir_grouped_mm_grad_w_raw(const void* x, const void* dy, in
   p.columns = out_in ? feat_out : feat_in;
   p.wide = wide_rows(dw, dw_type, p.features);
   p.idesc = tc05::instr_desc(map_format(type), 2 * kM, 0, 1, 1);
-  auto tiles = [&](int n) { return static_cast<long long>(num_groups) * ceil_div(p.columns, n); };
-  const int columns = set_tiles(fn, &p, false, tiles, tiles, ceil_div(ceil_div(rows, num_groups), 64), static_cast<long long>(num_groups) * p.columns);
+  const int columns = plan_grad(fn, &p);
   if (columns < 0) return -1;
-  p.nt = ceil_div(p.columns, columns);
-  p.per_group = Divisor(p.mt * p.nt);
   Operand oa{out_in ? x : dy, rows, p.features, 2}, ob{out_in ? dy : x, rows, p.columns, 2};
   const size_t bytes = oa.copy_bytes() + ob.copy_bytes() + part_bytes(p);
   CallScratch cs;
@@ -921,9 +949,21 @@ extern "C" int sparsetir_grouped_mm_workspace(int rows, int num_groups, int feat
   const char* fn = "sparsetir_grouped_mm_workspace";
   if (check_groups(fn, nullptr, rows, std::min(num_groups, 1), feat_in, feat_out, flags) != 0) return -1;
   if ((element_bytes != 1 && element_bytes != 2) || !scratch_bytes) return fail("%s: bad argument", fn);
+  *scratch_bytes = 0;
+  if (rows == 0 || num_groups == 0) return 0;
+  const bool out_in = element_bytes == 1 || (flags & SPARSETIR_GROUPED_W_OUT_IN) != 0;
+  // copies of both operands, whatever their addresses, and the sums of units that share a tile
   auto copy = [&](long long n, int cols) -> size_t { return (Operand{nullptr, n, cols, element_bytes}.padded() * n + 255) / 256 * 256; };
-  const bool out_in = (flags & SPARSETIR_GROUPED_W_OUT_IN) != 0;
-  const size_t w = copy(static_cast<long long>(num_groups) * (out_in ? feat_out : feat_in), out_in ? feat_in : feat_out);
-  *scratch_bytes = copy(rows, feat_in) + std::max(w, copy(rows, feat_out));
+  Args p{};
+  p.rows = rows;
+  p.groups = num_groups;
+  p.k = feat_in;
+  p.features = feat_out;
+  if (plan_product(fn, &p, 128 / element_bytes) < 0) return -1;
+  const size_t product = copy(static_cast<long long>(num_groups) * (out_in ? feat_out : feat_in), out_in ? feat_in : feat_out) + part_bytes(p);
+  p.features = out_in ? feat_in : feat_out;
+  p.columns = out_in ? feat_out : feat_in;
+  if (plan_grad(fn, &p) < 0) return -1;
+  *scratch_bytes = copy(rows, feat_in) + std::max(product, element_bytes == 1 ? 0 : copy(rows, feat_out) + part_bytes(p));
   return 0;
 }

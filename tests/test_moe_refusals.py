@@ -149,12 +149,20 @@ def test_scratch_queries():
         assert getattr(L.load(), name)(*sizes, ctypes.byref(out)) == 0, L.last_error()
         return out.value
 
-    assert ask("sparsetir_moe_route_workspace", 0, 8) == ask("sparsetir_moe_route_workspace", 128, 1024) == 0
-    assert ask("sparsetir_moe_route_workspace", 129, 8) == 2 * 8 * 4
+    assert ask("sparsetir_moe_route_workspace", 0, 8) == ask("sparsetir_moe_route_workspace", 32, 1024) == 0
+    assert ask("sparsetir_moe_route_workspace", 33, 8) == 2 * 8 * 4
     assert ask("sparsetir_moe_route_workspace", 2 ** 31 - 1, 1024) <= 148 * 1024 * 4
     # copies at rows of a multiple of 16 bytes
     assert ask("sparsetir_grouped_mm_workspace", 100, 4, 9, 16, 2, 1) == 100 * 32 + 128 + max(4 * 16 * 32, 100 * 32 + 128)
-    assert ask("sparsetir_grouped_mm_workspace", 0, 4, 17, 16, 1, 0) == 4 * 17 * 16 + 192
+    assert ask("sparsetir_grouped_mm_workspace", 100, 4, 17, 16, 1, 0) == 100 * 32 + 128 + 4 * 16 * 32
+    assert ask("sparsetir_grouped_mm_workspace", 0, 4, 17, 16, 1, 0) == ask("sparsetir_grouped_mm_workspace", 4, 0, 17, 16, 2, 0) == 0
+    # sums of units that share a tile: of the gradient, of the product; of no more units than run at a time
+    assert ask("sparsetir_grouped_mm_workspace", 64000, 1, 256, 256, 2, 0) == 2 * 64000 * 512 + 74 * 256 * 256 * 4
+    assert ask("sparsetir_grouped_mm_workspace", 300, 1, 4096, 256, 2, 1) == 300 * 8192 + 256 * 8192 + 16 * 300 * 256 * 4
+    for rows in (1, 100, 10_000, 1_000_000):
+        for sizes in ((1, 64, 64), (1, 4096, 64), (8, 512, 512), (64, 2048, 2048), (1, 100_000, 8)):
+            copies = 2 * (rows * sizes[1] + max(sizes[0] * sizes[1] * sizes[2], rows * sizes[2])) + 512
+            assert ask("sparsetir_grouped_mm_workspace", rows, *sizes, 2, 1) <= copies + (20 << 20)
     for name, sizes in (("sparsetir_moe_route_workspace", (-1, 8)), ("sparsetir_moe_route_workspace", (4, 0)),
                         ("sparsetir_grouped_mm_workspace", (4, 4, 0, 8, 2, 0)), ("sparsetir_grouped_mm_workspace", (4, 4, 8, 8, 3, 0))):
         assert getattr(L.load(), name)(*sizes, ctypes.byref(out)) == -1
