@@ -30,29 +30,52 @@ __device__ __forceinline__ float over_top(uint32_t key, uint32_t top) {
   if (key == 0u) return 0.f;
   return key == top ? 1.f : expf(key_value(key) - key_value(top));
 }
-__device__ __forceinline__ float warp_sum(float v) {
+
+// Reductions over the L lanes of a token.
+template <int L>
+__device__ __forceinline__ uint32_t most_of(uint32_t v) {
+  if constexpr (L == 32) {
+    return __reduce_max_sync(kFull, v);
+  } else {
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    for (int o = L / 2; o >= 1; o >>= 1) v = max(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+  }
+}
+template <int L>
+__device__ __forceinline__ int least_of(int v) {
+  if constexpr (L == 32) {
+    return __reduce_min_sync(kFull, v);
+  } else {
+#pragma unroll
+    for (int o = L / 2; o >= 1; o >>= 1) v = min(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+  }
+}
+template <int L>
+__device__ __forceinline__ float sum_of(float v) {
+#pragma unroll
+  for (int o = L / 2; o >= 1; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   return v;
 }
 
-// A token's logits, R to a lane: lane l has those of the experts l, l + 32, ...
-template <class T, int R>
-__device__ __forceinline__ void load_keys(const T* row, int num_experts, int lane, uint32_t (&key)[R]) {
+// A token's logits, R to each of L lanes: lane l has those of the experts l, l + L, ...
+template <class T, int L, int R>
+__device__ __forceinline__ void load_keys(const T* row, int num_experts, int l, bool live, uint32_t (&key)[R]) {
   constexpr int G = R < 8 ? R : 8;  // in flight
 #pragma unroll
   for (int r0 = 0; r0 < R; r0 += G) {
     T v[G];
 #pragma unroll
     for (int r = 0; r < G; ++r)
-      if (lane + 32 * (r0 + r) < num_experts) v[r] = ld_global(row + lane + 32 * (r0 + r));
+      if (live && l + L * (r0 + r) < num_experts) v[r] = ld_global(row + l + L * (r0 + r));
 #pragma unroll
-    for (int r = 0; r < G; ++r) key[r0 + r] = lane + 32 * (r0 + r) < num_experts ? order_key(to_float(v[r])) : 0u;
+    for (int r = 0; r < G; ++r) key[r0 + r] = live && l + L * (r0 + r) < num_experts ? order_key(to_float(v[r])) : 0u;
   }
 }
 
 // The router is two launches, or one where a single block has all tokens.  Each block of the first chooses for its share of
-// the tokens, a warp per token, and counts the pairs of every expert; each block of the second sums the counts of all
+// the tokens, L lanes to a token, and counts the pairs of every expert; each block of the second sums the counts of all
 // shares (they are few: 148 at most) and places its share's pairs.  Nothing depends on the order in which blocks run.
 constexpr int kRouteThreads = 1024, kRouteWarps = kRouteThreads / 32;
 constexpr int kRouteAlone = 32;   // tokens that a single block takes
@@ -116,30 +139,34 @@ __device__ __forceinline__ void place_pairs(PlaceShared& s, const int32_t* exper
   }
 }
 
-// p[i] = exp(z[i] - max z) / sum; the top_k largest are found one after the other, each by a maximum over the keys of the
-// warp and the lowest index that has it.
-template <class T, int R>
+// p[i] = exp(z[i] - max z) / sum; the top_k <= L largest are found one after the other, each by a maximum over the keys of the
+// token's lanes and the lowest index that has it.  What it costs is instructions, some hundred to a token, and one token's chain of
+// them where there are few: the 8.4 MB of 16,384 tokens of 128 logits would be 1.3 us, the launch takes 9.
+template <class T, int L, int R>
 __global__ void __launch_bounds__(kRouteThreads)
 choose_kernel(const T* logits, float* gates, int32_t* experts, int32_t* slots, int32_t* indptr, int32_t* counts, int tokens,
               int share, int num_experts, int top_k, int renormalize) {
   __shared__ PlaceShared s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int l = lane % L, first_lane = lane - l;
   s.next[tid] = 0;
   chain_wait();
   __syncthreads();
   const int t0 = blockIdx.x * share, t1 = t0 + min(share, tokens - t0);
-  for (int t = t0 + warp; t < t1; t += kRouteWarps) {
+  for (int tw = t0 + warp * (32 / L); tw < t1; tw += kRouteWarps * (32 / L)) {
+    const int t = tw + lane / L;
+    const bool live = t < t1;
     uint32_t key[R];
-    load_keys<T, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, lane, key);
+    load_keys<T, L, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, l, live, key);
     uint32_t most = 0u;
 #pragma unroll
     for (int r = 0; r < R; ++r) most = max(most, key[r]);
-    const uint32_t top = __reduce_max_sync(kFull, most);
+    const uint32_t top = most_of<L>(most);
     float sum = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) sum += over_top(key[r], top);
-    sum = warp_sum(sum);
-    int expert = -1;     // of choice `lane`
+    sum = sum_of<L>(sum);
+    int expert = -1;     // of choice l
     uint32_t chosen = 0u;
     for (int j = 0; j < top_k; ++j) {
       uint32_t best = 0u;  // the lane's largest that is left, and its first place
@@ -149,23 +176,25 @@ choose_kernel(const T* logits, float* gates, int32_t* experts, int32_t* slots, i
         at = key[r] >= best ? r : at;
         best = max(best, key[r]);
       }
-      const uint32_t found = __reduce_max_sync(kFull, best);
-      if (found == 0u) break;
-      const unsigned have = __ballot_sync(kFull, best == found);
-      // several lanes: the lowest expert, whose row of 32 comes first, and then its lane
+      const uint32_t found = most_of<L>(best);
+      if (!__any_sync(kFull, found != 0u)) break;
+      const unsigned have = (__ballot_sync(kFull, best == found) >> first_lane) & (L == 32 ? kFull : (1u << (L & 31)) - 1u);
+      // several lanes: the lowest expert, whose row of L comes first, and then its lane
       int src = __ffs(have) - 1;
-      if ((have & (have - 1u)) != 0u) src = __reduce_min_sync(kFull, best == found ? at * 32 + lane : 0x7fffffff) & 31;
-      const int row = __shfl_sync(kFull, at, src);
-      const int gone = lane == src ? row : -1;
+      if (__any_sync(kFull, (have & (have - 1u)) != 0u)) src = least_of<L>(best == found ? at * L + l : 0x7fffffff) % L;
+      const int row = __shfl_sync(kFull, at, first_lane + src);
+      const int gone = l == src ? row : -1;
 #pragma unroll
       for (int r = 0; r < R; ++r) key[r] = gone == r ? 0u : key[r];
-      expert = lane == j ? row * 32 + src : expert;
-      chosen = lane == j ? found : chosen;
+      if (l == j && found != 0u) {
+        expert = row * L + src;
+        chosen = found;
+      }
     }
     const float value = over_top(chosen, top);
-    if (renormalize) sum = warp_sum(value);
-    if (lane < top_k) {
-      const size_t p = static_cast<size_t>(t) * top_k + lane;
+    if (renormalize) sum = sum_of<L>(value);
+    if (live && l < top_k) {
+      const size_t p = static_cast<size_t>(t) * top_k + l;
       experts[p] = expert;
       gates[p] = expert < 0 ? 0.f : value / sum;
       if (expert >= 0) atomicAdd(&s.next[expert], 1);
@@ -221,26 +250,26 @@ place_kernel(const int32_t* experts, int32_t* slots, int32_t* indptr, const int3
   place_pairs(s, experts, slots, t0 * top_k, t1 * top_k, num_experts);
 }
 
-template <class T, int R>
+template <class T, int L, int R>
 __global__ void __launch_bounds__(kWarps * 32)
 route_grad_kernel(const T* logits, const float* gates, const int32_t* experts, const float* d_gates, T* d_logits, int tokens,
                   int num_experts, int top_k, int renormalize) {
   chain_wait();
-  const int lane = threadIdx.x & 31;
-  const int t = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (t >= tokens) return;
+  const int lane = threadIdx.x & 31, l = lane % L;
+  const int t = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * (32 / L) + lane / L;
+  const bool live = t < tokens;
   int expert = -1;
   float gate = 0.f, dg = 0.f;
-  if (lane < top_k) {
-    const size_t p = static_cast<size_t>(t) * top_k + lane;
+  if (live && l < top_k) {
+    const size_t p = static_cast<size_t>(t) * top_k + l;
     expert = ld_global(experts + p);
     gate = ld_global(gates + p);
     dg = ld_global(d_gates + p);
   }
   uint32_t key[R];
-  load_keys<T, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, lane, key);
+  load_keys<T, L, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, l, live, key);
   if (expert < 0) gate = dg = 0.f;
-  const float mean = warp_sum(gate * dg);
+  const float mean = sum_of<L>(gate * dg);
   float grad[R];
   if (renormalize) {
 #pragma unroll
@@ -250,39 +279,48 @@ route_grad_kernel(const T* logits, const float* gates, const int32_t* experts, c
     uint32_t most = 0u;
 #pragma unroll
     for (int r = 0; r < R; ++r) most = max(most, key[r]);
-    const uint32_t top = __reduce_max_sync(kFull, most);
+    const uint32_t top = most_of<L>(most);
     float sum = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       grad[r] = over_top(key[r], top);
       sum += grad[r];
     }
-    sum = warp_sum(sum);
+    sum = sum_of<L>(sum);
 #pragma unroll
     for (int r = 0; r < R; ++r) grad[r] = key[r] != 0u ? -mean * (grad[r] / sum) : 0.f;
   }
   for (int j = 0; j < top_k; ++j) {
-    const int e = __shfl_sync(kFull, expert, j);
-    const float add = __shfl_sync(kFull, gate * dg, j);
+    const int e = __shfl_sync(kFull, expert, lane - l + j);
+    const float add = __shfl_sync(kFull, gate * dg, lane - l + j);
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (lane + 32 * r == e) grad[r] += add;
+      if (l + L * r == e) grad[r] += add;
   }
+  if (!live) return;
   T* out = d_logits + static_cast<size_t>(t) * num_experts;
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    if (lane + 32 * r < num_experts) out[lane + 32 * r] = from_float<T>(grad[r]);
+    if (l + L * r < num_experts) out[l + L * r] = from_float<T>(grad[r]);
 }
 
-// f(integral constant R) with R * 32 >= num_experts
+// f(L, R) as integral constants, L * R >= num_experts.  8 lanes to a token, for up to `most` experts, where the SMs have warps
+// enough all the same (us, 32 lanes / 8: router of 16,384 tokens, 128 experts, 8 choices 20.4 / 17.5, 65,536 tokens, 64, 6 36.8 /
+// 27.0, 8,192, 128, 8 14.0 / 13.9, 2,000, 128, 8 8.8 / 9.8; the gradient of the first 7.4 / 7.8, of the second 16.4 / 11.6).
 template <class F>
-int with_lane_share(int num_experts, F&& f) {
-  if (num_experts <= 32) return f(std::integral_constant<int, 1>{});
-  if (num_experts <= 64) return f(std::integral_constant<int, 2>{});
-  if (num_experts <= 128) return f(std::integral_constant<int, 4>{});
-  if (num_experts <= 256) return f(std::integral_constant<int, 8>{});
-  if (num_experts <= 512) return f(std::integral_constant<int, 16>{});
-  return f(std::integral_constant<int, 32>{});
+int with_lanes(int tokens, int num_experts, int top_k, int most, F&& f) {
+  using std::integral_constant;
+  if (tokens >= 8192 && num_experts <= most && top_k <= 8) {
+    if (num_experts <= 32) return f(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+    if (num_experts <= 64) return f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+    return f(integral_constant<int, 8>{}, integral_constant<int, 16>{});
+  }
+  if (num_experts <= 32) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+  if (num_experts <= 64) return f(integral_constant<int, 32>{}, integral_constant<int, 2>{});
+  if (num_experts <= 128) return f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+  if (num_experts <= 256) return f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+  if (num_experts <= 512) return f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+  return f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
 }
 
 // ---- rows -----------------------------------------------------------------------------------------------------------
@@ -435,7 +473,7 @@ combine_grad_kernel(const Piece<B>* dy, const Piece<B>* z, const int32_t* slots,
           to[i * kRowThreads] = pack<T, B>(o);
         }
       }
-      dot = warp_sum(dot);
+      dot = sum_of<32>(dot);
       if (lane == 0) part[j][warp] += dot;
     };
     Piece<B> u[kRowHold], v[kRowHold];
@@ -580,8 +618,8 @@ extern "C" int sparsetir_moe_route_raw(const void* logits, int logits_type, floa
   int32_t* counts = reinterpret_cast<int32_t*>(cs.scratch);
   const int rc = with_type(logits_type, [&](auto t) {
     using T = decltype(t);
-    return with_lane_share(num_experts, [&](auto r) {
-      launch_chained(choose_kernel<T, r.value>, shares, kRouteThreads, 0, st, static_cast<const T*>(logits), gates, experts, slots,
+    return with_lanes(tokens, num_experts, top_k, 128, [&](auto l, auto r) {
+      launch_chained(choose_kernel<T, l.value, r.value>, shares, kRouteThreads, 0, st, static_cast<const T*>(logits), gates, experts, slots,
                      indptr, counts, tokens, share, num_experts, top_k, flags & SPARSETIR_MOE_RENORMALIZE);
       SPTIR_LAUNCH_OK("choose_kernel");
       return 0;
@@ -615,8 +653,8 @@ extern "C" int sparsetir_moe_route_grad_raw(const void* logits, int logits_type,
     return -1;
   return with_type(logits_type, [&](auto t) {
     using T = decltype(t);
-    return with_lane_share(num_experts, [&](auto r) {
-      launch_chained(route_grad_kernel<T, r.value>, ceil_div(tokens, kWarps), kWarps * 32, 0, st, static_cast<const T*>(logits),
+    return with_lanes(tokens, num_experts, top_k, 64, [&](auto l, auto r) {
+      launch_chained(route_grad_kernel<T, l.value, r.value>, ceil_div(tokens, kWarps * 32 / l.value), kWarps * 32, 0, st, static_cast<const T*>(logits),
                      gates, experts, d_gates, static_cast<T*>(d_logits), tokens, num_experts, top_k,
                      flags & SPARSETIR_MOE_RENORMALIZE);
       SPTIR_LAUNCH_OK("route_grad_kernel");

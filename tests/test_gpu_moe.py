@@ -102,7 +102,8 @@ def test_route(cuda_device, t, e, k, dtype, renorm):
     check_route(z, k, renorm)
 
 
-@pytest.mark.parametrize("t,e,k", [(3000, 8, 2), (4097, 64, 6), (5000, 256, 8), (2049, 1024, 4), (12345, 16, 1)])
+@pytest.mark.parametrize("t,e,k", [(3000, 8, 2), (4097, 64, 6), (5000, 256, 8), (2049, 1024, 4), (12345, 16, 1), (8192, 33, 8),
+                                   (8195, 128, 8), (9001, 100, 3), (8200, 5, 5), (33, 40, 2)])
 def test_route_of_many_tokens_is_a_stable_sort(cuda_device, t, e, k):
     # few distinct logits: mostly ties, and popular experts
     z = torch.randint(-3, 4, (t, e), generator=gen(t, cuda_device), device=cuda_device).float()
@@ -172,6 +173,26 @@ def test_route_grad(cuda_device, t, e, k, dtype, renorm):
     mags = (chosen * (d.abs() + size) if renorm else chosen * d.abs())
     most = (0 * p if renorm else p * size).scatter_add_(1, at, mags)
     near(got, want, 2 * (40 + e + k) * U * most, dtype)
+
+
+@pytest.mark.parametrize("t,e,k", [(8192, 64, 6), (8197, 30, 8), (9000, 64, 1)])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_many_tokens_are_routed_like_few(cuda_device, t, e, k, renorm):
+    """Batches from 8,192 tokens on give a token fewer lanes: the same bits but for the order of a sum of e terms."""
+    g = gen(t, cuda_device)
+    z = torch.randn(t, e, generator=g, device=cuda_device) * 2
+    z[torch.rand(t, e, generator=g, device=cuda_device) < 0.1] = -INF
+    z[5] = -INF
+    dg = torch.randn(t, k, generator=g, device=cuda_device)
+    gates, experts, _, _ = route(z, k, renorm)
+    dz = route_grad(z, gates, experts, dg, renorm)
+    half = t // 2
+    for part in (slice(0, half), slice(half, t)):
+        some = route(z[part].contiguous(), k, renorm)
+        assert torch.equal(experts[part], some[1])
+        near(gates[part], some[0].double(), 2 * e * U * some[0].double())
+        want = route_grad(z[part].contiguous(), some[0], some[1], dg[part].contiguous(), renorm)
+        near(dz[part], want.double(), 8 * (e + k) * U * (dg[part].abs().sum(1, keepdim=True).double() + 0 * want.double()))
 
 
 @pytest.mark.parametrize("renorm", [False, True])
