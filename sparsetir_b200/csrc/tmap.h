@@ -14,10 +14,11 @@
 namespace sptir {
 
 // Encodes a map of `rank` dimensions: dims and box in elements, strides (of all but the first dimension) in bytes, multiples of 16;
-// the box row (box[0] * element size) must equal the swizzle width for the swizzled modes.  Returns 0, or -1 with the
-// error message set.
+// the box row (box[0] * element size) must equal the swizzle width for the swizzled modes; `fetch` is
+// what L2 takes from memory at a time.  Returns 0, or -1 with the error message set.
 inline int make_tmap(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, int rank, const cuuint64_t* dims,
-                     const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+                     const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle,
+                     CUtensorMapL2promotion fetch = CU_TENSOR_MAP_L2_PROMOTION_L2_128B) {
   using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
@@ -33,8 +34,7 @@ inline int make_tmap(CUtensorMap* map, CUtensorMapDataType dtype, const void* ba
   if (!encode) return fail("cuTensorMapEncodeTiled is not available from this driver");
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult rc = encode(map, dtype, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, estr,
-                             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, fetch, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (rc != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed with code %d", static_cast<int>(rc));
   return 0;
 }
