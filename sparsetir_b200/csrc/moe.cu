@@ -25,10 +25,10 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) != 0u ? 0x80000000u : 0xffffffffu));
 }
-// exp(v - top) for the logits of a token; those of the largest are 1 even if it is +inf
-__device__ __forceinline__ float over_top(uint32_t key, uint32_t top) {
-  if (key == 0u) return 0.f;
-  return key == top ? 1.f : expf(key_value(key) - key_value(top));
+// exp(v - top) for a logit of a token whose largest is top; 0 for a masked one (-inf), 1 for the largest even if it is +inf
+__device__ __forceinline__ float over_top(float v, float top) {
+  const float e = expf(v - top);
+  return v == top ? 1.f : v > -INFINITY ? e : 0.f;
 }
 
 // Reductions over the L lanes of a token.
@@ -59,19 +59,27 @@ __device__ __forceinline__ float sum_of(float v) {
   return v;
 }
 
-// A token's logits, R to each of L lanes: lane l has those of the experts l, l + L, ...
+// A token's logits, R to each of L lanes: lane l has those of the experts l, l + L, ...; -inf for what masks an expert.
+// Returns the largest of the token, NaN if all are masked.
 template <class T, int L, int R>
-__device__ __forceinline__ void load_keys(const T* row, int num_experts, int l, bool live, uint32_t (&key)[R]) {
+__device__ __forceinline__ float load_logits(const T* row, int num_experts, int l, bool live, float (&v)[R]) {
   constexpr int G = R < 8 ? R : 8;  // in flight
 #pragma unroll
   for (int r0 = 0; r0 < R; r0 += G) {
-    T v[G];
+    T raw[G];
 #pragma unroll
     for (int r = 0; r < G; ++r)
-      if (live && l + L * (r0 + r) < num_experts) v[r] = ld_global(row + l + L * (r0 + r));
+      if (live && l + L * (r0 + r) < num_experts) raw[r] = ld_global(row + l + L * (r0 + r));
 #pragma unroll
-    for (int r = 0; r < G; ++r) key[r0 + r] = live && l + L * (r0 + r) < num_experts ? order_key(to_float(v[r])) : 0u;
+    for (int r = 0; r < G; ++r) {
+      const float x = live && l + L * (r0 + r) < num_experts ? to_float(raw[r]) : -INFINITY;
+      v[r0 + r] = x > -INFINITY ? x : -INFINITY;
+    }
   }
+  float most = v[0];
+#pragma unroll
+  for (int r = 1; r < R; ++r) most = fmaxf(most, v[r]);
+  return key_value(most_of<L>(order_key(most)));
 }
 
 // The router is two launches, or one where a single block has all tokens.  Each block of the first chooses for its share of
@@ -157,14 +165,16 @@ choose_kernel(const T* logits, float* gates, int32_t* experts, int32_t* slots, i
     const int t = tw + lane / L;
     const bool live = t < t1;
     uint32_t key[R];
-    load_keys<T, L, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, l, live, key);
-    uint32_t most = 0u;
+    float top, sum = 0.f;
+    {
+      float v[R];
+      top = load_logits<T, L, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, l, live, v);
 #pragma unroll
-    for (int r = 0; r < R; ++r) most = max(most, key[r]);
-    const uint32_t top = most_of<L>(most);
-    float sum = 0.f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) sum += over_top(key[r], top);
+      for (int r = 0; r < R; ++r) {
+        sum += over_top(v[r], top);
+        key[r] = order_key(v[r]);
+      }
+    }
     sum = sum_of<L>(sum);
     int expert = -1;     // of choice l
     uint32_t chosen = 0u;
@@ -191,7 +201,7 @@ choose_kernel(const T* logits, float* gates, int32_t* experts, int32_t* slots, i
         chosen = found;
       }
     }
-    const float value = over_top(chosen, top);
+    const float value = chosen != 0u ? over_top(key_value(chosen), top) : 0.f;
     if (renormalize) sum = sum_of<L>(value);
     if (live && l < top_k) {
       const size_t p = static_cast<size_t>(t) * top_k + l;
@@ -266,42 +276,37 @@ route_grad_kernel(const T* logits, const float* gates, const int32_t* experts, c
     gate = ld_global(gates + p);
     dg = ld_global(d_gates + p);
   }
-  uint32_t key[R];
-  load_keys<T, L, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, l, live, key);
-  if (expert < 0) gate = dg = 0.f;
+  float v[R];
+  const float top = load_logits<T, L, R>(logits + static_cast<size_t>(t) * num_experts, num_experts, l, live, v);
+  if (expert < 0 || expert >= num_experts) gate = dg = 0.f;
   const float mean = sum_of<L>(gate * dg);
-  float grad[R];
-  if (renormalize) {
+  // what the chosen experts have besides, in a row of the token's own
+  extern __shared__ float rows[];
+  float* const row = rows + static_cast<size_t>(threadIdx.x / L) * num_experts;
 #pragma unroll
-    for (int r = 0; r < R; ++r) grad[r] = 0.f;
-    dg -= mean;
-  } else {
-    uint32_t most = 0u;
-#pragma unroll
-    for (int r = 0; r < R; ++r) most = max(most, key[r]);
-    const uint32_t top = most_of<L>(most);
+  for (int r = 0; r < R; ++r)
+    if (l + L * r < num_experts) row[l + L * r] = 0.f;
+  __syncwarp();
+  if (gate != 0.f) row[expert] = gate * (renormalize ? dg - mean : dg);
+  __syncwarp();
+  float scale = 0.f;  // of the probabilities
+  if (!renormalize) {
     float sum = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      grad[r] = over_top(key[r], top);
-      sum += grad[r];
+      v[r] = over_top(v[r], top);
+      sum += v[r];
     }
     sum = sum_of<L>(sum);
-#pragma unroll
-    for (int r = 0; r < R; ++r) grad[r] = key[r] != 0u ? -mean * (grad[r] / sum) : 0.f;
-  }
-  for (int j = 0; j < top_k; ++j) {
-    const int e = __shfl_sync(kFull, expert, lane - l + j);
-    const float add = __shfl_sync(kFull, gate * dg, lane - l + j);
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (l + L * r == e) grad[r] += add;
+    scale = sum > 0.f ? -mean / sum : 0.f;
   }
   if (!live) return;
   T* out = d_logits + static_cast<size_t>(t) * num_experts;
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-    if (l + L * r < num_experts) out[l + L * r] = from_float<T>(grad[r]);
+  for (int r = 0; r < R; ++r) {
+    const int e = l + L * r;
+    if (e < num_experts) out[e] = from_float<T>(renormalize ? row[e] : fmaf(scale, v[r], row[e]));
+  }
 }
 
 // f(L, R) as integral constants, L * R >= num_experts.  8 lanes to a token, for up to `most` experts, where the SMs have warps
@@ -654,7 +659,8 @@ extern "C" int sparsetir_moe_route_grad_raw(const void* logits, int logits_type,
   return with_type(logits_type, [&](auto t) {
     using T = decltype(t);
     return with_lanes(tokens, num_experts, top_k, 64, [&](auto l, auto r) {
-      launch_chained(route_grad_kernel<T, l.value, r.value>, ceil_div(tokens, kWarps * 32 / l.value), kWarps * 32, 0, st, static_cast<const T*>(logits),
+      launch_chained(route_grad_kernel<T, l.value, r.value>, ceil_div(tokens, kWarps * 32 / l.value), kWarps * 32,
+                     kWarps * (32 / l.value) * num_experts * sizeof(float), st, static_cast<const T*>(logits),
                      gates, experts, d_gates, static_cast<T*>(d_logits), tokens, num_experts, top_k,
                      flags & SPARSETIR_MOE_RENORMALIZE);
       SPTIR_LAUNCH_OK("route_grad_kernel");
