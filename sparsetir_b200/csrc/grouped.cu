@@ -14,7 +14,7 @@
 // take the other one out; tiles that are not running yet are taken over by pairs that are done (cluster launch control).
 // With all operands in L2 a step of K (64 deep, 512 clocks of the tensor core) takes 0.28 us of loads, 117 GB/s into each SM:
 // loads and MMAs are even, and beyond about 1.2 PFLOP/s the power limit lowers the clock.  65,536 rows in 64 ragged groups, 2048 ->
-// 2048, bf16: 0.45-0.51 ms, 1.08-1.2 PFLOP/s, by the clock (8192^3 in one group: 0.71-0.83 ms; torch.matmul 0.75).  The
+// 2048, bf16: 0.45-0.51 ms, 1.08-1.2 PFLOP/s, by the clock (8192^3 in one group: 0.71-0.83 ms; a library product 0.75).  The
 // gradient of 64 weights of 2048 x 1024 over 32,768 rows, 8 steps to a tile, 0.13-0.17 ms: its 470 MB alone are 72 us.
 // Tried and taken back: equal column tiles instead of 256 and a remainder (more, smaller loads: 54 -> 45 us on 6,001 rows); a
 // prefetch of the next tiles' operands to L2 (44 -> 60); the whole tiles of all groups first (no change); one arrival
@@ -650,7 +650,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
   static_cast<OutT*>(p.out)[at] = from_float<OutT>(v);
 }
 
-// ---- rows at aligned addresses: TMA wants pitches that are multiples of 16 bytes
+// ---- rows at aligned addresses: TMA wants pitches that are multiples of 16 bytes.  A copy reads and writes the operand once more, which
+// the large products can bear and the small ones feel (us, the same without a copy behind it: 4,593 rows in 16 groups,
+// 3641 -> 3576 296, 3640 -> 3576 168; 16 rows in 8 groups, 1782 -> 1111 19, 1784 -> 1112 5.5).  Cutting 16 bytes out of two aligned
+// loads in the kernel for few rows instead gained where weights are small (8 groups, 1001 -> 999 11.9 -> 8.5) and lost where
+// they are not (64 rows, 2047 -> 2047 38 -> 62): taken back.
 
 template <class E>  // an element of 1 or 2 bytes
 __global__ void __launch_bounds__(256) pad_rows_kernel(const E* src, uint4* dst, long long rows, int cols, int pieces) {
@@ -829,18 +833,19 @@ int product(const char* fn, const void* x, const void* w, int type, void* y, int
   p.idesc = i8 ? tc05::instr_desc_i8(2 * kM, 0) : tc05::instr_desc(map_format(type), 2 * kM, 0, p.a_mn, 0);
   const int columns = plan_product(fn, &p, depth);
   if (columns < 0) return -1;
+  const bool few = few_rows_pay(rows, groups, fi, fo, out_in);
   Operand ox{x, rows, fi, size}, ow{w, static_cast<long long>(groups) * (out_in ? fo : fi), out_in ? fi : fo, size};
-  const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + part_bytes(p);
+  const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + (few ? 0 : part_bytes(p));
   CallScratch cs;
   if (bytes > 0 && take_scratch(device_id, st, bytes, 0, &cs) != 0) return -1;
   char* scratch = cs.scratch;
   if (place_operand(&ox, &scratch, st) != 0 || place_operand(&ow, &scratch, st) != 0) return -1;
-  p.parts = scratch;
-  if (few_rows_pay(rows, groups, fi, fo, out_in)) {
+  if (few) {
     FewArgs f{ox.data, ow.data, y, xs, ws, indptr, ox.pitch, ow.pitch, rows, groups, fi, fo, fi * size, 0, 0, 0};
     const int done = few_rows(f, type, y_type, out_in, st);
     return done != 0 ? done : return_scratch(cs, st);
   }
+  p.parts = scratch;
   CUtensorMap tm_w, tm_x64, tm_x16;
   const cuuint64_t each = out_in ? fo : fi;  // rows of one W
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(ow.cols), each, static_cast<cuuint64_t>(groups)};

@@ -449,6 +449,36 @@ def test_grouped_few_rows(cuda_device, sizes, fi, fo, dtype, out_in):
     check_grouped(sizes, fi, fo, dtype, out_in, dtype, cuda_device, tail=3)
 
 
+@pytest.mark.parametrize("sizes", [[1], [3, 0, 5, 2], [9, 16, 12], [1] * 40], ids=str)
+@pytest.mark.parametrize("fi,fo", [(1, 1), (7, 9), (63, 130), (264, 257), (1001, 24), (2047, 1111)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("out_in", [False, True])
+def test_grouped_few_rows_of_odd_widths(cuda_device, sizes, fi, fo, dtype, out_in):
+    check_grouped(sizes, fi, fo, dtype, out_in, torch.float32, cuda_device)
+    check_grouped(sizes, fi, fo, dtype, out_in, dtype, cuda_device, tail=2)
+
+
+@pytest.mark.parametrize("fi,fo", [(63, 65), (65, 130), (129, 7), (130, 136)])
+@pytest.mark.parametrize("out_in", [False, True])
+def test_grouped_values_stay_in_rows_of_odd_widths(cuda_device, fi, fo, out_in):
+    """What is not a number lies right before and behind the rows of x and W in use, in their own arrays and beyond."""
+    sizes, bad = [0, 3, 0, 1, 0], torch.tensor([NAN, INF, -INF], device=cuda_device)
+    rows, g = sum(sizes), gen(fi, cuda_device)
+    x = bad[torch.arange(rows + 2, device=cuda_device)[:, None].expand(-1, fi) % 3].half()
+    w = bad[torch.arange(5, device=cuda_device)[:, None, None].expand(-1, fi, fo) % 3].half()
+    x[1:4] = torch.randn(3, fi, generator=g, device=cuda_device).half()
+    w[1] = torch.randn(fi, fo, generator=g, device=cuda_device).half()
+    want = x[1:4].double() @ w[1].double()
+    slack = 2 * fi * U * (x[1:4].double().abs() @ w[1].double().abs())
+    flat = (w.transpose(1, 2) if out_in else w).contiguous()
+    y = torch.full(((rows + 2) * fo,), 7.0, device=cuda_device)
+    indptr = torch.tensor([1, 1, 4, 4, 5, 5], dtype=torch.int32, device=cuda_device)
+    ops.grouped_mm(x.view(-1), flat.view(-1), y, indptr, 5, fi, fo, ops.GROUPED_W_OUT_IN if out_in else 0)
+    y = y.view(rows + 2, fo)
+    near(y[1:4], want, slack)
+    assert (y[[0, 5]] == 7).all() and not torch.isfinite(y[4]).any()
+
+
 def test_grouped_values_stay_in_their_rows_and_groups(cuda_device):
     sizes, fi, fo = [40, 0, 25, 130], 96, 136
     g = gen(3, cuda_device)
@@ -641,6 +671,12 @@ def test_i8_operands_at_odd_addresses(cuda_device, shift, fi, fo):
 @pytest.mark.parametrize("sizes,fi,fo", [([100], 8200, 520), ([33, 0, 50, 41] * 10, 4112, 72), ([3], 4096, 2000), ([5, 0, 16, 17, 1, 0, 33], 1040, 520)])
 def test_i8_depth_shared(cuda_device, sizes, fi, fo):
     check_i8(sizes, fi, fo, torch.float32, cuda_device, tail=9)
+
+
+@pytest.mark.parametrize("sizes", [[1], [3, 0, 5, 2], [9, 16, 12]], ids=str)
+@pytest.mark.parametrize("fi,fo", [(1, 1), (7, 9), (63, 130), (1001, 24), (2047, 1111), (4098, 33)])
+def test_i8_few_rows_of_odd_widths(cuda_device, sizes, fi, fo):
+    check_i8(sizes, fi, fo, torch.float32, cuda_device, tail=2)
 
 
 def test_i8_extremes_and_one_dense_product(cuda_device):
