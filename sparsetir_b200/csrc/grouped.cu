@@ -804,14 +804,15 @@ bool wide_rows(const void* out, int type, int features) {
 
 // Whether the kernel for groups of a few rows takes a product, from what the host knows (us, that kernel / this one, 16-bit elements
 // unless said otherwise; rows, groups, features): W contiguous along the depth 2, 1, 4096 -> 4096 7.9 / 13.4; 16, 1, 4096 -> 4096
-// 9.0 / 14.0; 16, 8, 1024 -> 1024 3.8 / 8.8; 64, 8, 2048 -> 2048 15.5 / 15.8; 8-bit integers 1, 1, 4096 -> 8192 8.2 / 14; but 128, 8, 2048 -> 2048 20 / 16 and
-// 500, 64, 2048 -> 2048 114 / 90, which have tiles enough; along the features 16, 8, 512 -> 512 3.9 / 6.5, but 16, 8, 2048 ->
-// 2048 17.7 / 14.4.  The bound on the rows is for batches that meet in one group, which it walks 16 rows at a time.
+// 9.0 / 14.0; 16, 8, 1024 -> 1024 3.8 / 8.8; 64, 8, 2048 -> 2048 15.5 / 15.8; 8-bit integers 1, 1, 4096 -> 8192 8.2 / 14; but 128, 8,
+// 2048 -> 2048 20 / 16 and 500, 64, 2048 -> 2048 114 / 90, which have tiles enough; along the features 16, 8, 512 -> 512 3.2 / 6.5,
+// 1, 1, 4096 -> 4096 8.0 / 11.9, 16, 8, 1784 -> 1112 7.9 / 12.6, but 48, 8, 1024 -> 4096 17.4 / 14.2.  The bound on the rows is
+// for batches that meet in one group, which it walks 16 rows at a time.
 bool few_rows_pay(int rows, int groups, int fi, int fo, bool along_k) {
   const long long used = std::min(groups, rows);
   const long long tiles = used * ceil_div(fo, 2 * kM);
   if (rows > 256 || rows > (tiles < kNumSMs / 4 ? 16 : 8) * used || groups > 65535) return false;
-  return along_k ? tiles <= 256 : used * fi <= (8 << 20) / fo;
+  return along_k ? tiles <= 256 : used * fi <= (24 << 20) / fo;
 }
 
 // y = x * W: `type` of the elements of x and W, -1 for 8-bit integers

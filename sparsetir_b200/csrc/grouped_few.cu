@@ -3,7 +3,9 @@
 // most of the memory system idle; here the weights go straight from global memory into the registers of the matrix instructions
 // (m16n8k16, m16n8k32 for 8-bit integers: 16 features, 8 rows of x), by as many warps as it takes to keep it busy: the
 // warps of a block share its features and, where these are few, the depth, and their sums meet in shared memory in a fixed order.
-// Which element of a step of K plays which k is free as long as both operands agree, so every lane loads 16 bytes of W.
+// Which element of a step of K plays which k is free as long as both operands agree, so every lane loads 16 (8) bytes of W.
+// One row of 8-bit integers, 4096 -> 8192: 33.6 MB in 8.2 us out of HBM, 5.0 out of L2; prefetch sizes of 128 and 256 bytes at the
+// loads changed nothing and cost up to a third.
 #include <algorithm>
 #include <type_traits>
 
@@ -117,66 +119,65 @@ struct AlongK {
   }
 };
 
-// W contiguous along the features (16-bit elements).  A step is 16 of K of 64 features: lane l has 8 features from
-// 8 (l / 4) on of the four rows of W from 4 (l % 4) on, and four elements of its rows of x; instruction j takes the j-th and
-// the (j + 4)-th feature of every lane's eight.
+// W contiguous along the features (16-bit elements).  A step is 32 of K of 32 features: lane l has 4 features from 4 (l / 4) on of the
+// eight rows of W from 8 (l % 4) on, and eight elements of its rows of x; instruction j takes the j-th and the (j + 2)-th
+// feature of every lane's four, four rows at a time.  (With 8 features to a lane, 64 to a warp, there are half as many
+// warps: 1 row, 4096 -> 2000 12.6 us where now 7.9, 64 rows in 8 groups, 1024 -> 1024 8.1 where now 6.4; along K 5.0 and 4.8.)
 template <class T, int NT>
 struct AlongFeatures {
-  static constexpr int kFeatures = 64, kStepBytes = 32, kRows = 8 * NT;  // bytes of K in x
+  static constexpr int kFeatures = 32, kStepBytes = 64, kRows = 8 * NT;  // bytes of K in x
   using Sum = float;
-  float acc[4][NT][4];
-  struct Step { uint4 w[4]; uint2 x[NT]; };
+  float acc[2][NT][4];
+  struct Step { uint2 w[8]; uint4 x[NT]; };
 
   const char *wp, *xp[NT];
   int at, last;  // elements of K
   size_t pitch;
   __device__ __forceinline__ void start(const FewArgs& p, int group, int feat0, int row0, int live, int k0, int k1, int lane) {
-    const int f = feat0 + 8 * (lane / 4);
+    const int f = feat0 + 4 * (lane / 4);
     pitch = p.w_pitch;
-    at = k0 / 2 + 4 * (lane & 3);
+    at = k0 / 2 + 8 * (lane & 3);
     last = k1 / 2;
     wp = static_cast<const char*>(p.w) + (static_cast<size_t>(group) * p.fi + at) * pitch + static_cast<size_t>(f < p.fo ? f : 0) * 2;
 #pragma unroll
     for (int h = 0; h < NT; ++h) {
       xp[h] = static_cast<const char*>(p.x) + static_cast<size_t>(row0 + min(lane / 4 + 8 * h, live - 1)) * p.x_pitch + static_cast<size_t>(at) * 2;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[j][h][c] = 0.f;
+      for (int c = 0; c < 4; ++c) acc[0][h][c] = acc[1][h][c] = 0.f;
     }
   }
   __device__ __forceinline__ void load(Step& s) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_if(s.w[i], wp + i * pitch, at + i < last);
-    wp += 16 * pitch;
+    for (int i = 0; i < 8; ++i) load_if(s.w[i], wp + i * pitch, at + i < last);
+    wp += 32 * pitch;
 #pragma unroll
-    for (int h = 0; h < NT; ++h) {  // a row of x that does not end at a multiple of four elements is followed by zeros
+    for (int h = 0; h < NT; ++h) {  // a row of x that does not end at a multiple of eight elements is followed by zeros
       load_if(s.x[h], xp[h], at < last);
-      xp[h] += 32;
+      xp[h] += 64;
     }
-    at += 16;
+    at += 32;
   }
   __device__ __forceinline__ void multiply(const Step& s) {
-    // words of the four rows that hold features j and j + 1 (lo) and j + 4 and j + 5 (hi) of the lane's eight
-    auto two = [&](int j, uint32_t l0, uint32_t l1, uint32_t l2, uint32_t l3, uint32_t h0, uint32_t h1, uint32_t h2, uint32_t h3) {
-#pragma unroll
-      for (int h = 0; h < NT; ++h) {
-        mma<T>(acc[j][h], __byte_perm(l0, l1, 0x5410), __byte_perm(h0, h1, 0x5410), __byte_perm(l2, l3, 0x5410),
-               __byte_perm(h2, h3, 0x5410), s.x[h].x, s.x[h].y);
-        mma<T>(acc[j + 1][h], __byte_perm(l0, l1, 0x7632), __byte_perm(h0, h1, 0x7632), __byte_perm(l2, l3, 0x7632),
-               __byte_perm(h2, h3, 0x7632), s.x[h].x, s.x[h].y);
-      }
+    // words of four rows that hold the lane's features 0 and 1 (lo), and 2 and 3 (hi)
+    auto two = [&](const uint2& r0, const uint2& r1, const uint2& r2, const uint2& r3, int h, uint32_t x0, uint32_t x1) {
+      mma<T>(acc[0][h], __byte_perm(r0.x, r1.x, 0x5410), __byte_perm(r0.y, r1.y, 0x5410), __byte_perm(r2.x, r3.x, 0x5410),
+             __byte_perm(r2.y, r3.y, 0x5410), x0, x1);
+      mma<T>(acc[1][h], __byte_perm(r0.x, r1.x, 0x7632), __byte_perm(r0.y, r1.y, 0x7632), __byte_perm(r2.x, r3.x, 0x7632),
+             __byte_perm(r2.y, r3.y, 0x7632), x0, x1);
     };
-    two(0, s.w[0].x, s.w[1].x, s.w[2].x, s.w[3].x, s.w[0].z, s.w[1].z, s.w[2].z, s.w[3].z);
-    two(2, s.w[0].y, s.w[1].y, s.w[2].y, s.w[3].y, s.w[0].w, s.w[1].w, s.w[2].w, s.w[3].w);
+#pragma unroll
+    for (int h = 0; h < NT; ++h) {
+      two(s.w[0], s.w[1], s.w[2], s.w[3], h, s.x[h].x, s.x[h].y);
+      two(s.w[4], s.w[5], s.w[6], s.w[7], h, s.x[h].z, s.x[h].w);
+    }
   }
   __device__ __forceinline__ void put(float (*to)[kFeatures], int lane) const {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int h = 0; h < NT; ++h)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) to[8 * h + 2 * (lane & 3) + (c & 1)][8 * (lane / 4) + j + 4 * (c >> 1)] = acc[j][h][c];
+        for (int c = 0; c < 4; ++c) to[8 * h + 2 * (lane & 3) + (c & 1)][4 * (lane / 4) + j + 2 * (c >> 1)] = acc[j][h][c];
   }
 };
 
