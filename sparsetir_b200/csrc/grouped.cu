@@ -11,7 +11,7 @@
 // indptr on the device.
 //
 // A ring of six stages of 32 KB is fed by TMA, MMAs of 256 x 256 x 16 (x 32) go to one of two accumulators while eight warps
-// take the other one out; tiles that are not running yet are taken over by pairs that are done (cluster launch control).
+// take the other one out; a pair's units are those of its number, of its number plus the pairs, and so on.
 // With all operands in L2 a step of K (64 deep, 512 clocks of the tensor core) takes 0.28 us of loads, 117 GB/s into each SM:
 // loads and MMAs are even, and beyond about 1.2 PFLOP/s the power limit lowers the clock.  65,536 rows in 64 ragged groups, 2048 ->
 // 2048, bf16: 0.45-0.51 ms, 1.08-1.2 PFLOP/s, by the clock (8192^3 in one group: 0.71-0.83 ms; a library product 0.75).  The
@@ -35,9 +35,8 @@ namespace {
 constexpr int kM = 128;               // features per block
 constexpr int kABytes = 16 * 1024;    // left operand of a stage: 128 rows of 128 bytes
 constexpr int kAtom = 8 * 1024;       // 64 rows of 128 bytes
-constexpr int kFirstEpilogue = 4;     // warp 0 loads, 1 issues, 2 clears the tails of groups (grad_w), 3 hands out tiles, from 4 on the epilogue
+constexpr int kFirstEpilogue = 4;     // warp 0 loads, 1 issues, 2 clears the tails of groups (grad_w), from 4 on the epilogue
 constexpr int kStagedBytes = 32 * 64; // 32 columns of 32 features on their way out, per epilogue warp
-constexpr int kTiles = 4;             // entries of the ring of tiles
 constexpr int kBand = 8;              // column tiles of a group that are walked side by side
 
 // Columns of a tile, and what follows from them.  128 leave room for two pairs of blocks on two SMs: for many groups of few rows,
@@ -82,7 +81,6 @@ struct Args {
   int mt, nt;     // tiles of 256 features; grad_w: column tiles
   Divisor per_split, per_group, per_band;  // splits; grad_w: mt * nt; kBand * mt
   int max_tiles;  // no valid indptr has more; times splits
-  int deal;       // more of them than pairs of blocks run at a time
   int splits;     // units that share the depth of a tile, each with sums of its own in `parts`
   void* parts;    // [splits][rows of the result][features], 32 bits each
   long long part; // elements of one split's
@@ -105,7 +103,7 @@ struct Tile {
   int split, step0, steps; // the unit's share of the depth
 };
 
-// The tile of a unit.  All lanes of a warp call at() together; lane l holds the prefix of tile counts of group base + l.
+// The tile of a unit.  All lanes of a warp call at() together, with units that rise; lane l holds the prefix of tile counts of group base + l.
 // Sums stop at 2^30: wild pointers give tiles inside the arrays, and no more than max_tiles of them.
 template <bool GRAD, int kN, int kDepth>
 struct Walker {
@@ -130,10 +128,6 @@ struct Walker {
       out->depth = l - f;
     } else {
       const int lane = threadIdx.x & 31;
-      if (static_cast<unsigned>(t) < before) {
-        base = -32;
-        before = all = 0;
-      }
       while (static_cast<unsigned>(t) >= all) {
         base += 32;
         if (base >= p.groups) return false;
@@ -323,16 +317,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
   __shared__ __align__(8) uint64_t bar_acc_full[2];
   __shared__ __align__(8) uint64_t bar_acc_empty[2];    // rank 0: both blocks have taken the result
   __shared__ __align__(8) uint64_t bar_drain;
-  __shared__ __align__(8) uint64_t bar_tile_full[kTiles];
-  __shared__ __align__(8) uint64_t bar_tile_empty[kTiles];  // rank 0: the roles of both blocks have read the entry
-  __shared__ __align__(8) uint64_t bar_answer;
-  __shared__ __align__(16) int4 s_tiles[kTiles][2];
-  __shared__ __align__(16) int4 s_answer;
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = tc05::pair::rank();
   const uint32_t base = (tc05::smem_u32(smem_raw) + 1023u) & ~1023u;
-  const int pair = blockIdx.x >> 1;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -346,11 +335,6 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         tc05::mbar_init(&bar_acc_empty[b], 2 * kEpilogue);
       }
       tc05::mbar_init(&bar_drain, 1);
-      for (int b = 0; b < kTiles; ++b) {
-        tc05::mbar_init(&bar_tile_full[b], 1);
-        tc05::mbar_init(&bar_tile_empty[b], 3 + 2 * kEpilogue + (GRAD ? 2 : 0));
-      }
-      tc05::mbar_init(&bar_answer, 1);
       tc05::fence_mbar_init();
       tc05::prefetch_tensormap(&tm_a);
       tc05::prefetch_tensormap(&tm_b64);
@@ -378,23 +362,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
   };
   Walker<GRAD, kN, kDepth> walk(p);
   Tile tile;
-  // A role's next tile: the pair's own, then those that warp 3 of rank 0 hands to both blocks.
-  int turn = -1;
-  auto next = [&]() {
-    if (turn < 0) {
-      turn = 0;
-      return walk.at(pair, &tile);
-    }
-    if (p.deal == 0) return false;
-    const int s = turn % kTiles;
-    ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_tile_full[s], (turn / kTiles) & 1));
-    if (!ok) return false;
-    const int4 a = s_tiles[s][0], b = s_tiles[s][1];
-    __syncwarp();
-    if (lane == 0) tc05::pair::arrive(tc05::pair::at_first(&bar_tile_empty[s]));
-    ++turn;
-    tile = Tile{a.x, a.y, a.z, a.w & 0xffff, ((a.w & 0xffff) + 31) & ~31, b.x, b.y, a.w >> 16, b.z, b.w};
-    return tile.steps >= 0;
+  // Every role of both blocks finds them by itself.  Units taken over from pairs that do not run yet (cluster launch control), handed to
+  // the roles through a ring of entries in both blocks' shared memory, were faster by up to 15 %, but about one launch in a
+  // million had a role of the other block read an entry from before: taken back.
+  int unit = -1;
+  auto next = [&]() {  // a role's next tile
+    unit = unit < 0 ? pair : unit + pairs;
+    return unit < p.max_tiles && walk.at(unit, &tile);
   };
 
   if (warp == 0) {
@@ -503,41 +477,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         }
         tc05::fence_async_smem();
         __syncwarp();
-        if (lane == 0) tc05::pair::arrive(tc05::pair::at_first(&bar_full[s]));
+        if (lane == 0) tc05::pair::arrive_release(tc05::pair::at_first(&bar_full[s]));
       }
       advance(tile.steps);
-    }
-  } else if (warp == 3) {
-    // ---- tiles.  The launch has a pair of blocks for every unit; a pair that runs takes over the work of one that does not yet,
-    // until there is none.  (us, units dealt out beforehand / this: 65,536 rows in 64 groups, 512 -> 2048 170 / 148; 16,000
-    // rows, 1024 -> 1024 61 / 57.)
-    int at = 0;
-    bool more = rank == 0 && p.deal != 0 && walk.at(pair, &tile);  // there are readers
-    while (rank == 0 && p.deal != 0) {
-      if (lane == 0) {
-        tc05::mbar_arrive_expect_tx(&bar_answer, 16);
-        tc05::pair::try_cancel(&s_answer, &bar_answer);
-      }
-      ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_answer, at & 1));
-      ++at;
-      int block = 0;
-      const bool one = ok && tc05::pair::cancelled(&s_answer, &block);
-      tc05::fence_async_smem();  // the answer has been read before it is written again
-      __syncwarp();
-      if (more) {
-        if (!one || !walk.at(block >> 1, &tile)) tile.steps = -1;  // the readers' last entry
-        more = tile.steps >= 0;
-        const int n = turn < 0 ? 0 : turn, s = n % kTiles;
-        turn = n + 1;
-        ok = ok && __all_sync(0xffffffffu, tc05::mbar_wait(&bar_tile_empty[s], ((n / kTiles) & 1) ^ 1));
-        if (ok && lane < 2) {  // to the block of rank `lane`
-          const uint32_t to = tc05::pair::at_rank(&s_tiles[s][0], lane), bar = tc05::pair::at_rank(&bar_tile_full[s], lane);
-          tc05::pair::arrive_expect_tx(bar, 32);
-          tc05::pair::store_async(to, make_int4(tile.group, tile.feat0, tile.col0, tile.n | tile.split << 16), bar);
-          tc05::pair::store_async(to + 16, make_int4(tile.row0, tile.depth, tile.step0, tile.steps), bar);
-        }
-      }
-      if (!one || !ok) break;
     }
   } else if (warp >= kFirstEpilogue) {
     // ---- epilogue: a warp takes the 32 features of its lanes of TMEM, columns 32 at a time; two warps share them
@@ -714,7 +656,7 @@ int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap
                                        cudaSharedmemCarveoutMaxShared));
     configured_device = dev;
   }
-  launch_chained(grouped_kernel<I8, GRAD, OutT, N>, 2 * p.max_tiles, Shape<N>::kThreads, smem, st, tm_a, tm_b64, tm_b16, p);
+  launch_chained(grouped_kernel<I8, GRAD, OutT, N>, 2 * std::min(p.max_tiles, kNumSMs / 2 * Shape<N>::kBlocks), Shape<N>::kThreads, smem, st, tm_a, tm_b64, tm_b16, p);
   SPTIR_LAUNCH_OK("grouped_kernel");
   if (p.splits > 1) {
     const long long rows = p.part / p.features;
@@ -768,7 +710,6 @@ int set_tiles(const char* fn, Args* p, bool few_columns, Bound&& bound, Some&& s
   const long long units = bound(columns) * p->mt;
   if (units > (1 << 29) / p->splits) return fail("%s: too many tiles for 32-bit indices", fn);
   p->max_tiles = static_cast<int>(units) * p->splits;
-  p->deal = p->max_tiles > kNumSMs / 2 * (columns == 128 ? Shape<128>::kBlocks : Shape<256>::kBlocks);
   p->per_split = Divisor(p->splits);
   p->per_band = Divisor(kBand * p->mt);
   p->part = rows * p->features;

@@ -275,42 +275,13 @@ __device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
   return a;
 }
 __device__ __forceinline__ uint32_t at_first(const void* p) { return at_rank(p, 0); }
-// An arrival at a barrier of either block.  (With release.cluster it waits until all stores of this thread have arrived, those
-// to global memory among them.)
+// An arrival at a barrier of either block, which orders nothing but reads that are over (of TMEM).
 __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void arrive_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-// 16 bytes to shared memory of a block of the cluster; they count at its barrier when they are there.
-__device__ __forceinline__ void store_async(uint32_t to, int4 v, uint32_t bar) {
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(v.x),
-               "r"(v.y), "r"(v.z), "r"(v.w), "r"(bar)
-               : "memory");
-}
-// Takes over the work of a cluster of this launch that has not been started: 16 bytes for cancelled() at `answer`, which
-// count at `bar`.  Not to be asked again once there was none.
-__device__ __forceinline__ void try_cancel(void* answer, uint64_t* bar) {
-  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
-               "r"(smem_u32(bar))
-               : "memory");
-}
-// Whether there was one; *block is the x index of its first block.
-__device__ __forceinline__ bool cancelled(const void* answer, int* block) {
-  uint32_t yes, x;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
-      "ld.shared.b128 r, [%2];\n\t"
-      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "mov.u32 %1, 0;\n\t"
-      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, r;\n\t}"
-      : "=r"(yes), "=r"(x)
-      : "r"(smem_u32(answer))
-      : "memory");
-  *block = static_cast<int>(x);
-  return yes != 0;
+// The same behind this thread's stores, which waits until all of them have arrived, those to global memory among them.
+__device__ __forceinline__ void arrive_release(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // mbar_wait for a barrier at which threads of the other block arrive
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
