@@ -589,6 +589,23 @@ def test_grad_w_of_groups_without_rows(cuda_device, out_in, fo):
     check_grad_w([0] * 20 + [3] + [0] * 20, 264, fo, torch.bfloat16, out_in, torch.bfloat16, cuda_device)
 
 
+def test_grad_w_of_many_groups_with_few_rows_repeats(cuda_device):
+    """Thousands of launches whose tiles are mostly zeros: every tile is found by all roles alike, every time."""
+    groups, fi, fo, rows = 64, 1444, 2024, 9
+    g = gen(11, cuda_device)
+    sizes = torch.bincount(torch.randint(0, groups, (rows,), generator=g, device=cuda_device), minlength=groups)
+    x = torch.randn(rows, fi, generator=g, device=cuda_device).half()
+    dy = torch.randn(rows, fo, generator=g, device=cuda_device).half()
+    indptr = pointers(sizes.tolist(), cuda_device)
+    first, dw = (torch.full((groups * fi * fo,), 9.0, dtype=torch.float16, device=cuda_device) for _ in range(2))
+    ops.grouped_mm_grad_w(x.view(-1), dy.view(-1), first, indptr, groups, fi, fo)
+    for _ in range(10):
+        dw.fill_(9.0)
+        for _ in range(200):
+            ops.grouped_mm_grad_w(x.view(-1), dy.view(-1), dw, indptr, groups, fi, fo)
+        assert torch.equal(dw, first)
+
+
 def test_grad_w_rows_of_other_groups_do_not_matter(cuda_device):
     """A neighbour's infinities and NaNs, whichever rows of a step they share with this group's."""
     fi, fo, sizes = 72, 136, [5, 0, 58, 1, 100, 64, 20]
