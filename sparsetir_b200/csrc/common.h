@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <mutex>
 
 #include "sparsetir_b200.h"
 
@@ -24,22 +25,45 @@ int use_device(int device_id);
 
 cudaStream_t stream_for(int device_id);
 
+// The scratch buffers of a (device, stream): plain, and all zero whenever no kernel is using it.
+struct StreamBuffers {
+  struct Buffer {
+    void* ptr = nullptr;
+    size_t bytes = 0;
+  };
+  Buffer kind[2];
+  std::recursive_mutex busy;
+};
+
+// A call's hold on the buffers of its stream, from its first request to the end of the hold's life, behind the call's last
+// launch.  The stream orders launches as they are queued: without it a host thread that uses the same stream could queue a
+// launch of its own, on the same buffer, between two launches of this call, or free the buffer for a larger one
+// before this call's launches are queued.  The stages of one call may each have one.
+class ScratchHold {
+ public:
+  StreamBuffers& take(int device_id, cudaStream_t stream);
+
+ private:
+  StreamBuffers* buffers_ = nullptr;
+  std::unique_lock<std::recursive_mutex> lock_;
+};
+
 // Scratch memory for kernels that need an intermediate buffer: one grow-only allocation per
 // (device, stream), kept until the library is unloaded, so that steady-state calls allocate
-// nothing.  Calls that use it on the same stream are ordered by the stream; calls on different
+// nothing.  Calls that use it on the same stream are ordered by the stream and by their holds; calls on different
 // streams get different buffers.  Returns nullptr (after recording the error) when the device
 // cannot provide `bytes`.  Growing an existing buffer frees the old one, which synchronises the
 // device once.
-void* workspace(int device_id, cudaStream_t stream, size_t bytes);
+void* workspace(ScratchHold* hold, int device_id, cudaStream_t stream, size_t bytes);
 
 // The same for counters and flags that kernels find at zero and leave at zero: the buffer is
 // cleared (on `stream`) when it is allocated, and every kernel that uses it restores the zeros
 // before it ends, so steady-state calls neither allocate nor clear.
-void* zeroed_workspace(int device_id, cudaStream_t stream, size_t bytes);
+void* zeroed_workspace(ScratchHold* hold, int device_id, cudaStream_t stream, size_t bytes);
 
 // Whether both buffers of (device, stream) already hold that much, so that asking for them neither
 // allocates nor synchronises (neither is possible while the stream is being captured).
-bool workspace_fits(int device_id, cudaStream_t stream, size_t bytes, size_t zeroed_bytes);
+bool workspace_fits(ScratchHold* hold, int device_id, cudaStream_t stream, size_t bytes, size_t zeroed_bytes);
 
 // Scratch and zeroed counters of one operator call: the buffers above, or, while the stream is being
 // captured, memory that belongs to the graph.  A captured launch must not keep the addresses of the
@@ -49,6 +73,7 @@ struct CallScratch {
   char* scratch = nullptr;
   unsigned* counters = nullptr;
   void* owned = nullptr;  // allocated by the graph
+  ScratchHold hold;       // on the buffers above
 };
 int take_scratch(int device_id, cudaStream_t stream, size_t bytes, size_t counter_bytes, CallScratch* out);
 // After the last launch that uses it.

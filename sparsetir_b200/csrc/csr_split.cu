@@ -500,7 +500,7 @@ int csr_split_run(const float* a, const float* b, float* c, const int32_t* indpt
   CallScratch cs;
   if (pieces != nullptr) {
     cs.scratch = static_cast<char*>(pieces);
-    cs.counters = static_cast<unsigned*>(zeroed_workspace(device_id, st, p.counter_bytes));
+    cs.counters = static_cast<unsigned*>(zeroed_workspace(&cs.hold, device_id, st, p.counter_bytes));
     if (cs.counters == nullptr) return -1;
   } else if (take_scratch(device_id, st, p.part_bytes, p.counter_bytes, &cs) != 0) {
     return -1;

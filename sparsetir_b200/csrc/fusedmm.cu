@@ -223,7 +223,8 @@ extern "C" int sparsetir_fusedmm_raw(const float* q, const float* k, const float
   SPTIR_CUDA_OK(cudaStreamIsCapturing(st, &capture));
   const bool eager = capture == cudaStreamCaptureStatusNone;
   const size_t piece_bytes = eager ? csrmm_scratch(v, o, m, n, feat, nnz) : 0;
-  char* ws = static_cast<char*>(workspace(device_id, st, piece_bytes > 0 ? pieces_at(m, nnz) + piece_bytes : stage_bytes(m, nnz)));
+  ScratchHold hold;
+  char* ws = static_cast<char*>(workspace(&hold, device_id, st, piece_bytes > 0 ? pieces_at(m, nnz) + piece_bytes : stage_bytes(m, nnz)));
   if (!ws) return -1;
   float* scores = reinterpret_cast<float*>(ws);
   float* probs = softmax_by_blocks(m, nnz) ? scores : scores + nnz;

@@ -1148,9 +1148,9 @@ int hyb_spmm_run(const float* b, float* c, const SparsetirEllBucket* buckets, co
         // Whole tiles are captured with the stream's own buffers where these have been reserved; everything
         // else that is being captured gets memory of the graph (ragged feature counts and unaligned
         // operands need no reservation: the kernels that they took before this one had no scratch).
-        if (vec4 && feat % (lane_w * lanes) == 0 && workspace_fits(device_id, st, part_bytes, counter_bytes)) {
-          cs.scratch = static_cast<char*>(workspace(device_id, st, part_bytes));
-          cs.counters = static_cast<unsigned*>(zeroed_workspace(device_id, st, counter_bytes));
+        if (vec4 && feat % (lane_w * lanes) == 0 && workspace_fits(&cs.hold, device_id, st, part_bytes, counter_bytes)) {
+          cs.scratch = static_cast<char*>(workspace(&cs.hold, device_id, st, part_bytes));
+          cs.counters = static_cast<unsigned*>(zeroed_workspace(&cs.hold, device_id, st, counter_bytes));
         } else if (take_scratch(device_id, st, part_bytes, counter_bytes, &cs) != 0) {
           return -1;
         }

@@ -257,8 +257,9 @@ extern "C" int sparsetir_rgms_raw(const float* a, const float* w, const float* x
         if (rc1 <= 0) return rc1;
       }
       float* z = nullptr;
+      ScratchHold hold;
       if (!fused)
-        z = static_cast<float*>(workspace(device_id, st, static_cast<size_t>(nnz_i) * 64 * sizeof(float)));
+        z = static_cast<float*>(workspace(&hold, device_id, st, static_cast<size_t>(nnz_i) * 64 * sizeof(float)));
       if (z != nullptr && single_rows()) {
         if (rgms_pairs_launch(a, x, z, indptr_j, indices_j, nnz_i, nnz_j, st) != 0) return -1;
         return rgms_tma_launch_pairs(a, w, x, y, indptr_i, indices_i, indptr_j, indices_j, num_rels, nnz_i, z, st);

@@ -149,6 +149,7 @@ extern "C" int sparsetir_rgms_ell3d_raw(const float* w, const float* x, float* y
   if (num_rels == 0) return fail("sparsetir_rgms_ell3d: rows but no relations");
   if (use_device(device_id) != 0) return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ScratchHold hold;
 
   if (feat == 64 && num_buckets <= kMaxBuckets) {
     // ---- three launches for all buckets
@@ -175,7 +176,7 @@ extern "C" int sparsetir_rgms_ell3d_raw(const float* w, const float* x, float* y
       tb.z_base[tb.nb] = static_cast<int32_t>(total);
       const size_t zb = (static_cast<size_t>(total) * feat * sizeof(float) + 255) & ~static_cast<size_t>(255);
       const size_t rb = (static_cast<size_t>(num_ranges + 1) * sizeof(int32_t) + 255) & ~static_cast<size_t>(255);
-      char* wsp = static_cast<char*>(workspace(device_id, st, zb + rb + static_cast<size_t>(total) * sizeof(int32_t)));
+      char* wsp = static_cast<char*>(workspace(&hold, device_id, st, zb + rb + static_cast<size_t>(total) * sizeof(int32_t)));
       if (!wsp) return -1;
       float* zall = reinterpret_cast<float*>(wsp);
       int32_t* rng = reinterpret_cast<int32_t*>(wsp + zb);
@@ -196,7 +197,7 @@ extern "C" int sparsetir_rgms_ell3d_raw(const float* w, const float* x, float* y
   // workspace: Z of the largest bucket, then the relation ranges
   const size_t z_bytes = (static_cast<size_t>(max_rows) * feat * sizeof(float) + 255) & ~static_cast<size_t>(255);
   const size_t ptr_bytes = static_cast<size_t>(num_rels + 1) * sizeof(int32_t);
-  char* ws = static_cast<char*>(workspace(device_id, st, z_bytes + ptr_bytes));
+  char* ws = static_cast<char*>(workspace(&hold, device_id, st, z_bytes + ptr_bytes));
   if (!ws) return -1;
   float* z = reinterpret_cast<float*>(ws);
   int32_t* ranges = reinterpret_cast<int32_t*>(ws + z_bytes);

@@ -1072,6 +1072,7 @@ int run(const BucketTable& tb, const __half* w, const __half* x, OutT* y, int m,
         int feat_out, int device_id, cudaStream_t st) {
   const int total = tb.z_base[tb.nb];
   const long long num_ranges = static_cast<long long>(tb.nb) * num_rels;
+  ScratchHold hold;
   if (num_ranges >= INT32_MAX) return fail("sparsetir_rgms_ell3d_f16: too many (bucket, relation) pairs");
   // SPARSETIR_RGMS_F16_PATH=simt keeps the transform on the CUDA cores, =two keeps the two-launch
   // form where the one-launch form would be taken, =atomic keeps the one-launch form with
@@ -1102,7 +1103,7 @@ int run(const BucketTable& tb, const __half* w, const __half* x, OutT* y, int m,
                         static_cast<long long>(m) * num_rels < (1ll << 30);
     const size_t rb1 = (static_cast<size_t>(num_ranges + 1) * sizeof(int32_t) + 255) & ~static_cast<size_t>(255);
     const size_t map_bytes = try_os ? static_cast<size_t>(m) * num_rels * sizeof(int32_t) : 0;
-    char* ws1 = static_cast<char*>(workspace(device_id, st, rb1 + 256 + map_bytes));
+    char* ws1 = static_cast<char*>(workspace(&hold, device_id, st, rb1 + 256 + map_bytes));
     if (!ws1) return -1;
     int32_t* ranges1 = reinterpret_cast<int32_t*>(ws1);
     int32_t* flag = reinterpret_cast<int32_t*>(ws1 + rb1);
@@ -1132,7 +1133,7 @@ int run(const BucketTable& tb, const __half* w, const __half* x, OutT* y, int m,
   if (single >= 0) {
     const BucketTable one = only_bucket(tb, single), rest = without_bucket(tb, single);
     const size_t rb1 = (static_cast<size_t>(num_rels + 2) * sizeof(int32_t) + 255) & ~static_cast<size_t>(255);
-    char* ws1 = static_cast<char*>(workspace(device_id, st, rb1 + z_bytes(rest, num_rels, feat_in)));
+    char* ws1 = static_cast<char*>(workspace(&hold, device_id, st, rb1 + z_bytes(rest, num_rels, feat_in)));
     if (!ws1) return -1;
     int32_t* ranges1 = reinterpret_cast<int32_t*>(ws1);
     int32_t* passed = ranges1 + num_rels + 1;
@@ -1143,7 +1144,7 @@ int run(const BucketTable& tb, const __half* w, const __half* x, OutT* y, int m,
     if (rc < 0) return rc;
     if (rc == 0) return run_z<OutT>(rest, w, x, y, num_rels, feat_in, feat_out, path, ws1 + rb1, passed, st);
   }
-  char* ws = static_cast<char*>(workspace(device_id, st, z_bytes(tb, num_rels, feat_in)));
+  char* ws = static_cast<char*>(workspace(&hold, device_id, st, z_bytes(tb, num_rels, feat_in)));
   if (!ws) return -1;
   return run_z<OutT>(tb, w, x, y, num_rels, feat_in, feat_out, path, ws, nullptr, st);
 }

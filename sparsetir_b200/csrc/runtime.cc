@@ -5,7 +5,7 @@
 #include <map>
 #include <mutex>
 #include <string>
-#include <utility>
+#include <tuple>
 
 #include "common.h"
 
@@ -49,19 +49,44 @@ cudaStream_t stream_for(int device_id) {
 }
 
 namespace {
-struct Scratch {
-  void* ptr = nullptr;
-  size_t bytes = 0;
-};
-std::mutex g_ws_mutex;
-// [0]: plain scratch; [1]: scratch that is all zero whenever no kernel is using it
-std::map<std::pair<int, cudaStream_t>, Scratch> g_ws[2];
+std::mutex g_ws_mutex;  // of the table; a stream's buffers are used under their own `busy`
+// (device, stream, thread): the thread is 0 but for cudaStreamPerThread, one handle that is another stream in every thread.
+using StreamKey = std::tuple<int, cudaStream_t, unsigned>;
+// Never destroyed: threads may end after the library's other objects.
+std::map<StreamKey, StreamBuffers>& buffer_table() {
+  static auto& table = *new std::map<StreamKey, StreamBuffers>;
+  return table;
+}
 
-// Grows the buffer of (device, stream) to at least `bytes`; with `zeroed`, a new buffer is cleared
+// The number of a thread that has used its own stream, whose buffers go when it ends.
+struct ThreadNumber {
+  unsigned number = 0;
+  unsigned get() {
+    static std::atomic<unsigned> last{0};
+    if (number == 0) number = ++last;
+    return number;
+  }
+  ~ThreadNumber() {
+    if (number == 0) return;
+    std::lock_guard<std::mutex> lock(g_ws_mutex);
+    auto& table = buffer_table();
+    for (auto it = table.begin(); it != table.end();) {
+      if (std::get<2>(it->first) != number) {
+        ++it;
+        continue;
+      }
+      for (const auto& s : it->second.kind)
+        if (s.ptr != nullptr) cudaFree(s.ptr);  // synchronises, as in grow()
+      it = table.erase(it);
+    }
+  }
+};
+thread_local ThreadNumber tls_number;
+
+// Grows one of the buffers that a call holds to at least `bytes`; a new zeroed one is cleared
 // on `stream` before anything queued later can touch it.
-void* grow(int kind, int device_id, cudaStream_t stream, size_t bytes) {
-  std::lock_guard<std::mutex> lock(g_ws_mutex);
-  Scratch& s = g_ws[kind][{device_id, stream}];
+void* grow(ScratchHold* hold, int kind, int device_id, cudaStream_t stream, size_t bytes) {
+  StreamBuffers::Buffer& s = hold->take(device_id, stream).kind[kind];
   if (s.bytes >= bytes && s.ptr != nullptr) return s.ptr;
   if (s.ptr != nullptr) {
     cudaFree(s.ptr);  // synchronises: nothing in flight can still use the old buffer
@@ -103,30 +128,38 @@ int peer_table(const char* fn, const void* own, int n_peers, void* const* peers,
   return 0;
 }
 
-bool workspace_fits(int device_id, cudaStream_t stream, size_t bytes, size_t zeroed_bytes) {
-  std::lock_guard<std::mutex> lock(g_ws_mutex);
-  const std::pair<int, cudaStream_t> key{device_id, stream};
-  const auto a = g_ws[0].find(key), b = g_ws[1].find(key);
-  return a != g_ws[0].end() && a->second.bytes >= bytes &&
-         (zeroed_bytes == 0 || (b != g_ws[1].end() && b->second.bytes >= zeroed_bytes));
+StreamBuffers& ScratchHold::take(int device_id, cudaStream_t stream) {
+  if (buffers_ == nullptr) {
+    {
+      std::lock_guard<std::mutex> lock(g_ws_mutex);
+      buffers_ = &buffer_table()[{device_id, stream, stream == cudaStreamPerThread ? tls_number.get() : 0u}];
+    }
+    lock_ = std::unique_lock<std::recursive_mutex>(buffers_->busy);
+  }
+  return *buffers_;
 }
 
-void* workspace(int device_id, cudaStream_t stream, size_t bytes) {
-  return grow(0, device_id, stream, bytes);
+bool workspace_fits(ScratchHold* hold, int device_id, cudaStream_t stream, size_t bytes, size_t zeroed_bytes) {
+  const StreamBuffers& b = hold->take(device_id, stream);
+  return b.kind[0].bytes >= bytes && b.kind[0].ptr != nullptr && b.kind[1].bytes >= zeroed_bytes;
 }
 
-void* zeroed_workspace(int device_id, cudaStream_t stream, size_t bytes) {
-  return grow(1, device_id, stream, bytes);
+void* workspace(ScratchHold* hold, int device_id, cudaStream_t stream, size_t bytes) {
+  return grow(hold, 0, device_id, stream, bytes);
+}
+
+void* zeroed_workspace(ScratchHold* hold, int device_id, cudaStream_t stream, size_t bytes) {
+  return grow(hold, 1, device_id, stream, bytes);
 }
 
 int take_scratch(int device_id, cudaStream_t stream, size_t bytes, size_t counter_bytes, CallScratch* out) {
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   SPTIR_CUDA_OK(cudaStreamIsCapturing(stream, &capture));
   if (capture == cudaStreamCaptureStatusNone) {
-    out->scratch = static_cast<char*>(workspace(device_id, stream, bytes));
+    out->scratch = static_cast<char*>(workspace(&out->hold, device_id, stream, bytes));
     if (out->scratch == nullptr) return -1;
     if (counter_bytes > 0) {
-      out->counters = static_cast<unsigned*>(zeroed_workspace(device_id, stream, counter_bytes));
+      out->counters = static_cast<unsigned*>(zeroed_workspace(&out->hold, device_id, stream, counter_bytes));
       if (out->counters == nullptr) return -1;
     }
     return 0;
@@ -171,8 +204,9 @@ int sparsetir_reserve_workspace(int device_id, void* stream, size_t scratch_byte
                                 size_t counter_bytes) {
   if (sptir::use_device(device_id) != 0) return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (scratch_bytes > 0 && sptir::workspace(device_id, st, scratch_bytes) == nullptr) return -1;
-  if (counter_bytes > 0 && sptir::zeroed_workspace(device_id, st, counter_bytes) == nullptr) return -1;
+  sptir::ScratchHold hold;
+  if (scratch_bytes > 0 && sptir::workspace(&hold, device_id, st, scratch_bytes) == nullptr) return -1;
+  if (counter_bytes > 0 && sptir::zeroed_workspace(&hold, device_id, st, counter_bytes) == nullptr) return -1;
   return 0;
 }
 
