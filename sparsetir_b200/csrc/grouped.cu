@@ -418,6 +418,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       ok = __all_sync(0xffffffffu, ok);
       advance(tile.steps);
     }
+    // The last arrivals at this block's barriers come from the other block too: they have come before the block ends.
+    for (int i = 0; i < kStages && ok; ++i) {
+      ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_empty[stage], phase ^ 1u));
+      advance(1);
+    }
   } else if (warp == 1) {
     // ---- MMAs of both blocks, from rank 0: M = 256 features, N = the tile's columns
     int acc = 0;
