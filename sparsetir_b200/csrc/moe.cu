@@ -708,8 +708,9 @@ extern "C" int sparsetir_moe_dispatch_i8_raw(const void* x, int type, const int3
                                              int rows, int feat, int top_k, int device_id, void* stream) {
   const char* fn = "sparsetir_moe_dispatch_i8";
   if (check_rows(fn, type, tokens, rows, feat, top_k) != 0) return -1;
+  if (tokens == 0) return 0;
   if (!slots && (top_k != 1 || rows != tokens)) return fail("%s: slots may be null with top_k 1 and a row per token only", fn);
-  if (tokens == 0 || rows == 0 || feat == 0) return 0;
+  if (rows == 0 || feat == 0) return 0;
   if (!x || !q || !scale) return fail("%s: null pointer argument", fn);
   if (use_device(device_id) != 0) return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
