@@ -323,7 +323,8 @@ SPARSETIR_API int sparsetir_sparse_conv_f16(SPARSETIR_PACKED_ARGS);
  * one expert in the order of the tokens: indptr i32[num_experts+1] bounds the experts' rows like the row pointers
  * of a CSR matrix, slots i32[T*top_k] is the row of every pair, or -1 for a pair without an expert.
  * Element types: f32, f16, bf16 (DLPack code kDLBfloat); sums are formed in f32 whatever the type.  top_k <= 32,
- * num_experts <= 1024.  Results do not depend on the order in which blocks run. */
+ * num_experts <= 1024; tokens, rows, groups and features up to 2^31 - 4097.  Results do not depend on the order in which blocks
+ * run. */
 #define SPARSETIR_MOE_RENORMALIZE 1 /* gates of a token are divided by their sum */
 #define SPARSETIR_MOE_MAX_TOP_K 32
 #define SPARSETIR_MOE_MAX_EXPERTS 1024

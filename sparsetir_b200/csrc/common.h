@@ -104,6 +104,9 @@ int peer_table(const char* fn, const void* own, int n_peers, void* const* peers,
 
 constexpr int kNumSMs = 148;  // B200
 
+// Sizes up to here may be rounded up to tiles, steps and strides of a block in 32 bits.
+constexpr int kLargestSize = INT32_MAX - 4096;
+
 inline int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
 }  // namespace sptir

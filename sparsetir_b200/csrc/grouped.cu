@@ -688,6 +688,9 @@ int launch_type(int columns, int type, const CUtensorMap& tm_a, const CUtensorMa
 int check_groups(const char* fn, const int32_t* indptr, int rows, int groups, int fi, int fo, int flags) {
   if (rows < 0 || groups < 0) return fail("%s: negative size", fn);
   if (fi < 1 || fo < 1) return fail("%s: feat_in and feat_out must be positive", fn);
+  if (std::max(std::max(rows, groups), std::max(fi, fo)) > kLargestSize ||
+      (groups > 0 && static_cast<long long>(fi) * fo > INT64_MAX / groups))
+    return fail("%s: too large for 32-bit indices", fn);
   if ((flags & ~SPARSETIR_GROUPED_W_OUT_IN) != 0) return fail("%s: unknown flags %d", fn, flags);
   if (!indptr && groups > 1) return fail("%s: indptr may be null with num_groups 1 only", fn);
   return 0;
@@ -753,11 +756,11 @@ bool wide_rows(const void* out, int type, int features) {
 // 9.0 / 14.0; 16, 8, 1024 -> 1024 3.8 / 8.8; 64, 8, 2048 -> 2048 15.5 / 15.8; 8-bit integers 1, 1, 4096 -> 8192 8.2 / 14; but 128, 8,
 // 2048 -> 2048 20 / 16 and 500, 64, 2048 -> 2048 114 / 90, which have tiles enough; along the features 16, 8, 512 -> 512 3.2 / 6.5,
 // 1, 1, 4096 -> 4096 8.0 / 11.9, 16, 8, 1784 -> 1112 7.9 / 12.6, but 48, 8, 1024 -> 4096 17.4 / 14.2.  The bound on the rows is
-// for batches that meet in one group, which it walks 16 rows at a time.
+// for batches that meet in one group, which it walks 16 rows at a time; it holds bytes of the depth in 32 bits.
 bool few_rows_pay(int rows, int groups, int fi, int fo, bool along_k) {
   const long long used = std::min(groups, rows);
   const long long tiles = used * ceil_div(fo, 2 * kM);
-  if (rows > 256 || rows > (tiles < kNumSMs / 4 ? 16 : 8) * used || groups > 65535) return false;
+  if (rows > 256 || rows > (tiles < kNumSMs / 4 ? 16 : 8) * used || groups > 65535 || fi > (1 << 29)) return false;
   return along_k ? tiles <= 256 : used * fi <= (24 << 20) / fo;
 }
 
@@ -901,7 +904,8 @@ extern "C" int sparsetir_grouped_mm_grad_w_raw(const void* x, const void* dy, in
 extern "C" int sparsetir_grouped_mm_workspace(int rows, int num_groups, int feat_in, int feat_out, int element_bytes, int flags,
                                               size_t* scratch_bytes) {
   const char* fn = "sparsetir_grouped_mm_workspace";
-  if (check_groups(fn, nullptr, rows, std::min(num_groups, 1), feat_in, feat_out, flags) != 0) return -1;
+  const int32_t some = 0;  // pointers are not looked at
+  if (check_groups(fn, &some, rows, num_groups, feat_in, feat_out, flags) != 0) return -1;
   if ((element_bytes != 1 && element_bytes != 2) || !scratch_bytes) return fail("%s: bad argument", fn);
   *scratch_bytes = 0;
   if (rows == 0 || num_groups == 0) return 0;

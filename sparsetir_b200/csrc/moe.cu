@@ -594,6 +594,7 @@ int with_piece(int b, F&& f) {
 int check_rows(const char* fn, int type, int tokens, int rows, int feat, int top_k) {
   if (type < SPARSETIR_F32 || type > SPARSETIR_BF16) return fail("%s: unknown element type %d", fn, type);
   if (tokens < 0 || rows < 0 || feat < 0) return fail("%s: negative size", fn);
+  if (std::max(tokens, std::max(rows, feat)) > kLargestSize) return fail("%s: too large for 32-bit indices", fn);
   if (top_k < 1 || top_k > SPARSETIR_MOE_MAX_TOP_K)
     return fail("%s: top_k = %d is not in [1, %d]", fn, top_k, SPARSETIR_MOE_MAX_TOP_K);
   return 0;
