@@ -371,7 +371,9 @@ SPARSETIR_API int sparsetir_moe_combine_grad(SPARSETIR_PACKED_ARGS);
 /* Products grouped by expert, ragged sizes: y[s, :] = x[s, :] * W[g] for the rows s in [indptr[g], indptr[g+1]).
  * W is [num_groups, feat_in, feat_out], or with SPARSETIR_GROUPED_W_OUT_IN [num_groups, feat_out, feat_in]; the
  * gradient with respect to x is the same call on dy with the flag the other way round and the sizes exchanged.
- * Rows of no group are not written.  indptr may be null with num_groups 1: all rows.
+ * Rows of no group are not written.  indptr may be null with num_groups 1: all rows.  It starts at 0, like the row pointers of
+ * a CSR matrix: where index arrays are checked (sparsetir_set_validate) another start is refused, otherwise the rows ahead of it
+ * belong to no group.  It may end before the last row, as it does behind a router that masked experts.
  * args: (x f16|bf16 [S*feat_in], w (type of x), y (type of x, or f32) [S*feat_out], indptr i32[num_groups+1] or null,
  *        num_groups, feat_in, feat_out [, flags]). */
 #define SPARSETIR_GROUPED_W_OUT_IN 1
