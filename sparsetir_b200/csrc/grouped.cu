@@ -565,17 +565,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
     if (row >= p.rows) return;
     if (p.indptr != nullptr) {
       if (row < ld_global(p.indptr) || row >= ld_global(p.indptr + p.groups)) return;
-      if constexpr (I8) {  // the last group that starts at or before the row: 32 pointers at a time
-        int lo = 0, n = p.groups;
-        while (n > 1) {
-          const int step = (n + 31) / 32;
-          const bool in = lane * step < n && ld_global(p.indptr + lo + min(lane * step, n - 1)) <= row;
-          const int last = 31 - __clz(__ballot_sync(0xffffffffu, in) | 1u);
-          lo += last * step;
-          n = min(step, n - last * step);
-        }
-        group = lo;
-      }
+      if constexpr (I8) group = group_of_row(p.indptr, p.groups, row, lane);
     }
   } else if (row >= static_cast<long long>(p.groups) * p.columns) {
     return;
@@ -755,12 +745,13 @@ bool wide_rows(const void* out, int type, int features) {
 // unless said otherwise; rows, groups, features): W contiguous along the depth 2, 1, 4096 -> 4096 7.9 / 13.4; 16, 1, 4096 -> 4096
 // 9.0 / 14.0; 16, 8, 1024 -> 1024 3.8 / 8.8; 64, 8, 2048 -> 2048 15.5 / 15.8; 8-bit integers 1, 1, 4096 -> 8192 8.2 / 14; but 128, 8,
 // 2048 -> 2048 20 / 16 and 500, 64, 2048 -> 2048 114 / 90, which have tiles enough; along the features 16, 8, 512 -> 512 3.2 / 6.5,
-// 1, 1, 4096 -> 4096 8.0 / 11.9, 16, 8, 1784 -> 1112 7.9 / 12.6, but 48, 8, 1024 -> 4096 17.4 / 14.2.  The bound on the rows is
-// for batches that meet in one group, which it walks 16 rows at a time; it holds bytes of the depth in 32 bits.
+// 1, 1, 4096 -> 4096 8.0 / 11.9, 16, 8, 1784 -> 1112 7.9 / 12.6, but 48, 8, 1024 -> 4096 17.4 / 14.2.  The bound on the rows
+// is for batches that meet in one group, whose weights it reads again for every 8 or 16 rows (256 rows in one of 64 groups,
+// 2048 -> 1024 28 / 15; 8-bit integers 17 / 10; 512 -> 512 6.9 / 7.6); it holds bytes of the depth in 32 bits.
 bool few_rows_pay(int rows, int groups, int fi, int fo, bool along_k) {
   const long long used = std::min(groups, rows);
   const long long tiles = used * ceil_div(fo, 2 * kM);
-  if (rows > 256 || rows > (tiles < kNumSMs / 4 ? 16 : 8) * used || groups > 65535 || fi > (1 << 29)) return false;
+  if (rows > 256 || rows > (tiles < kNumSMs / 4 ? 16 : 8) * used || groups > 65000 || fi > (1 << 29)) return false;
   return along_k ? tiles <= 256 : used * fi <= (24 << 20) / fo;
 }
 

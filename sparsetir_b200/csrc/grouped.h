@@ -1,10 +1,25 @@
-// What grouped.cu hands to grouped_few.cu.
+// What grouped.cu and grouped_few.cu share, and what the first hands to the second.
 #ifndef SPARSETIR_B200_GROUPED_H_
 #define SPARSETIR_B200_GROUPED_H_
 
 #include "common.h"
+#include "launch.cuh"
 
 namespace sptir {
+
+// The last of the groups that starts at or before the row, group 0 if none does: 32 pointers at a time, by all lanes of a warp
+// together.
+__device__ __forceinline__ int group_of_row(const int32_t* indptr, int groups, long long row, int lane) {
+  int lo = 0, n = groups;
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const bool in = lane * step < n && ld_global(indptr + lo + min(lane * step, n - 1)) <= row;
+    const int last = 31 - __clz(__ballot_sync(0xffffffffu, in) | 1u);
+    lo += last * step;
+    n = min(step, n - last * step);
+  }
+  return lo;
+}
 
 struct FewArgs {
   const void* x;

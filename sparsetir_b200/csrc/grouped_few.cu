@@ -181,7 +181,12 @@ struct AlongFeatures {
   }
 };
 
-// Block = (group, features); `splits` of its warps share the depth of the same features.
+// Block = (rows, features); `splits` of its warps share the depth of the same features.  Blocks y < groups have the first kRows rows
+// of group y; one more block for every further kRows rows of the operand has what lies in them of the rest of a group: of
+// the one that their first row belongs to, since the rest of a group that begins among them lies behind them.  They come last and
+// find the weights in L2.  With a group's rows walked by its own few blocks, a batch that met in a few groups waited for
+// these (256 rows, 64 groups, 2048 -> 1024, W along the depth, us, spread evenly / a quarter in one group / all in one:
+// 50 / 175 / 437, this way 50 / 50 / 28; the kernel of grouped.cu 47 / 46 / 15).
 template <class Operand, class OutT>
 __global__ void __launch_bounds__(32 * kMaxWarps, 1) few_rows_kernel(const __grid_constant__ FewArgs p) {
   using Sum = typename Operand::Sum;
@@ -190,18 +195,27 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 1) few_rows_kernel(const __gri
   Sum(*const part)[kRows][F] = reinterpret_cast<Sum(*)[kRows][F]>(smem);  // of every warp
   chain_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int group = blockIdx.y;
-  int first = 0, last = p.rows;
-  if (p.indptr != nullptr) {
-    first = min(max(ld_global(p.indptr + group), 0), p.rows);
-    last = min(ld_global(p.indptr + group + 1), p.rows);
+  int group = blockIdx.y, from = 0;
+  const bool rest = group >= p.groups;
+  if (__builtin_expect(rest, 0)) {
+    from = (group - p.groups + 1) * kRows;
+    group = p.indptr != nullptr ? group_of_row(p.indptr, p.groups, from, lane) : 0;
   }
+  int row0 = 0, end = p.rows;
+  if (p.indptr != nullptr) {
+    row0 = min(max(ld_global(p.indptr + group), 0), p.rows);
+    end = min(ld_global(p.indptr + group + 1), p.rows);
+  }
+  if (rest) row0 = max(row0 + kRows, from);
+  end = min(end, (rest ? from : row0) + kRows);
   const int fw = warp / p.splits, ks = warp - fw * p.splits;
   const int block_feats = p.feature_warps * F;
   const int block_feat0 = blockIdx.x * block_feats;
   const int k0 = ks * p.split_bytes, k1 = min(k0 + p.split_bytes, p.k_bytes);
-  for (int row0 = first; row0 < last; row0 += kRows) {
-    const int live = min(kRows, last - row0);
+  // Once.  Without the loop the compiler moves what is behind the steps ahead of them and spills 70 bytes of registers (one row,
+  // 4096 -> 8192 in 8 bits, quantised: 10.0 us where now 8.7).
+  for (; row0 < end; row0 += kRows) {
+    const int live = end - row0;
     Operand op;
     op.start(p, group, block_feat0 + fw * F, row0, live, k0, k1, lane);
     const int steps = (k1 - k0 + Operand::kStepBytes - 1) / Operand::kStepBytes;  // <= 0: nothing of the depth left
@@ -246,7 +260,7 @@ int launch(FewArgs p, cudaStream_t st) {
   while (p.feature_warps > 1 && warps / p.feature_warps < kNumSMs) p.feature_warps /= 2;
   p.splits = splits;
   p.split_bytes = (ceil_div(p.k_bytes, splits) + 127) / 128 * 128;
-  const dim3 grid(ceil_div(p.fo, p.feature_warps * Operand::kFeatures), p.groups);
+  const dim3 grid(ceil_div(p.fo, p.feature_warps * Operand::kFeatures), p.groups + (p.rows - 1) / Operand::kRows);
   const int block_warps = p.feature_warps * splits, smem = block_warps * Operand::kRows * Operand::kFeatures * 4;
   static thread_local int configured_device = -1;
   int dev = 0;
