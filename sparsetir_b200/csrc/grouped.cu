@@ -14,7 +14,7 @@
 // take the other one out; a pair's units are those of its number, of its number plus the pairs, and so on.
 // With all operands in L2 a step of K (64 deep, 512 clocks of the tensor core) takes 0.28 us of loads, 117 GB/s into each SM:
 // loads and MMAs are even, and beyond about 1.2 PFLOP/s the power limit lowers the clock.  65,536 rows in 64 ragged groups, 2048 ->
-// 2048, bf16: 0.45-0.51 ms, 1.08-1.2 PFLOP/s, by the clock (8192^3 in one group: 0.71-0.83 ms; a library product 0.75).  The
+// 2048, bf16: 0.45-0.53 ms, 1.04-1.2 PFLOP/s, by the clock (8192^3 in one group: 0.71-0.83 ms; a library product 0.75).  The
 // gradient of 64 weights of 2048 x 1024 over 32,768 rows, 8 steps to a tile, 0.16-0.17 ms: its 470 MB alone are 72 us.
 // Tried and taken back: equal column tiles instead of 256 and a remainder (more, smaller loads: 45 -> 54 us on 6,001 rows); a
 // prefetch of the next tiles' operands to L2 (44 -> 60); the whole tiles of all groups first (no change); one arrival

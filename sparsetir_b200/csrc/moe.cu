@@ -373,7 +373,8 @@ dispatch_kernel(const Piece<B>* x, const int32_t* slots, Piece<B>* z, int tokens
 }
 
 // A warp sums up to 64 pieces of a token's rows, four rows requested together, in 32 bits and in the order of the choices.  HBM
-// bounds the large ones; those of a decoding step are the chain slots -> rows and a launch (24 tokens: 2.5 us in a graph).
+// bounds the large ones (8,192 x 8 rows of 2048 in 16 bits, 302 MB in 49.8 us, 6.06 TB/s); those of a decoding step are the chain
+// slots -> rows and a launch (24 tokens: 2.5 us in a graph).
 template <class T, class OutT, int B>
 __global__ void __launch_bounds__(kWarps * 32)
 combine_kernel(const Piece<B>* z, const int32_t* slots, const float* gates, OutT* y, int tokens, int rows, int pieces,
