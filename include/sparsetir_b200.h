@@ -43,7 +43,7 @@ extern "C" {
 #ifndef DLPACK_DLPACK_H_
 typedef enum { kDLCPU = 1, kDLCUDA = 2, kDLCUDAHost = 3 } SpDLDeviceType;
 typedef struct { int32_t device_type; int32_t device_id; } DLDevice;
-typedef enum { kDLInt = 0U, kDLUInt = 1U, kDLFloat = 2U, kDLBfloat = 4U } SpDLDataTypeCode;
+typedef enum { kDLInt = 0U, kDLUInt = 1U, kDLFloat = 2U, kDLBfloat = 4U, kDLFloat8E4M3 = 10U } SpDLDataTypeCode;
 typedef struct { uint8_t code; uint8_t bits; uint16_t lanes; } DLDataType;
 typedef struct {
   void* data;
@@ -392,6 +392,49 @@ SPARSETIR_API int sparsetir_grouped_mm_grad_w(SPARSETIR_PACKED_ARGS);
  * feat_in < 131072. */
 SPARSETIR_API int sparsetir_grouped_mm_i8(SPARSETIR_PACKED_ARGS);
 
+/* The gated block of an expert in one product: with h = x[s, :] * W[g]^T of 2 * width features, the gate's first,
+ *   y[s, j] = f(h[j]) * h[width + j],   f(v) = v * sigmoid(v), with SPARSETIR_GATED_GELU v * sigmoid(2 u),
+ *   u = sqrt(2 / pi) * (v + 0.044715 v^3): the form of gelu with tanh.
+ * W is [num_groups, 2 * width, feat_in].  y is formed from the sums themselves; `hidden` (null: not kept) receives h in the type of
+ * x, for the gradient.  Rows of no group are not written; indptr as for sparsetir_grouped_mm.
+ * args: (x f16|bf16 [S*feat_in], w (type of x) [num_groups*2*width*feat_in], y (type of x) [S*width],
+ *        hidden (type of x) [S*2*width] or null, indptr i32[num_groups+1] or null, num_groups, feat_in, width [, flags]). */
+#define SPARSETIR_GATED_GELU 2
+SPARSETIR_API int sparsetir_grouped_mm_gated(SPARSETIR_PACKED_ARGS);
+
+/* Gradient of the gated block through the product that follows it: with d = dy[s, :] * W[g], W of that product, [num_groups, feat,
+ * width] (with SPARSETIR_GROUPED_W_OUT_IN [num_groups, width, feat]), and h = hidden[s, :],
+ *   d_hidden[s, j] = d[j] h[width + j] f'(h[j]),   d_hidden[s, width + j] = d[j] f(h[j]);
+ * `act` (null: not wanted) receives f(h[j]) h[width + j], formed again from h for the gradient of W.  The gradients to the block's
+ * input and weights are sparsetir_grouped_mm and sparsetir_grouped_mm_grad_w on d_hidden.  Rows of no group are not written.
+ * args: (dy f16|bf16 [S*feat], w (type of dy) [num_groups*feat*width], hidden (type of dy) [S*2*width], d_hidden (type of dy)
+ *        [S*2*width], act (type of dy) [S*width] or null, indptr i32[num_groups+1] or null, num_groups, feat, width [, flags]). */
+SPARSETIR_API int sparsetir_grouped_mm_gated_grad(SPARSETIR_PACKED_ARGS);
+
+/* ---- products in 8-bit floating point (e4m3, DLPack code kDLFloat8E4M3) with a scale for each block of 128 ----
+ * A scale belongs to 128 consecutive features of a row of x, and to 128 x 128 of W (fewer at the ends). */
+#define SPARSETIR_F8_BLOCK 128
+
+/* Rows of the tokens to expert order in 8 bits: for each 128 features of a row, a = max |x|,
+ *   scale = a / 448,  q = 448 x / a to the nearest e4m3, ties to even.
+ * Features with a below 2^-110 become zeros with scale 0; with an infinity or a NaN among them zeros with that as their
+ * scale.  scale is [ceil(feat / 128), S]: those of one block of features side by side.  slots may be null with top_k 1: row t goes
+ * to row t.
+ * args: (x f32|f16|bf16 [T*feat], slots i32[T*top_k] or null, q e4m3 [S*feat], scale f32[ceil(feat/128)*S], feat, top_k). */
+SPARSETIR_API int sparsetir_moe_dispatch_f8(SPARSETIR_PACKED_ARGS);
+
+/* y[s, fo] = sum over the blocks b of 128 of feat_in of  x_scale[b, s] * w_scale[g, fo / 128, b] * sum_{fi in b} x[s, fi] * w[g, fo, fi],
+ * sums in f32.
+ * args: (x e4m3 [S*feat_in], x_scale f32[ceil(feat_in/128)*S], w e4m3 [num_groups*feat_out*feat_in],
+ *        w_scale f32[num_groups*ceil(feat_out/128)*ceil(feat_in/128)], y f16|bf16|f32 [S*feat_out], indptr i32[num_groups+1] or null,
+ *        num_groups, feat_in, feat_out). */
+SPARSETIR_API int sparsetir_grouped_mm_f8(SPARSETIR_PACKED_ARGS);
+
+/* The gated block (sparsetir_grouped_mm_gated) of such operands, W [num_groups, 2 * width, feat_in].
+ * args: (x, x_scale, w, w_scale as above with feat_out = 2 * width, y f16|bf16 [S*width], indptr or null, num_groups, feat_in,
+ *        width [, flags]). */
+SPARSETIR_API int sparsetir_grouped_mm_gated_f8(SPARSETIR_PACKED_ARGS);
+
 /* ---- operators, plain-pointer form (device pointers; stream is a cudaStream_t) -------- */
 SPARSETIR_API int sparsetir_csrmm_raw(const float* a, const float* b, float* c,
                                       const int32_t* indptr, const int32_t* indices, int m, int n,
@@ -552,7 +595,9 @@ SPARSETIR_API int sparsetir_moe_combine_grad_raw(const void* dy, const void* z, 
                                                  const float* gates, void* dz, float* d_gates, int tokens, int rows,
                                                  int feat, int top_k, int device_id, void* stream);
 /* Scratch bytes at most of sparsetir_grouped_mm and its gradient (element_bytes 2) or of sparsetir_grouped_mm_i8 (1): copies of
- * operands whose rows do not start at 16-byte addresses, and sums of thread blocks that share a tile (20 MB at most). */
+ * operands whose rows do not start at 16-byte addresses, and sums of thread blocks that share a tile (20 MB at most).  Of the
+ * gated products with feat_out = 2 * width, of sparsetir_grouped_mm_gated_grad with feat and width as feat_in and feat_out, of the products
+ * of 8-bit floating point with element_bytes 1. */
 SPARSETIR_API int sparsetir_grouped_mm_workspace(int rows, int num_groups, int feat_in, int feat_out, int element_bytes,
                                                  int flags, size_t* scratch_bytes);
 /* rows: how many x and y have; row pointers outside of [0, rows] are taken as the nearer bound */
@@ -566,6 +611,20 @@ SPARSETIR_API int sparsetir_grouped_mm_i8_raw(const int8_t* x, const float* x_sc
                                               const float* w_scale, void* y, int y_type, const int32_t* indptr,
                                               int rows, int num_groups, int feat_in, int feat_out, int device_id,
                                               void* stream);
+SPARSETIR_API int sparsetir_grouped_mm_gated_raw(const void* x, const void* w, void* y, void* hidden, int type,
+                                                 const int32_t* indptr, int rows, int num_groups, int feat_in, int width,
+                                                 int flags, int device_id, void* stream);
+SPARSETIR_API int sparsetir_grouped_mm_gated_grad_raw(const void* dy, const void* w, const void* hidden, void* d_hidden, void* act,
+                                                      int type, const int32_t* indptr, int rows, int num_groups, int feat,
+                                                      int width, int flags, int device_id, void* stream);
+SPARSETIR_API int sparsetir_moe_dispatch_f8_raw(const void* x, int type, const int32_t* slots, void* q, float* scale, int tokens,
+                                                int rows, int feat, int top_k, int device_id, void* stream);
+SPARSETIR_API int sparsetir_grouped_mm_f8_raw(const void* x, const float* x_scale, const void* w, const float* w_scale, void* y,
+                                              int y_type, const int32_t* indptr, int rows, int num_groups, int feat_in,
+                                              int feat_out, int device_id, void* stream);
+SPARSETIR_API int sparsetir_grouped_mm_gated_f8_raw(const void* x, const float* x_scale, const void* w, const float* w_scale,
+                                                    void* y, int y_type, const int32_t* indptr, int rows, int num_groups,
+                                                    int feat_in, int width, int flags, int device_id, void* stream);
 
 /* ---- host-side format conversion (CPU int32 arrays) ----------------------------------- */
 

@@ -57,7 +57,7 @@ class EllBucket(ctypes.Structure):
 
 
 kDLCPU, kDLCUDA, kDLCUDAHost = 1, 2, 3
-kDLInt, kDLUInt, kDLFloat, kDLBfloat = 0, 1, 2, 4
+kDLInt, kDLUInt, kDLFloat, kDLBfloat, kDLFloat8E4M3 = 0, 1, 2, 4, 10
 kTVMArgInt, kTVMArgFloat, kTVMOpaqueHandle, kTVMNullptr = 0, 2, 3, 4
 kTVMDLTensorHandle, kTVMNDArrayHandle = 7, 13
 
@@ -66,6 +66,8 @@ HYB_MAX_BUCKETS = 64
 MOE_RENORMALIZE = 1
 MOE_MAX_TOP_K, MOE_MAX_EXPERTS = 32, 1024
 GROUPED_W_OUT_IN = 1
+GATED_GELU = 2
+F8_BLOCK = 128
 
 PACKED_SYMBOLS = (
     "sparsetir_csrmm",
@@ -94,6 +96,11 @@ PACKED_SYMBOLS = (
     "sparsetir_grouped_mm",
     "sparsetir_grouped_mm_grad_w",
     "sparsetir_grouped_mm_i8",
+    "sparsetir_grouped_mm_gated",
+    "sparsetir_grouped_mm_gated_grad",
+    "sparsetir_moe_dispatch_f8",
+    "sparsetir_grouped_mm_f8",
+    "sparsetir_grouped_mm_gated_f8",
 )
 
 # every other exported symbol: name -> (restype, argtypes)
@@ -150,6 +157,11 @@ PLAIN_SYMBOLS = {
     "sparsetir_grouped_mm_raw": (_i, [_vp, _vp, _i, _vp, _i, _vp] + [_i] * 6 + [_vp]),
     "sparsetir_grouped_mm_grad_w_raw": (_i, [_vp, _vp, _i, _vp, _i, _vp] + [_i] * 6 + [_vp]),
     "sparsetir_grouped_mm_i8_raw": (_i, [_vp] * 5 + [_i, _vp] + [_i] * 5 + [_vp]),
+    "sparsetir_grouped_mm_gated_raw": (_i, [_vp] * 4 + [_i, _vp] + [_i] * 6 + [_vp]),
+    "sparsetir_grouped_mm_gated_grad_raw": (_i, [_vp] * 5 + [_i, _vp] + [_i] * 6 + [_vp]),
+    "sparsetir_moe_dispatch_f8_raw": (_i, [_vp, _i] + [_vp] * 3 + [_i] * 5 + [_vp]),
+    "sparsetir_grouped_mm_f8_raw": (_i, [_vp] * 5 + [_i, _vp] + [_i] * 5 + [_vp]),
+    "sparsetir_grouped_mm_gated_f8_raw": (_i, [_vp] * 5 + [_i, _vp] + [_i] * 6 + [_vp]),
     "sparsetir_column_part_hyb": (_vp, [_i, _i, _i32p, _i32p, _i, _i32p, _i, _i]),
     "sparsetir_hyb_num_rows": (_i64, [_vp, _i, _i]),
     "sparsetir_hyb_copy_bucket": (_i, [_vp, _i, _i, _i32p, _i32p, _i32p, _i32p, _f32p, _f32p]),

@@ -35,7 +35,7 @@ struct Packed {
       return fail("%s: %s.ndim is expected to equal 1 (flat buffer), got %d", fn, name, t->ndim);
     if (t->dtype.code != code || t->dtype.bits != bits || t->dtype.lanes != 1)
       return fail("%s: %s.dtype is expected to be %s%d, got code=%d bits=%d lanes=%d", fn, name,
-                  code == kDLFloat ? "float" : (code == kDLInt ? "int" : "uint"), bits,
+                  code == kDLFloat ? "float" : code == kDLInt ? "int" : code == kDLFloat8E4M3 ? "e4m3 float" : "uint", bits,
                   t->dtype.code, t->dtype.bits, t->dtype.lanes);
     if (t->strides != nullptr && t->shape[0] > 1 && t->strides[0] != 1)
       return fail("%s: %s.strides: expected to be compact array", fn, name);
@@ -958,17 +958,18 @@ struct Groups {
   void* indptr = nullptr;
   int64_t num = 0, feat_in = 0, feat_out = 0, flags = 0;
 };
-static int groups(Packed& p, int at, bool with_flags, Groups* g) {
+static int groups(Packed& p, int at, bool with_flags, Groups* g, int64_t known = SPARSETIR_GROUPED_W_OUT_IN,
+                  const char* in = "feat_in", const char* out = "feat_out") {
   int64_t lp = 0;
   if (!p.absent(at)) TRY(p.tensor(at, "indptr", kDLInt, 32, &g->indptr, &lp));
   TRY(p.integer(at + 1, "num_groups", &g->num));
-  TRY(p.integer(at + 2, "feat_in", &g->feat_in));
-  TRY(p.integer(at + 3, "feat_out", &g->feat_out));
+  TRY(p.integer(at + 2, in, &g->feat_in));
+  TRY(p.integer(at + 3, out, &g->feat_out));
   if (with_flags && p.n == at + 5) TRY(p.integer(at + 4, "flags", &g->flags));
   TRY(fits_i32(p.fn, "num_groups", g->num));
-  if (g->feat_in < 1 || g->feat_out < 1) return fail("%s: feat_in and feat_out must be positive", p.fn);
-  TRY(fits_i32(p.fn, "feat_in", g->feat_in)); TRY(fits_i32(p.fn, "feat_out", g->feat_out));
-  if (g->flags & ~int64_t{SPARSETIR_GROUPED_W_OUT_IN}) return fail("%s: unknown flags %lld", p.fn, (long long)g->flags);
+  if (g->feat_in < 1 || g->feat_out < 1) return fail("%s: %s and %s must be positive", p.fn, in, out);
+  TRY(fits_i32(p.fn, in, g->feat_in)); TRY(fits_i32(p.fn, out, g->feat_out));
+  if (g->flags & ~known) return fail("%s: unknown flags %lld", p.fn, (long long)g->flags);
   if (p.absent(at)) {
     if (g->num != 1) return fail("%s: indptr may be null with num_groups 1 only, got %lld", p.fn, (long long)g->num);
     return 0;
@@ -977,8 +978,8 @@ static int groups(Packed& p, int at, bool with_flags, Groups* g) {
 }
 
 // num_groups matrices of feat_in x feat_out
-static int check_weights(const char* fn, const char* name, int64_t len, const Groups& g) {
-  const int64_t each = g.feat_in * g.feat_out;  // both below 2^31
+static int check_weights(const char* fn, const char* name, int64_t len, const Groups& g, int64_t times = 1) {
+  const int64_t each = g.feat_in * g.feat_out * times;  // both below 2^31, 1 or 2 of them
   if (g.num > 0 && each > INT64_MAX / g.num) return fail("%s: %s is too large", fn, name);
   return check_len(fn, name, len, g.num * each);
 }
@@ -1048,6 +1049,134 @@ int sparsetir_grouped_mm_i8(SPARSETIR_PACKED_ARGS) {
   return sparsetir_grouped_mm_i8_raw(static_cast<const int8_t*>(x), static_cast<const float*>(xs), static_cast<const int8_t*>(w),
                                      static_cast<const float*>(ws), y, ytype, static_cast<const int32_t*>(g.indptr), (int)rows,
                                      (int)g.num, (int)g.feat_in, (int)g.feat_out, p.device_id, sptir::stream_for(p.device_id));
+}
+
+int sparsetir_grouped_mm_gated(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_grouped_mm_gated", args, type_codes, num_args};
+  if (num_args != 8 && num_args != 9) return fail("sparsetir_grouped_mm_gated: num_args should be 8 or 9, got %d", num_args);
+  void *x = nullptr, *w = nullptr, *y = nullptr, *h = nullptr;
+  int64_t lx = 0, lw = 0, ly = 0, lh = 0, rows = 0;
+  int type = 0, same = 0;
+  Groups g;
+  TRY(p.floating(0, "x", kHalves, &type, &x, &lx));
+  TRY(p.floating(1, "w", 1u << type, &same, &w, &lw));
+  TRY(p.floating(2, "y", 1u << type, &same, &y, &ly));
+  if (!p.absent(3)) TRY(p.floating(3, "hidden", 1u << type, &same, &h, &lh));
+  TRY(groups(p, 4, true, &g, SPARSETIR_GATED_GELU, "feat_in", "width"));
+  TRY(whole_rows(p.fn, "x", lx, g.feat_in, &rows));
+  TRY(check_weights(p.fn, "w", lw, g, 2));
+  TRY(check_len(p.fn, "y", ly, rows * g.feat_out));
+  if (!p.absent(3)) TRY(check_len(p.fn, "hidden", lh, rows * g.feat_out * 2));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_grouped_mm_gated_raw(x, w, y, h, type, static_cast<const int32_t*>(g.indptr), (int)rows, (int)g.num,
+                                        (int)g.feat_in, (int)g.feat_out, (int)g.flags, p.device_id, sptir::stream_for(p.device_id));
+}
+
+int sparsetir_grouped_mm_gated_grad(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_grouped_mm_gated_grad", args, type_codes, num_args};
+  if (num_args != 9 && num_args != 10)
+    return fail("sparsetir_grouped_mm_gated_grad: num_args should be 9 or 10, got %d", num_args);
+  void *dy = nullptr, *w = nullptr, *h = nullptr, *dh = nullptr, *act = nullptr;
+  int64_t ldy = 0, lw = 0, lh = 0, ldh = 0, la = 0, rows = 0;
+  int type = 0, same = 0;
+  Groups g;
+  TRY(p.floating(0, "dy", kHalves, &type, &dy, &ldy));
+  TRY(p.floating(1, "w", 1u << type, &same, &w, &lw));
+  TRY(p.floating(2, "hidden", 1u << type, &same, &h, &lh));
+  TRY(p.floating(3, "d_hidden", 1u << type, &same, &dh, &ldh));
+  if (!p.absent(4)) TRY(p.floating(4, "act", 1u << type, &same, &act, &la));
+  TRY(groups(p, 5, true, &g, SPARSETIR_GATED_GELU | SPARSETIR_GROUPED_W_OUT_IN, "feat", "width"));
+  TRY(whole_rows(p.fn, "dy", ldy, g.feat_in, &rows));
+  TRY(check_weights(p.fn, "w", lw, g));
+  TRY(check_len(p.fn, "hidden", lh, rows * g.feat_out * 2));
+  TRY(check_len(p.fn, "d_hidden", ldh, rows * g.feat_out * 2));
+  if (!p.absent(4)) TRY(check_len(p.fn, "act", la, rows * g.feat_out));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_grouped_mm_gated_grad_raw(dy, w, h, dh, act, type, static_cast<const int32_t*>(g.indptr), (int)rows, (int)g.num,
+                                             (int)g.feat_in, (int)g.feat_out, (int)g.flags, p.device_id,
+                                             sptir::stream_for(p.device_id));
+}
+
+// Blocks of features that share a scale
+static int64_t scale_blocks(int64_t n) { return (n + SPARSETIR_F8_BLOCK - 1) / SPARSETIR_F8_BLOCK; }
+
+int sparsetir_moe_dispatch_f8(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_moe_dispatch_f8", args, type_codes, num_args};
+  if (num_args != 6) return fail("sparsetir_moe_dispatch_f8: num_args should be 6, got %d", num_args);
+  void *x = nullptr, *slots = nullptr, *q = nullptr, *scale = nullptr;
+  int64_t lx = 0, ls = 0, lq = 0, lc = 0, feat = 0, k = 0, tokens = 0, rows = 0;
+  int type = 0;
+  TRY(p.floating(0, "x", kAnyFloat, &type, &x, &lx));
+  if (!p.absent(1)) TRY(p.tensor(1, "slots", kDLInt, 32, &slots, &ls));
+  TRY(p.tensor(2, "q", kDLFloat8E4M3, 8, &q, &lq));
+  TRY(p.tensor(3, "scale", kDLFloat, 32, &scale, &lc));
+  TRY(p.integer(4, "feat_size", &feat));
+  TRY(p.integer(5, "top_k", &k));
+  TRY(check_top_k(p.fn, k));
+  TRY(whole_rows(p.fn, "x", lx, feat, &tokens));
+  TRY(whole_rows(p.fn, "q", lq, feat, &rows));
+  TRY(fits_i32(p.fn, "feat_size", feat)); TRY(fits_i32(p.fn, "the number of pairs", tokens * k));
+  TRY(check_len(p.fn, "scale", lc, scale_blocks(feat) * rows));
+  if (p.absent(1)) {
+    if (k != 1) return fail("sparsetir_moe_dispatch_f8: slots may be null with top_k 1 only, got %lld", (long long)k);
+    TRY(check_len(p.fn, "q", lq, lx));
+  } else {
+    TRY(check_len(p.fn, "slots", ls, tokens * k));
+  }
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_moe_dispatch_f8_raw(x, type, static_cast<const int32_t*>(slots), q, static_cast<float*>(scale), (int)tokens,
+                                       (int)rows, (int)feat, (int)k, p.device_id, sptir::stream_for(p.device_id));
+}
+
+// x, x_scale, w, w_scale, y and the groups of a product in 8-bit floating point; `times` W's rows to a feature of y
+struct ProductF8 {
+  void *x = nullptr, *xs = nullptr, *w = nullptr, *ws = nullptr, *y = nullptr;
+  int ytype = 0;
+  int64_t rows = 0;
+  Groups g;
+};
+static int product_f8(Packed& p, int64_t times, unsigned y_types, ProductF8* a) {
+  int64_t lx = 0, lxs = 0, lw = 0, lws = 0, ly = 0;
+  TRY(p.tensor(0, "x", kDLFloat8E4M3, 8, &a->x, &lx));
+  TRY(p.tensor(1, "x_scale", kDLFloat, 32, &a->xs, &lxs));
+  TRY(p.tensor(2, "w", kDLFloat8E4M3, 8, &a->w, &lw));
+  TRY(p.tensor(3, "w_scale", kDLFloat, 32, &a->ws, &lws));
+  TRY(p.floating(4, "y", y_types, &a->ytype, &a->y, &ly));
+  Groups& g = a->g;
+  TRY(groups(p, 5, times == 2, &g, SPARSETIR_GATED_GELU, "feat_in", times == 2 ? "width" : "feat_out"));
+  TRY(whole_rows(p.fn, "x", lx, g.feat_in, &a->rows));
+  TRY(check_len(p.fn, "x_scale", lxs, scale_blocks(g.feat_in) * a->rows));
+  TRY(check_weights(p.fn, "w", lw, g, times));
+  TRY(check_len(p.fn, "w_scale", lws, g.num * scale_blocks(g.feat_out * times) * scale_blocks(g.feat_in)));
+  return check_len(p.fn, "y", ly, a->rows * g.feat_out);
+}
+
+int sparsetir_grouped_mm_f8(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_grouped_mm_f8", args, type_codes, num_args};
+  if (num_args != 9) return fail("sparsetir_grouped_mm_f8: num_args should be 9, got %d", num_args);
+  ProductF8 a;
+  TRY(product_f8(p, 1, kAnyFloat, &a));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_grouped_mm_f8_raw(a.x, static_cast<const float*>(a.xs), a.w, static_cast<const float*>(a.ws), a.y, a.ytype,
+                                     static_cast<const int32_t*>(a.g.indptr), (int)a.rows, (int)a.g.num, (int)a.g.feat_in,
+                                     (int)a.g.feat_out, p.device_id, sptir::stream_for(p.device_id));
+}
+
+int sparsetir_grouped_mm_gated_f8(SPARSETIR_PACKED_ARGS) {
+  (void)resource_handle;
+  Packed p{"sparsetir_grouped_mm_gated_f8", args, type_codes, num_args};
+  if (num_args != 9 && num_args != 10)
+    return fail("sparsetir_grouped_mm_gated_f8: num_args should be 9 or 10, got %d", num_args);
+  ProductF8 a;
+  TRY(product_f8(p, 2, kHalves, &a));
+  set_void_return(out_ret_value, out_ret_tcode);
+  return sparsetir_grouped_mm_gated_f8_raw(a.x, static_cast<const float*>(a.xs), a.w, static_cast<const float*>(a.ws), a.y, a.ytype,
+                                           static_cast<const int32_t*>(a.g.indptr), (int)a.rows, (int)a.g.num, (int)a.g.feat_in,
+                                           (int)a.g.feat_out, (int)a.g.flags, p.device_id, sptir::stream_for(p.device_id));
 }
 
 }  // extern "C"

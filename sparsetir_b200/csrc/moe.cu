@@ -1,5 +1,7 @@
 // Router of a mixture of experts, and the exchange of rows between the order of the tokens and that of the experts.
 // The products between the two are in grouped.cu.
+#include <cuda_fp8.h>
+
 #include <algorithm>
 #include <cmath>
 
@@ -574,6 +576,91 @@ dispatch_i8_kernel(const Piece<B>* x, const int32_t* slots, Piece<B / sizeof(T)>
   }
 }
 
+// Rows to 8-bit floating point with a scale for each block of 128 features: L lanes have a block, P pieces each, and a warp kF8Hold
+// times as many blocks as it has room for.  The quotient 448 x / a is 0.875 x over a / 512: both are exact for elements of 16 bits,
+// and so is the quotient's place between the numbers of 8 bits, ties among them.
+constexpr int kF8Hold = 4;
+template <class T, int B>
+struct F8Lanes {
+  static constexpr int N = B / sizeof(T);  // elements of a piece
+  static constexpr int kLanes = SPARSETIR_F8_BLOCK / N < 32 ? SPARSETIR_F8_BLOCK / N : 32;
+  static constexpr int kPieces = SPARSETIR_F8_BLOCK / N / kLanes;
+  static constexpr int kBlocks = 32 / kLanes;  // of 128 features that a warp has side by side
+  static constexpr int kHold = kF8Hold / kPieces > 0 ? kF8Hold / kPieces : 1;
+};
+template <class T, int B>
+__global__ void __launch_bounds__(kWarps * 32)
+dispatch_f8_kernel(const Piece<B>* x, const int32_t* slots, Piece<B / sizeof(T)>* q, float* scale, int tokens, int rows, int pieces,
+                   int blocks, int chunks, int top_k) {
+  using Lanes = F8Lanes<T, B>;
+  constexpr int N = Lanes::N, L = Lanes::kLanes, P = Lanes::kPieces, H = Lanes::kHold;
+  chain_wait();
+  const int lane = threadIdx.x & 31;
+  const long long item = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int t = static_cast<int>(item / chunks), c = static_cast<int>(item - static_cast<long long>(t) * chunks);
+  if (t >= tokens) return;
+  const int slot = slots != nullptr ? pair_slot(slots, t, top_k, rows, lane) : (lane == 0 ? t : -1);
+  const int block0 = c * (H * Lanes::kBlocks) + lane / L;  // and every kBlocks further
+  const int first = block0 * (L * P) + lane % L;
+  Piece<B> v[H][P];
+  Piece<N> o[H][P];
+  float s_of[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int at = first + h * (Lanes::kBlocks * L * P) + i * L;
+      v[h][i] = Piece<B>{};
+      if (at < pieces) v[h][i] = ld_global(x + static_cast<size_t>(t) * pieces + at);
+    }
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    float f[P][N];
+    uint32_t bits = 0u;  // the largest magnitude without its sign: an infinity or a NaN is larger than all numbers
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      unpack<T, B>(v[h][i], f[i]);
+#pragma unroll
+      for (int n = 0; n < N; ++n) bits = max(bits, __float_as_uint(f[i][n]) & 0x7fffffffu);
+    }
+    bits = most_of<L>(bits);
+    const float a = __uint_as_float(bits);
+    const bool zeros = !(a >= 0x1p-110f && a < INFINITY);
+    const float unit = zeros ? INFINITY : a * 0x1p-9f;
+    s_of[h] = a < 0x1p-110f ? 0.f : a / 448.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      uint8_t* b = reinterpret_cast<uint8_t*>(&o[h][i]);
+#pragma unroll
+      for (int n = 0; n < N; n += 2) {
+        const float lo = zeros ? 0.f : f[i][n] * 0.875f / unit;
+        if constexpr (N > 1) {
+          const float hi = zeros ? 0.f : f[i][n + 1] * 0.875f / unit;
+          const __nv_fp8x2_storage_t both = __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+          b[n] = static_cast<uint8_t>(both & 0xff);
+          b[n + 1] = static_cast<uint8_t>(both >> 8);
+        } else {
+          b[n] = __nv_cvt_float_to_fp8(lo, __NV_SATFINITE, __NV_E4M3);
+        }
+      }
+    }
+  }
+  for (int j = 0; j < top_k; ++j) {
+    const int s = __shfl_sync(kFull, slot, j);
+    if (s < 0) continue;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int block = block0 + h * Lanes::kBlocks;
+      if (lane % L == 0 && block < blocks) scale[static_cast<size_t>(block) * rows + s] = s_of[h];
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int at = first + h * (Lanes::kBlocks * L * P) + i * L;
+        if (at < pieces) q[static_cast<size_t>(s) * pieces + at] = o[h][i];
+      }
+    }
+  }
+}
+
 // Widest piece, in bytes, that divides rows of `row_bytes` and fits the pointers.
 int piece_bytes(size_t row_bytes, uintptr_t pointers) {
   for (int b : {16, 8, 4})
@@ -728,6 +815,37 @@ extern "C" int sparsetir_moe_dispatch_i8_raw(const void* x, int type, const int3
       launch_chained(dispatch_i8_kernel<T, B>, tokens, kRowThreads, 0, st, static_cast<const Piece<B>*>(x), slots,
                      reinterpret_cast<Q*>(q), scale, rows, static_cast<int>(sizeof(T) * feat / B), top_k);
       SPTIR_LAUNCH_OK("dispatch_i8_kernel");
+      return 0;
+    });
+  });
+}
+
+extern "C" int sparsetir_moe_dispatch_f8_raw(const void* x, int type, const int32_t* slots, void* q, float* scale, int tokens,
+                                             int rows, int feat, int top_k, int device_id, void* stream) {
+  const char* fn = "sparsetir_moe_dispatch_f8";
+  if (check_rows(fn, type, tokens, rows, feat, top_k) != 0) return -1;
+  if (tokens == 0) return 0;
+  if (!slots && (top_k != 1 || rows != tokens)) return fail("%s: slots may be null with top_k 1 and a row per token only", fn);
+  if (rows == 0 || feat == 0) return 0;
+  if (!x || !q || !scale) return fail("%s: null pointer argument", fn);
+  if (use_device(device_id) != 0) return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (slots && check_slots(fn, slots, tokens, rows, top_k, st) != 0) return -1;
+  return with_type(type, [&](auto t) {
+    using T = decltype(t);
+    // a piece of N elements leaves as N bytes
+    int b = piece_bytes(sizeof(T) * feat, bits_of(x));
+    while (b > static_cast<int>(sizeof(T)) && bits_of(q) % (b / sizeof(T)) != 0) b /= 2;
+    return with_piece<sizeof(T)>(b, [&](auto bytes) {
+      constexpr int B = bytes.value;
+      using Lanes = F8Lanes<T, B>;
+      const int scales = ceil_div(feat, SPARSETIR_F8_BLOCK), chunks = ceil_div(scales, Lanes::kBlocks * Lanes::kHold);
+      const long long blocks = (static_cast<long long>(tokens) * chunks + kWarps - 1) / kWarps;
+      if (blocks > INT32_MAX) return fail("%s: too large for one launch", fn);
+      launch_chained(dispatch_f8_kernel<T, B>, static_cast<unsigned>(blocks), kWarps * 32, 0, st, static_cast<const Piece<B>*>(x),
+                     slots, static_cast<Piece<Lanes::N>*>(q), scale, tokens, rows, static_cast<int>(sizeof(T) * feat / B), scales,
+                     chunks, top_k);
+      SPTIR_LAUNCH_OK("dispatch_f8_kernel");
       return 0;
     });
   });

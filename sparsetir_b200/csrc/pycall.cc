@@ -30,6 +30,7 @@ bool dl_type(at::ScalarType t, bool more, DLDataType* out) {
   out->lanes = 1;
   switch (t) {
     case at::kBFloat16: out->code = kDLBfloat; out->bits = 16; return more;
+    case at::kFloat8_e4m3fn: out->code = kDLFloat8E4M3; out->bits = 8; return more;
     case at::kChar: out->code = kDLInt; out->bits = 8; return more;
     case at::kFloat: out->code = kDLFloat; out->bits = 32; return true;
     case at::kHalf: out->code = kDLFloat; out->bits = 16; return true;
@@ -70,7 +71,7 @@ int run(PackedFn fn, SetStreamFn set_stream, TVMValue* values, int* codes, int n
 // end the process.
 
 // invoke(fn, set_stream, args) -> return code, or None when an argument is of a kind that only the
-// general packing on the Python side takes (or refuses with its message).  invoke_more takes bfloat16 and int8 too.
+// general packing on the Python side takes (or refuses with its message).  invoke_more takes bfloat16, int8 and e4m3 too.
 template <bool MORE>
 PyObject* invoke(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   HANDLE_TH_ERRORS

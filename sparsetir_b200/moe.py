@@ -5,8 +5,9 @@
     expert_e(x) = (silu(x gate_e^T) * (x up_e^T)) down_e^T
 
 ``ExpertLayer`` holds the weights; ``forward`` returns the result and what ``backward`` needs, ``backward`` the gradients of the
-input and of all weights, each from the library's own operator.  ``QuantizedExpertLayer`` is the same layer for serving with
-weights and activations in 8-bit integers.  Everything runs on torch's current stream, nothing is read back to the host:
+input and of all weights, each from the library's own operator; with ``gated`` the projections, the activation and their product are
+one operator, and so is the gradient of it.  ``QuantizedExpertLayer`` is the same layer for serving with weights and activations in
+8-bit integers, ``Float8ExpertLayer`` in 8-bit floating point with a scale for each block of 128.  Everything runs on torch's current stream, nothing is read back to the host:
 how many tokens an expert has is known on the device alone, so that a step can be captured into a CUDA graph.
 """
 from __future__ import annotations
@@ -39,7 +40,7 @@ class Saved:
     routing: Routing
     rows: torch.Tensor    # the tokens' rows in the experts' order
     hidden: torch.Tensor  # [pairs, 2 * width]: gate and up projections
-    act: torch.Tensor     # silu(gate) * up
+    act: Optional[torch.Tensor]  # silu(gate) * up; a gated layer forms it again
     out: torch.Tensor     # the experts' results
 
 
@@ -54,6 +55,9 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = False) -> Routin
     return Routing(logits, gates, chosen, slots, indptr)
 
 
+ACTIVATIONS = {"silu": 0, "gelu": ops.GATED_GELU}  # gelu in its form with tanh
+
+
 class _Layer:
     def _logits(self, x: torch.Tensor, padding: Optional[torch.Tensor]) -> torch.Tensor:
         if x.dim() != 2 or x.shape[1] != self.features or not x.is_contiguous():
@@ -66,15 +70,20 @@ class _Layer:
 
 class ExpertLayer(_Layer):
     """``router [experts, features]``, ``gate_up [experts, 2 * width, features]`` (the gate projection's rows first), ``down
-    [experts, features, width]``; ``gate_up`` and ``down`` in float16 or bfloat16."""
+    [experts, features, width]``; ``gate_up`` and ``down`` in float16 or bfloat16.  ``gated``: "silu" or "gelu", the activation of a
+    layer that runs its gated block as one operator (``ops.grouped_mm_gated``), from the unrounded projections; None: silu in passes
+    of its own."""
 
-    def __init__(self, router: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, top_k: int, renormalize: bool = False):
+    def __init__(self, router: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, top_k: int, renormalize: bool = False,
+                 gated: Optional[str] = None):
         self.experts, self.features = router.shape
         self.width = down.shape[2]
         if tuple(gate_up.shape) != (self.experts, 2 * self.width, self.features) or tuple(down.shape) != (self.experts, self.features, self.width):
             raise ValueError("gate_up must be [experts, 2 * width, features] and down [experts, features, width]")
         self.router, self.gate_up, self.down = router, gate_up.contiguous(), down.contiguous()
-        self.top_k, self.renormalize = top_k, renormalize
+        if gated is not None and gated not in ACTIVATIONS:
+            raise ValueError(f"gated must be None or one of {sorted(ACTIVATIONS)}, got {gated!r}")
+        self.top_k, self.renormalize, self.gated = top_k, renormalize, gated
 
     def _product(self, x: torch.Tensor, w: torch.Tensor, indptr: torch.Tensor, transposed: bool) -> torch.Tensor:
         """x times every expert's ``w[e]^T`` (its layout is [out, in]), or times ``w[e]``: the gradient's product."""
@@ -88,28 +97,51 @@ class ExpertLayer(_Layer):
         ops.grouped_mm_grad_w(x.view(-1), dy.view(-1), dw.view(-1), indptr, self.experts, w.shape[2], w.shape[1], ops.GROUPED_W_OUT_IN)
         return dw
 
-    def forward(self, x: torch.Tensor, padding: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Saved]:
+    def _gated(self, rows: torch.Tensor, hidden: Optional[torch.Tensor], indptr: torch.Tensor) -> torch.Tensor:
+        act = torch.empty(rows.shape[0], self.width, dtype=rows.dtype, device=rows.device)
+        ops.grouped_mm_gated(rows.view(-1), self.gate_up.view(-1), act.view(-1), None if hidden is None else hidden.view(-1), indptr,
+                             self.experts, self.features, self.width, ACTIVATIONS[self.gated])
+        return act
+
+    def _gated_grad(self, d_out: torch.Tensor, s: Saved) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The gradient of ``hidden``, and the activations."""
+        d_hidden = torch.empty_like(s.hidden)
+        act = torch.empty(s.hidden.shape[0], self.width, dtype=s.hidden.dtype, device=s.hidden.device)
+        ops.grouped_mm_gated_grad(d_out.view(-1), self.down.view(-1), s.hidden.view(-1), d_hidden.view(-1), act.view(-1),
+                                  s.routing.indptr, self.experts, self.features, self.width, ACTIVATIONS[self.gated])
+        return d_hidden, act
+
+    def forward(self, x: torch.Tensor, padding: Optional[torch.Tensor] = None, train: bool = True) -> Tuple[torch.Tensor, Saved]:
+        """The result, and what ``backward`` needs; without ``train`` a gated layer does not keep that."""
         r = route(self._logits(x, padding), self.top_k, self.renormalize)
         rows = torch.empty(x.shape[0] * self.top_k, self.features, dtype=x.dtype, device=x.device)
         ops.moe_dispatch(x.view(-1), r.slots.view(-1), rows.view(-1), self.features, self.top_k)
-        hidden = self._product(rows, self.gate_up, r.indptr, False)
-        # rounded to 16 bits behind silu and behind the product: in 32 bits the two would take three more passes over [pairs, width]
-        act = F.silu(hidden[:, :self.width]) * hidden[:, self.width:]
+        if self.gated is not None:
+            hidden = torch.empty(rows.shape[0], 2 * self.width, dtype=x.dtype, device=x.device) if train else None
+            act = self._gated(rows, hidden, r.indptr)
+        else:
+            hidden = self._product(rows, self.gate_up, r.indptr, False)
+            # rounded to 16 bits behind silu and behind the product: in 32 bits the two would take three more passes over [pairs, width]
+            act = F.silu(hidden[:, :self.width]) * hidden[:, self.width:]
         out = self._product(act, self.down, r.indptr, False)
         y = torch.empty_like(x)
         ops.moe_combine(out.view(-1), r.slots.view(-1), r.gates.view(-1), y.view(-1), self.features, self.top_k)
-        return y, Saved(x, r, rows, hidden, act, out)
+        return y, Saved(x, r, rows, hidden, act if self.gated is None else None, out)
 
     def backward(self, dy: torch.Tensor, s: Saved) -> Dict[str, torch.Tensor]:
         r, k = s.routing, self.top_k
         d_out, d_gates = torch.empty_like(s.out), torch.empty_like(r.gates)
         ops.moe_combine_grad(dy.contiguous().view(-1), s.out.view(-1), r.slots.view(-1), r.gates.view(-1), d_out.view(-1),
                              d_gates.view(-1), self.features, k)
-        d_down = self._weight_grad(s.act, d_out, self.down, r.indptr)
-        d_act = self._product(d_out, self.down, r.indptr, True)
-        gate, up = s.hidden[:, :self.width].float(), s.hidden[:, self.width:].float()
-        sig = torch.sigmoid(gate)
-        d_hidden = torch.cat([d_act * up * sig * (1 + gate * (1 - sig)), d_act * gate * sig], 1).to(s.hidden.dtype)
+        if self.gated is not None:
+            d_hidden, act = self._gated_grad(d_out, s)
+            d_down = self._weight_grad(act, d_out, self.down, r.indptr)
+        else:
+            d_down = self._weight_grad(s.act, d_out, self.down, r.indptr)
+            d_act = self._product(d_out, self.down, r.indptr, True)
+            gate, up = s.hidden[:, :self.width].float(), s.hidden[:, self.width:].float()
+            sig = torch.sigmoid(gate)
+            d_hidden = torch.cat([d_act * up * sig * (1 + gate * (1 - sig)), d_act * gate * sig], 1).to(s.hidden.dtype)
         d_gate_up = self._weight_grad(s.rows, d_hidden, self.gate_up, r.indptr)
         d_rows = self._product(d_hidden, self.gate_up, r.indptr, True)
         dx = torch.empty(s.x.shape, device=s.x.device)
@@ -121,10 +153,13 @@ class ExpertLayer(_Layer):
         return {"x": dx.to(s.x.dtype), "router": d_logits.t() @ s.x.float(), "gate_up": d_gate_up, "down": d_down}
 
     def __call__(self, x: torch.Tensor, padding: Optional[torch.Tensor] = None) -> torch.Tensor:
-        return self.forward(x, padding)[0]
+        return self.forward(x, padding, train=False)[0]
 
-    def quantized(self) -> "QuantizedExpertLayer":
-        return QuantizedExpertLayer(self)
+    def quantized(self, kind: str = "int8") -> "_Layer":
+        """The layer for serving in 8 bits: "int8" (``QuantizedExpertLayer``) or "float8" (``Float8ExpertLayer``)."""
+        if kind not in ("int8", "float8"):
+            raise ValueError(f'kind must be "int8" or "float8", got {kind!r}')
+        return QuantizedExpertLayer(self) if kind == "int8" else Float8ExpertLayer(self)
 
 
 def quantize_channels(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -140,7 +175,7 @@ class QuantizedExpertLayer(_Layer):
 
     def __init__(self, layer: ExpertLayer):
         self.router, self.top_k, self.renormalize = layer.router, layer.top_k, layer.renormalize
-        self.experts, self.features, self.width = layer.experts, layer.features, layer.width
+        self.experts, self.features, self.width, self.gated = layer.experts, layer.features, layer.width, layer.gated
         self.gate_up, self.gate_up_scale = quantize_channels(layer.gate_up)
         self.down, self.down_scale = quantize_channels(layer.down)
 
@@ -157,8 +192,53 @@ class QuantizedExpertLayer(_Layer):
         r = route(self._logits(x, padding), self.top_k, self.renormalize)
         pairs = x.shape[0] * self.top_k
         hidden = self._product(x, r.slots.view(-1), pairs, self.gate_up, self.gate_up_scale, r.indptr)
-        act = F.silu(hidden[:, :self.width]) * hidden[:, self.width:]
+        gate = hidden[:, :self.width]
+        act = (F.gelu(gate, approximate="tanh") if self.gated == "gelu" else F.silu(gate)) * hidden[:, self.width:]
         out = self._product(act, None, pairs, self.down, self.down_scale, r.indptr)
+        y = torch.empty_like(x)
+        ops.moe_combine(out.view(-1), r.slots.view(-1), r.gates.view(-1), y.view(-1), self.features, self.top_k)
+        return y
+
+
+def quantize_blocks(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Weights [..., out, in] in 8-bit floating point with a scale for each 128 x 128 of them: [..., ceil(out / 128), ceil(in / 128)]."""
+    n = ops.F8_BLOCK
+    out, features = w.shape[-2:]
+    padded = F.pad(w.float(), (0, -features % n, 0, -out % n)).unflatten(-1, (-1, n)).unflatten(-3, (-1, n))  # [..., blocks, n, blocks, n]
+    scale = padded.abs().amax((-3, -1)) / 448
+    unit = torch.where(scale > 0, scale, torch.ones_like(scale))[..., :, None, :, None]
+    q = (padded / unit).clamp(-448, 448).flatten(-4, -3).flatten(-2, -1)[..., :out, :features]
+    return q.to(torch.float8_e4m3fn).contiguous(), scale
+
+
+class Float8ExpertLayer(_Layer):
+    """An ``ExpertLayer`` for serving: weights and activations in 8-bit floating point (e4m3) with a scale for each 128 x 128 of the
+    weights and each 128 features of a row; the gated block is one product."""
+
+    def __init__(self, layer: ExpertLayer):
+        self.router, self.top_k, self.renormalize = layer.router, layer.top_k, layer.renormalize
+        self.experts, self.features, self.width, self.gated = layer.experts, layer.features, layer.width, layer.gated or "silu"
+        self.gate_up, self.gate_up_scale = quantize_blocks(layer.gate_up)
+        self.down, self.down_scale = quantize_blocks(layer.down)
+
+    def _quantized(self, x: torch.Tensor, slots: Optional[torch.Tensor], rows: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        features = x.shape[1]
+        q = torch.empty(rows * features, dtype=torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty(-(-features // ops.F8_BLOCK) * rows, device=x.device)
+        ops.moe_dispatch_f8(x.view(-1), slots, q, scale, features, 1 if slots is None else self.top_k)
+        return q, scale
+
+    def __call__(self, x: torch.Tensor, padding: Optional[torch.Tensor] = None) -> torch.Tensor:
+        r = route(self._logits(x, padding), self.top_k, self.renormalize)
+        pairs = x.shape[0] * self.top_k
+        q, scale = self._quantized(x, r.slots.view(-1), pairs)
+        act = torch.empty(pairs, self.width, dtype=x.dtype, device=x.device)
+        ops.grouped_mm_gated_f8(q, scale, self.gate_up.view(-1), self.gate_up_scale.view(-1), act.view(-1), r.indptr, self.experts,
+                                self.features, self.width, ACTIVATIONS[self.gated])
+        q, scale = self._quantized(act, None, pairs)
+        out = torch.empty(pairs, self.features, dtype=x.dtype, device=x.device)
+        ops.grouped_mm_f8(q, scale, self.down.view(-1), self.down_scale.view(-1), out.view(-1), r.indptr, self.experts, self.width,
+                          self.features)
         y = torch.empty_like(x)
         ops.moe_combine(out.view(-1), r.slots.view(-1), r.gates.view(-1), y.view(-1), self.features, self.top_k)
         return y

@@ -36,11 +36,12 @@ _DTYPES = {
     torch.uint8: (L.kDLUInt, 8),
 }
 # what the mixture-of-experts operators take besides
-_MORE_DTYPES = {**_DTYPES, torch.bfloat16: (L.kDLBfloat, 16), torch.int8: (L.kDLInt, 8)}
+_MORE_DTYPES = {**_DTYPES, torch.bfloat16: (L.kDLBfloat, 16), torch.int8: (L.kDLInt, 8),
+                torch.float8_e4m3fn: (L.kDLFloat8E4M3, 8)}
 
 
 def to_dltensor(t: torch.Tensor, keepalive: List, more: bool = False) -> L.DLTensor:
-    """Borrowed DLTensor view of a torch tensor (no copy); with ``more``, of bfloat16 and int8 too."""
+    """Borrowed DLTensor view of a torch tensor (no copy); with ``more``, of bfloat16, int8 and float8_e4m3fn too."""
     dtypes = _MORE_DTYPES if more else _DTYPES
     if t.dtype not in dtypes:
         raise TypeError(f"unsupported dtype {t.dtype}")
@@ -92,7 +93,7 @@ class PreparedCall:
 
 class PackedFunc:
     """A TVMBackendPackedCFunc symbol of the library, callable like the reference's functions.  ``more``: it takes
-    bfloat16 and int8 tensors besides the types of the reference's operators."""
+    bfloat16, int8 and float8_e4m3fn tensors besides the types of the reference's operators."""
 
     def __init__(self, symbol: str, more: bool = False):
         self.symbol = symbol
@@ -203,8 +204,13 @@ moe_combine_grad = PackedFunc("sparsetir_moe_combine_grad", more=True)
 grouped_mm = PackedFunc("sparsetir_grouped_mm", more=True)
 grouped_mm_grad_w = PackedFunc("sparsetir_grouped_mm_grad_w", more=True)
 grouped_mm_i8 = PackedFunc("sparsetir_grouped_mm_i8", more=True)
+grouped_mm_gated = PackedFunc("sparsetir_grouped_mm_gated", more=True)
+grouped_mm_gated_grad = PackedFunc("sparsetir_grouped_mm_gated_grad", more=True)
+moe_dispatch_f8 = PackedFunc("sparsetir_moe_dispatch_f8", more=True)
+grouped_mm_f8 = PackedFunc("sparsetir_grouped_mm_f8", more=True)
+grouped_mm_gated_f8 = PackedFunc("sparsetir_grouped_mm_gated_f8", more=True)
 
-MOE_RENORMALIZE, GROUPED_W_OUT_IN = L.MOE_RENORMALIZE, L.GROUPED_W_OUT_IN
+MOE_RENORMALIZE, GROUPED_W_OUT_IN, GATED_GELU, F8_BLOCK = L.MOE_RENORMALIZE, L.GROUPED_W_OUT_IN, L.GATED_GELU, L.F8_BLOCK
 
 
 def hyb_args(x: torch.Tensor, y: torch.Tensor, buckets: Sequence[Sequence[torch.Tensor]],
