@@ -42,6 +42,8 @@ int rgms_f16_timeouts(unsigned int* count);  // ... and of rgms_f16.cu
 int rgms_fused_timeouts(unsigned int* count);  // ... and of rgms_fused.cu
 int conv_timeouts(unsigned int* count);        // ... and of sparse_conv.cu
 int grouped_timeouts(unsigned int* count);     // ... and of grouped.cu
+int gated_timeouts(unsigned int* count);       // ... and of grouped_gated.cu
+int f8_timeouts(unsigned int* count);          // ... and of grouped_f8.cu
 
 namespace {
 
@@ -606,6 +608,8 @@ extern "C" int sparsetir_tc_timeouts(int device_id, unsigned int* count) {
   if (conv_timeouts(&cv) != 0) return -1;
   unsigned int gr = 0;
   if (grouped_timeouts(&gr) != 0) return -1;
-  *count = bsr + rgms + rh + rf + cv + gr;
+  unsigned int gd = 0, f8 = 0;
+  if (gated_timeouts(&gd) != 0 || f8_timeouts(&f8) != 0) return -1;
+  *count = bsr + rgms + rh + rf + cv + gr + gd + f8;
   return 0;
 }

@@ -1,0 +1,105 @@
+// The gated block of an expert in one product, and its gradient through the product that follows it, on the tensor cores
+// (grouped_tile.cuh; the epilogues are in grouped_gated.cuh):
+//   grouped_mm_gated       h = x W[g]^T of 2 * width features, act = f(h[:, :width]) * h[:, width:]  (gate.cuh)
+//   grouped_mm_gated_grad  d = dy W[g], and from d and h the gradient to h
+#include "grouped_tile.cuh"
+
+namespace sptir {
+namespace {
+
+template <int OUT>
+int launch_half(int columns, int type, const CUtensorMap& w, const CUtensorMap& x64, const CUtensorMap& x16, const Args& p, cudaStream_t st) {
+  return with_half(type, [&](auto t) {
+    using T = decltype(t);
+    if (columns == 128) return launch<kHalf, OUT, T, 128>(w, x64, x16, p, st);
+    return launch<kHalf, OUT, T, 256>(w, x64, x16, p, st);
+  });
+}
+
+}  // namespace
+
+int gated_timeouts(unsigned int* count) {
+  SPTIR_CUDA_OK(cudaMemcpyFromSymbol(count, g_grouped_timeouts, sizeof(unsigned int)));
+  return 0;
+}
+
+}  // namespace sptir
+
+using namespace sptir;
+
+extern "C" int sparsetir_grouped_mm_gated_raw(const void* x, const void* w, void* y, void* hidden, int type, const int32_t* indptr,
+                                              int rows, int num_groups, int feat_in, int width, int flags, int device_id,
+                                              void* stream) {
+  const char* fn = "sparsetir_grouped_mm_gated";
+  if (check_block(fn, indptr, rows, num_groups, feat_in, width, true, flags, SPARSETIR_GATED_GELU) != 0) return -1;
+  if (type != SPARSETIR_F16 && type != SPARSETIR_BF16) return fail("%s: x, w, y and hidden are f16 or bf16", fn);
+  if (rows == 0 || num_groups == 0) return 0;
+  if (!x || !w || !y) return fail("%s: null pointer argument", fn);
+  if (use_device(device_id) != 0) return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (check_pointers(fn, indptr, rows, num_groups, st) != 0) return -1;
+  Args p{};
+  p.out = y;
+  p.hidden = hidden;
+  p.gate = Gate((flags & SPARSETIR_GATED_GELU) != 0);
+  p.indptr = indptr;
+  p.rows = rows;
+  p.groups = num_groups;
+  p.k = feat_in;
+  p.features = width;
+  p.wide = wide_rows(y, type, width) && aligned16(hidden);
+  p.idesc = tc05::instr_desc(map_format(type), 2 * kM, 0, 0, 0);
+  const int columns = plan_product(fn, &p, 2 * width, 64);
+  if (columns < 0) return -1;
+  Operand ox{x, rows, feat_in, 2}, ow{w, static_cast<long long>(num_groups) * 2 * width, feat_in, 2};
+  const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + part_bytes(p);
+  CallScratch cs;
+  if (bytes > 0 && take_scratch(device_id, st, bytes, 0, &cs) != 0) return -1;
+  char* scratch = cs.scratch;
+  if (place_operand(&ox, &scratch, st) != 0 || place_operand(&ow, &scratch, st) != 0) return -1;
+  p.parts = scratch;
+  CUtensorMap tm_w, tm_x64, tm_x16;
+  if (map_operands(&tm_w, &tm_x64, &tm_x16, map_type(type), ow, ox, width, num_groups, true, true) != 0) return -1;
+  const int rc = launch_half<kGated>(columns, type, tm_w, tm_x64, tm_x16, p, st);
+  return rc != 0 ? rc : return_scratch(cs, st);
+}
+
+extern "C" int sparsetir_grouped_mm_gated_grad_raw(const void* dy, const void* w, const void* hidden, void* d_hidden, void* act,
+                                                   int type, const int32_t* indptr, int rows, int num_groups, int feat, int width,
+                                                   int flags, int device_id, void* stream) {
+  const char* fn = "sparsetir_grouped_mm_gated_grad";
+  if (check_block(fn, indptr, rows, num_groups, feat, width, true, flags, SPARSETIR_GATED_GELU | SPARSETIR_GROUPED_W_OUT_IN) != 0) return -1;
+  if (type != SPARSETIR_F16 && type != SPARSETIR_BF16) return fail("%s: all tensors are f16 or bf16", fn);
+  if (rows == 0 || num_groups == 0) return 0;
+  if (!dy || !w || !hidden || !d_hidden) return fail("%s: null pointer argument", fn);
+  if (use_device(device_id) != 0) return -1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (check_pointers(fn, indptr, rows, num_groups, st) != 0) return -1;
+  const bool out_in = (flags & SPARSETIR_GROUPED_W_OUT_IN) != 0;
+  Args p{};
+  p.out = act;
+  p.hidden_in = hidden;
+  p.hidden = d_hidden;
+  p.gate = Gate((flags & SPARSETIR_GATED_GELU) != 0);
+  p.indptr = indptr;
+  p.rows = rows;
+  p.groups = num_groups;
+  p.k = feat;
+  p.features = width;
+  p.a_mn = out_in ? 0 : 1;
+  p.wide = wide_rows(d_hidden, type, width) && aligned16(hidden) && aligned16(act);
+  p.idesc = tc05::instr_desc(map_format(type), 2 * kM, 0, p.a_mn, 0);
+  const int columns = plan_product(fn, &p, width, 64);
+  if (columns < 0) return -1;
+  Operand ox{dy, rows, feat, 2}, ow{w, static_cast<long long>(num_groups) * (out_in ? width : feat), out_in ? feat : width, 2};
+  const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + part_bytes(p);
+  CallScratch cs;
+  if (bytes > 0 && take_scratch(device_id, st, bytes, 0, &cs) != 0) return -1;
+  char* scratch = cs.scratch;
+  if (place_operand(&ox, &scratch, st) != 0 || place_operand(&ow, &scratch, st) != 0) return -1;
+  p.parts = scratch;
+  CUtensorMap tm_w, tm_x64, tm_x16;
+  if (map_operands(&tm_w, &tm_x64, &tm_x16, map_type(type), ow, ox, out_in ? width : feat, num_groups, out_in, false) != 0) return -1;
+  const int rc = launch_half<kGatedGrad>(columns, type, tm_w, tm_x64, tm_x16, p, st);
+  return rc != 0 ? rc : return_scratch(cs, st);
+}

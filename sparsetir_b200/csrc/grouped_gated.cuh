@@ -1,0 +1,431 @@
+// Epilogues of grouped_kernel (grouped_tile.cuh, which includes this): a gated block, the gradient of one, and sums with a scale for each
+// 128 of K.  All take the sums as fragments (tmem_ld16x32): 16 lanes of TMEM, 32 columns, v[4 i + 2 h + c] = lane 8 h + l / 4 of the 16, column
+// 8 i + 2 (l % 4) + c, for lane l of the warp.
+//   Gated: of the 32 rows of W that a warp's lanes of TMEM stand for, the first 16 are the gate's and the last 16 the other projection's of
+//   the same features: the two fragments that a thread loads belong together, and nothing is exchanged.
+#ifndef SPARSETIR_B200_GROUPED_GATED_CUH_
+#define SPARSETIR_B200_GROUPED_GATED_CUH_
+
+namespace sptir {
+namespace {
+
+// Registers of a thread in the kernel with scaled sums: a thread of the epilogue holds 128 sums, the others need few.  What a block
+// was launched with is shared out again: (kN = 256) 128 * 56 + 256 * 224 = 384 * 168, (128) 128 * 56 + 128 * 200 = 256 * 128.
+template <int N> struct F8Registers {
+  static constexpr int kOthers = 56;
+  static constexpr int kEpilogue = N == 256 ? 224 : 200;
+};
+
+// (x, y) += (a, b) * (s, t)
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float s, float t) {
+  asm("{\n\t.reg .b64 p, q, r;\n\t"
+      "mov.b64 p, {%2, %3};\n\t"
+      "mov.b64 q, {%4, %5};\n\t"
+      "mov.b64 r, {%0, %1};\n\t"
+      "fma.rn.f32x2 r, p, q, r;\n\t"
+      "mov.b64 {%0, %1}, r;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b), "f"(s), "f"(t));
+}
+
+// An epilogue warp's share of a tile: features feat0 and so on, columns first, first + step and so on, 32 at a time.
+template <class OutT>
+struct Warp {
+  const Args& p;
+  const Tile& t;
+  const int feat0, first, step;
+  unsigned char* const staged;
+  const int lane;
+  const int feats;  // live ones from feat0 on, may be <= 0
+
+  __device__ __forceinline__ Warp(const Args& args, const Tile& tile, int feat, int column, int stride, unsigned char* mem, int l)
+      : p(args), t(tile), feat0(feat), first(column), step(stride), staged(mem), lane(l), feats(args.features - feat) {}
+
+  // Row of column c of the tile
+  __device__ __forceinline__ size_t row(int c) const { return static_cast<size_t>(t.col0) + c; }
+
+  // ---- one element to a store, whatever the alignment; eight lanes have neighbouring features
+  template <class O>
+  __device__ __forceinline__ void direct(O* to, size_t pitch, int live, const float* v, int c0) const {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int f = 8 * ((i >> 1) & 1) + lane / 4, c = 8 * (i >> 2) + 2 * (lane & 3) + (i & 1);
+      if (f < live && c0 + c < t.n) to[c * pitch + f] = from_float<O>(v[i]);
+    }
+  }
+  // Sums of a unit that shares the depth: both fragments' rows of the left operand
+  template <int OUT>
+  __device__ __forceinline__ void to_parts(const float* a, const float* b, int c0) const {
+    const size_t pitch = OUT == kGated ? 2 * static_cast<size_t>(p.features) : p.features;
+    float* to = static_cast<float*>(p.parts) + t.split * p.part + row(c0) * pitch + feat0;
+    direct(to, pitch, feats, a, c0);
+    if constexpr (OUT == kGated) direct(to + p.features, pitch, feats, b, c0);
+    else direct(to + 16, pitch, feats - 16, b, c0);
+  }
+  template <int OUT>
+  __device__ __forceinline__ void zeros(int chunks) const {
+    const float none[16] = {};
+    for (int j = 0; j < chunks; ++j)
+      if (first + j * step < t.n) to_parts<OUT>(none, none, first + j * step);
+  }
+
+  // ---- 16-bit elements at 16-byte addresses, through shared memory: 32 rows (columns of the tile) of 64 bytes, pieces of 16 bytes exchanged
+  // so that neither side collides.  v[q]: features 8 q + l / 4, columns 8 i + 2 (l % 4) and the next
+  __device__ __forceinline__ static uint32_t place64(int r, int q) { return static_cast<uint32_t>(r * 64 + ((q ^ ((r >> 1) & 3)) << 4)); }
+  __device__ __forceinline__ void put64(int at, int i, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) const {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                     tc05::smem_u32(staged) + at + place64(8 * i + (lane & 7), lane >> 3)),
+                 "r"(v0), "r"(v1), "r"(v2), "r"(v3)
+                 : "memory");
+  }
+  __device__ __forceinline__ void get64(int at, int i, uint32_t (&v)[4]) const {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(tc05::smem_u32(staged) + at + place64(8 * i + (lane & 7), lane >> 3))
+                 : "memory");
+  }
+  // A lane has the piece lane % 4 of the rows lane / 4, 8 further and so on: to `to`, where its piece of row lane / 4 goes
+  __device__ __forceinline__ void leave64(int at, OutT* to, size_t pitch, bool live, int c0) const {
+    const unsigned char* from = staged + at + place64(lane >> 2, lane & 3);  // rows 8 apart alike
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(from + 8 * i * 64);
+      if (live && c0 + 8 * i + (lane >> 2) < t.n) *reinterpret_cast<uint4*>(to + 8 * i * pitch) = v;
+    }
+  }
+  // The same for 16 features: rows of 32 bytes
+  __device__ __forceinline__ static uint32_t place32(int r, int q) { return static_cast<uint32_t>(r * 32 + ((q ^ ((r >> 2) & 1)) << 4)); }
+  __device__ __forceinline__ void put32(int at, int i, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) const {  // of columns 8 i.., 8 i + 8..
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                     tc05::smem_u32(staged) + at + place32(8 * (i + (lane >> 4)) + (lane & 7), (lane >> 3) & 1)),
+                 "r"(v0), "r"(v1), "r"(v2), "r"(v3)
+                 : "memory");
+  }
+  __device__ __forceinline__ void leave32(int at, OutT* to, size_t pitch, bool live, int c0) const {
+    const unsigned char* from = staged + at + place32(lane >> 1, lane & 1);  // rows 16 apart alike
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(from + 16 * i * 32);
+      if (live && c0 + 16 * i + (lane >> 1) < t.n) *reinterpret_cast<uint4*>(to + 16 * i * pitch) = v;
+    }
+  }
+
+  // ---- what becomes of 32 columns' sums; next(): they are not needed any more
+  template <class Next>
+  __device__ __forceinline__ void plain(const float* a, const float* b, int c0, Next&& next) const {
+    OutT* to = static_cast<OutT*>(p.out) + row(c0) * p.features + feat0;
+    if constexpr (sizeof(OutT) == 2) {
+      if (p.wide) {
+        __syncwarp();  // the reads of the last 32 columns are over
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          put64(0, i, pack2<OutT>(a[4 * i], a[4 * i + 1]), pack2<OutT>(a[4 * i + 2], a[4 * i + 3]), pack2<OutT>(b[4 * i], b[4 * i + 1]),
+                pack2<OutT>(b[4 * i + 2], b[4 * i + 3]));
+        next();
+        __syncwarp();
+        leave64(0, to + static_cast<size_t>(lane >> 2) * p.features + 8 * (lane & 3), p.features, 8 * (lane & 3) < feats, c0);
+        return;
+      }
+    }
+    direct(to, p.features, feats, a, c0);
+    direct(to + 16, p.features, feats - 16, b, c0);
+    next();
+  }
+  template <class Next>
+  __device__ __forceinline__ void gated(const float* g, const float* u, int c0, Next&& next) const {
+    const size_t width = p.features;
+    OutT* const to = static_cast<OutT*>(p.out) + row(c0) * width + feat0;
+    OutT* const kept = static_cast<OutT*>(p.hidden) + row(c0) * 2 * width + feat0;
+    if (p.wide) {
+      uint32_t act[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) act[i] = pack2<OutT>(p.gate.act(g[2 * i], u[2 * i]), p.gate.act(g[2 * i + 1], u[2 * i + 1]));
+      __syncwarp();  // the reads of the last 32 columns are over
+      put32(kStagedBytes, 0, act[0], act[1], act[2], act[3]);
+      put32(kStagedBytes, 2, act[4], act[5], act[6], act[7]);
+      if (p.hidden != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          put64(0, i, pack2<OutT>(g[4 * i], g[4 * i + 1]), pack2<OutT>(g[4 * i + 2], g[4 * i + 3]), pack2<OutT>(u[4 * i], u[4 * i + 1]),
+                pack2<OutT>(u[4 * i + 2], u[4 * i + 3]));
+      }
+      next();
+      __syncwarp();
+      leave32(kStagedBytes, to + static_cast<size_t>(lane >> 1) * width + 8 * (lane & 1), width, 8 * (lane & 1) < feats, c0);
+      if (p.hidden != nullptr)  // pieces 0 and 1 are the gate's
+        leave64(0, kept + static_cast<size_t>(lane >> 2) * 2 * width + ((lane & 2) != 0 ? width : 0) + 8 * (lane & 1), 2 * width,
+                8 * (lane & 1) < feats, c0);
+      return;
+    }
+    float act[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) act[i] = p.gate.act(g[i], u[i]);
+    direct(to, width, feats, act, c0);
+    if (p.hidden != nullptr) {
+      direct(kept, 2 * width, feats, g, c0);
+      direct(kept + width, 2 * width, feats, u, c0);
+    }
+    next();
+  }
+
+  // The projections of 32 features and columns, for the gradient: asked for ahead, put where put64 puts them.
+  struct Ahead { uint4 g[4], u[4]; };
+  __device__ __forceinline__ void ask(int c0, Ahead& h) const {
+    const size_t width = p.features;
+    const OutT* from = static_cast<const OutT*>(p.hidden_in) + row(c0 + (lane >> 2)) * 2 * width + feat0 + 8 * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (8 * (lane & 3) < feats && c0 + 8 * i + (lane >> 2) < t.n) {
+        h.g[i] = ld_global(reinterpret_cast<const uint4*>(from + 8 * i * 2 * width));
+        h.u[i] = ld_global(reinterpret_cast<const uint4*>(from + 8 * i * 2 * width + width));
+      } else {
+        h.g[i] = h.u[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  }
+  __device__ __forceinline__ static float half_of(uint32_t v, int c) {
+    const uint32_t one = c == 0 ? v & 0xffffu : v >> 16;
+    const uint16_t bits = static_cast<uint16_t>(one);
+    return to_float(reinterpret_cast<const OutT&>(bits));
+  }
+  template <class Next>
+  __device__ __forceinline__ void gated_grad(const float* da, const float* db, int c0, Ahead& ahead, Next&& next) const {
+    const size_t width = p.features;
+    OutT* const dg = static_cast<OutT*>(p.hidden) + row(c0) * 2 * width + feat0;
+    if (p.wide) {
+      __syncwarp();  // the reads of the last 32 columns are over
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = static_cast<int>(place64(8 * i + (lane >> 2), lane & 3));
+        *reinterpret_cast<uint4*>(staged + at) = ahead.g[i];
+        *reinterpret_cast<uint4*>(staged + kStagedBytes + at) = ahead.u[i];
+      }
+      if (c0 + step < t.n) ask(c0 + step, ahead);
+      __syncwarp();
+      uint32_t act[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t g[4], u[4], og[4], ou[4];
+        get64(0, i, g);
+        get64(kStagedBytes, i, u);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float* d = (q < 2 ? da : db) + 4 * i + 2 * (q & 1);
+          float xg[2], xu[2], xa[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) p.gate.grad(half_of(g[q], c), half_of(u[q], c), d[c], &xg[c], &xu[c], &xa[c]);
+          og[q] = pack2<OutT>(xg[0], xg[1]);
+          ou[q] = pack2<OutT>(xu[0], xu[1]);
+          act[4 * i + q] = pack2<OutT>(xa[0], xa[1]);
+        }
+        __syncwarp();
+        put64(0, i, og[0], og[1], og[2], og[3]);  // in the place of what was read
+        put64(kStagedBytes, i, ou[0], ou[1], ou[2], ou[3]);
+      }
+      next();
+      __syncwarp();
+      OutT* const to = dg + static_cast<size_t>(lane >> 2) * 2 * width + 8 * (lane & 3);
+      const bool live = 8 * (lane & 3) < feats;
+      leave64(0, to, 2 * width, live, c0);
+      leave64(kStagedBytes, to + width, 2 * width, live, c0);
+      if (p.out != nullptr) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put64(0, i, act[4 * i], act[4 * i + 1], act[4 * i + 2], act[4 * i + 3]);
+        __syncwarp();
+        leave64(0, static_cast<OutT*>(p.out) + row(c0 + (lane >> 2)) * width + feat0 + 8 * (lane & 3), width, live, c0);
+      }
+      return;
+    }
+    const OutT* const h = static_cast<const OutT*>(p.hidden_in) + row(c0) * 2 * width + feat0;
+    OutT* const act = static_cast<OutT*>(p.out) + row(c0) * width + feat0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int f = 16 * (i >> 4) + 8 * ((i >> 1) & 1) + lane / 4, c = 8 * ((i >> 2) & 3) + 2 * (lane & 3) + (i & 1);
+      if (f >= feats || c0 + c >= t.n) continue;
+      const size_t at = c * 2 * width + f;
+      float xg, xu, xa;
+      p.gate.grad(to_float(ld_global(h + at)), to_float(ld_global(h + at + width)), i < 16 ? da[i & 15] : db[i & 15], &xg, &xu, &xa);
+      dg[at] = from_float<OutT>(xg);
+      dg[at + width] = from_float<OutT>(xu);
+      if (p.out != nullptr) act[c * width + f] = from_float<OutT>(xa);
+    }
+    next();
+  }
+
+  // ---- a tile whose sums are complete in TMEM; false: the wait ran out
+  template <int OUT>
+  __device__ __forceinline__ bool out_of_tmem(uint32_t taddr, uint64_t* full, uint32_t taken, uint32_t parity) const {
+    Ahead ahead;
+    const bool reads = OUT == kGatedGrad && p.wide != 0 && p.splits == 1;
+    if (reads && first < t.n) ask(first, ahead);
+    if (!__all_sync(0xffffffffu, tc05::mbar_wait(full, parity))) return false;
+    tc05::fence_after_sync();
+    auto take = [&]() {  // the warp's last columns are in registers: the accumulator may be written again
+      tc05::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc05::pair::arrive(taken);
+    };
+    if (first >= t.n) {
+      take();
+      return true;
+    }
+    uint32_t a[16], b[16];
+    tc05::tmem_ld16x32(taddr + first, a);
+    tc05::tmem_ld16x32(taddr + (16u << 16) + first, b);
+    for (int c0 = first; c0 < t.n; c0 += step) {
+      tc05::tmem_ld_wait();
+      if (c0 + step >= t.n) take();
+      float va[16], vb[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        va[i] = __uint_as_float(a[i]);
+        vb[i] = __uint_as_float(b[i]);
+      }
+      auto next = [&]() {  // the next columns while these leave
+        if (c0 + step >= t.n) return;
+        tc05::tmem_ld16x32(taddr + c0 + step, a);
+        tc05::tmem_ld16x32(taddr + (16u << 16) + c0 + step, b);
+      };
+      if (p.splits > 1) {
+        to_parts<OUT>(va, vb, c0);
+        next();
+      } else if constexpr (OUT == kGated) {
+        gated(va, vb, c0, next);
+      } else {
+        gated_grad(va, vb, c0, ahead, next);
+      }
+    }
+    return true;
+  }
+
+  // ---- a tile of 8-bit floating point: the sums of every 128 of K come by themselves, from accumulators that change by turns, and are
+  // scaled and added in registers: 128 columns of the warp's 32 lanes.  The columns' scales go through shared memory; plain: times the scale
+  // of W, one for all 128 features of a block; gated: the rows of the other projection may lie in two blocks of W.
+  template <int OUT>
+  __device__ __forceinline__ bool scaled(uint32_t taddr, int buffer, uint64_t* full, uint64_t* empty, int acc) const {
+    constexpr bool kTwo = OUT == kGated;
+    float sum[4][32];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sum[j][i] = 0.f;
+    const int live = t.n - first;  // columns, may be <= 0
+    const int blocks = (p.k + SPARSETIR_F8_BLOCK - 1) / SPARSETIR_F8_BLOCK;
+    const int of_w = ((kTwo ? 2 : 1) * p.features + SPARSETIR_F8_BLOCK - 1) / SPARSETIR_F8_BLOCK;
+    const float* const ws = p.w_scale + static_cast<size_t>(t.group) * of_w * blocks + t.step0;
+    const float* xs = p.x_scale + static_cast<size_t>(t.step0) * p.rows + row(first + lane);
+    auto scale_of = [&](int f) { return ws + static_cast<size_t>(f / SPARSETIR_F8_BLOCK) * blocks; };
+    const int f = min(feat0, p.features - 1), fu = feat0 + lane / 4;
+    const float* const w0 = scale_of(f);
+    const float* const w1 = scale_of(p.features + min(fu, p.features - 1));      // gated
+    const float* const w2 = scale_of(p.features + min(fu + 8, p.features - 1));
+    float x[4], w[3];
+    auto fetch = [&](int k) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = lane + 32 * j < live ? ld_global(xs + 32 * j) : 0.f;
+      xs += p.rows;
+      w[0] = ld_global(w0 + k);
+      if constexpr (kTwo) {
+        w[1] = ld_global(w1 + k);
+        w[2] = ld_global(w2 + k);
+      }
+    };
+    fetch(0);
+    float* const shared = reinterpret_cast<float*>(staged);
+    __syncwarp();  // the last tile has left it
+    for (int k = 0; k < t.steps; ++k, ++acc) {
+      float* const s = shared + (k & 1) * 128;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[32 * j + lane] = kTwo ? x[j] : x[j] * w[0];
+      const float wg = w[0], wu0 = w[1], wu1 = w[2];
+      __syncwarp();
+      if (k + 1 < t.steps) fetch(k + 1);
+      const int buf = acc & 1;
+      if (!__all_sync(0xffffffffu, tc05::mbar_wait(full + buf, (acc >> 1) & 1))) return false;
+      tc05::fence_after_sync();
+      const uint32_t taken = tc05::pair::at_first(empty + buf);
+      auto take = [&]() {
+        tc05::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc05::pair::arrive(taken);
+      };
+      if (live <= 0) take();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (32 * j >= live) break;
+        uint32_t a[16], b[16];
+        tc05::tmem_ld16x32(taddr + buf * buffer + first + 32 * j, a);
+        tc05::tmem_ld16x32(taddr + (16u << 16) + buf * buffer + first + 32 * j, b);
+        tc05::tmem_ld_wait();
+        if (j == 3 || 32 * (j + 1) >= live) take();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 sc = *reinterpret_cast<const float2*>(s + 32 * j + 8 * i + 2 * (lane & 3));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int at = 4 * i + 2 * h;
+            const float ws_g = kTwo ? wg : 1.f, ws_u = kTwo ? (h == 0 ? wu0 : wu1) : 1.f;
+            fma2(sum[j][at], sum[j][at + 1], __uint_as_float(a[at]), __uint_as_float(a[at + 1]), kTwo ? sc.x * ws_g : sc.x,
+                 kTwo ? sc.y * ws_g : sc.y);
+            fma2(sum[j][16 + at], sum[j][17 + at], __uint_as_float(b[at]), __uint_as_float(b[at + 1]), kTwo ? sc.x * ws_u : sc.x,
+                 kTwo ? sc.y * ws_u : sc.y);
+          }
+        }
+      }
+    }
+    __syncwarp();  // the scales are read
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c0 = first + 32 * j;
+      if (c0 >= t.n) break;
+      if (p.splits > 1) {
+        to_parts<OUT>(sum[j], sum[j] + 16, c0);
+      } else if constexpr (kTwo) {
+        gated(sum[j], sum[j] + 16, c0, [] {});
+      } else {
+        plain(sum[j], sum[j] + 16, c0, [] {});
+      }
+    }
+    return true;
+  }
+};
+
+// The sums of the units that share a tile, added in their order, and what becomes of them: thread = a feature of a row
+template <int OUT, class T>
+__global__ void __launch_bounds__(256) join_gated_kernel(const __grid_constant__ Args p) {
+  chain_wait();
+  const long long row = blockIdx.y + static_cast<long long>(blockIdx.z) * gridDim.y;
+  const int feat = blockIdx.x * 256 + threadIdx.x;
+  if (row >= p.rows || feat >= p.features) return;
+  if (p.indptr != nullptr && (row < ld_global(p.indptr) || row >= ld_global(p.indptr + p.groups))) return;  // of no group
+  const size_t width = p.features;
+  const float* from = static_cast<const float*>(p.parts) + static_cast<size_t>(row) * (OUT == kGated ? 2 : 1) * width + feat;
+  float a = 0.f, b = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < p.splits; ++s) {
+    a += ld_global(from + s * p.part);
+    if constexpr (OUT == kGated) b += ld_global(from + s * p.part + width);
+  }
+  const size_t at = static_cast<size_t>(row) * width + feat, two = static_cast<size_t>(row) * 2 * width + feat;
+  T* const hidden = static_cast<T*>(p.hidden);
+  T* const out = static_cast<T*>(p.out);
+  if constexpr (OUT == kGated) {
+    out[at] = from_float<T>(p.gate.act(a, b));
+    if (hidden != nullptr) {
+      hidden[two] = from_float<T>(a);
+      hidden[two + width] = from_float<T>(b);
+    }
+  } else {
+    const T* const h = static_cast<const T*>(p.hidden_in);
+    float xg, xu, xa;
+    p.gate.grad(to_float(ld_global(h + two)), to_float(ld_global(h + two + width)), a, &xg, &xu, &xa);
+    hidden[two] = from_float<T>(xg);
+    hidden[two + width] = from_float<T>(xu);
+    if (out != nullptr) out[at] = from_float<T>(xa);
+  }
+}
+
+}  // namespace
+}  // namespace sptir
+#endif  // SPARSETIR_B200_GROUPED_GATED_CUH_

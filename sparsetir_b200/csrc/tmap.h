@@ -32,7 +32,7 @@ inline int make_tmap(CUtensorMap* map, CUtensorMapDataType dtype, const void* ba
     return reinterpret_cast<EncodeFn>(fn);
   }();
   if (!encode) return fail("cuTensorMapEncodeTiled is not available from this driver");
-  const cuuint32_t estr[3] = {1, 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult rc = encode(map, dtype, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, estr,
                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, fetch, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (rc != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed with code %d", static_cast<int>(rc));
