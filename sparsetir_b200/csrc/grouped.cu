@@ -85,7 +85,7 @@ int product(const char* fn, const void* x, const void* w, int type, void* y, int
   char* scratch = cs.scratch;
   if (place_operand(&ox, &scratch, st) != 0 || place_operand(&ow, &scratch, st) != 0) return -1;
   if (few) {
-    FewArgs f{ox.data, ow.data, y, xs, ws, indptr, ox.pitch, ow.pitch, rows, groups, fi, fo, fi * size, 0, 0, 0};
+    FewArgs f{ox.data, ow.data, y, xs, ws, indptr, ox.pitch, ow.pitch, rows, groups, fi, fo, fi * size, 0, 0, 0, nullptr, Gate()};
     const int done = few_rows(f, type, y_type, out_in, st);
     return done != 0 ? done : return_scratch(cs, st);
   }

@@ -3,6 +3,7 @@
 #define SPARSETIR_B200_GROUPED_H_
 
 #include "common.h"
+#include "gate.cuh"
 #include "launch.cuh"
 
 namespace sptir {
@@ -32,11 +33,16 @@ struct FewArgs {
   int rows, groups, fi, fo;
   int k_bytes;              // of a row of x
   int splits, split_bytes, feature_warps;  // set by the launcher
+  void* hidden;  // gated: the projections, or null; fo is the width
+  Gate gate;
 };
 
 // y = x * W by the kernel for groups of a few rows; `type` as SPARSETIR_F16 / BF16, -1 for 8-bit integers; along_k: W is
 // contiguous along the depth.
 int few_rows(const FewArgs& p, int type, int y_type, bool along_k, cudaStream_t st);
+// The gated block (W along the depth) of 16-bit elements, and the product or the gated block of 8-bit floating point.
+int few_rows_gated(const FewArgs& p, int type, cudaStream_t st);
+int few_rows_f8(const FewArgs& p, int y_type, bool gated, cudaStream_t st);
 
 }  // namespace sptir
 #endif  // SPARSETIR_B200_GROUPED_H_

@@ -26,11 +26,17 @@ int product_f8(const char* fn, const void* x, const float* x_scale, const void* 
   const int columns = plan_product(fn, &p, each, 128);
   if (columns < 0) return -1;
   Operand ox{x, rows, fi, 1}, ow{w, static_cast<long long>(groups) * each, fi, 1};
-  const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + part_bytes(p);
+  const bool few = few_rows_pay(rows, groups, fi, each, true);
+  const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + (few ? 0 : part_bytes(p));
   CallScratch cs;
   if (bytes > 0 && take_scratch(device_id, st, bytes, 0, &cs) != 0) return -1;
   char* scratch = cs.scratch;
   if (place_operand(&ox, &scratch, st) != 0 || place_operand(&ow, &scratch, st) != 0) return -1;
+  if (few) {
+    const FewArgs f{ox.data, ow.data, y, x_scale, w_scale, indptr, ox.pitch, ow.pitch, rows, groups, fi, fo, fi, 0, 0, 0, nullptr, gate};
+    const int done = few_rows_f8(f, y_type, gated, st);
+    return done != 0 ? done : return_scratch(cs, st);
+  }
   p.parts = scratch;
   CUtensorMap tm_w, tm_x64, tm_x16;
   if (map_operands(&tm_w, &tm_x64, &tm_x16, CU_TENSOR_MAP_DATA_TYPE_UINT8, ow, ox, fo, groups, true, gated) != 0) return -1;

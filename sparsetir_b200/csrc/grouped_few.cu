@@ -6,10 +6,13 @@
 // Which element of a step of K plays which k is free as long as both operands agree, so every lane loads 16 (8) bytes of W.
 // One row of 8-bit integers, 4096 -> 8192: 33.6 MB in 8.2 us out of HBM, 5.0 out of L2; prefetch sizes of 128 and 256 bytes at the
 // loads changed nothing and cost up to a third.
+#include <cuda_fp8.h>
+
 #include <algorithm>
 #include <type_traits>
 
 #include "common.h"
+#include "gate.cuh"
 #include "grouped.h"
 #include "launch.cuh"
 #include "lowp.cuh"
@@ -30,6 +33,13 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__nv_fp8_e4m3>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                                   uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 template <class T>
 __device__ __forceinline__ void mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -61,9 +71,11 @@ __device__ __forceinline__ void load_if(uint2& v, const char* p, bool in) {
 
 // W contiguous along K.  A step is 64 bytes of K of 32 features and 8 NT rows: lane l has 16 bytes, at 16 (l % 4), of
 // features l / 4 + 8 i and of rows l / 4 + 8 h; registers 0, 1 of them make one instruction, 2, 3 another.
-template <class T, int NT>
+// Gated: the 32 are 16 of the gate (i = 0, 1) and the same 16 of the other projection.
+template <class T, int NT, bool GATED = false>
 struct AlongK {
   static constexpr int kFeatures = 32, kStepBytes = 64, kRows = 8 * NT;
+  static constexpr bool kGated = GATED;
   using Sum = typename SumOf<T>::type;
   Sum acc[2][NT][4];
   struct Step { uint4 w[4], x[NT]; };
@@ -76,8 +88,10 @@ struct AlongK {
     bytes = k1;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int f = feat0 + lane / 4 + 8 * i;
-      wp[i] = static_cast<const char*>(p.w) + (static_cast<size_t>(group) * p.fo + min(f, p.fo - 1)) * p.w_pitch + at;
+      const int f = feat0 + lane / 4 + 8 * (GATED ? i & 1 : i);
+      size_t r = static_cast<size_t>(group) * (GATED ? 2 : 1) * p.fo + min(f, p.fo - 1);
+      if (GATED && i >= 2) r += p.fo;
+      wp[i] = static_cast<const char*>(p.w) + r * p.w_pitch + at;
     }
 #pragma unroll
     for (int h = 0; h < NT; ++h) {
@@ -119,6 +133,74 @@ struct AlongK {
   }
 };
 
+// The same for 8-bit floating point: the sums of a step, half of a block of K that shares scales, are scaled and added to those of the steps
+// before it.
+template <int NT, bool GATED>
+struct Scaled : AlongK<__nv_fp8_e4m3, NT, GATED> {
+  using Base = AlongK<__nv_fp8_e4m3, NT, GATED>;
+  struct Step : Base::Step { float x_scale[NT][2], w_scale[3]; };
+  float sum[2][NT][4];
+  const float *xs, *ws[3];
+  int base, rows, row[NT][2];  // base: of K, of the next step
+  __device__ __forceinline__ void start(const FewArgs& p, int group, int feat0, int row0, int live, int k0, int k1, int lane) {
+    Base::start(p, group, feat0, row0, live, k0, k1, lane);
+    base = k0;
+    rows = p.rows;
+    const int blocks = (p.fi + SPARSETIR_F8_BLOCK - 1) / SPARSETIR_F8_BLOCK;
+    const int of_w = ((GATED ? 2 : 1) * p.fo + SPARSETIR_F8_BLOCK - 1) / SPARSETIR_F8_BLOCK;
+    auto of = [&](int f) { return p.w_scale + (static_cast<size_t>(group) * of_w + f / SPARSETIR_F8_BLOCK) * blocks; };
+    const int f = feat0 + lane / 4;
+    ws[0] = of(min(feat0, p.fo - 1));              // of all 32 features (gated: 16) of the warp
+    ws[1] = of(p.fo + min(f, p.fo - 1));           // gated: the other projection's may lie in two blocks
+    ws[2] = of(p.fo + min(f + 8, p.fo - 1));
+    xs = p.x_scale + row0;
+#pragma unroll
+    for (int h = 0; h < NT; ++h)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) row[h][c] = min(8 * h + 2 * (lane & 3) + c, live - 1);
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int h = 0; h < NT; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[m][h][c] = 0.f;
+  }
+  __device__ __forceinline__ void load(Step& s) {
+    const int block = base / SPARSETIR_F8_BLOCK;
+    const bool in = base < this->bytes;
+#pragma unroll
+    for (int i = 0; i < (GATED ? 3 : 1); ++i) s.w_scale[i] = in ? ld_global(ws[i] + block) : 0.f;
+#pragma unroll
+    for (int h = 0; h < NT; ++h)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) s.x_scale[h][c] = in ? ld_global(xs + static_cast<size_t>(block) * rows + row[h][c]) : 0.f;
+    base += Base::kStepBytes;
+    Base::load(s);
+  }
+  __device__ __forceinline__ void multiply(const Step& s) {
+    Base::multiply(s);
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int h = 0; h < NT; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float w = s.w_scale[GATED && m == 1 ? 1 + (c >> 1) : 0];
+          sum[m][h][c] = fmaf(this->acc[m][h][c], s.x_scale[h][c & 1] * w, sum[m][h][c]);
+          this->acc[m][h][c] = 0.f;
+        }
+  }
+  __device__ __forceinline__ void put(float (*to)[Base::kFeatures], int lane) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int h = 0; h < NT; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) this->acc[m][h][c] = sum[m][h][c];
+    Base::put(to, lane);
+  }
+};
+
 // W contiguous along the features (16-bit elements).  A step is 32 of K of 32 features: lane l has 4 features from 4 (l / 4) on of the
 // eight rows of W from 8 (l % 4) on, and eight elements of its rows of x; instruction j takes the j-th and the (j + 2)-th
 // feature of every lane's four, four rows at a time.  (With 8 features to a lane, 64 to a warp, there are half as many
@@ -126,6 +208,7 @@ struct AlongK {
 template <class T, int NT>
 struct AlongFeatures {
   static constexpr int kFeatures = 32, kStepBytes = 64, kRows = 8 * NT;  // bytes of K in x
+  static constexpr bool kGated = false;
   using Sum = float;
   float acc[2][NT][4];
   struct Step { uint2 w[8]; uint4 x[NT]; };
@@ -191,6 +274,7 @@ template <class Operand, class OutT>
 __global__ void __launch_bounds__(32 * kMaxWarps, 1) few_rows_kernel(const __grid_constant__ FewArgs p) {
   using Sum = typename Operand::Sum;
   constexpr int F = Operand::kFeatures, kRows = Operand::kRows;
+  constexpr int O = Operand::kGated ? F / 2 : F;  // features of the result to a warp
   extern __shared__ __align__(16) unsigned char smem[];
   Sum(*const part)[kRows][F] = reinterpret_cast<Sum(*)[kRows][F]>(smem);  // of every warp
   chain_wait();
@@ -209,7 +293,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 1) few_rows_kernel(const __gri
   if (rest) row0 = max(row0 + kRows, from);
   end = min(end, (rest ? from : row0) + kRows);
   const int fw = warp / p.splits, ks = warp - fw * p.splits;
-  const int block_feats = p.feature_warps * F;
+  const int block_feats = p.feature_warps * O;
   const int block_feat0 = blockIdx.x * block_feats;
   const int k0 = ks * p.split_bytes, k1 = min(k0 + p.split_bytes, p.k_bytes);
   // Once.  Without the loop the compiler moves what is behind the steps ahead of them and spills 70 bytes of registers (one row,
@@ -217,7 +301,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 1) few_rows_kernel(const __gri
   for (; row0 < end; row0 += kRows) {
     const int live = end - row0;
     Operand op;
-    op.start(p, group, block_feat0 + fw * F, row0, live, k0, k1, lane);
+    op.start(p, group, block_feat0 + fw * O, row0, live, k0, k1, lane);
     const int steps = (k1 - k0 + Operand::kStepBytes - 1) / Operand::kStepBytes;  // <= 0: nothing of the depth left
     // two or three steps requested ahead of the one that is multiplied
     typename Operand::Step a, b, c;
@@ -238,7 +322,18 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 1) few_rows_kernel(const __gri
       const int feat = block_feat0 + f;
       if (feat >= p.fo) continue;
       Sum sum = 0;
-      for (int q = 0; q < p.splits; ++q) sum += part[f / F * p.splits + q][r][f % F];
+      for (int q = 0; q < p.splits; ++q) sum += part[f / O * p.splits + q][r][f % O];
+      if constexpr (Operand::kGated) {
+        float up = 0.f;
+        for (int q = 0; q < p.splits; ++q) up += part[f / O * p.splits + q][r][O + f % O];
+        static_cast<OutT*>(p.y)[static_cast<size_t>(row0 + r) * p.fo + feat] = from_float<OutT>(p.gate.act(sum, up));
+        if (p.hidden != nullptr) {
+          OutT* const h = static_cast<OutT*>(p.hidden) + static_cast<size_t>(row0 + r) * 2 * p.fo + feat;
+          h[0] = from_float<OutT>(sum);
+          h[p.fo] = from_float<OutT>(up);
+        }
+        continue;
+      }
       float v = static_cast<float>(sum);
       if constexpr (std::is_same<Sum, int>::value)
         v *= ld_global(p.x_scale + row0 + r) * ld_global(p.w_scale + static_cast<size_t>(group) * p.fo + feat);
@@ -253,14 +348,15 @@ int launch(FewArgs p, cudaStream_t st) {
   // as many warps as keep the memory busy: the depth is split where the features of the groups are too few, into parts of four
   // steps at least.  Eight warps to a block, fewer where blocks would not be found on every SM.
   const int used = std::min(p.groups, p.rows);
-  const long long warps = static_cast<long long>(ceil_div(p.fo, Operand::kFeatures)) * used;
+  constexpr int O = Operand::kGated ? Operand::kFeatures / 2 : Operand::kFeatures;
+  const long long warps = static_cast<long long>(ceil_div(p.fo, O)) * used;
   int splits = 1;
   while (splits < kMaxWarps && 2 * warps * splits <= kNumSMs * kMaxWarps && p.k_bytes / splits > 4 * Operand::kStepBytes) splits *= 2;
   p.feature_warps = std::max(1, 8 / splits);
   while (p.feature_warps > 1 && warps / p.feature_warps < kNumSMs) p.feature_warps /= 2;
   p.splits = splits;
   p.split_bytes = (ceil_div(p.k_bytes, splits) + 127) / 128 * 128;
-  const dim3 grid(ceil_div(p.fo, p.feature_warps * Operand::kFeatures), p.groups + (p.rows - 1) / Operand::kRows);
+  const dim3 grid(ceil_div(p.fo, p.feature_warps * O), p.groups + (p.rows - 1) / Operand::kRows);
   const int block_warps = p.feature_warps * splits, smem = block_warps * Operand::kRows * Operand::kFeatures * 4;
   static thread_local int configured_device = -1;
   int dev = 0;
@@ -282,12 +378,18 @@ int launch_layout(const FewArgs& p, bool along_k, cudaStream_t st) {
   return launch<AlongK<T, NT>, OutT>(p, st);
 }
 
+// f(integral constant NT): 8 rows at a time, or 16
+template <class F>
+int with_rows(const FewArgs& p, F&& f) {
+  if (p.rows <= 4ll * std::min(p.groups, p.rows)) return f(std::integral_constant<int, 1>{});
+  return f(std::integral_constant<int, 2>{});
+}
+
 template <class T>
 int launch_type(const FewArgs& p, int y_type, bool along_k, cudaStream_t st) {
-  const bool eight = p.rows <= 4ll * std::min(p.groups, p.rows);
   return with_type(y_type, [&](auto o) {
     using O = decltype(o);
-    return eight ? launch_layout<T, 1, O>(p, along_k, st) : launch_layout<T, 2, O>(p, along_k, st);
+    return with_rows(p, [&](auto nt) { return launch_layout<T, nt.value, O>(p, along_k, st); });
   });
 }
 
@@ -297,6 +399,24 @@ int few_rows(const FewArgs& p, int type, int y_type, bool along_k, cudaStream_t 
   if (type < 0) return launch_type<int8_t>(p, y_type, along_k, st);
   if (type == SPARSETIR_F16) return launch_type<__half>(p, y_type, along_k, st);
   return launch_type<__nv_bfloat16>(p, y_type, along_k, st);
+}
+
+int few_rows_gated(const FewArgs& p, int type, cudaStream_t st) {
+  return with_rows(p, [&](auto nt) {
+    if (type == SPARSETIR_F16) return launch<AlongK<__half, nt.value, true>, __half>(p, st);
+    return launch<AlongK<__nv_bfloat16, nt.value, true>, __nv_bfloat16>(p, st);
+  });
+}
+
+int few_rows_f8(const FewArgs& p, int y_type, bool gated, cudaStream_t st) {
+  return with_rows(p, [&](auto nt) {
+    return with_type(y_type, [&](auto o) {
+      using O = decltype(o);
+      if constexpr (!std::is_same<O, float>::value)
+        if (gated) return launch<Scaled<nt.value, true>, O>(p, st);
+      return launch<Scaled<nt.value, false>, O>(p, st);
+    });
+  });
 }
 
 }  // namespace sptir

@@ -51,12 +51,19 @@ extern "C" int sparsetir_grouped_mm_gated_raw(const void* x, const void* w, void
   p.idesc = tc05::instr_desc(map_format(type), 2 * kM, 0, 0, 0);
   const int columns = plan_product(fn, &p, 2 * width, 64);
   if (columns < 0) return -1;
+  const bool few = few_rows_pay(rows, num_groups, feat_in, 2 * width, true);
   Operand ox{x, rows, feat_in, 2}, ow{w, static_cast<long long>(num_groups) * 2 * width, feat_in, 2};
-  const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + part_bytes(p);
+  const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + (few ? 0 : part_bytes(p));
   CallScratch cs;
   if (bytes > 0 && take_scratch(device_id, st, bytes, 0, &cs) != 0) return -1;
   char* scratch = cs.scratch;
   if (place_operand(&ox, &scratch, st) != 0 || place_operand(&ow, &scratch, st) != 0) return -1;
+  if (few) {
+    const FewArgs f{ox.data, ow.data, y, nullptr, nullptr, indptr, ox.pitch, ow.pitch, rows, num_groups, feat_in, width, feat_in * 2, 0, 0, 0, hidden,
+                    p.gate};
+    const int done = few_rows_gated(f, type, st);
+    return done != 0 ? done : return_scratch(cs, st);
+  }
   p.parts = scratch;
   CUtensorMap tm_w, tm_x64, tm_x16;
   if (map_operands(&tm_w, &tm_x64, &tm_x16, map_type(type), ow, ox, width, num_groups, true, true) != 0) return -1;

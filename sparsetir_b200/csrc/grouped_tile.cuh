@@ -33,15 +33,17 @@ enum Out { kPlain, kWeights, kGated, kGatedGrad };
 // Columns of a tile, and what follows from them.  128 leave room for two pairs of blocks on two SMs: for many groups of few rows,
 // where the loads of one pair hide the other's beginning and end (us, 256 / 128 columns: 64 groups of 16 rows, 512 -> 512
 // 13.6 / 7.6; 500 rows in 64 groups, 2048 -> 2048 91.4 / 90.3; 8 groups of 500 rows 39 / 41).
-template <int N, int OUT = kPlain> struct Shape {
+template <int N, int OUT = kPlain, int ELEM = kHalf> struct Shape {
   static constexpr int kBytes = kABytes + N / 2 * 128;  // of a stage
-  static constexpr int kStages = N == 256 ? 6 : OUT == kGatedGrad ? 3 : 4;  // what shared memory holds
+  static constexpr int kStages = N == 256 ? 6 : OUT == kGatedGrad || ELEM == kFloat8 ? 3 : 4;  // what shared memory holds
   static constexpr int kBlocks = N == 256 ? 1 : 2;      // per SM
   static constexpr int kTmemCols = 2 * N;               // two accumulators
   static constexpr int kEpilogue = N == 256 ? 8 : 4;    // warps
   static constexpr int kThreads = (kFirstEpilogue + kEpilogue) * 32;
-  static constexpr int kStaged = OUT == kGatedGrad ? 2 * kStagedBytes : OUT == kGated ? kStagedBytes + kStagedBytes / 2 : kStagedBytes;
-  static constexpr int kSmem = kStages * kBytes + kEpilogue * kStaged + 1024;
+  // of an epilogue warp: what leaves, and 8-bit floating point's scales behind it
+  static constexpr int kStaged = OUT == kGatedGrad ? 2 * kStagedBytes : OUT == kGated ? kStagedBytes + kStagedBytes / 2 + 128 : kStagedBytes;
+  static constexpr int kWarp = kStaged + (ELEM == kFloat8 && N == 128 ? 4 * (128 + 32 * (OUT == kGated ? 3 : 1)) * 4 : 0);
+  static constexpr int kSmem = kStages * kBytes + kEpilogue * kWarp + 1024;
 };
 
 __device__ unsigned int g_grouped_timeouts = 0;
@@ -309,13 +311,18 @@ template <int ELEM, int OUT, class OutT, int kN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kN>::kThreads, Shape<kN>::kBlocks)
 grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b64,
                const __grid_constant__ CUtensorMap tm_b16, const __grid_constant__ Args p) {
-  using S = Shape<kN, OUT>;
+  using S = Shape<kN, OUT, ELEM>;
   constexpr bool I8 = ELEM == kInt8, F8 = ELEM == kFloat8, GRAD = OUT == kWeights;
   constexpr int kDepth = ELEM == kHalf ? 64 : 128;  // of K per stage
   constexpr int kInstr = ELEM == kHalf ? 16 : 32;   // of K per instruction
   constexpr int kStages = S::kStages, kStageBytes = S::kBytes, kTmemCols = S::kTmemCols;
   constexpr int kEpilogue = S::kEpilogue;
   constexpr int kBlockFeatures = OUT == kGated ? kM / 2 : kM;  // of the result, per block
+  constexpr bool ROWS = F8 && kN == 256;  // rows of x are the left operand, rows of W the columns
+  // of a tile with ROWS, in whole blocks of the halves that the two blocks of the pair bring
+  auto columns_of = [&](const Tile& t) {
+    return OUT == kGated ? min(256, (2 * (p.features - t.feat0) + 63) & ~63) : min(256, (p.features - t.feat0 + 31) & ~31);
+  };
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kStages];   // rank 0: both blocks' operands are there
   __shared__ __align__(8) uint64_t bar_empty[kStages];  // the tensor core has read the stage
@@ -384,23 +391,56 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     int acc = 0;
     const int mine = (warp - kFirstEpilogue) / 4 * 32;  // first columns of the warp
     constexpr int kStep = kEpilogue / 4 * 32;
-    unsigned char* const staged = smem_raw + (base - tc05::smem_u32(smem_raw)) + kStages * kStageBytes + (warp - kFirstEpilogue) * S::kStaged;
-    while (ok && next()) {
-      const int feat0 = tile.feat0 + static_cast<int>(rank) * kBlockFeatures + (warp & 3) * (kBlockFeatures / 4);
+    unsigned char* const staged = smem_raw + (base - tc05::smem_u32(smem_raw)) + kStages * kStageBytes + (warp - kFirstEpilogue) * S::kWarp;
+    auto first_feature = [&]() { return tile.feat0 + static_cast<int>(rank) * kBlockFeatures + (warp & 3) * (kBlockFeatures / 4); };
+    if constexpr (ROWS) {
+      const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 4 * mine;
+      while (ok && next()) {
+        RowWarp<OUT, OutT> w(p, tile, columns_of(tile), mine / 32, static_cast<int>(rank) * kM + (warp & 3) * 32, staged, lane);
+        if (tile.steps == 0) {  // nothing of the depth is left for this unit
+          w.zeros();
+          continue;
+        }
+        ok = w.add(taddr, kN, bar_acc_full, bar_acc_empty, acc);
+        acc += tile.steps;
+        if (ok) w.emit();
+      }
+    } else if constexpr (F8) {  // 128 neighbouring columns to a warp
+      static_assert(S::kWarp == S::kStaged + Scales<OUT>::kBytes && Scales<OUT>::kProducts <= S::kStaged, "shared memory of a warp");
+      float* const slots = reinterpret_cast<float*>(staged + S::kStaged);
+      const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+      Scales<OUT> scales;
+      bool more = next();
+      if (more) scales.begin(p, tile, first_feature(), 4 * mine, 128, slots, lane);
+      while (ok && more) {
+        const Tile t = tile;
+        const Warp<OutT> w(p, t, first_feature(), 4 * mine, 32, 128, staged, lane);
+        if (t.steps > 0) ok = w.template add_scaled<OUT>(taddr, kN, bar_acc_full, bar_acc_empty, acc, scales, slots);
+        if (!ok) break;
+        acc += t.steps;
+        more = next();
+        if (more) scales.begin(p, tile, first_feature(), 4 * mine, 128, slots, lane);  // on their way while this tile leaves
+        if (t.steps > 0) {
+          const int buf = (acc - 1) & 1;
+          typename Warp<OutT>::Ahead none;
+          w.template emit<OUT>(taddr + buf * kN, none, [&] { w.taken(&bar_acc_empty[buf]); });
+        } else {  // nothing of the depth is left for this unit
+          w.template zeros<OUT>();
+        }
+      }
+    }
+    while (!F8 && ok && next()) {
+      const int feat0 = first_feature();
       size_t row = static_cast<size_t>(tile.col0);
       if constexpr (GRAD) row += static_cast<size_t>(tile.group) * p.columns;
-      if constexpr (F8 || OUT == kGated || OUT == kGatedGrad) {
-        // 8-bit floating point: 128 neighbouring columns
-        const Warp<OutT> w(p, tile, feat0, F8 ? 4 * mine : mine, F8 ? 32 : kStep, staged, lane);
+      if constexpr (OUT == kGated || OUT == kGatedGrad) {
+        const Warp<OutT> w(p, tile, feat0, mine, kStep, kN, staged, lane);
         const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         if (tile.steps == 0) {  // nothing of the depth is left for this unit
-          w.template zeros<OUT>(F8 ? 4 : kN / kStep);
-        } else if constexpr (F8) {
-          ok = w.template scaled<OUT>(taddr, kN, bar_acc_full, bar_acc_empty, acc);
-          acc += tile.steps;
+          w.template zeros<OUT>();
         } else {
           const int buf = acc & 1;
-          ok = w.template out_of_tmem<OUT>(taddr + buf * kN, &bar_acc_full[buf], tc05::pair::at_first(&bar_acc_empty[buf]), (acc >> 1) & 1);
+          ok = w.template out_of_tmem<OUT>(taddr + buf * kN, &bar_acc_full[buf], &bar_acc_empty[buf], (acc >> 1) & 1);
           ++acc;
         }
         continue;
@@ -451,10 +491,14 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     if (warp == 0) {
       // ---- loads.  Each block fetches its 128 features and its half of the columns, and tells rank 0's barrier.
       while (ok && next()) {
-        const int half = tile.n_mma / 2, units = half / 16;
-        const int feat = tile.feat0 + static_cast<int>(rank) * kBlockFeatures, col = tile.col0 + static_cast<int>(rank) * half;
+        const int half = ROWS ? kM : tile.n_mma / 2;
+        auto units_of = [&](int r) { return ROWS ? max(0, min(kM, tile.n - r * kM) + 15) / 16 : half / 16; };  // rows of x, 16 at a time
+        const int units = units_of(static_cast<int>(rank));
+        const int feat = tile.feat0 + static_cast<int>(rank) * (ROWS ? columns_of(tile) / (OUT == kGated ? 4 : 2) : kBlockFeatures);
+        const int col = tile.col0 + static_cast<int>(rank) * half;
         if (tc05::elect_one()) {
           const uint32_t bytes = kABytes + (GRAD ? (half > 64 ? 2 : 1) * kAtom : units * 2048);
+          const uint32_t both = ROWS ? 2 * kABytes + (units_of(0) + units_of(1)) * 2048 : 2 * bytes;
           int s = stage;
           uint32_t ph = phase;
           for (int k = tile.step0; k < tile.step0 + tile.steps; ++k) {
@@ -467,7 +511,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             } else {
               bar = tc05::pair::at_first(&bar_full[s]);
               if (rank == 0) {  // for both blocks: an arrival from the other one at every step took 1 us each
-                tc05::mbar_arrive_expect_tx(&bar_full[s], 2 * bytes);
+                tc05::mbar_arrive_expect_tx(&bar_full[s], both);
                 tc05::mbar_arrive(&bar_full[s]);
               }
             }
@@ -508,13 +552,14 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       int acc = 0;
       const bool a_mn = GRAD || p.a_mn != 0;
       const uint32_t a_step = a_mn ? 2048u : 32u, b_step = GRAD ? 2048u : 32u;
-      const uint64_t da0 = tc05::smem_desc_swizzled(base, a_mn ? kAtom : 0, 1024, tc05::kSwizzle128B);
-      const uint64_t db0 = tc05::smem_desc_swizzled(base + kABytes, GRAD ? kAtom : 0, 1024, tc05::kSwizzle128B);
+      // left operand: W, or x with ROWS
+      const uint64_t da0 = tc05::smem_desc_swizzled(base + (ROWS ? kABytes : 0), a_mn ? kAtom : 0, 1024, tc05::kSwizzle128B);
+      const uint64_t db0 = tc05::smem_desc_swizzled(base + (ROWS ? 0 : kABytes), GRAD ? kAtom : 0, 1024, tc05::kSwizzle128B);
       while (rank == 0 && ok && next()) {
         if (tile.steps == 0) continue;
         if (tc05::elect_one()) {
           const int buf = acc & 1;
-          const uint32_t idesc = p.idesc | static_cast<uint32_t>(tile.n_mma >> 3) << 17;
+          const uint32_t idesc = p.idesc | static_cast<uint32_t>((ROWS ? columns_of(tile) : tile.n_mma) >> 3) << 17;
           uint32_t d = tmem + buf * kN;
           int s = stage;
           uint32_t ph = phase;
@@ -677,7 +722,7 @@ inline int place_operand(Operand* o, char** scratch, cudaStream_t st) {
 
 template <int ELEM, int OUT, class OutT, int N>
 int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap& tm_b16, const Args& p, cudaStream_t st) {
-  using S = Shape<N, OUT>;
+  using S = Shape<N, OUT, ELEM>;
   static thread_local int configured_device = -1;
   constexpr int smem = S::kSmem;
   const auto kernel = grouped_kernel<ELEM, OUT, OutT, N>;
