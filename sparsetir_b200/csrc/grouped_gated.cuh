@@ -6,6 +6,8 @@
 #ifndef SPARSETIR_B200_GROUPED_GATED_CUH_
 #define SPARSETIR_B200_GROUPED_GATED_CUH_
 
+#include <type_traits>
+
 namespace sptir {
 namespace {
 
@@ -319,7 +321,8 @@ struct Warp {
     tc05::tmem_ld16x32(taddr + first, a);
     tc05::tmem_ld16x32(taddr + (16u << 16) + first, b);
     for (int c0 = first; c0 < last; c0 += step) {
-      tc05::tmem_ld_wait();
+      tc05::tmem_ld_wait(a);
+      tc05::tmem_ld_wait(b);
       if (c0 + step >= last) take();
       float va[16], vb[16];
 #pragma unroll
@@ -390,7 +393,7 @@ struct Warp {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if (16 * j >= live) break;
-        tc05::tmem_ld_wait();
+        tc05::tmem_ld_wait(r[j & 1]);
         if (j < 7 && 16 * (j + 1) < live) tc05::tmem_ld16(from + 16 * (j + 1), r[(j + 1) & 1]);
         else if (!ends) taken(empty + buf);
 #pragma unroll
@@ -429,14 +432,14 @@ struct RowWarp {
   const Args& p;
   const Tile t;
   const int feat0;        // of the result, of the warp's first column
-  const int columns;      // that the tensor core fills for the warp, may be <= 0
+  const int columns;      // that the tensor core fills for the warp, 128 at most, may be <= 0
   const int row0, rows;   // of the warp's lanes: the first, and how many live, may be <= 0 or > 32
   unsigned char* const staged;
   const int lane;
   float sum[128];
 
   __device__ __forceinline__ RowWarp(const Args& args, const Tile& tile, int n_mma, int half, int first_row, unsigned char* mem, int l)
-      : p(args), t(tile), feat0(tile.feat0 + half * (kTwo ? 64 : 128)), columns(n_mma - half * 128), row0(tile.col0 + first_row),
+      : p(args), t(tile), feat0(tile.feat0 + half * (kTwo ? 64 : 128)), columns(min(n_mma - half * 128, 128)), row0(tile.col0 + first_row),
         rows(tile.n - first_row), staged(mem), lane(l) {}
 
   // false: a wait ran out
@@ -467,36 +470,67 @@ struct RowWarp {
 #pragma unroll
     for (int i = 0; i < 128; ++i) sum[i] = 0.f;
     const bool dead = columns <= 0 || rows <= 0;
+    auto wait = [&](int n) { return __all_sync(0xffffffffu, tc05::mbar_spin(full + (n & 1), (n >> 1) & 1)) != 0; };
+    // 32 columns; those of a gated block: 16 of the gate, 16 of the other projection
+    auto add32 = [&](int j, const uint32_t (&r)[32], float s, float u, float v, auto mixed) {
+      const int left = change - 16 * j;  // features with the scales of u
+      const float by = !kTwo ? s : left > 0 ? u : v;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float f = i < 16 ? s : mixed.value && kTwo ? (i - 16 < left ? u : v) : by;
+        sum[32 * j + i] = fmaf(__uint_as_float(r[i]), f, sum[32 * j + i]);
+      }
+    };
+    if (!dead && columns == 128 && !(kTwo && change < 64 && change % 16 != 0)) {
+      // All of it: the loads of the next 32 columns, across the steps, while these are added.  Whether the next step's sums are complete is
+      // asked ahead, since the answer takes 0.1 us.
+      if (!wait(acc)) return false;
+      tc05::fence_after_sync();
+      uint32_t r[2][32];
+      tc05::tmem_ask32(taddr + (acc & 1) * buffer, r[0]);
+      for (int k = 0; k < t.steps; ++k, ++acc) {
+        const float s = a.x * a.w, u = a.x * a.u, v = a.x * a.v;
+        a = b;
+        b = fetch(k + 2);
+        const uint32_t from = taddr + (acc & 1) * buffer, next = taddr + ((acc + 1) & 1) * buffer;
+        const bool more = k + 1 < t.steps;
+        bool over = true;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          tc05::tmem_ld_wait(r[j & 1]);
+          if (j < 3) {
+            tc05::tmem_ask32(from + 32 * (j + 1), r[(j + 1) & 1]);
+          } else {
+            taken(empty + (acc & 1));
+            if (more) {
+              if (!__all_sync(0xffffffffu, over) && !wait(acc + 1)) return false;
+              tc05::fence_after_sync();
+              tc05::tmem_ask32(next, r[0]);
+            }
+          }
+          if (j == 2 && more) over = tc05::mbar_over(full + ((acc + 1) & 1), ((acc + 1) >> 1) & 1);
+          add32(j, r[j & 1], s, u, v, std::false_type{});
+        }
+      }
+      return true;
+    }
     for (int k = 0; k < t.steps; ++k, ++acc) {
       const float s = a.x * a.w, u = a.x * a.u, v = a.x * a.v;
       a = b;
       b = fetch(k + 2);
-      const int buf = acc & 1;
-      if (!__all_sync(0xffffffffu, tc05::mbar_wait(full + buf, (acc >> 1) & 1))) return false;
+      if (!wait(acc)) return false;
       tc05::fence_after_sync();
-      const uint32_t from = taddr + buf * buffer;
       if (dead) {
-        taken(empty + buf);
+        taken(empty + (acc & 1));
         continue;
       }
-      uint32_t r[2][16];
-      tc05::tmem_ld16(from, r[0]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (16 * j >= columns) break;
-        tc05::tmem_ld_wait();
-        if (j < 7 && 16 * (j + 1) < columns) tc05::tmem_ld16(from + 16 * (j + 1), r[(j + 1) & 1]);
-        else taken(empty + buf);
-        const bool mixed = kTwo && (j & 1) != 0 && 8 * (j - 1) < change && 8 * (j - 1) + 16 > change;
-        if (!mixed) {
-          const float by = !kTwo || (j & 1) == 0 ? s : 8 * (j - 1) < change ? u : v;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sum[16 * j + i] = fmaf(__uint_as_float(r[j & 1][i]), by, sum[16 * j + i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            sum[16 * j + i] = fmaf(__uint_as_float(r[j & 1][i]), 8 * (j - 1) + i < change ? u : v, sum[16 * j + i]);
-        }
+      for (int j = 0; j < 4; ++j) {
+        if (32 * j >= columns) break;
+        uint32_t r[32];
+        tc05::tmem_ld32(taddr + (acc & 1) * buffer + 32 * j, r);
+        if (32 * (j + 1) >= columns) taken(empty + (acc & 1));
+        add32(j, r, s, u, v, std::true_type{});
       }
     }
     return true;

@@ -566,13 +566,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
           if constexpr (!F8) ok = tc05::pair::mbar_wait(&bar_acc_empty[buf], ((acc >> 1) & 1) ^ 1);
           tc05::fence_after_sync();
           for (int k = tile.step0; k < tile.step0 + tile.steps && ok; ++k) {
-            if constexpr (F8) {  // every step has sums of its own
-              const int n = acc + k - tile.step0;
-              d = tmem + (n & 1) * kN;
-              if (!tc05::pair::mbar_wait(&bar_acc_empty[n & 1], ((n >> 1) & 1) ^ 1)) { ok = false; break; }
-            }
             const bool cleared = GRAD && (k + 1) * kDepth > tile.depth;  // by threads of both blocks
             if (!(cleared ? tc05::pair::mbar_wait(&bar_full[s], ph) : tc05::mbar_wait(&bar_full[s], ph))) { ok = false; break; }
+            if constexpr (F8) {  // every step has sums of its own; the operands are there long before
+              const int n = acc + k - tile.step0;
+              d = tmem + (n & 1) * kN;
+              if (!tc05::mbar_spin(&bar_acc_empty[n & 1], ((n >> 1) & 1) ^ 1)) { ok = false; break; }
+            }
             tc05::fence_after_sync();
             const uint64_t da = tc05::desc_advance(da0, s * kStageBytes), db = tc05::desc_advance(db0, s * kStageBytes);
             const int left = tile.depth - k * kDepth;
