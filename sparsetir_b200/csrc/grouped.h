@@ -42,6 +42,7 @@ struct FewArgs {
 int few_rows(const FewArgs& p, int type, int y_type, bool along_k, cudaStream_t st);
 // The gated block (W along the depth) of 16-bit elements, and the product or the gated block of 8-bit floating point.
 int few_rows_gated(const FewArgs& p, int type, cudaStream_t st);
+constexpr int kFewF8Depth = 16384;  // at most, whose scales shared memory holds
 int few_rows_f8(const FewArgs& p, int y_type, bool gated, cudaStream_t st);
 
 }  // namespace sptir

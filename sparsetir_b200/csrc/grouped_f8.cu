@@ -26,7 +26,7 @@ int product_f8(const char* fn, const void* x, const float* x_scale, const void* 
   const int columns = plan_product(fn, &p, each, 128);
   if (columns < 0) return -1;
   Operand ox{x, rows, fi, 1}, ow{w, static_cast<long long>(groups) * each, fi, 1};
-  const bool few = few_rows_pay(rows, groups, fi, each, true);
+  const bool few = fi <= kFewF8Depth && few_rows_pay(rows, groups, fi, each, true);
   const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + (few ? 0 : part_bytes(p));
   CallScratch cs;
   if (bytes > 0 && take_scratch(device_id, st, bytes, 0, &cs) != 0) return -1;

@@ -567,7 +567,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
           tc05::fence_after_sync();
           for (int k = tile.step0; k < tile.step0 + tile.steps && ok; ++k) {
             const bool cleared = GRAD && (k + 1) * kDepth > tile.depth;  // by threads of both blocks
-            if (!(cleared ? tc05::pair::mbar_wait(&bar_full[s], ph) : tc05::mbar_wait(&bar_full[s], ph))) { ok = false; break; }
+            if (!(cleared ? tc05::pair::mbar_wait(&bar_full[s], ph) : F8 ? tc05::mbar_spin(&bar_full[s], ph) : tc05::mbar_wait(&bar_full[s], ph))) { ok = false; break; }
             if constexpr (F8) {  // every step has sums of its own; the operands are there long before
               const int n = acc + k - tile.step0;
               d = tmem + (n & 1) * kN;
@@ -581,8 +581,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
               if (i * kInstr < left)
                 tc05::pair::mma<kKind>(d, tc05::desc_advance(da, i * a_step), tc05::desc_advance(db, i * b_step), idesc,
                                        ((!F8 && k > tile.step0) || i > 0) ? 1u : 0u);
-            tc05::pair::mma_commit(&bar_empty[s]);
             if constexpr (F8) tc05::pair::mma_commit(&bar_acc_full[(acc + k - tile.step0) & 1]);
+            tc05::pair::mma_commit(&bar_empty[s]);
             if (++s == kStages) { s = 0; ph ^= 1u; }
           }
           if constexpr (!F8) tc05::pair::mma_commit(&bar_acc_full[buf]);

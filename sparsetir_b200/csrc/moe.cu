@@ -576,24 +576,62 @@ dispatch_i8_kernel(const Piece<B>* x, const int32_t* slots, Piece<B / sizeof(T)>
   }
 }
 
-// Rows to 8-bit floating point with a scale for each block of 128 features: L lanes have a block, P pieces each, and a warp kF8Hold
-// times as many blocks as it has room for.  The quotient 448 x / a is 0.875 x over a / 512: both are exact for elements of 16 bits,
-// and so is the quotient's place between the numbers of 8 bits, ties among them.
-constexpr int kF8Hold = 4;
-template <class T, int B>
+// Four numbers to e4m3, to nearest, ties to even.
+__device__ __forceinline__ uint32_t pack_f8(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return __byte_perm(lo, hi, 0x5410);
+}
+// 448 x / a to the nearest e4m3, ties to even, for |x| <= a: the quotient of 0.875 x by unit = a / 512.  Both are exact for elements of 16 bits, and
+// so is the place of their rounded quotient between the numbers of 8 bits, ties among them.  below and above are 0.875 / unit moved by
+// four units of its last place: where x times both has one place, so has the quotient, and four divisions are spared.
+__device__ __forceinline__ uint32_t quotients_f8(const float* x, float unit, float below, float above) {
+  uint32_t q = pack_f8(x[0] * below, x[1] * below, x[2] * below, x[3] * below);
+  if (q != pack_f8(x[0] * above, x[1] * above, x[2] * above, x[3] * above))
+    q = pack_f8(0.875f * x[0] / unit, 0.875f * x[1] / unit, 0.875f * x[2] / unit, 0.875f * x[3] / unit);
+  return q;
+}
+// The largest magnitude of pieces, in the order of unsigned integers (so that an infinity or a NaN is larger than all numbers), and as the bits of
+// a float: of 16-bit elements two at a time.
+template <class T>
+struct Largest {
+  uint32_t bits = 0u;
+  template <int B>
+  __device__ __forceinline__ void take(const Piece<B>& v) {
+    if constexpr (sizeof(T) == 2 && B == 2) {
+      bits = max(bits, static_cast<uint32_t>(v) & 0x7fffu);
+    } else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+      for (int i = 0; i < B / 4; ++i) bits = sizeof(T) == 2 ? __vmaxs2(bits, w[i] & 0x7fff7fffu) : max(bits, w[i] & 0x7fffffffu);
+    }
+  }
+  template <int L>
+  __device__ __forceinline__ float over_lanes() const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(most_of<L>(bits));
+    const uint16_t most = static_cast<uint16_t>(most_of<L>(max(bits & 0xffffu, bits >> 16)));
+    return to_float(reinterpret_cast<const T&>(most));
+  }
+};
+
+// Rows to 8-bit floating point with a scale for each block of 128 features: L lanes have a block, P pieces each that lie side by side, and a
+// warp kHold times as many blocks as it has room for.  (Us, 8,192 rows of 2048 in 16 bits to eight slots each, 172 MB: 36.0 with a
+// division to an element and 8 bytes to a store, now 30.0; one slot each, 16,384 rows of 4096, 201 MB: 71 and 47.)
+template <class T, int B, bool WIDE>
 struct F8Lanes {
   static constexpr int N = B / sizeof(T);  // elements of a piece
-  static constexpr int kLanes = SPARSETIR_F8_BLOCK / N < 32 ? SPARSETIR_F8_BLOCK / N : 32;
-  static constexpr int kPieces = SPARSETIR_F8_BLOCK / N / kLanes;
+  static constexpr int kPieces = SPARSETIR_F8_BLOCK / N > 32 ? SPARSETIR_F8_BLOCK / N / 32 : WIDE ? 16 / N : 1;
+  static constexpr int kLanes = SPARSETIR_F8_BLOCK / N / kPieces;
   static constexpr int kBlocks = 32 / kLanes;  // of 128 features that a warp has side by side
-  static constexpr int kHold = kF8Hold / kPieces > 0 ? kF8Hold / kPieces : 1;
+  static constexpr int kHold = kPieces < 4 ? 4 / kPieces : 1;
+  static constexpr int kOut = WIDE ? kPieces * N : N;  // bytes of a store
 };
-template <class T, int B>
+template <class T, int B, bool WIDE>
 __global__ void __launch_bounds__(kWarps * 32)
-dispatch_f8_kernel(const Piece<B>* x, const int32_t* slots, Piece<B / sizeof(T)>* q, float* scale, int tokens, int rows, int pieces,
-                   int blocks, int chunks, int top_k) {
-  using Lanes = F8Lanes<T, B>;
-  constexpr int N = Lanes::N, L = Lanes::kLanes, P = Lanes::kPieces, H = Lanes::kHold;
+dispatch_f8_kernel(const Piece<B>* x, const int32_t* slots, uint8_t* q, float* scale, int tokens, int rows, int pieces, int blocks,
+                   int chunks, int top_k) {
+  using Lanes = F8Lanes<T, B, WIDE>;
+  constexpr int N = Lanes::N, L = Lanes::kLanes, P = Lanes::kPieces, H = Lanes::kHold, OUT = Lanes::kOut;
   chain_wait();
   const int lane = threadIdx.x & 31;
   const long long item = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
@@ -601,61 +639,60 @@ dispatch_f8_kernel(const Piece<B>* x, const int32_t* slots, Piece<B / sizeof(T)>
   if (t >= tokens) return;
   const int slot = slots != nullptr ? pair_slot(slots, t, top_k, rows, lane) : (lane == 0 ? t : -1);
   const int block0 = c * (H * Lanes::kBlocks) + lane / L;  // and every kBlocks further
-  const int first = block0 * (L * P) + lane % L;
+  const int first = (block0 * L + lane % L) * P;
   Piece<B> v[H][P];
-  Piece<N> o[H][P];
+  constexpr int E = P * N;  // elements of a lane in a block, a multiple of four
+  __align__(16) uint32_t o[H][E / 4];
   float s_of[H];
 #pragma unroll
   for (int h = 0; h < H; ++h)
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const int at = first + h * (Lanes::kBlocks * L * P) + i * L;
+      const int at = first + h * (Lanes::kBlocks * L * P) + i;
       v[h][i] = Piece<B>{};
       if (at < pieces) v[h][i] = ld_global(x + static_cast<size_t>(t) * pieces + at);
     }
 #pragma unroll
   for (int h = 0; h < H; ++h) {
-    float f[P][N];
-    uint32_t bits = 0u;  // the largest magnitude without its sign: an infinity or a NaN is larger than all numbers
+    Largest<T> largest;
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      unpack<T, B>(v[h][i], f[i]);
-#pragma unroll
-      for (int n = 0; n < N; ++n) bits = max(bits, __float_as_uint(f[i][n]) & 0x7fffffffu);
-    }
-    bits = most_of<L>(bits);
-    const float a = __uint_as_float(bits);
+    for (int i = 0; i < P; ++i) largest.template take<B>(v[h][i]);
+    const float a = largest.template over_lanes<L>();
     const bool zeros = !(a >= 0x1p-110f && a < INFINITY);
-    const float unit = zeros ? INFINITY : a * 0x1p-9f;
+    const float unit = zeros ? 1.f : a * 0x1p-9f, times = __fdividef(0.875f, unit);  // two units off at most
     s_of[h] = a < 0x1p-110f ? 0.f : a / 448.f;
+    float f[E];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      uint8_t* b = reinterpret_cast<uint8_t*>(&o[h][i]);
+      float part[N];
+      unpack<T, B>(v[h][i], part);
 #pragma unroll
-      for (int n = 0; n < N; n += 2) {
-        const float lo = zeros ? 0.f : f[i][n] * 0.875f / unit;
-        if constexpr (N > 1) {
-          const float hi = zeros ? 0.f : f[i][n + 1] * 0.875f / unit;
-          const __nv_fp8x2_storage_t both = __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
-          b[n] = static_cast<uint8_t>(both & 0xff);
-          b[n + 1] = static_cast<uint8_t>(both >> 8);
-        } else {
-          b[n] = __nv_cvt_float_to_fp8(lo, __NV_SATFINITE, __NV_E4M3);
-        }
-      }
+      for (int n = 0; n < N; ++n) f[i * N + n] = part[n];
+    }
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const uint32_t q4 = quotients_f8(f + e, unit, times * (1.f - 0x1p-21f), times * (1.f + 0x1p-21f));
+      o[h][e / 4] = zeros ? 0u : q4;
     }
   }
   for (int j = 0; j < top_k; ++j) {
     const int s = __shfl_sync(kFull, slot, j);
     if (s < 0) continue;
+    uint8_t* const to = q + static_cast<size_t>(s) * pieces * N;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       const int block = block0 + h * Lanes::kBlocks;
       if (lane % L == 0 && block < blocks) scale[static_cast<size_t>(block) * rows + s] = s_of[h];
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const int at = first + h * (Lanes::kBlocks * L * P) + i * L;
-        if (at < pieces) q[static_cast<size_t>(s) * pieces + at] = o[h][i];
+      for (int i = 0; i < E / OUT; ++i) {
+        const int at = first * N + h * (Lanes::kBlocks * L * E) + i * OUT;  // rows are whole stores
+        Piece<OUT> out;
+        if constexpr (OUT >= 4) {
+          out = *reinterpret_cast<const Piece<OUT>*>(&o[h][i * OUT / 4]);
+        } else {
+          out = static_cast<Piece<OUT>>(o[h][i * OUT / 4] >> (8 * (i * OUT % 4)));
+        }
+        if (at < pieces * N) *reinterpret_cast<Piece<OUT>*>(to + at) = out;
       }
     }
   }
@@ -833,21 +870,23 @@ extern "C" int sparsetir_moe_dispatch_f8_raw(const void* x, int type, const int3
   if (slots && check_slots(fn, slots, tokens, rows, top_k, st) != 0) return -1;
   return with_type(type, [&](auto t) {
     using T = decltype(t);
-    // a piece of N elements leaves as N bytes
+    // a piece of N elements leaves as N bytes, or two (four) as 16
     int b = piece_bytes(sizeof(T) * feat, bits_of(x));
     while (b > static_cast<int>(sizeof(T)) && bits_of(q) % (b / sizeof(T)) != 0) b /= 2;
-    return with_piece<sizeof(T)>(b, [&](auto bytes) {
+    auto run = [&](auto bytes, auto wide) {
       constexpr int B = bytes.value;
-      using Lanes = F8Lanes<T, B>;
+      using Lanes = F8Lanes<T, B, wide.value>;
       const int scales = ceil_div(feat, SPARSETIR_F8_BLOCK), chunks = ceil_div(scales, Lanes::kBlocks * Lanes::kHold);
       const long long blocks = (static_cast<long long>(tokens) * chunks + kWarps - 1) / kWarps;
       if (blocks > INT32_MAX) return fail("%s: too large for one launch", fn);
-      launch_chained(dispatch_f8_kernel<T, B>, static_cast<unsigned>(blocks), kWarps * 32, 0, st, static_cast<const Piece<B>*>(x),
-                     slots, static_cast<Piece<Lanes::N>*>(q), scale, tokens, rows, static_cast<int>(sizeof(T) * feat / B), scales,
-                     chunks, top_k);
+      launch_chained(dispatch_f8_kernel<T, B, wide.value>, static_cast<unsigned>(blocks), kWarps * 32, 0, st,
+                     static_cast<const Piece<B>*>(x), slots, static_cast<uint8_t*>(q), scale, tokens, rows,
+                     static_cast<int>(sizeof(T) * feat / B), scales, chunks, top_k);
       SPTIR_LAUNCH_OK("dispatch_f8_kernel");
       return 0;
-    });
+    };
+    if (b == 16 && feat % 16 == 0 && bits_of(q) % 16 == 0) return run(std::integral_constant<int, 16>{}, std::true_type{});
+    return with_piece<sizeof(T)>(b, [&](auto bytes) { return run(bytes, std::false_type{}); });
   });
 }
 
