@@ -9,29 +9,93 @@
 
 #include <cuda_runtime.h>
 
+#include <cstdint>
+
 namespace sptir {
 
+// Two floats that go through one instruction: the epilogues of the products wait for the results of most of their instructions, and this halves
+// their number.
+struct Two {
+  uint64_t v;
+  Two() = default;
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+  __device__ __forceinline__ float lo() const { return __uint_as_float(static_cast<uint32_t>(v)); }
+  __device__ __forceinline__ float hi() const { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+  __device__ __forceinline__ friend Two operator*(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+  }
+  __device__ __forceinline__ friend Two operator+(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+  }
+};
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {  // a b + c
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float exp2_near(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_near(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 struct Gate {
-  float c1 = 1.f, c3 = 0.f;  // z = g (c1 + c3 g^2)
+  bool gelu = false;
+  static constexpr float kC1 = 1.5957691216057308f;   // 2 sqrt(2 / pi)
+  static constexpr float kC3 = 0.07135481282652936f;  // and times 0.044715
   Gate() = default;
-  explicit Gate(bool gelu) {
-    if (gelu) {
-      c1 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
-      c3 = 0.07135481282652936f;  // and times 0.044715
-    }
+  explicit Gate(bool g) : gelu(g) {}
+
+  // An infinite square would make z' g s (1 - s) = inf * 0.
+  __device__ __forceinline__ static Two square(Two g) {
+    const Two q = g * g;
+    return Two(fminf(q.lo(), 1e30f), fminf(q.hi(), 1e30f));
   }
-  __device__ __forceinline__ float sigmoid(float g, float g2) const {
-    return __fdividef(1.f, 1.f + __expf(-g * fmaf(c3, g2, c1)));  // exp is infinite from about 88 on: 1 / inf = 0
+  template <bool GELU>
+  __device__ __forceinline__ static Two sigmoid(Two g, Two squares) {
+    constexpr float kLog2e = 1.4426950408889634f;
+    const Two z = GELU ? g * fma(Two(-kLog2e * kC3), squares, Two(-kLog2e * kC1)) : g * Two(-kLog2e);
+    // 2^z is infinite from 128 on: 1 / inf = 0
+    const Two t = Two(exp2_near(z.lo()), exp2_near(z.hi())) + Two(1.f);
+    return Two(reciprocal_near(t.lo()), reciprocal_near(t.hi()));
   }
-  // bounded: c3 = 0 times an infinite square would not be a number
-  static __device__ __forceinline__ float square(float g) { return fminf(g * g, 1e30f); }
-  __device__ __forceinline__ float act(float g, float up) const { return g * sigmoid(g, square(g)) * up; }
+  // f(g) up
+  template <bool GELU>
+  __device__ __forceinline__ static Two act(Two g, Two up) {
+    return g * sigmoid<GELU>(g, GELU ? square(g) : g) * up;
+  }
   // d: gradient of act
-  __device__ __forceinline__ void grad(float g, float up, float d, float* d_gate, float* d_up, float* act) const {
-    const float g2 = square(g), s = sigmoid(g, g2), f = g * s;
-    *d_gate = d * up * fmaf(f * (1.f - s), fmaf(3.f * c3, g2, c1), s);
+  template <bool GELU>
+  __device__ __forceinline__ static void grad(Two g, Two up, Two d, Two* d_gate, Two* d_up, Two* act) {
+    const Two squares = GELU ? square(g) : g;
+    const Two s = sigmoid<GELU>(g, squares), f = g * s, rest = fma(s, Two(-1.f), Two(1.f));
+    Two slope = f * rest;  // f' = s + f (1 - s) z'
+    if (GELU) slope = slope * fma(Two(3.f * kC3), squares, Two(kC1));
+    *d_gate = d * up * (slope + s);
     *d_up = d * f;
     *act = f * up;
+  }
+  // One at a time, where speed does not matter
+  __device__ __forceinline__ float act(float g, float up) const {
+    return (gelu ? act<true>(Two(g), Two(up)) : act<false>(Two(g), Two(up))).lo();
+  }
+  __device__ __forceinline__ void grad(float g, float up, float d, float* d_gate, float* d_up, float* of_act) const {
+    Two a, b, c;
+    if (gelu) grad<true>(Two(g), Two(up), Two(d), &a, &b, &c);
+    else grad<false>(Two(g), Two(up), Two(d), &a, &b, &c);
+    *d_gate = a.lo();
+    *d_up = b.lo();
+    *of_act = c.lo();
   }
 };
 

@@ -195,8 +195,15 @@ struct Warp {
     OutT* const kept = static_cast<OutT*>(p.hidden) + row(c0) * 2 * width + feat0;
     if (p.wide) {
       uint32_t act[8];
+      auto activate = [&](auto gelu) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) act[i] = pack2<OutT>(p.gate.act(g[2 * i], u[2 * i]), p.gate.act(g[2 * i + 1], u[2 * i + 1]));
+        for (int i = 0; i < 8; ++i) {
+          const Two a = Gate::act<gelu.value>(Two(g[2 * i], g[2 * i + 1]), Two(u[2 * i], u[2 * i + 1]));
+          act[i] = pack2<OutT>(a.lo(), a.hi());
+        }
+      };
+      if (p.gate.gelu) activate(std::true_type{});
+      else activate(std::false_type{});
       __syncwarp();  // the reads of the last 32 columns are over
       put32(kStagedBytes, 0, act[0], act[1], act[2], act[3]);
       put32(kStagedBytes, 2, act[4], act[5], act[6], act[7]);
@@ -240,10 +247,13 @@ struct Warp {
       }
     }
   }
-  __device__ __forceinline__ static float half_of(uint32_t v, int c) {
-    const uint32_t one = c == 0 ? v & 0xffffu : v >> 16;
-    const uint16_t bits = static_cast<uint16_t>(one);
-    return to_float(reinterpret_cast<const OutT&>(bits));
+  __device__ __forceinline__ static Two halves_of(uint32_t v) {
+    if constexpr (std::is_same<OutT, __half>::value) {
+      const float2 f = __half22float2(reinterpret_cast<const __half2&>(v));
+      return Two(f.x, f.y);
+    } else {
+      return Two(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    }
   }
   template <class Next>
   __device__ __forceinline__ void gated_grad(const float* da, const float* db, int c0, Ahead& ahead, Next&& next) const {
@@ -260,25 +270,28 @@ struct Warp {
       if (c0 + step < t.n) ask(c0 + step, ahead);
       __syncwarp();
       uint32_t act[16];
+      auto differentiate = [&](auto gelu) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t g[4], u[4], og[4], ou[4];
-        get64(0, i, g);
-        get64(kStagedBytes, i, u);
+        for (int i = 0; i < 4; ++i) {
+          uint32_t g[4], u[4], og[4], ou[4];
+          get64(0, i, g);
+          get64(kStagedBytes, i, u);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float* d = (q < 2 ? da : db) + 4 * i + 2 * (q & 1);
-          float xg[2], xu[2], xa[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) p.gate.grad(half_of(g[q], c), half_of(u[q], c), d[c], &xg[c], &xu[c], &xa[c]);
-          og[q] = pack2<OutT>(xg[0], xg[1]);
-          ou[q] = pack2<OutT>(xu[0], xu[1]);
-          act[4 * i + q] = pack2<OutT>(xa[0], xa[1]);
+          for (int q = 0; q < 4; ++q) {
+            const float* d = (q < 2 ? da : db) + 4 * i + 2 * (q & 1);
+            Two xg, xu, xa;
+            Gate::grad<gelu.value>(halves_of(g[q]), halves_of(u[q]), Two(d[0], d[1]), &xg, &xu, &xa);
+            og[q] = pack2<OutT>(xg.lo(), xg.hi());
+            ou[q] = pack2<OutT>(xu.lo(), xu.hi());
+            act[4 * i + q] = pack2<OutT>(xa.lo(), xa.hi());
+          }
+          __syncwarp();
+          put64(0, i, og[0], og[1], og[2], og[3]);  // in the place of what was read
+          put64(kStagedBytes, i, ou[0], ou[1], ou[2], ou[3]);
         }
-        __syncwarp();
-        put64(0, i, og[0], og[1], og[2], og[3]);  // in the place of what was read
-        put64(kStagedBytes, i, ou[0], ou[1], ou[2], ou[3]);
-      }
+      };
+      if (p.gate.gelu) differentiate(std::true_type{});
+      else differentiate(std::false_type{});
       next();
       __syncwarp();
       OutT* const to = dg + static_cast<size_t>(lane >> 2) * 2 * width + 8 * (lane & 3);
@@ -596,7 +609,9 @@ struct RowWarp {
         for (int i = 0; i < 16; ++i) {
           if constexpr (kTwo) {
             const int at = 64 * j + 32 * (i >> 3) + 2 * (i & 7);
-            w[i] = pack2<OutT>(p.gate.act(sum[at], sum[at + 16]), p.gate.act(sum[at + 1], sum[at + 17]));
+            const Two g(sum[at], sum[at + 1]), u(sum[at + 16], sum[at + 17]);
+            const Two a = p.gate.gelu ? Gate::act<true>(g, u) : Gate::act<false>(g, u);
+            w[i] = pack2<OutT>(a.lo(), a.hi());
           } else {
             w[i] = pack2<OutT>(sum[32 * j + 2 * i], sum[32 * j + 2 * i + 1]);
           }
