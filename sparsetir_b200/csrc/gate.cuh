@@ -3,7 +3,7 @@
 //   gelu, form of tanh  0.5 g (1 + tanh(u)) = g * sigmoid(2 u):  z = 2 sqrt(2 / pi) (g + 0.044715 g^3)
 // and its gradient: with s = sigmoid(z),  f' = s + g s (1 - s) z'.
 // All of it in f32; exp and the quotient by the hardware's approximations (a few units of 2^-22: nothing beside the rounding of a 16-bit
-// result, and z is at most 88 in magnitude where s is not 0 or 1 to that precision).
+// result).
 #ifndef SPARSETIR_B200_GATE_CUH_
 #define SPARSETIR_B200_GATE_CUH_
 
@@ -40,7 +40,7 @@ __device__ __forceinline__ Two fma(Two a, Two b, Two c) {  // a b + c
 }
 __device__ __forceinline__ float exp2_near(float x) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));  // without ftz: results down to 2^-149
   return r;
 }
 __device__ __forceinline__ float reciprocal_near(float x) {
@@ -64,10 +64,11 @@ struct Gate {
   template <bool GELU>
   __device__ __forceinline__ static Two sigmoid(Two g, Two squares) {
     constexpr float kLog2e = 1.4426950408889634f;
-    const Two z = GELU ? g * fma(Two(-kLog2e * kC3), squares, Two(-kLog2e * kC1)) : g * Two(-kLog2e);
-    // 2^z is infinite from 128 on: 1 / inf = 0
-    const Two t = Two(exp2_near(z.lo()), exp2_near(z.hi())) + Two(1.f);
-    return Two(reciprocal_near(t.lo()), reciprocal_near(t.hi()));
+    const Two z = GELU ? g * fma(Two(kLog2e * kC3), squares, Two(kLog2e * kC1)) : g * Two(kLog2e);
+    // of e = 2^-|z|, which is 1 at most: 1 / (1 + e), or e / (1 + e) where z < 0, small as it may be
+    const float e0 = exp2_near(-fabsf(z.lo())), e1 = exp2_near(-fabsf(z.hi()));
+    const Two t = Two(e0, e1) + Two(1.f);
+    return Two(z.lo() < 0.f ? e0 : 1.f, z.hi() < 0.f ? e1 : 1.f) * Two(reciprocal_near(t.lo()), reciprocal_near(t.hi()));
   }
   // f(g) up
   template <bool GELU>
