@@ -406,7 +406,8 @@ SPARSETIR_API int sparsetir_grouped_mm_gated(SPARSETIR_PACKED_ARGS);
  * width] (with SPARSETIR_GROUPED_W_OUT_IN [num_groups, width, feat]), and h = hidden[s, :],
  *   d_hidden[s, j] = d[j] h[width + j] f'(h[j]),   d_hidden[s, width + j] = d[j] f(h[j]);
  * `act` (null: not wanted) receives f(h[j]) h[width + j], formed again from h for the gradient of W.  The gradients to the block's
- * input and weights are sparsetir_grouped_mm and sparsetir_grouped_mm_grad_w on d_hidden.  Rows of no group are not written.
+ * input and weights are sparsetir_grouped_mm and sparsetir_grouped_mm_grad_w on d_hidden.  d_hidden may be hidden itself.  Rows of no group
+ * are not written.
  * args: (dy f16|bf16 [S*feat], w (type of dy) [num_groups*feat*width], hidden (type of dy) [S*2*width], d_hidden (type of dy)
  *        [S*2*width], act (type of dy) [S*width] or null, indptr i32[num_groups+1] or null, num_groups, feat, width [, flags]). */
 SPARSETIR_API int sparsetir_grouped_mm_gated_grad(SPARSETIR_PACKED_ARGS);

@@ -10,6 +10,7 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -53,11 +54,17 @@ def _newest_header() -> float:
     return newest
 
 
+def _newest_source(path: str) -> float:
+    """Of a source and of those that it includes."""
+    with open(path) as f:
+        included = re.findall(r'^#include "(\w+\.cu)"', f.read(), re.M)
+    return max([os.path.getmtime(path)] + [os.path.getmtime(os.path.join(CSRC, i)) for i in included])
+
+
 def _compile(src: str, force: bool, verbose: bool, hdr_mtime: float) -> str:
     obj = os.path.join(OBJ_DIR, src + ".o")
     path = os.path.join(CSRC, src)
-    if (not force and os.path.exists(obj)
-            and os.path.getmtime(obj) > max(os.path.getmtime(path), hdr_mtime)):
+    if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(_newest_source(path), hdr_mtime):
         return obj
     cmd = [_nvcc(), *NVCC_FLAGS, "-x", "cu", "-c", path, "-o", obj]
     if verbose:

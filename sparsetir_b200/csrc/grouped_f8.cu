@@ -1,9 +1,12 @@
 // Products of 8-bit floating point (e4m3) grouped by expert, with a scale for each 128 of a row of x and for each 128 x 128 of W, and the gated
-// block of such operands, on the tensor cores (grouped_tile.cuh; the epilogue is in grouped_gated.cuh).
-// A step of the ring is 128 of K: its sums are complete in one of two accumulators, which change by turns, and eight warps add them, scaled, to
-// sums in their registers while the tensor core fills the other.  The MMAs of a step are 512 clocks of the tensor core; the eight
-// warps' 256 loads of TMEM and the additions, two to an instruction, are about 340 of each scheduler's.
-#include "grouped_tile.cuh"
+// block of such operands, on the tensor cores (grouped.cu; the epilogue is in grouped_gated.cuh).
+// A step of the ring is 128 of K: its sums are complete in one of two accumulators, which change by turns, and the epilogue's warps add them, scaled, to
+// sums in their registers while the tensor core fills the other.  Tiles of 256 rows have the rows of x as the left operand (one scale to a lane);
+// those of 128 rows, for groups of few rows, the features, as the other products have (us, tiles of 128 / 256 rows: 500 rows in 64
+// groups, 2048 -> 2048 56 / 76, 4,096 rows 71 / 81, 6,400 rows 1024 -> 1024 28 / 32).
+// Power: 8192^3 505 us, 2.18 PFLOP/s of values of one sign.
+#define SPARSETIR_GROUPED_KERNEL_ONLY
+#include "grouped.cu"
 
 namespace sptir {
 namespace {
@@ -26,6 +29,8 @@ int product_f8(const char* fn, const void* x, const float* x_scale, const void* 
   const int columns = plan_product(fn, &p, each, 128);
   if (columns < 0) return -1;
   Operand ox{x, rows, fi, 1}, ow{w, static_cast<long long>(groups) * each, fi, 1};
+  // us, the kernel for few rows / this one: 1 row, 4096 -> 8192 7.6 / 16.7; 16 rows 10.8 / 17.4; 48 rows, 8 groups, 1024 -> 4096 8.5 / 16.7; 64 rows,
+  // 8 groups, 2048 -> 2048 10.3 / 14.3, gated 17.3 / 29.3
   const bool few = fi <= kFewF8Depth && few_rows_pay(rows, groups, fi, each, true);
   const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + (few ? 0 : part_bytes(p));
   CallScratch cs;

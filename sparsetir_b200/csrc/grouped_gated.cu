@@ -1,8 +1,14 @@
 // The gated block of an expert in one product, and its gradient through the product that follows it, on the tensor cores
-// (grouped_tile.cuh; the epilogues are in grouped_gated.cuh):
+// (grouped.cu; the epilogues are in grouped_gated.cuh):
 //   grouped_mm_gated       h = x W[g]^T of 2 * width features, act = f(h[:, :width]) * h[:, width:]  (gate.cuh)
 //   grouped_mm_gated_grad  d = dy W[g], and from d and h the gradient to h
-#include "grouped_tile.cuh"
+// A gated tile is 128 features of act, 256 rows of W: in every 32 of them 16 of the gate and the same 16 of the other projection, which TMA brings
+// side by side (a box of 16 x 2 rows), so that both meet in one thread of the epilogue.  The gradient's epilogue has the projections of the next 32
+// rows on their way while it works, and puts their gradients where they lay in shared memory.
+// 65,536 rows, 64 groups, 2048 -> 2 x 1024, bf16: 434 us with both projections kept (even groups; 1.27 PFLOP/s, the plain product of that size
+// 404 to 460), 545 with ragged ones; the gradient 285 and 354: without its loads and stores of the projections 226, its 1.2 GB alone are 184.
+#define SPARSETIR_GROUPED_KERNEL_ONLY
+#include "grouped.cu"
 
 namespace sptir {
 namespace {

@@ -1,4 +1,4 @@
-// Epilogues of grouped_kernel (grouped_tile.cuh, which includes this): a gated block, the gradient of one, and sums with a scale for each
+// Epilogues of grouped_kernel (grouped.cu, which includes this): a gated block, the gradient of one, and sums with a scale for each
 // 128 of K.  All take the sums as fragments (tmem_ld16x32): 16 lanes of TMEM, 32 columns, v[4 i + 2 h + c] = lane 8 h + l / 4 of the 16, column
 // 8 i + 2 (l % 4) + c, for lane l of the warp.
 //   Gated: of the 32 rows of W that a warp's lanes of TMEM stand for, the first 16 are the gate's and the last 16 the other projection's of
@@ -18,9 +18,8 @@ template <int N> struct F8Registers {
   static constexpr int kEpilogue = N == 256 ? 232 : 216;
 };
 
-// The scales of 8-bit floating point on their way to an epilogue warp: every lane copies its four columns' and those of W's rows, four steps of K
-// ahead, into places that it alone reads.  (Read into registers one step ahead, they held the warps up: each step then lasted as long
-// as a load takes, 0.8 us where it now is 0.4.)
+// The scales of 8-bit floating point on their way to an epilogue warp whose columns are rows of x: every lane copies its four columns' and those of
+// W's rows, four steps of K ahead, into places that it alone reads, and multiplies them for all lanes when their step comes.
 template <int OUT>
 struct Scales {
   static constexpr int kW = OUT == kGated ? 3 : 1;  // of W: gated: the gate's, and two of the other projection's, whose rows may lie in two blocks
@@ -438,7 +437,11 @@ struct Warp {
 
 // ---- 8-bit floating point, tiles of 256 rows: the rows of x are those of the tensor core's left operand, 256 features (gated: 128 and 128, 16 by
 // 16) its columns.  A lane's 128 sums are of one row and, but for a gated block's other projection, of one block of W: they share one scale, and
-// nothing but TMEM is read between one step of K and the next.
+// nothing but TMEM is read between one step of K and the next.  Us, 65,536 rows in 64 equal groups, 2048 -> 2048: with the features as the left
+// operand and the rows' scales out of shared memory 512 to 566, this way 367, with the loads of TMEM in flight across the steps 328, with waits that
+// ask again and again 310 (the same product of 8-bit integers, scaled at the end alone, 228).  What is left is the way there and back: from the issue of
+// a step's MMAs (512 clocks) to their sums in registers 1,160 clocks, 350 to take them and 200 until the issuing thread knows, with two accumulators
+// on the way.  The same in two halves of 128 columns with barriers of their own was slower (345), and TMEM has no room for a third of 256.
 template <int OUT, class OutT>
 struct RowWarp {
   static constexpr bool kTwo = OUT == kGated;

@@ -134,11 +134,11 @@ __device__ __forceinline__ bool mbar_over(uint64_t* bar, uint32_t parity) {
   return done != 0;
 }
 
-// mbar_wait by asking again and again: the answer comes sooner than to a thread that the barrier has to wake.
+// mbar_wait by asking again and again, for waits that are short: the answer comes sooner than to a thread that the barrier has to wake.
 __device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity) {
-  for (uint32_t spin = 0; spin < kSpinLimit; ++spin)
+  for (int spin = 0; spin < 4096; ++spin)
     if (mbar_over(bar, parity)) return true;
-  return false;
+  return mbar_wait(bar, parity);
 }
 
 // Producer side of a TMA pipeline: one arrival plus the number of bytes the copies will deliver.

@@ -297,6 +297,18 @@ def test_grad_values_stay_in_their_rows(cuda_device):
     assert torch.equal(d[~bad_d], d0[~bad_d]) and torch.equal(a[~bad_a], a0[~bad_a])
 
 
+@pytest.mark.parametrize("sizes,feat,width", [([70, 0, 300, 1], 200, 136), ([90], 4096, 72), ([40, 500], 65, 33), ([60] * 40, 72, 520)], ids=str)
+def test_gradient_in_the_place_of_the_projections(cuda_device, sizes, feat, width):
+    g = gen(8, cuda_device)
+    rand = lambda *s: torch.randn(*s, generator=g, device=cuda_device).bfloat16()  # noqa: E731
+    rows, n = sum(sizes), len(sizes)
+    dy, w, hidden, ptr = rand(rows * feat), rand(n * feat * width), rand(rows * 2 * width), pointers(sizes, cuda_device)
+    d, act, act2 = torch.empty_like(hidden), torch.empty_like(hidden[:rows * width]), torch.empty_like(hidden[:rows * width])
+    ops.grouped_mm_gated_grad(dy, w, hidden, d, act, ptr, n, feat, width)
+    ops.grouped_mm_gated_grad(dy, w, hidden, hidden, act2, ptr, n, feat, width)
+    assert torch.equal(hidden, d) and torch.equal(act, act2)
+
+
 # ------------------------------------------------------------------ both
 @pytest.mark.parametrize("fi,rows,width", [(64, 30, 64), (2048, 30, 136), (64, 3000, 132), (4096, 900, 136)])
 def test_wild_pointers_stay_inside(cuda_device, fi, rows, width):
