@@ -41,8 +41,6 @@ constexpr int kFirstEpilogue = 4;     // warp 0 loads, 1 issues, 2 clears the ta
 constexpr int kStagedBytes = 32 * 64; // 32 columns of 32 features on their way, per epilogue warp
 constexpr int kBand = 8;              // column tiles of a group that are walked side by side
 
-// Elements of the operands: 16 bits, 8-bit integers, 8-bit floating point with a scale for each 128 of K.
-enum Elem { kHalf, kInt8, kFloat8 };
 // What becomes of the sums: the result, a gradient of weights (rows of a group are the depth), or, in grouped_gated.cuh, a gated block
 // (two rows of W to a feature) and the gradient of one.
 enum Out { kPlain, kWeights, kGated, kGatedGrad };
@@ -50,17 +48,15 @@ enum Out { kPlain, kWeights, kGated, kGatedGrad };
 // Columns of a tile, and what follows from them.  128 leave room for two pairs of blocks on two SMs: for many groups of few rows,
 // where the loads of one pair hide the other's beginning and end (us, 256 / 128 columns: 64 groups of 16 rows, 512 -> 512
 // 13.6 / 7.6; 500 rows in 64 groups, 2048 -> 2048 91.4 / 90.3; 8 groups of 500 rows 39 / 41).
-template <int N, int OUT = kPlain, int ELEM = kHalf> struct Shape {
+template <int N, int OUT = kPlain> struct Shape {
   static constexpr int kBytes = kABytes + N / 2 * 128;  // of a stage
-  static constexpr int kStages = N == 256 ? 6 : OUT == kGatedGrad || ELEM == kFloat8 ? 3 : 4;  // what shared memory holds
+  static constexpr int kStages = N == 256 ? 6 : OUT == kGatedGrad ? 3 : 4;  // what shared memory holds
   static constexpr int kBlocks = N == 256 ? 1 : 2;      // per SM
   static constexpr int kTmemCols = 2 * N;               // two accumulators
   static constexpr int kEpilogue = N == 256 ? 8 : 4;    // warps
   static constexpr int kThreads = (kFirstEpilogue + kEpilogue) * 32;
-  // of an epilogue warp: what leaves, and 8-bit floating point's scales behind it
-  static constexpr int kStaged = OUT == kGatedGrad ? 2 * kStagedBytes : OUT == kGated ? kStagedBytes + kStagedBytes / 2 + 128 : kStagedBytes;
-  static constexpr int kWarp = kStaged + (ELEM == kFloat8 && N == 128 ? 4 * (128 + 32 * (OUT == kGated ? 3 : 1)) * 4 : 0);
-  static constexpr int kSmem = kStages * kBytes + kEpilogue * kWarp + 1024;
+  static constexpr int kStaged = OUT == kGatedGrad ? 2 * kStagedBytes : OUT == kGated ? kStagedBytes + kStagedBytes / 2 : kStagedBytes;
+  static constexpr int kSmem = kStages * kBytes + kEpilogue * kStaged + 1024;
 };
 
 __device__ unsigned int g_grouped_timeouts = 0;
@@ -324,22 +320,17 @@ __device__ __forceinline__ void store_lanes(OutT* to, int pitch, int feats, int 
 namespace sptir {
 namespace {
 
-template <int ELEM, int OUT, class OutT, int kN>
+template <bool I8, int OUT, class OutT, int kN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kN>::kThreads, Shape<kN>::kBlocks)
 grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b64,
                const __grid_constant__ CUtensorMap tm_b16, const __grid_constant__ Args p) {
-  using S = Shape<kN, OUT, ELEM>;
-  constexpr bool I8 = ELEM == kInt8, F8 = ELEM == kFloat8, GRAD = OUT == kWeights;
-  constexpr int kDepth = ELEM == kHalf ? 64 : 128;  // of K per stage
-  constexpr int kInstr = ELEM == kHalf ? 16 : 32;   // of K per instruction
+  constexpr int kDepth = I8 ? 128 : 64;  // of K per stage
+  constexpr int kInstr = I8 ? 32 : 16;   // of K per instruction
+  using S = Shape<kN, OUT>;
+  constexpr bool GRAD = OUT == kWeights;
   constexpr int kStages = S::kStages, kStageBytes = S::kBytes, kTmemCols = S::kTmemCols;
   constexpr int kEpilogue = S::kEpilogue;
   constexpr int kBlockFeatures = OUT == kGated ? kM / 2 : kM;  // of the result, per block
-  constexpr bool ROWS = F8 && kN == 256;  // rows of x are the left operand, rows of W the columns
-  // of a tile with ROWS, in whole blocks of the halves that the two blocks of the pair bring
-  auto columns_of = [&](const Tile& t) {
-    return OUT == kGated ? min(256, (2 * (p.features - t.feat0) + 63) & ~63) : min(256, (p.features - t.feat0 + 31) & ~31);
-  };
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kStages];   // rank 0: both blocks' operands are there
   __shared__ __align__(8) uint64_t bar_empty[kStages];  // the tensor core has read the stage
@@ -349,7 +340,6 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
   __shared__ __align__(8) uint64_t bar_drain;
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr tc05::pair::Kind kKind = F8 ? tc05::pair::kF8 : I8 ? tc05::pair::kI8 : tc05::pair::kF16;
   const uint32_t rank = tc05::pair::rank();
   const uint32_t base = (tc05::smem_u32(smem_raw) + 1023u) & ~1023u;
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -402,56 +392,136 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     return unit < p.max_tiles && walk.at(unit, &tile);
   };
 
-  if (warp >= kFirstEpilogue) {
-    if constexpr (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8Registers<kN>::kEpilogue));
+  if (warp == 0) {
+    // ---- loads.  Each block fetches its 128 features and its half of the columns, and tells rank 0's barrier.
+    while (ok && next()) {
+      const int half = tile.n_mma / 2, units = half / 16;
+      const int feat = tile.feat0 + static_cast<int>(rank) * kBlockFeatures, col = tile.col0 + static_cast<int>(rank) * half;
+      if (tc05::elect_one()) {
+        const uint32_t bytes = kABytes + (GRAD ? (half > 64 ? 2 : 1) * kAtom : units * 2048);
+        int s = stage;
+        uint32_t ph = phase;
+        for (int k = tile.step0; k < tile.step0 + tile.steps; ++k) {
+          if (!tc05::mbar_wait(&bar_empty[s], ph ^ 1u)) { ok = false; break; }
+          const uint32_t st = base + s * kStageBytes;
+          uint32_t bar;
+          if (GRAD && (k + 1) * kDepth > tile.depth) {
+            bar = tc05::smem_u32(&bar_tail[s]);
+            tc05::mbar_arrive_expect_tx(&bar_tail[s], bytes);
+          } else {
+            bar = tc05::pair::at_first(&bar_full[s]);
+            if (rank == 0) {  // for both blocks: an arrival from the other one at every step took 1 us each
+              tc05::mbar_arrive_expect_tx(&bar_full[s], 2 * bytes);
+              tc05::mbar_arrive(&bar_full[s]);
+            }
+          }
+          if constexpr (GRAD) {
+            const int row = tile.row0 + k * kDepth;
+            tc05::pair::tma_load_2d(st, &tm_a, feat, row, bar);
+            tc05::pair::tma_load_2d(st + kAtom, &tm_a, feat + 64, row, bar);
+            tc05::pair::tma_load_2d(st + kABytes, &tm_b64, col, row, bar);
+            if (half > 64) tc05::pair::tma_load_2d(st + kABytes + kAtom, &tm_b64, col + 64, row, bar);
+          } else {
+            if constexpr (OUT == kGated) {  // 16 rows of the gate, 16 of the other projection, and so on
+#pragma unroll
+              for (int q = 0; q < 4; ++q) tc05::pair::tma_load_4d(st + q * 4096, &tm_a, k * kDepth, feat + 16 * q, 0, tile.group, bar);
+            } else if (p.a_mn) {
+              tc05::pair::tma_load_3d(st, &tm_a, feat, k * kDepth, tile.group, bar);
+              tc05::pair::tma_load_3d(st + kAtom, &tm_a, feat + 64, k * kDepth, tile.group, bar);
+            } else {
+              tc05::pair::tma_load_3d(st, &tm_a, k * kDepth, feat, tile.group, bar);
+            }
+            int u = 0;
+            for (; u + 4 <= units; u += 4) tc05::pair::tma_load_2d(st + kABytes + u * 2048, &tm_b64, k * kDepth, col + u * 16, bar);
+            for (; u < units; ++u) tc05::pair::tma_load_2d(st + kABytes + u * 2048, &tm_b16, k * kDepth, col + u * 16, bar);
+          }
+          ++armed;
+          if (++s == kStages) { s = 0; ph ^= 1u; }
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      advance(tile.steps);
+    }
+    // The last arrivals at this block's barriers come from the other block too: they have come before the block ends.
+    for (int i = 0; i < kStages && ok; ++i) {
+      ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_empty[stage], phase ^ 1u));
+      advance(1);
+    }
+  } else if (warp == 1) {
+    // ---- MMAs of both blocks, from rank 0: M = 256 features, N = the tile's columns
+    int acc = 0;
+    const bool a_mn = GRAD || p.a_mn != 0;
+    const uint32_t a_step = a_mn ? 2048u : 32u, b_step = GRAD ? 2048u : 32u;
+    const uint64_t da0 = tc05::smem_desc_swizzled(base, a_mn ? kAtom : 0, 1024, tc05::kSwizzle128B);
+    const uint64_t db0 = tc05::smem_desc_swizzled(base + kABytes, GRAD ? kAtom : 0, 1024, tc05::kSwizzle128B);
+    while (rank == 0 && ok && next()) {
+      if (tile.steps == 0) continue;
+      if (tc05::elect_one()) {
+        const int buf = acc & 1;
+        const uint32_t idesc = p.idesc | static_cast<uint32_t>(tile.n_mma >> 3) << 17;
+        const uint32_t d = tmem + buf * kN;
+        int s = stage;
+        uint32_t ph = phase;
+        ok = tc05::pair::mbar_wait(&bar_acc_empty[buf], ((acc >> 1) & 1) ^ 1);
+        tc05::fence_after_sync();
+        for (int k = tile.step0; k < tile.step0 + tile.steps && ok; ++k) {
+          const bool cleared = GRAD && (k + 1) * kDepth > tile.depth;  // by threads of both blocks
+          if (!(cleared ? tc05::pair::mbar_wait(&bar_full[s], ph) : tc05::mbar_wait(&bar_full[s], ph))) { ok = false; break; }
+          tc05::fence_after_sync();
+          const uint64_t da = tc05::desc_advance(da0, s * kStageBytes), db = tc05::desc_advance(db0, s * kStageBytes);
+          const int left = tile.depth - k * kDepth;
+#pragma unroll
+          for (int i = 0; i < kDepth / kInstr; ++i)
+            if (i * kInstr < left)
+              tc05::pair::mma<I8>(d, tc05::desc_advance(da, i * a_step), tc05::desc_advance(db, i * b_step), idesc,
+                                  (k > tile.step0 || i > 0) ? 1u : 0u);
+          tc05::pair::mma_commit(&bar_empty[s]);
+          if (++s == kStages) { s = 0; ph ^= 1u; }
+        }
+        tc05::pair::mma_commit(&bar_acc_full[buf]);
+        if (!ok) {  // gave up: what has been issued is over before the block's memory is released
+          tc05::pair::mma_commit(&bar_drain);
+          tc05::mbar_wait(&bar_drain, 0);
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      ++acc;
+      advance(tile.steps);
+    }
+  } else if (GRAD && warp == 2) {
+    // ---- The last step of a group holds rows of its neighbours: zeros in their place, in both operands (0 times what is
+    // not a number would not be zero), up to where the instructions read.
+    uint32_t tail_phase = 0;
+    while (ok && next()) {
+      const int rem = tile.depth % kDepth;
+      if (rem != 0 && tile.steps > 0 && (tile.step0 + tile.steps) * kDepth > tile.depth) {
+        const int s = (stage + tile.steps - 1) % kStages;
+        ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_tail[s], (tail_phase >> s) & 1u));
+        tail_phase ^= 1u << s;
+        const int clear = (((rem + kInstr - 1) / kInstr) * kInstr - rem) * 8;  // pieces of 16 bytes in each atom
+        unsigned char* at = smem_raw + (base - tc05::smem_u32(smem_raw)) + s * kStageBytes + rem * 128;
+        for (int i = lane; i < kStageBytes / kAtom * clear; i += 32) {
+          const int atom = i / clear;
+          *reinterpret_cast<uint4*>(at + atom * kAtom + (i - atom * clear) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        tc05::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) tc05::pair::arrive_release(tc05::pair::at_first(&bar_full[s]));
+      }
+      advance(tile.steps);
+    }
+  } else if (warp >= kFirstEpilogue) {
     // ---- epilogue: a warp takes the 32 features of its lanes of TMEM, columns 32 at a time; two warps share them
     int acc = 0;
     const int mine = (warp - kFirstEpilogue) / 4 * 32;  // first columns of the warp
     constexpr int kStep = kEpilogue / 4 * 32;
-    unsigned char* const staged = smem_raw + (base - tc05::smem_u32(smem_raw)) + kStages * kStageBytes + (warp - kFirstEpilogue) * S::kWarp;
-    auto first_feature = [&]() { return tile.feat0 + static_cast<int>(rank) * kBlockFeatures + (warp & 3) * (kBlockFeatures / 4); };
-    if constexpr (ROWS) {
-      const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 4 * mine;
-      while (ok && next()) {
-        RowWarp<OUT, OutT> w(p, tile, columns_of(tile), mine / 32, static_cast<int>(rank) * kM + (warp & 3) * 32, staged, lane);
-        if (tile.steps == 0) {  // nothing of the depth is left for this unit
-          w.zeros();
-          continue;
-        }
-        ok = w.add(taddr, kN, bar_acc_full, bar_acc_empty, acc);
-        acc += tile.steps;
-        if (ok) w.emit();
-      }
-    } else if constexpr (F8) {  // 128 neighbouring columns to a warp
-      static_assert(S::kWarp == S::kStaged + Scales<OUT>::kBytes && Scales<OUT>::kProducts <= S::kStaged, "shared memory of a warp");
-      float* const slots = reinterpret_cast<float*>(staged + S::kStaged);
-      const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-      Scales<OUT> scales;
-      bool more = next();
-      if (more) scales.begin(p, tile, first_feature(), 4 * mine, 128, slots, lane);
-      while (ok && more) {
-        const Tile t = tile;
-        const Warp<OutT> w(p, t, first_feature(), 4 * mine, 32, 128, staged, lane);
-        if (t.steps > 0) ok = w.template add_scaled<OUT>(taddr, kN, bar_acc_full, bar_acc_empty, acc, scales, slots);
-        if (!ok) break;
-        acc += t.steps;
-        more = next();
-        if (more) scales.begin(p, tile, first_feature(), 4 * mine, 128, slots, lane);  // on their way while this tile leaves
-        if (t.steps > 0) {
-          const int buf = (acc - 1) & 1;
-          typename Warp<OutT>::Ahead none;
-          w.template emit<OUT>(taddr + buf * kN, none, [&] { w.taken(&bar_acc_empty[buf]); });
-        } else {  // nothing of the depth is left for this unit
-          w.template zeros<OUT>();
-        }
-      }
-    }
-    while (!F8 && ok && next()) {
-      const int feat0 = first_feature();
+    unsigned char* const staged = smem_raw + (base - tc05::smem_u32(smem_raw)) + kStages * kStageBytes + (warp - kFirstEpilogue) * S::kStaged;
+    while (ok && next()) {
+      const int feat0 = tile.feat0 + static_cast<int>(rank) * kBlockFeatures + (warp & 3) * (kBlockFeatures / 4);
       size_t row = static_cast<size_t>(tile.col0);
       if constexpr (GRAD) row += static_cast<size_t>(tile.group) * p.columns;
       if constexpr (OUT == kGated || OUT == kGatedGrad) {
-        const Warp<OutT> w(p, tile, feat0, mine, kStep, kN, staged, lane);
+        const Warp<OutT> w(p, tile, feat0, mine, kStep, staged, lane);
         const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         if (tile.steps == 0) {  // nothing of the depth is left for this unit
           w.template zeros<OUT>();
@@ -502,138 +572,6 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       }
       if (!done) store_lanes<I8, kStep>(to, p.features, feats, mine, tile.n, taddr, xs, ws, lane, take);
       ++acc;
-    }
-  } else {
-    if constexpr (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F8Registers<kN>::kOthers));
-    if (warp == 0) {
-      // ---- loads.  Each block fetches its 128 features and its half of the columns, and tells rank 0's barrier.
-      while (ok && next()) {
-        const int half = ROWS ? kM : tile.n_mma / 2;
-        auto units_of = [&](int r) { return ROWS ? max(0, min(kM, tile.n - r * kM) + 15) / 16 : half / 16; };  // rows of x, 16 at a time
-        const int units = units_of(static_cast<int>(rank));
-        const int feat = tile.feat0 + static_cast<int>(rank) * (ROWS ? columns_of(tile) / (OUT == kGated ? 4 : 2) : kBlockFeatures);
-        const int col = tile.col0 + static_cast<int>(rank) * half;
-        if (tc05::elect_one()) {
-          const uint32_t bytes = kABytes + (GRAD ? (half > 64 ? 2 : 1) * kAtom : units * 2048);
-          const uint32_t both = ROWS ? 2 * kABytes + (units_of(0) + units_of(1)) * 2048 : 2 * bytes;
-          int s = stage;
-          uint32_t ph = phase;
-          for (int k = tile.step0; k < tile.step0 + tile.steps; ++k) {
-            if (!tc05::mbar_wait(&bar_empty[s], ph ^ 1u)) { ok = false; break; }
-            const uint32_t st = base + s * kStageBytes;
-            uint32_t bar;
-            if (GRAD && (k + 1) * kDepth > tile.depth) {
-              bar = tc05::smem_u32(&bar_tail[s]);
-              tc05::mbar_arrive_expect_tx(&bar_tail[s], bytes);
-            } else {
-              bar = tc05::pair::at_first(&bar_full[s]);
-              if (rank == 0) {  // for both blocks: an arrival from the other one at every step took 1 us each
-                tc05::mbar_arrive_expect_tx(&bar_full[s], both);
-                tc05::mbar_arrive(&bar_full[s]);
-              }
-            }
-            if constexpr (GRAD) {
-              const int row = tile.row0 + k * kDepth;
-              tc05::pair::tma_load_2d(st, &tm_a, feat, row, bar);
-              tc05::pair::tma_load_2d(st + kAtom, &tm_a, feat + 64, row, bar);
-              tc05::pair::tma_load_2d(st + kABytes, &tm_b64, col, row, bar);
-              if (half > 64) tc05::pair::tma_load_2d(st + kABytes + kAtom, &tm_b64, col + 64, row, bar);
-            } else {
-              if constexpr (OUT == kGated) {  // 16 rows of the gate, 16 of the other projection, and so on
-  #pragma unroll
-                for (int q = 0; q < 4; ++q) tc05::pair::tma_load_4d(st + q * 4096, &tm_a, k * kDepth, feat + 16 * q, 0, tile.group, bar);
-              } else if (p.a_mn) {
-                tc05::pair::tma_load_3d(st, &tm_a, feat, k * kDepth, tile.group, bar);
-                tc05::pair::tma_load_3d(st + kAtom, &tm_a, feat + 64, k * kDepth, tile.group, bar);
-              } else {
-                tc05::pair::tma_load_3d(st, &tm_a, k * kDepth, feat, tile.group, bar);
-              }
-              int u = 0;
-              for (; u + 4 <= units; u += 4) tc05::pair::tma_load_2d(st + kABytes + u * 2048, &tm_b64, k * kDepth, col + u * 16, bar);
-              for (; u < units; ++u) tc05::pair::tma_load_2d(st + kABytes + u * 2048, &tm_b16, k * kDepth, col + u * 16, bar);
-            }
-            ++armed;
-            if (++s == kStages) { s = 0; ph ^= 1u; }
-          }
-        }
-        ok = __all_sync(0xffffffffu, ok);
-        advance(tile.steps);
-      }
-      // The last arrivals at this block's barriers come from the other block too: they have come before the block ends.
-      for (int i = 0; i < kStages && ok; ++i) {
-        ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_empty[stage], phase ^ 1u));
-        advance(1);
-      }
-    } else if (warp == 1) {
-      // ---- MMAs of both blocks, from rank 0: M = 256 features, N = the tile's columns
-      int acc = 0;
-      const bool a_mn = GRAD || p.a_mn != 0;
-      const uint32_t a_step = a_mn ? 2048u : 32u, b_step = GRAD ? 2048u : 32u;
-      // left operand: W, or x with ROWS
-      const uint64_t da0 = tc05::smem_desc_swizzled(base + (ROWS ? kABytes : 0), a_mn ? kAtom : 0, 1024, tc05::kSwizzle128B);
-      const uint64_t db0 = tc05::smem_desc_swizzled(base + (ROWS ? 0 : kABytes), GRAD ? kAtom : 0, 1024, tc05::kSwizzle128B);
-      while (rank == 0 && ok && next()) {
-        if (tile.steps == 0) continue;
-        if (tc05::elect_one()) {
-          const int buf = acc & 1;
-          const uint32_t idesc = p.idesc | static_cast<uint32_t>((ROWS ? columns_of(tile) : tile.n_mma) >> 3) << 17;
-          uint32_t d = tmem + buf * kN;
-          int s = stage;
-          uint32_t ph = phase;
-          if constexpr (!F8) ok = tc05::pair::mbar_wait(&bar_acc_empty[buf], ((acc >> 1) & 1) ^ 1);
-          tc05::fence_after_sync();
-          for (int k = tile.step0; k < tile.step0 + tile.steps && ok; ++k) {
-            const bool cleared = GRAD && (k + 1) * kDepth > tile.depth;  // by threads of both blocks
-            if (!(cleared ? tc05::pair::mbar_wait(&bar_full[s], ph) : F8 ? tc05::mbar_spin(&bar_full[s], ph) : tc05::mbar_wait(&bar_full[s], ph))) { ok = false; break; }
-            if constexpr (F8) {  // every step has sums of its own; the operands are there long before
-              const int n = acc + k - tile.step0;
-              d = tmem + (n & 1) * kN;
-              if (!tc05::mbar_spin(&bar_acc_empty[n & 1], ((n >> 1) & 1) ^ 1)) { ok = false; break; }
-            }
-            tc05::fence_after_sync();
-            const uint64_t da = tc05::desc_advance(da0, s * kStageBytes), db = tc05::desc_advance(db0, s * kStageBytes);
-            const int left = tile.depth - k * kDepth;
-  #pragma unroll
-            for (int i = 0; i < kDepth / kInstr; ++i)
-              if (i * kInstr < left)
-                tc05::pair::mma<kKind>(d, tc05::desc_advance(da, i * a_step), tc05::desc_advance(db, i * b_step), idesc,
-                                       ((!F8 && k > tile.step0) || i > 0) ? 1u : 0u);
-            if constexpr (F8) tc05::pair::mma_commit(&bar_acc_full[(acc + k - tile.step0) & 1]);
-            tc05::pair::mma_commit(&bar_empty[s]);
-            if (++s == kStages) { s = 0; ph ^= 1u; }
-          }
-          if constexpr (!F8) tc05::pair::mma_commit(&bar_acc_full[buf]);
-          if (!ok) {  // gave up: what has been issued is over before the block's memory is released
-            tc05::pair::mma_commit(&bar_drain);
-            tc05::mbar_wait(&bar_drain, 0);
-          }
-        }
-        ok = __all_sync(0xffffffffu, ok);
-        acc += F8 ? tile.steps : 1;
-        advance(tile.steps);
-      }
-    } else if (GRAD && warp == 2) {
-      // ---- The last step of a group holds rows of its neighbours: zeros in their place, in both operands (0 times what is
-      // not a number would not be zero), up to where the instructions read.
-      uint32_t tail_phase = 0;
-      while (ok && next()) {
-        const int rem = tile.depth % kDepth;
-        if (rem != 0 && tile.steps > 0 && (tile.step0 + tile.steps) * kDepth > tile.depth) {
-          const int s = (stage + tile.steps - 1) % kStages;
-          ok = __all_sync(0xffffffffu, tc05::mbar_wait(&bar_tail[s], (tail_phase >> s) & 1u));
-          tail_phase ^= 1u << s;
-          const int clear = (((rem + kInstr - 1) / kInstr) * kInstr - rem) * 8;  // pieces of 16 bytes in each atom
-          unsigned char* at = smem_raw + (base - tc05::smem_u32(smem_raw)) + s * kStageBytes + rem * 128;
-          for (int i = lane; i < kStageBytes / kAtom * clear; i += 32) {
-            const int atom = i / clear;
-            *reinterpret_cast<uint4*>(at + atom * kAtom + (i - atom * clear) * 16) = make_uint4(0u, 0u, 0u, 0u);
-          }
-          tc05::fence_async_smem();
-          __syncwarp();
-          if (lane == 0) tc05::pair::arrive_release(tc05::pair::at_first(&bar_full[s]));
-        }
-        advance(tile.steps);
-      }
     }
   }
 
@@ -737,27 +675,9 @@ inline int place_operand(Operand* o, char** scratch, cudaStream_t st) {
   return 0;
 }
 
-template <int ELEM, int OUT, class OutT, int N>
-int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap& tm_b16, const Args& p, cudaStream_t st) {
-  using S = Shape<N, OUT, ELEM>;
-  static thread_local int configured_device = -1;
-  constexpr int smem = S::kSmem;
-  const auto kernel = grouped_kernel<ELEM, OUT, OutT, N>;
-  int dev = 0;
-  SPTIR_CUDA_OK(cudaGetDevice(&dev));
-  if (configured_device != dev) {
-    SPTIR_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    SPTIR_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-    if constexpr (ELEM == kFloat8) {  // a share of more registers than the block has would be waited for for good
-      cudaFuncAttributes attr;
-      SPTIR_CUDA_OK(cudaFuncGetAttributes(&attr, kernel));
-      constexpr int wanted = 128 * F8Registers<N>::kOthers + (S::kThreads - 128) * F8Registers<N>::kEpilogue;
-      if (attr.numRegs * S::kThreads < wanted) return fail("grouped_kernel was built with %d registers to a thread", attr.numRegs);
-    }
-    configured_device = dev;
-  }
-  launch_chained(kernel, 2 * std::min(p.max_tiles, kNumSMs / 2 * S::kBlocks), S::kThreads, smem, st, tm_a, tm_b64, tm_b16, p);
-  SPTIR_LAUNCH_OK("grouped_kernel");
+// Behind a product whose depth units share
+template <bool I8, int OUT, class OutT>
+int join_parts(const Args& p, cudaStream_t st) {
   if (p.splits > 1) {
     const long long rows = p.part / (OUT == kGated ? 2ll * p.features : p.features);
     const unsigned y = static_cast<unsigned>(std::min<long long>(rows, 32768));
@@ -765,11 +685,29 @@ int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap
     if constexpr (OUT == kGated || OUT == kGatedGrad) {
       launch_chained(join_gated_kernel<OUT, OutT>, grid, 256, 0, st, p);
     } else {
-      launch_chained(join_kernel<ELEM == kInt8, OUT == kWeights, OutT>, grid, 256, 0, st, p);
+      launch_chained(join_kernel<I8, OUT == kWeights, OutT>, grid, 256, 0, st, p);
     }
     SPTIR_LAUNCH_OK("join_kernel");
   }
   return 0;
+}
+
+template <bool I8, int OUT, class OutT, int N>
+int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap& tm_b16, const Args& p, cudaStream_t st) {
+  using S = Shape<N, OUT>;
+  static thread_local int configured_device = -1;
+  constexpr int smem = S::kSmem;
+  const auto kernel = grouped_kernel<I8, OUT, OutT, N>;
+  int dev = 0;
+  SPTIR_CUDA_OK(cudaGetDevice(&dev));
+  if (configured_device != dev) {
+    SPTIR_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    SPTIR_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    configured_device = dev;
+  }
+  launch_chained(kernel, 2 * std::min(p.max_tiles, kNumSMs / 2 * S::kBlocks), S::kThreads, smem, st, tm_a, tm_b64, tm_b16, p);
+  SPTIR_LAUNCH_OK("grouped_kernel");
+  return join_parts<I8, OUT, OutT>(p, st);
 }
 
 inline int check_pointers(const char* fn, const int32_t* indptr, int rows, int groups, cudaStream_t st) {
@@ -806,6 +744,21 @@ inline int plan_product(const char* fn, Args* p, int wide, int depth) {
   return set_tiles(fn, p, wide, rows <= 128 * used, [&](int n) { return rows / n + used; },
                    [&](int n) { return used * ((rows + used * n - 1) / (used * n)); }, ceil_div(p->k, depth), rows);
 }
+// The same for f8_kernel (grouped_f8.cu): tiles of 128 rows x 256 rows of W, one to a block, by the same rule for a shared depth.
+inline int plan_f8(const char* fn, Args* p, int wide) {
+  const long long rows = p->rows, used = std::min(p->groups, p->rows);
+  p->mt = ceil_div(wide, 2 * kM);
+  const long long tiles = used * ((rows + used * 128 - 1) / (used * 128)) * p->mt, units = (rows / 128 + used) * p->mt;
+  const int depth = ceil_div(p->k, 128);
+  const int most = static_cast<int>(std::min<long long>(kNumSMs / std::max<long long>(tiles, 1), depth / 4));
+  p->splits = most > 1 && depth - depth / most >= 12 ? most : 1;
+  if (units > (1 << 29) / p->splits) return fail("%s: too many tiles for 32-bit indices", fn);
+  p->max_tiles = static_cast<int>(units) * p->splits;
+  p->per_split = Divisor(p->splits);
+  p->per_band = Divisor(kBand * p->mt);
+  p->part = rows * wide;
+  return 0;
+}
 inline size_t part_bytes(const Args& p) { return p.splits > 1 ? p.part * p.splits * sizeof(float) : 0; }
 
 inline CUtensorMapDataType map_type(int type) {
@@ -815,7 +768,7 @@ inline CUtensorMapDataType map_type(int type) {
 inline uint32_t map_format(int type) { return type == SPARSETIR_F16 ? tc05::kFmtF16 : tc05::kFmtBF16; }
 
 // What the gated products and those of 8-bit floating point check; `half`: feat_out is the width of a gated block, half of W's rows
-inline int check_block(const char* fn, const int32_t* indptr, int rows, int groups, int fi, int fo, bool half, int flags, int known) {
+[[maybe_unused]] inline int check_block(const char* fn, const int32_t* indptr, int rows, int groups, int fi, int fo, bool half, int flags, int known) {
   if (rows < 0 || groups < 0) return fail("%s: negative size", fn);
   if (fi < 1 || fo < 1) return fail("%s: feat_in and %s must be positive", fn, half ? "width" : "feat_out");
   if (std::max(std::max(rows, groups), std::max(fi, fo)) > kLargestSize || (half && fo > kLargestSize / 2) ||
@@ -828,13 +781,13 @@ inline int check_block(const char* fn, const int32_t* indptr, int rows, int grou
 // Maps of a product's operands, in boxes of `depth` of K: W (`each` rows to a group) along K or along the features, or a gated block's along K,
 // 16 rows of the gate and 16 of the other projection, `each` rows further on, to a box.
 inline int map_operands(CUtensorMap* w, CUtensorMap* x64, CUtensorMap* x16, CUtensorMapDataType dt, const Operand& ow, const Operand& ox,
-                        int each, int groups, bool along_k, bool gated) {
+                        int each, int groups, bool along_k, bool gated, cuuint32_t box_rows = kM) {
   const cuuint32_t depth = 128 / ow.size;
   // the weights of the next step come with this one's (us, 128 / 256 bytes: 500 rows, 64 groups, 2048 -> 2048 90.8 / 84.8)
   const CUtensorMapL2promotion fetch = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
   const cuuint64_t cols = ow.cols, n = each, g = groups;
   const cuuint64_t dims[3] = {cols, n, g}, strides[2] = {ow.pitch, ow.pitch * n};
-  const cuuint32_t box[3] = {along_k ? depth : 64, along_k ? kM : depth, 1};
+  const cuuint32_t box[3] = {along_k ? depth : 64, along_k ? box_rows : depth, 1};
   const cuuint64_t two_dims[4] = {cols, n, 2, g}, two_strides[3] = {ow.pitch, ow.pitch * n, ow.pitch * n * 2};
   const cuuint32_t two_box[4] = {depth, 16, 2, 1};
   if (make_tmap(w, dt, ow.data, gated ? 4 : 3, gated ? two_dims : dims, gated ? two_strides : strides, gated ? two_box : box,
@@ -878,14 +831,14 @@ namespace sptir {
 namespace {
 
 // The kernel for results of `type`, with tiles of `columns` columns.
-template <int ELEM, int OUT>
+template <bool I8, int OUT>
 int launch_type(int columns, int type, const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap& tm_b16, const Args& p,
                 cudaStream_t st) {
   return with_type(type, [&](auto o) {
     using O = decltype(o);
     if constexpr (OUT != kWeights)
-      if (columns == 128) return launch<ELEM, OUT, O, 128>(tm_a, tm_b64, tm_b16, p, st);
-    return launch<ELEM, OUT, O, 256>(tm_a, tm_b64, tm_b16, p, st);
+      if (columns == 128) return launch<I8, OUT, O, 128>(tm_a, tm_b64, tm_b16, p, st);
+    return launch<I8, OUT, O, 256>(tm_a, tm_b64, tm_b16, p, st);
   });
 }
 
@@ -943,8 +896,8 @@ int product(const char* fn, const void* x, const void* w, int type, void* y, int
   p.parts = scratch;
   CUtensorMap tm_w, tm_x64, tm_x16;
   if (map_operands(&tm_w, &tm_x64, &tm_x16, map_type(type), ow, ox, out_in ? fo : fi, groups, out_in, false) != 0) return -1;
-  const int rc = i8 ? launch_type<kInt8, kPlain>(columns, y_type, tm_w, tm_x64, tm_x16, p, st)
-                    : launch_type<kHalf, kPlain>(columns, y_type, tm_w, tm_x64, tm_x16, p, st);
+  const int rc = i8 ? launch_type<true, kPlain>(columns, y_type, tm_w, tm_x64, tm_x16, p, st)
+                    : launch_type<false, kPlain>(columns, y_type, tm_w, tm_x64, tm_x16, p, st);
   return rc != 0 ? rc : return_scratch(cs, st);
 }
 
@@ -1032,7 +985,7 @@ extern "C" int sparsetir_grouped_mm_grad_w_raw(const void* x, const void* dy, in
   if (make_tmap_2d(&tm_a, dt, oa.data, oa.cols, rows, oa.pitch, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
       make_tmap_2d(&tm_b, dt, ob.data, ob.cols, rows, ob.pitch, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) != 0)
     return -1;
-  const int rc = launch_type<kHalf, kWeights>(columns, dw_type, tm_a, tm_b, tm_b, p, st);
+  const int rc = launch_type<false, kWeights>(columns, dw_type, tm_a, tm_b, tm_b, p, st);
   return rc != 0 ? rc : return_scratch(cs, st);
 }
 
@@ -1053,7 +1006,12 @@ extern "C" int sparsetir_grouped_mm_workspace(int rows, int num_groups, int feat
   p.k = feat_in;
   p.features = feat_out;
   if (plan_product(fn, &p, feat_out, 128 / element_bytes) < 0) return -1;
-  const size_t product = copy(static_cast<long long>(num_groups) * (out_in ? feat_out : feat_in), out_in ? feat_in : feat_out) + part_bytes(p);
+  size_t parts = part_bytes(p);
+  if (element_bytes == 1) {  // of 8-bit integers, or of floating point
+    if (plan_f8(fn, &p, feat_out) != 0) return -1;
+    parts = std::max(parts, part_bytes(p));
+  }
+  const size_t product = copy(static_cast<long long>(num_groups) * (out_in ? feat_out : feat_in), out_in ? feat_in : feat_out) + parts;
   p.features = out_in ? feat_in : feat_out;
   p.columns = out_in ? feat_out : feat_in;
   if (plan_grad(fn, &p) < 0) return -1;

@@ -17,8 +17,8 @@ template <int OUT>
 int launch_half(int columns, int type, const CUtensorMap& w, const CUtensorMap& x64, const CUtensorMap& x16, const Args& p, cudaStream_t st) {
   return with_half(type, [&](auto t) {
     using T = decltype(t);
-    if (columns == 128) return launch<kHalf, OUT, T, 128>(w, x64, x16, p, st);
-    return launch<kHalf, OUT, T, 256>(w, x64, x16, p, st);
+    if (columns == 128) return launch<false, OUT, T, 128>(w, x64, x16, p, st);
+    return launch<false, OUT, T, 256>(w, x64, x16, p, st);
   });
 }
 
