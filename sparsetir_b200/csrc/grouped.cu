@@ -21,6 +21,7 @@
 // prefetch of the next tiles' operands to L2 (44 -> 60); the whole tiles of all groups first (no change); one arrival
 // of the loading thread at the other block's barrier per step (935 us where now 500).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "gate.cuh"
@@ -42,20 +43,20 @@ constexpr int kStagedBytes = 32 * 64; // 32 columns of 32 features on their way,
 constexpr int kBand = 8;              // column tiles of a group that are walked side by side
 
 // What becomes of the sums: the result, a gradient of weights (rows of a group are the depth), or, in grouped_gated.cuh, a gated block
-// (two rows of W to a feature) and the gradient of one.
-enum Out { kPlain, kWeights, kGated, kGatedGrad };
+// (two rows of W to a feature) and the gradient of one, with rows at 16-byte addresses or at any.
+enum Out { kPlain, kWeights, kGated, kGatedGrad, kGatedGradAny };
 
 // Columns of a tile, and what follows from them.  128 leave room for two pairs of blocks on two SMs: for many groups of few rows,
 // where the loads of one pair hide the other's beginning and end (us, 256 / 128 columns: 64 groups of 16 rows, 512 -> 512
 // 13.6 / 7.6; 500 rows in 64 groups, 2048 -> 2048 91.4 / 90.3; 8 groups of 500 rows 39 / 41).
 template <int N, int OUT = kPlain> struct Shape {
   static constexpr int kBytes = kABytes + N / 2 * 128;  // of a stage
-  static constexpr int kStages = N == 256 ? 6 : OUT == kGatedGrad ? 3 : 4;  // what shared memory holds
+  static constexpr int kStages = N == 256 ? 6 : OUT >= kGatedGrad ? 3 : 4;  // what shared memory holds
   static constexpr int kBlocks = N == 256 ? 1 : 2;      // per SM
   static constexpr int kTmemCols = 2 * N;               // two accumulators
   static constexpr int kEpilogue = N == 256 ? 8 : 4;    // warps
   static constexpr int kThreads = (kFirstEpilogue + kEpilogue) * 32;
-  static constexpr int kStaged = OUT == kGatedGrad ? 2 * kStagedBytes : OUT == kGated ? kStagedBytes + kStagedBytes / 2 : kStagedBytes;
+  static constexpr int kStaged = OUT >= kGatedGrad ? 2 * kStagedBytes : OUT == kGated ? kStagedBytes + kStagedBytes / 2 : kStagedBytes;
   static constexpr int kSmem = kStages * kBytes + kEpilogue * kStaged + 1024;
 };
 
@@ -520,7 +521,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
       const int feat0 = tile.feat0 + static_cast<int>(rank) * kBlockFeatures + (warp & 3) * (kBlockFeatures / 4);
       size_t row = static_cast<size_t>(tile.col0);
       if constexpr (GRAD) row += static_cast<size_t>(tile.group) * p.columns;
-      if constexpr (OUT == kGated || OUT == kGatedGrad) {
+      if constexpr (OUT >= kGated) {
         const Warp<OutT> w(p, tile, feat0, mine, kStep, staged, lane);
         const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         if (tile.steps == 0) {  // nothing of the depth is left for this unit
@@ -629,17 +630,19 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
 // loads in the kernel for few rows instead gained where weights are small (8 groups, 1001 -> 999 11.9 -> 8.5) and lost where
 // they are not (64 rows, 2047 -> 2047 38 -> 62): taken back.
 
-template <class E>  // an element of 1 or 2 bytes
-__global__ void __launch_bounds__(256) pad_rows_kernel(const E* src, uint4* dst, long long rows, int cols, int pieces) {
-  constexpr int N = 16 / sizeof(E);
+// A thread has 16 bytes of a row, in units of U bytes, the largest that rows and operand are multiples of (a gated block in 8 bits, 396
+// rows in 16 groups, 1832 -> 1224: 91 us with units of a byte, 70 with units of 8).
+template <int U>
+__global__ void __launch_bounds__(256) pad_rows_kernel(const Piece<U>* src, uint4* dst, long long rows, int cols, int pieces) {
+  constexpr int N = 16 / U;
   chain_wait();
   const long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   const long long row = at / pieces;
   const int c0 = static_cast<int>(at - row * pieces) * N;
   if (row >= rows) return;
-  const E* from = src + row * cols + c0;
+  const Piece<U>* from = src + row * cols + c0;
   Piece<16> v = make_uint4(0u, 0u, 0u, 0u);
-  E* e = reinterpret_cast<E*>(&v);
+  Piece<U>* e = reinterpret_cast<Piece<U>*>(&v);
 #pragma unroll
   for (int i = 0; i < N; ++i)
     if (c0 + i < cols) e[i] = from[i];
@@ -663,12 +666,17 @@ inline int place_operand(Operand* o, char** scratch, cudaStream_t st) {
   const long long blocks = (o->rows * pieces + 255) / 256;
   if (blocks > INT32_MAX) return fail("operand too large to be copied to aligned rows");
   uint4* to = reinterpret_cast<uint4*>(*scratch);
-  if (o->size == 2)
-    launch_chained(pad_rows_kernel<uint16_t>, static_cast<unsigned>(blocks), 256, 0, st, static_cast<const uint16_t*>(o->data), to,
-                   o->rows, o->cols, pieces);
-  else
-    launch_chained(pad_rows_kernel<uint8_t>, static_cast<unsigned>(blocks), 256, 0, st, static_cast<const uint8_t*>(o->data), to,
-                   o->rows, o->cols, pieces);
+  const size_t row_bytes = static_cast<size_t>(o->cols) * o->size;
+  auto run = [&](auto unit) {
+    constexpr int U = unit.value;
+    launch_chained(pad_rows_kernel<U>, static_cast<unsigned>(blocks), 256, 0, st, static_cast<const Piece<U>*>(o->data), to, o->rows,
+                   static_cast<int>(row_bytes / U), pieces);
+  };
+  const size_t both = row_bytes | reinterpret_cast<uintptr_t>(o->data);
+  if (both % 8 == 0) run(std::integral_constant<int, 8>{});
+  else if (both % 4 == 0) run(std::integral_constant<int, 4>{});
+  else if (both % 2 == 0) run(std::integral_constant<int, 2>{});
+  else run(std::integral_constant<int, 1>{});
   SPTIR_LAUNCH_OK("pad_rows_kernel");
   *scratch += o->copy_bytes();
   o->data = to;
@@ -682,7 +690,7 @@ int join_parts(const Args& p, cudaStream_t st) {
     const long long rows = p.part / (OUT == kGated ? 2ll * p.features : p.features);
     const unsigned y = static_cast<unsigned>(std::min<long long>(rows, 32768));
     const dim3 grid(ceil_div(p.features, 256), y, ceil_div(rows, y));
-    if constexpr (OUT == kGated || OUT == kGatedGrad) {
+    if constexpr (OUT >= kGated) {
       launch_chained(join_gated_kernel<OUT, OutT>, grid, 256, 0, st, p);
     } else {
       launch_chained(join_kernel<I8, OUT == kWeights, OutT>, grid, 256, 0, st, p);

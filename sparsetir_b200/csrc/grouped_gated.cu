@@ -113,6 +113,7 @@ extern "C" int sparsetir_grouped_mm_gated_grad_raw(const void* dy, const void* w
   p.parts = scratch;
   CUtensorMap tm_w, tm_x64, tm_x16;
   if (map_operands(&tm_w, &tm_x64, &tm_x16, map_type(type), ow, ox, out_in ? width : feat, num_groups, out_in, false) != 0) return -1;
-  const int rc = launch_half<kGatedGrad>(columns, type, tm_w, tm_x64, tm_x16, p, st);
+  const int rc = p.wide ? launch_half<kGatedGrad>(columns, type, tm_w, tm_x64, tm_x16, p, st)
+                        : launch_half<kGatedGradAny>(columns, type, tm_w, tm_x64, tm_x16, p, st);
   return rc != 0 ? rc : return_scratch(cs, st);
 }

@@ -163,68 +163,92 @@ struct Warp {
   __device__ __forceinline__ void gated_grad(const float* da, const float* db, int c0, Ahead& ahead, Next&& next) const {
     const size_t width = p.features;
     OutT* const dg = static_cast<OutT*>(p.hidden) + row(c0) * 2 * width + feat0;
-    if (p.wide) {
-      __syncwarp();  // the reads of the last 32 columns are over
+    __syncwarp();  // the reads of the last 32 columns are over
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = static_cast<int>(place64(8 * i + (lane >> 2), lane & 3));
+      *reinterpret_cast<uint4*>(staged + at) = ahead.g[i];
+      *reinterpret_cast<uint4*>(staged + kStagedBytes + at) = ahead.u[i];
+    }
+    if (c0 + step < t.n) ask(c0 + step, ahead);
+    __syncwarp();
+    uint32_t act[16];
+    auto differentiate = [&](auto gelu) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int at = static_cast<int>(place64(8 * i + (lane >> 2), lane & 3));
-        *reinterpret_cast<uint4*>(staged + at) = ahead.g[i];
-        *reinterpret_cast<uint4*>(staged + kStagedBytes + at) = ahead.u[i];
-      }
-      if (c0 + step < t.n) ask(c0 + step, ahead);
-      __syncwarp();
-      uint32_t act[16];
-      auto differentiate = [&](auto gelu) {
+        uint32_t g[4], u[4], og[4], ou[4];
+        get64(0, i, g);
+        get64(kStagedBytes, i, u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t g[4], u[4], og[4], ou[4];
-          get64(0, i, g);
-          get64(kStagedBytes, i, u);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float* d = (q < 2 ? da : db) + 4 * i + 2 * (q & 1);
-            Two xg, xu, xa;
-            Gate::grad<gelu.value>(halves_of(g[q]), halves_of(u[q]), Two(d[0], d[1]), &xg, &xu, &xa);
-            og[q] = pack2<OutT>(xg.lo(), xg.hi());
-            ou[q] = pack2<OutT>(xu.lo(), xu.hi());
-            act[4 * i + q] = pack2<OutT>(xa.lo(), xa.hi());
-          }
-          __syncwarp();
-          put64(0, i, og[0], og[1], og[2], og[3]);  // in the place of what was read
-          put64(kStagedBytes, i, ou[0], ou[1], ou[2], ou[3]);
+        for (int q = 0; q < 4; ++q) {
+          const float* d = (q < 2 ? da : db) + 4 * i + 2 * (q & 1);
+          Two xg, xu, xa;
+          Gate::grad<gelu.value>(halves_of(g[q]), halves_of(u[q]), Two(d[0], d[1]), &xg, &xu, &xa);
+          og[q] = pack2<OutT>(xg.lo(), xg.hi());
+          ou[q] = pack2<OutT>(xu.lo(), xu.hi());
+          act[4 * i + q] = pack2<OutT>(xa.lo(), xa.hi());
         }
-      };
-      if (p.gate.gelu) differentiate(std::true_type{});
-      else differentiate(std::false_type{});
-      next();
-      __syncwarp();
-      OutT* const to = dg + static_cast<size_t>(lane >> 2) * 2 * width + 8 * (lane & 3);
-      const bool live = 8 * (lane & 3) < feats;
-      leave64(0, to, 2 * width, live, c0);
-      leave64(kStagedBytes, to + width, 2 * width, live, c0);
-      if (p.out != nullptr) {
         __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) put64(0, i, act[4 * i], act[4 * i + 1], act[4 * i + 2], act[4 * i + 3]);
-        __syncwarp();
-        leave64(0, static_cast<OutT*>(p.out) + row(c0 + (lane >> 2)) * width + feat0 + 8 * (lane & 3), width, live, c0);
+        put64(0, i, og[0], og[1], og[2], og[3]);  // in the place of what was read
+        put64(kStagedBytes, i, ou[0], ou[1], ou[2], ou[3]);
       }
-      return;
-    }
-    const OutT* const h = static_cast<const OutT*>(p.hidden_in) + row(c0) * 2 * width + feat0;
-    OutT* const act = static_cast<OutT*>(p.out) + row(c0) * width + feat0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int f = 16 * (i >> 4) + 8 * ((i >> 1) & 1) + lane / 4, c = 8 * ((i >> 2) & 3) + 2 * (lane & 3) + (i & 1);
-      if (f >= feats || c0 + c >= t.n) continue;
-      const size_t at = c * 2 * width + f;
-      float xg, xu, xa;
-      p.gate.grad(to_float(ld_global(h + at)), to_float(ld_global(h + at + width)), i < 16 ? da[i & 15] : db[i & 15], &xg, &xu, &xa);
-      dg[at] = from_float<OutT>(xg);
-      dg[at + width] = from_float<OutT>(xu);
-      if (p.out != nullptr) act[c * width + f] = from_float<OutT>(xa);
-    }
+    };
+    if (p.gate.gelu) differentiate(std::true_type{});
+    else differentiate(std::false_type{});
     next();
+    __syncwarp();
+    OutT* const to = dg + static_cast<size_t>(lane >> 2) * 2 * width + 8 * (lane & 3);
+    const bool live = 8 * (lane & 3) < feats;
+    leave64(0, to, 2 * width, live, c0);
+    leave64(kStagedBytes, to + width, 2 * width, live, c0);
+    if (p.out != nullptr) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) put64(0, i, act[4 * i], act[4 * i + 1], act[4 * i + 2], act[4 * i + 3]);
+      __syncwarp();
+      leave64(0, static_cast<OutT*>(p.out) + row(c0 + (lane >> 2)) * width + feat0 + 8 * (lane & 3), width, live, c0);
+    }
+  }
+  template <class Next>
+  __device__ __forceinline__ void gated_grad_any(const float* da, const float* db, int c0, Next&& next) const {
+    const size_t width = p.features;
+    OutT* const dg = static_cast<OutT*>(p.hidden) + row(c0) * 2 * width + feat0;
+    // At any address: the sums through shared memory, lane = feature, eight columns' projections on their way at a time (14,774 rows in 8
+    // groups, 1024 -> 826: 138 us, one element after the other out of the fragments 243).  An instantiation of its own: its registers cost
+    // the form for aligned rows 10% (65,536 rows in 64 groups, 2048 -> 1024: 291 us, with both in one kernel 316).
+    float* const sums = reinterpret_cast<float*>(staged);
+    auto place = [](int c, int f) { return c * 32 + (f ^ ((c & 14) << 1)); };  // lanes of a column, and of a fragment, in different banks
+    __syncwarp();  // the reads of the last 32 columns are over
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      sums[place(8 * ((i >> 2) & 3) + 2 * (lane & 3) + (i & 1), 16 * (i >> 4) + 8 * ((i >> 1) & 1) + lane / 4)] = i < 16 ? da[i & 15] : db[i & 15];
+    next();
+    __syncwarp();
+    const OutT* const h = static_cast<const OutT*>(p.hidden_in) + row(c0) * 2 * width + feat0 + lane;
+    OutT* const act = static_cast<OutT*>(p.out) + row(c0) * width + feat0 + lane;
+    const int n = min(32, t.n - c0);
+    for (int c = 0; lane < feats && c < n; c += 8) {
+      OutT hg[8], hu[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        hg[q] = hu[q] = OutT{};
+        if (c + q < n) {
+          hg[q] = ld_global(h + (c + q) * 2 * width);
+          hu[q] = ld_global(h + (c + q) * 2 * width + width);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        if (c + q >= n) break;
+        float xg, xu, xa;
+        p.gate.grad(to_float(hg[q]), to_float(hu[q]), sums[place(c + q, lane)], &xg, &xu, &xa);
+        OutT* const to = dg + (c + q) * 2 * width + lane;
+        to[0] = from_float<OutT>(xg);
+        to[width] = from_float<OutT>(xu);
+        if (p.out != nullptr) act[(c + q) * width] = from_float<OutT>(xa);
+      }
+    }
+    __syncwarp();
   }
 
   // ---- sums that are complete in TMEM; take(): the warp's last columns are in registers, the accumulator may be written again
@@ -257,8 +281,10 @@ struct Warp {
         next();
       } else if constexpr (OUT == kGated) {
         gated(va, vb, c0, next);
-      } else {
+      } else if constexpr (OUT == kGatedGrad) {
         gated_grad(va, vb, c0, ahead, next);
+      } else {
+        gated_grad_any(va, vb, c0, next);
       }
     }
   }
@@ -271,7 +297,7 @@ struct Warp {
   template <int OUT>
   __device__ __forceinline__ bool out_of_tmem(uint32_t taddr, uint64_t* full, uint64_t* empty, uint32_t parity) const {
     Ahead ahead;
-    if (OUT == kGatedGrad && p.wide != 0 && p.splits == 1 && first < t.n) ask(first, ahead);
+    if (OUT == kGatedGrad && p.splits == 1 && first < t.n) ask(first, ahead);
     if (!__all_sync(0xffffffffu, tc05::mbar_wait(full, parity))) return false;
     tc05::fence_after_sync();
     emit<OUT>(taddr, ahead, [&] { taken(empty); });
