@@ -598,7 +598,8 @@ SPARSETIR_API int sparsetir_moe_combine_grad_raw(const void* dy, const void* z, 
 /* Scratch bytes at most of sparsetir_grouped_mm and its gradient (element_bytes 2) or of sparsetir_grouped_mm_i8 (1): copies of
  * operands whose rows do not start at 16-byte addresses, and sums of thread blocks that share a tile (20 MB at most).  Of the
  * gated products with feat_out = 2 * width, of sparsetir_grouped_mm_gated_grad with feat and width as feat_in and feat_out, of the products
- * of 8-bit floating point with element_bytes 1. */
+ * of 8-bit floating point with element_bytes 1.  flags: those of the call, of which SPARSETIR_GATED_GELU changes nothing; without
+ * SPARSETIR_GROUPED_W_OUT_IN the answer is enough for both layouts of W. */
 SPARSETIR_API int sparsetir_grouped_mm_workspace(int rows, int num_groups, int feat_in, int feat_out, int element_bytes,
                                                  int flags, size_t* scratch_bytes);
 /* rows: how many x and y have; row pointers outside of [0, rows] are taken as the nearer bound */

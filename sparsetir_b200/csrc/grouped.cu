@@ -1001,7 +1001,7 @@ extern "C" int sparsetir_grouped_mm_workspace(int rows, int num_groups, int feat
                                               size_t* scratch_bytes) {
   const char* fn = "sparsetir_grouped_mm_workspace";
   const int32_t some = 0;  // pointers are not looked at
-  if (check_groups(fn, &some, rows, num_groups, feat_in, feat_out, flags) != 0) return -1;
+  if (check_block(fn, &some, rows, num_groups, feat_in, feat_out, false, flags, SPARSETIR_GROUPED_W_OUT_IN | SPARSETIR_GATED_GELU) != 0) return -1;
   if ((element_bytes != 1 && element_bytes != 2) || !scratch_bytes) return fail("%s: bad argument", fn);
   *scratch_bytes = 0;
   if (rows == 0 || num_groups == 0) return 0;
@@ -1019,7 +1019,9 @@ extern "C" int sparsetir_grouped_mm_workspace(int rows, int num_groups, int feat
     if (plan_f8(fn, &p, feat_out) != 0) return -1;
     parts = std::max(parts, part_bytes(p));
   }
-  const size_t product = copy(static_cast<long long>(num_groups) * (out_in ? feat_out : feat_in), out_in ? feat_in : feat_out) + parts;
+  // W along the depth, or, where the flags do not say so, the larger of the two: a gated product has it so without a flag
+  const size_t along_k = copy(static_cast<long long>(num_groups) * feat_out, feat_in);
+  const size_t product = (out_in ? along_k : std::max(along_k, copy(static_cast<long long>(num_groups) * feat_in, feat_out))) + parts;
   p.features = out_in ? feat_in : feat_out;
   p.columns = out_in ? feat_out : feat_in;
   if (plan_grad(fn, &p) < 0) return -1;
