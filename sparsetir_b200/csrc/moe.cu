@@ -582,14 +582,32 @@ __device__ __forceinline__ uint32_t pack_f8(float a, float b, float c, float d) 
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return __byte_perm(lo, hi, 0x5410);
 }
-// 448 x / a to the nearest e4m3, ties to even, for |x| <= a: the quotient of 0.875 x by unit = a / 512.  Both are exact for elements of 16 bits, and
-// so is the place of their rounded quotient between the numbers of 8 bits, ties among them.  below and above are 0.875 / unit moved by
-// four units of its last place: where x times both has one place, so has the quotient, and four divisions are spared.
+__device__ __forceinline__ float2 unpack_f8(uint32_t two) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3)));
+}
+// Of lo and hi, neighbours or the same, the nearer one to 0.875 x / unit, or their middle, which is rounded to the even one: by the sign of
+// 0.875 x - middle * unit.  Each product and what its rounding leaves are exact, so are their differences, a few bits beside each other, and
+// that of the products themselves, which are next to each other.  `by`: a power of two that keeps what is left above the smallest numbers.
+__device__ __forceinline__ float nearer(float x, float unit, float lo, float hi, float by) {
+  const float middle = 0.5f * (lo + hi), y = x * by, u = unit * by, a = __fmul_rn(0.875f, y), b = __fmul_rn(middle, u);
+  const float d = (a - b) + (fmaf(0.875f, y, -a) - fmaf(middle, u, -b));
+  return d == 0.f ? middle : d > 0.f ? fmaxf(lo, hi) : fminf(lo, hi);
+}
+// 448 x / a to the nearest e4m3, ties to even, for |x| <= a: the quotient of 0.875 x by unit = a / 512.  below and above are 0.875 / unit moved by
+// four units of its last place: where x times both has one place between the numbers of 8 bits, so has the quotient, and four divisions are spared.
+// For elements of 16 bits 0.875 x is exact, and so is the place of the rounded quotient, ties among them; for 32 bits it is not.
+template <class T>
 __device__ __forceinline__ uint32_t quotients_f8(const float* x, float unit, float below, float above) {
-  uint32_t q = pack_f8(x[0] * below, x[1] * below, x[2] * below, x[3] * below);
-  if (q != pack_f8(x[0] * above, x[1] * above, x[2] * above, x[3] * above))
-    q = pack_f8(0.875f * x[0] / unit, 0.875f * x[1] / unit, 0.875f * x[2] / unit, 0.875f * x[3] / unit);
-  return q;
+  const uint32_t q = pack_f8(x[0] * below, x[1] * below, x[2] * below, x[3] * below);
+  const uint32_t r = pack_f8(x[0] * above, x[1] * above, x[2] * above, x[3] * above);
+  if (q == r) return q;
+  if constexpr (sizeof(T) == 4) {
+    const float by = unit < 1.f ? 0x1p20f : 0x1p-20f;
+    const float2 q01 = unpack_f8(q & 0xffffu), q23 = unpack_f8(q >> 16), r01 = unpack_f8(r & 0xffffu), r23 = unpack_f8(r >> 16);
+    return pack_f8(nearer(x[0], unit, q01.x, r01.x, by), nearer(x[1], unit, q01.y, r01.y, by), nearer(x[2], unit, q23.x, r23.x, by),
+                   nearer(x[3], unit, q23.y, r23.y, by));
+  }
+  return pack_f8(0.875f * x[0] / unit, 0.875f * x[1] / unit, 0.875f * x[2] / unit, 0.875f * x[3] / unit);
 }
 // The largest magnitude of pieces, in the order of unsigned integers (so that an infinity or a NaN is larger than all numbers), and as the bits of
 // a float: of 16-bit elements two at a time.
@@ -671,7 +689,7 @@ dispatch_f8_kernel(const Piece<B>* x, const int32_t* slots, uint8_t* q, float* s
     }
 #pragma unroll
     for (int e = 0; e < E; e += 4) {
-      const uint32_t q4 = quotients_f8(f + e, unit, times * (1.f - 0x1p-21f), times * (1.f + 0x1p-21f));
+      const uint32_t q4 = quotients_f8<T>(f + e, unit, times * (1.f - 0x1p-21f), times * (1.f + 0x1p-21f));
       o[h][e / 4] = zeros ? 0u : q4;
     }
   }
