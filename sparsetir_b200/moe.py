@@ -39,7 +39,7 @@ class Saved:
     x: torch.Tensor
     routing: Routing
     rows: torch.Tensor    # the tokens' rows in the experts' order
-    hidden: torch.Tensor  # [pairs, 2 * width]: gate and up projections
+    hidden: Optional[torch.Tensor]  # [pairs, 2 * width]: gate and up projections; None where a gated layer was to keep nothing
     act: Optional[torch.Tensor]  # silu(gate) * up; a gated layer forms it again
     out: torch.Tensor     # the experts' results
 
@@ -112,7 +112,7 @@ class ExpertLayer(_Layer):
         return d_hidden, act
 
     def forward(self, x: torch.Tensor, padding: Optional[torch.Tensor] = None, train: bool = True) -> Tuple[torch.Tensor, Saved]:
-        """The result, and what ``backward`` needs; without ``train`` a gated layer does not keep that."""
+        """The result, and what ``backward`` needs; without ``train`` a gated layer does not keep that, and ``backward`` refuses."""
         r = route(self._logits(x, padding), self.top_k, self.renormalize)
         rows = torch.empty(x.shape[0] * self.top_k, self.features, dtype=x.dtype, device=x.device)
         ops.moe_dispatch(x.view(-1), r.slots.view(-1), rows.view(-1), self.features, self.top_k)
@@ -129,6 +129,8 @@ class ExpertLayer(_Layer):
         return y, Saved(x, r, rows, hidden, act if self.gated is None else None, out)
 
     def backward(self, dy: torch.Tensor, s: Saved) -> Dict[str, torch.Tensor]:
+        if s.hidden is None:
+            raise ValueError("backward needs the projections, which forward keeps with train=True")
         r, k = s.routing, self.top_k
         d_out, d_gates = torch.empty_like(s.out), torch.empty_like(r.gates)
         ops.moe_combine_grad(dy.contiguous().view(-1), s.out.view(-1), r.slots.view(-1), r.gates.view(-1), d_out.view(-1),
