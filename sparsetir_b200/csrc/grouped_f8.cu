@@ -422,7 +422,6 @@ int product_f8(const char* fn, const void* x, const float* x_scale, const void* 
   p.groups = groups;
   p.k = fi;
   p.features = fo;
-  p.wide = wide_rows(y, y_type, fo);
   p.idesc = tc05::instr_desc(tc05::kFmtE4M3, kM, 0, 0, 0);
   const int each = gated ? 2 * fo : fo;  // rows of one W
   if (plan_f8(fn, &p, each) != 0) return -1;
