@@ -425,7 +425,7 @@ SPARSETIR_API int sparsetir_grouped_mm_gated_grad(SPARSETIR_PACKED_ARGS);
 SPARSETIR_API int sparsetir_moe_dispatch_f8(SPARSETIR_PACKED_ARGS);
 
 /* y[s, fo] = sum over the blocks b of 128 of feat_in of  x_scale[b, s] * w_scale[g, fo / 128, b] * sum_{fi in b} x[s, fi] * w[g, fo, fi],
- * sums in f32.
+ * sums in f32, the product of the two scales formed first.
  * args: (x e4m3 [S*feat_in], x_scale f32[ceil(feat_in/128)*S], w e4m3 [num_groups*feat_out*feat_in],
  *        w_scale f32[num_groups*ceil(feat_out/128)*ceil(feat_in/128)], y f16|bf16|f32 [S*feat_out], indptr i32[num_groups+1] or null,
  *        num_groups, feat_in, feat_out). */

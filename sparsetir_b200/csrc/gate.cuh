@@ -2,8 +2,9 @@
 //   silu                z = g
 //   gelu, form of tanh  0.5 g (1 + tanh(u)) = g * sigmoid(2 u):  z = 2 sqrt(2 / pi) (g + 0.044715 g^3)
 // and its gradient: with s = sigmoid(z),  f' = s + g s (1 - s) z'.
-// All of it in f32; exp and the quotient by the hardware's approximations (a few units of 2^-22: nothing beside the rounding of a 16-bit
-// result).
+// All of it in f32; exp and the quotient by the hardware's approximations.  The exponential multiplies the few roundings of its argument by |z|:
+// f and act are off by (8 |z| + 32) 2^-24 of their value at most, 2^-14 where they are still above 2^-140 (|z| = 104).  That is little beside the
+// rounding of a 16-bit result; one of 32 bits would show it.
 #ifndef SPARSETIR_B200_GATE_CUH_
 #define SPARSETIR_B200_GATE_CUH_
 
@@ -13,8 +14,9 @@
 
 namespace sptir {
 
-// Two floats that go through one instruction: the epilogues of the products wait for the results of most of their instructions, and this halves
-// their number.
+// Two floats that go through one instruction, half as many of them to issue in the epilogues of the products.  (Us, floats one by one / this, two
+// runs each: gated products of 6,001 rows 73.4 73.6 / 73.0 73.2, of 65,536 rows 463 463 / 462 462, the gradient 320 361 / 322 317, in 8-bit
+// floating point 186 182 / 179 184.)
 struct Two {
   uint64_t v;
   Two() = default;

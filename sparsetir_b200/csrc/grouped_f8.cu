@@ -8,13 +8,16 @@
 // one step and the next.
 //
 // What bounds it is the way there and back: from the issue of a step's MMAs (512 clocks) to their sums in registers, to take them (350 clocks) and
-// until the issuing thread knows, with two accumulators on the way.  Us, 65,536 rows in 64 equal groups, 2048 -> 2048, by pairs of blocks on
+// until the issuing thread knows, with two accumulators on the way.  Of the 2,100 clocks of that round trip some 570 are not accounted for.
+// Us, 65,536 rows in 64 equal groups, 2048 -> 2048, by pairs of blocks on
 // 256 rows: with the features as the left operand and the rows' scales out of shared memory 512 to 566, rows as the left operand 367, with
 // the loads of TMEM in flight across the steps 328, with waits that ask again and again 310 to 320.  This kernel, without another block to wait for,
-// takes 328, wastes less on ragged groups and reads weights for few rows as well as tiles of their own did (perf of both, us, pairs / this: 8,192
+// takes 331, and 562 for 8192^3 where the pairs took 513; it wastes less on ragged groups and reads weights for few rows as well as tiles of
+// their own did (us, calls in a row of two sets of inputs, pairs / this: 8,192
 // rows to eight of 64 ragged groups with their quantisation 391 / 382, 4,096 to four of 32 120 / 107, gated 230 / 192; 4,096 rows in 64 groups, 2048 ->
-// 2048 71 / 60, 6,400 rows 1024 -> 1024 28 / 19, 500 rows 2048 -> 2048 56 / 56: 268 MB of weights).
-// 8-bit integers, which are scaled at the end alone, take 228 where this takes 328.
+// 2048 71 / 60, 6,400 rows 1024 -> 1024 28 / 19, 500 rows 2048 -> 2048 56 / 56: 268 MB of weights).  The gated form spills 76 bytes of a thread's
+// registers.
+// 8-bit integers, which are scaled at the end alone, take 228 where this takes 331.
 #define SPARSETIR_GROUPED_KERNEL_ONLY
 #include "grouped.cu"
 
@@ -426,8 +429,8 @@ int product_f8(const char* fn, const void* x, const float* x_scale, const void* 
   const int each = gated ? 2 * fo : fo;  // rows of one W
   if (plan_f8(fn, &p, each) != 0) return -1;
   Operand ox{x, rows, fi, 1}, ow{w, static_cast<long long>(groups) * each, fi, 1};
-  // us, the kernel for few rows / this one: 1 row, 4096 -> 8192 7.6 / 16.7; 16 rows 10.8 / 17.4; 48 rows, 8 groups, 1024 -> 4096 8.5 / 16.7; 64 rows,
-  // 8 groups, 2048 -> 2048 10.3 / 14.3, gated 17.3 / 29.3
+  // us, weights out of HBM, the kernel for few rows / this one: 1 row, 4096 -> 8192 10.3 / 14.2; 16 rows 12.5 / 15.1; 8 groups of 8 rows, 2048 -> 2048
+  // 12.2 / 14.0 (of 10 and more rows this one: 14.1), gated, 1024 -> 2 x 2048 12.9 / 15.0; 32 groups, 1024 -> 1024, of 4 rows 10.8 / 11.4, of 8 12.7 / 11.7
   const bool few = fi <= kFewF8Depth && few_rows_pay(rows, groups, fi, each, true);
   const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + (few ? 0 : part_bytes(p));
   CallScratch cs;

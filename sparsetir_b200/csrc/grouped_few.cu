@@ -135,7 +135,8 @@ struct AlongK {
 
 // The same for 8-bit floating point: the sums of a step, half of a block of K that shares scales, are scaled and added to those of the steps
 // before it.  The scales of a block's rows of x and W, for all of the depth, are in shared memory: in registers with the steps
-// ahead they were spilled (48 rows, 8 groups, 1024 -> 2 x 2048: 17.2 us where now 9.9).
+// ahead they were spilled (48 rows, 8 groups, 1024 -> 2 x 2048, weights in L2: 17.2 us where now 8.6).  With 16 rows at a time 52 bytes of a
+// thread's registers are spilled all the same, 72 in the gated form.
 template <int NT, bool GATED>
 struct Scaled : AlongK<__nv_fp8_e4m3, NT, GATED> {
   using Base = AlongK<__nv_fp8_e4m3, NT, GATED>;
@@ -406,8 +407,10 @@ int with_rows(const FewArgs& p, int each, F&& f) {
   if (p.rows <= static_cast<long long>(each) * std::min(p.groups, p.rows)) return f(std::integral_constant<int, 1>{});
   return f(std::integral_constant<int, 2>{});
 }
-// Of the gated products and those of 8-bit floating point (us, 8 rows at a time / 16: 48 rows, 8 groups, 1024 -> 2 x 2048 9.2 / 10.1, in
-// 8 bits 8.8 / 11.1; 16 rows, 1 group, 4096 -> 2 x 4096 16.6 / 10.7, 4096 -> 8192 in 8 bits 13.8 / 10.7).
+// Of the gated products and those of 8-bit floating point.  Us, weights out of HBM, 8 rows at a time / 16.  Even groups: 8 groups of 4, 6 and 8
+// rows, 1024 -> 2 x 2048 14.0 / 13.9, 14.5 / 14.5, 14.6 / 14.6, in 8 bits 10.3 / 12.3, 10.8 / 12.8, 10.9 / 12.9; one group of 10 rows, 4096 -> 2 x 4096
+// 20.1 / 14.0, 4096 -> 8192 in 8 bits 15.8 / 12.3: beyond 8 rows the weights are read again.  So they are for the larger ones of ragged groups: 40
+// and 64 rows over 8 groups, the same sizes, 18.7 / 14.5 and 20.3 / 15.0, in 8 bits 10.8 / 13.2 and 16.5 / 13.2.
 constexpr int kRowsEach = 6;
 
 template <class T>

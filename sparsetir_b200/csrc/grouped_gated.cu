@@ -6,7 +6,7 @@
 // side by side (a box of 16 x 2 rows), so that both meet in one thread of the epilogue.  The gradient's epilogue has the projections of the next 32
 // rows on their way while it works, and puts their gradients where they lay in shared memory.
 // 65,536 rows, 64 groups, 2048 -> 2 x 1024, bf16: 434 us with both projections kept (even groups; 1.27 PFLOP/s, the plain product of that size
-// 404 to 460), 545 with ragged ones; the gradient 285 and 354: without its loads and stores of the projections 226, its 1.2 GB alone are 184.
+// 404 to 460), 462 to 564 with ragged ones (calls in a row, runs of seconds); the gradient 285 and 317 to 362: without its loads and stores of the projections 226, its 1.2 GB alone are 184.
 #define SPARSETIR_GROUPED_KERNEL_ONLY
 #include "grouped.cu"
 
@@ -57,6 +57,8 @@ extern "C" int sparsetir_grouped_mm_gated_raw(const void* x, const void* w, void
   p.idesc = tc05::instr_desc(map_format(type), 2 * kM, 0, 0, 0);
   const int columns = plan_product(fn, &p, 2 * width, 64);
   if (columns < 0) return -1;
+  // us, weights out of HBM, the kernel for few rows / this one: 8 groups of 3 and 8 rows, 1024 -> 2 x 2048 13.8 / 14.8, 14.6 / 14.9; one group of 1 and
+  // 16 rows, 4096 -> 2 x 4096 13.2 / 17.9, 14.2 / 18.4
   const bool few = few_rows_pay(rows, num_groups, feat_in, 2 * width, true);
   Operand ox{x, rows, feat_in, 2}, ow{w, static_cast<long long>(num_groups) * 2 * width, feat_in, 2};
   const size_t bytes = ox.copy_bytes() + ow.copy_bytes() + (few ? 0 : part_bytes(p));

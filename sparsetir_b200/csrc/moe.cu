@@ -633,8 +633,8 @@ struct Largest {
 };
 
 // Rows to 8-bit floating point with a scale for each block of 128 features: L lanes have a block, P pieces each that lie side by side, and a
-// warp kHold times as many blocks as it has room for.  (Us, 8,192 rows of 2048 in 16 bits to eight slots each, 172 MB: 36.0 with a
-// division to an element and 8 bytes to a store, now 30.0; one slot each, 16,384 rows of 4096, 201 MB: 71 and 47.)
+// warp kHold times as many blocks as it has room for.  (Us, 8,192 rows of 2048 in bfloat16 to eight slots each, 172 MB: 36.0 with a
+// division to an element and 8 bytes to a store, now 29.2; one slot each, 16,384 rows of 4096, 201 MB: 71 and 47, in float16 38, in 32 bits, 336 MB, 53.)
 template <class T, int B, bool WIDE>
 struct F8Lanes {
   static constexpr int N = B / sizeof(T);  // elements of a piece
