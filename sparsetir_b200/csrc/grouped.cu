@@ -94,11 +94,16 @@ struct Args {
   long long part; // elements of one split's
   uint32_t idesc; // without N
   int a_mn;       // the left operand is contiguous along the features
-  int wide;       // rows of the result start at 16-byte addresses, and so do the following
-  const void* hidden_in;  // gradient of a gated block: its projections
-  void* hidden;   // gated: the projections, or null; gradient: theirs.  `out` is act, in the gradient it may be null
+  int wide;       // rows of the result start at 16-byte addresses, and so do those of GatedArgs
+};
+static_assert(sizeof(Args) == 136, "what a launch was measured with (FewGatedArgs)");
+// Of a gated block and its gradient.
+struct GatedArgs : Args {
+  const void* hidden_in;  // gradient: the block's projections
+  void* hidden;   // the projections, or null; gradient: theirs.  `out` is act, in the gradient it may be null
   Gate gate;
 };
+template <int OUT> using ArgsOf = std::conditional_t<(OUT >= kGated), GatedArgs, Args>;
 
 // First and past the last row of group g, inside the array whatever the pointers say.
 __device__ __forceinline__ void group_rows(const Args& p, int g, int* first, int* last) {
@@ -324,7 +329,7 @@ namespace {
 template <bool I8, int OUT, class OutT, int kN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kN>::kThreads, Shape<kN>::kBlocks)
 grouped_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b64,
-               const __grid_constant__ CUtensorMap tm_b16, const __grid_constant__ Args p) {
+               const __grid_constant__ CUtensorMap tm_b16, const __grid_constant__ ArgsOf<OUT> p) {
   constexpr int kDepth = I8 ? 128 : 64;  // of K per stage
   constexpr int kInstr = I8 ? 32 : 16;   // of K per instruction
   using S = Shape<kN, OUT>;
@@ -685,7 +690,7 @@ inline int place_operand(Operand* o, char** scratch, cudaStream_t st) {
 
 // Behind a product whose depth units share
 template <bool I8, int OUT, class OutT>
-int join_parts(const Args& p, cudaStream_t st) {
+int join_parts(const ArgsOf<OUT>& p, cudaStream_t st) {
   if (p.splits > 1) {
     const long long rows = p.part / (OUT == kGated ? 2ll * p.features : p.features);
     const unsigned y = static_cast<unsigned>(std::min<long long>(rows, 32768));
@@ -701,7 +706,7 @@ int join_parts(const Args& p, cudaStream_t st) {
 }
 
 template <bool I8, int OUT, class OutT, int N>
-int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap& tm_b16, const Args& p, cudaStream_t st) {
+int launch(const CUtensorMap& tm_a, const CUtensorMap& tm_b64, const CUtensorMap& tm_b16, const ArgsOf<OUT>& p, cudaStream_t st) {
   using S = Shape<N, OUT>;
   static thread_local int configured_device = -1;
   constexpr int smem = S::kSmem;
@@ -897,7 +902,7 @@ int product(const char* fn, const void* x, const void* w, int type, void* y, int
   char* scratch = cs.scratch;
   if (place_operand(&ox, &scratch, st) != 0 || place_operand(&ow, &scratch, st) != 0) return -1;
   if (few) {
-    FewArgs f{ox.data, ow.data, y, xs, ws, indptr, ox.pitch, ow.pitch, rows, groups, fi, fo, fi * size, 0, 0, 0, nullptr, Gate()};
+    FewArgs f{ox.data, ow.data, y, xs, ws, indptr, ox.pitch, ow.pitch, rows, groups, fi, fo, fi * size, 0, 0, 0};
     const int done = few_rows(f, type, y_type, out_in, st);
     return done != 0 ? done : return_scratch(cs, st);
   }

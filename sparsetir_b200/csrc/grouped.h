@@ -33,7 +33,13 @@ struct FewArgs {
   int rows, groups, fi, fo;
   int k_bytes;              // of a row of x
   int splits, split_bytes, feature_warps;  // set by the launcher
-  void* hidden;  // gated: the projections, or null; fo is the width
+};
+// Of a gated block; fo is the width.  Apart from what the other kernels take: a launch's time on the host depends on where the bytes of its
+// parameters end within 64 (us, one row, 512 -> 64, calls in a row, with 96 bytes / 112: 2.96 / 3.38; the kernel for tiles, whose parameters end
+// elsewhere, with 520 / 544: 3.33 / 3.66).
+static_assert(sizeof(FewArgs) == 96, "what a launch was measured with");
+struct FewGatedArgs : FewArgs {
+  void* hidden;  // the projections, or null
   Gate gate;
 };
 
@@ -41,9 +47,9 @@ struct FewArgs {
 // contiguous along the depth.
 int few_rows(const FewArgs& p, int type, int y_type, bool along_k, cudaStream_t st);
 // The gated block (W along the depth) of 16-bit elements, and the product or the gated block of 8-bit floating point.
-int few_rows_gated(const FewArgs& p, int type, cudaStream_t st);
+int few_rows_gated(const FewGatedArgs& p, int type, cudaStream_t st);
 constexpr int kFewF8Depth = 16384;  // at most, whose scales shared memory holds
-int few_rows_f8(const FewArgs& p, int y_type, bool gated, cudaStream_t st);
+int few_rows_f8(const FewGatedArgs& p, int y_type, bool gated, cudaStream_t st);
 
 }  // namespace sptir
 #endif  // SPARSETIR_B200_GROUPED_H_

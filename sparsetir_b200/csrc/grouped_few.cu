@@ -76,6 +76,7 @@ template <class T, int NT, bool GATED = false>
 struct AlongK {
   static constexpr int kFeatures = 32, kStepBytes = 64, kRows = 8 * NT;
   static constexpr bool kGated = GATED;
+  using Args = std::conditional_t<GATED, FewGatedArgs, FewArgs>;
   using Sum = typename SumOf<T>::type;
   Sum acc[2][NT][4];
   struct Step { uint4 w[4], x[NT]; };
@@ -221,6 +222,7 @@ template <class T, int NT>
 struct AlongFeatures {
   static constexpr int kFeatures = 32, kStepBytes = 64, kRows = 8 * NT;  // bytes of K in x
   static constexpr bool kGated = false;
+  using Args = FewArgs;
   using Sum = float;
   float acc[2][NT][4];
   struct Step { uint2 w[8]; uint4 x[NT]; };
@@ -283,7 +285,7 @@ struct AlongFeatures {
 // these (256 rows, 64 groups, 2048 -> 1024, W along the depth, us, spread evenly / a quarter in one group / all in one:
 // 50 / 175 / 437, this way 50 / 50 / 28; the kernel of grouped.cu 47 / 46 / 15).
 template <class Operand, class OutT>
-__global__ void __launch_bounds__(32 * kMaxWarps, 1) few_rows_kernel(const __grid_constant__ FewArgs p) {
+__global__ void __launch_bounds__(32 * kMaxWarps, 1) few_rows_kernel(const __grid_constant__ typename Operand::Args p) {
   using Sum = typename Operand::Sum;
   constexpr int F = Operand::kFeatures, kRows = Operand::kRows;
   constexpr int O = Operand::kGated ? F / 2 : F;  // features of the result to a warp
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 1) few_rows_kernel(const __gri
 }
 
 template <class Operand, class OutT>
-int launch(FewArgs p, cudaStream_t st) {
+int launch(typename Operand::Args p, cudaStream_t st) {
   // as many warps as keep the memory busy: the depth is split where the features of the groups are too few, into parts of four
   // steps at least.  Eight warps to a block, fewer where blocks would not be found on every SM.
   const int used = std::min(p.groups, p.rows);
@@ -429,14 +431,14 @@ int few_rows(const FewArgs& p, int type, int y_type, bool along_k, cudaStream_t 
   return launch_type<__nv_bfloat16>(p, y_type, along_k, st);
 }
 
-int few_rows_gated(const FewArgs& p, int type, cudaStream_t st) {
+int few_rows_gated(const FewGatedArgs& p, int type, cudaStream_t st) {
   return with_rows(p, kRowsEach, [&](auto nt) {
     if (type == SPARSETIR_F16) return launch<AlongK<__half, nt.value, true>, __half>(p, st);
     return launch<AlongK<__nv_bfloat16, nt.value, true>, __nv_bfloat16>(p, st);
   });
 }
 
-int few_rows_f8(const FewArgs& p, int y_type, bool gated, cudaStream_t st) {
+int few_rows_f8(const FewGatedArgs& p, int y_type, bool gated, cudaStream_t st) {
   return with_rows(p, kRowsEach, [&](auto nt) {
     return with_type(y_type, [&](auto o) {
       using O = decltype(o);

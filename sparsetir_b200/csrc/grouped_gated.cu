@@ -14,7 +14,7 @@ namespace sptir {
 namespace {
 
 template <int OUT>
-int launch_half(int columns, int type, const CUtensorMap& w, const CUtensorMap& x64, const CUtensorMap& x16, const Args& p, cudaStream_t st) {
+int launch_half(int columns, int type, const CUtensorMap& w, const CUtensorMap& x64, const CUtensorMap& x16, const GatedArgs& p, cudaStream_t st) {
   return with_half(type, [&](auto t) {
     using T = decltype(t);
     if (columns == 128) return launch<false, OUT, T, 128>(w, x64, x16, p, st);
@@ -44,7 +44,7 @@ extern "C" int sparsetir_grouped_mm_gated_raw(const void* x, const void* w, void
   if (use_device(device_id) != 0) return -1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (check_pointers(fn, indptr, rows, num_groups, st) != 0) return -1;
-  Args p{};
+  GatedArgs p{};
   p.out = y;
   p.hidden = hidden;
   p.gate = Gate((flags & SPARSETIR_GATED_GELU) != 0);
@@ -67,8 +67,8 @@ extern "C" int sparsetir_grouped_mm_gated_raw(const void* x, const void* w, void
   char* scratch = cs.scratch;
   if (place_operand(&ox, &scratch, st) != 0 || place_operand(&ow, &scratch, st) != 0) return -1;
   if (few) {
-    const FewArgs f{ox.data, ow.data, y, nullptr, nullptr, indptr, ox.pitch, ow.pitch, rows, num_groups, feat_in, width, feat_in * 2, 0, 0, 0, hidden,
-                    p.gate};
+    const FewGatedArgs f{{ox.data, ow.data, y, nullptr, nullptr, indptr, ox.pitch, ow.pitch, rows, num_groups, feat_in, width, feat_in * 2, 0, 0, 0},
+                         hidden, p.gate};
     const int done = few_rows_gated(f, type, st);
     return done != 0 ? done : return_scratch(cs, st);
   }
@@ -91,7 +91,7 @@ extern "C" int sparsetir_grouped_mm_gated_grad_raw(const void* dy, const void* w
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (check_pointers(fn, indptr, rows, num_groups, st) != 0) return -1;
   const bool out_in = (flags & SPARSETIR_GROUPED_W_OUT_IN) != 0;
-  Args p{};
+  GatedArgs p{};
   p.out = act;
   p.hidden_in = hidden;
   p.hidden = d_hidden;

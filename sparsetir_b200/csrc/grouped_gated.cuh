@@ -13,14 +13,14 @@ namespace {
 // An epilogue warp's share of a tile: features feat0 and so on, columns first, first + step and so on 32 at a time.
 template <class OutT>
 struct Warp {
-  const Args& p;
+  const GatedArgs& p;
   const Tile& t;
   const int feat0, first, step;
   unsigned char* const staged;
   const int lane;
   const int feats;  // live ones from feat0 on, may be <= 0
 
-  __device__ __forceinline__ Warp(const Args& args, const Tile& tile, int feat, int column, int stride, unsigned char* mem, int l)
+  __device__ __forceinline__ Warp(const GatedArgs& args, const Tile& tile, int feat, int column, int stride, unsigned char* mem, int l)
       : p(args), t(tile), feat0(feat), first(column), step(stride), staged(mem), lane(l), feats(args.features - feat) {}
 
   // Row of column c of the tile
@@ -307,7 +307,7 @@ struct Warp {
 
 // The sums of the units that share a tile, added in their order, and what becomes of them: thread = a feature of a row
 template <int OUT, class T>
-__global__ void __launch_bounds__(256) join_gated_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(256) join_gated_kernel(const __grid_constant__ GatedArgs p) {
   chain_wait();
   const long long row = blockIdx.y + static_cast<long long>(blockIdx.z) * gridDim.y;
   const int feat = blockIdx.x * 256 + threadIdx.x;
