@@ -3,7 +3,8 @@
 //   grouped_mm_i8      the same in 8-bit integers, scaled per row and per output feature
 //   grouped_mm_grad_w  dW[g, a, b] = sum over the rows s of group g of pa[s, a] * pb[s, b]
 //
-// All three are one kernel, and so are the products of grouped_gated.cu and grouped_f8.cu, which take the kernel and what its hosts share from here.  A
+// All three are one kernel, and so are the products of grouped_gated.cu, which includes this file; grouped_f8.cu, which does too, has a kernel of its own
+// and takes the walk over the tiles and what the hosts share.  A
 // pair of blocks (cta_group::2) holds 256 of what is contiguous in the result (output
 // features; b) as the rows of the tensor core's left operand, and up to 256 of what is not (rows of the group; a) as the columns:
 // the result comes out of TMEM with neighbouring lanes at neighbouring addresses, and a ragged group costs its rows rounded
